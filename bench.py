@@ -74,7 +74,7 @@ def _peaks():
 
 
 DECODE_SOURCES = ("dsa_decode.cu", "dsa_decode_h16.cuh", "dsa_decode_hm.cuh", "dsa_pipeline.cuh",
-                  "sm100_ptx.cuh")
+                  "dsa_common.cuh", "dsa_host.cuh", "sm100_ptx.cuh")
 
 
 def kernel_digest() -> str:

@@ -21,15 +21,13 @@
 #include <utility>
 
 #include "dsa_b200.h"
+#include "dsa_common.cuh"
+#include "dsa_host.cuh"
 #include "sm100_ptx.cuh"
 
 namespace dsa {
 
-constexpr int kDCkv = 512;            // latent (value) width
-constexpr int kDKpe = 64;             // rope key width
-constexpr float kTau = 8.0f;          // lazy-rescale threshold (log2 units)
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint64_t kWaitCycles = 4000000000ull;  // default wait bound: ~2 s at ~2 GHz
+constexpr float kTau = 8.0f;  // lazy-rescale threshold (log2 units)
 
 struct Params {
   const int32_t* idx;
@@ -58,57 +56,6 @@ struct Params {
   const uint8_t* member;
   int64_t member_sb;
   int32_t tok_shift;
-};
-
-// UMMA shared-memory descriptor, 128-byte swizzle, sm_100 (version 1).
-__device__ __forceinline__ uint64_t sdesc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-  d |= (uint64_t)((lbo >> 4) & 0x3FFFu) << 16;
-  d |= (uint64_t)((sbo >> 4) & 0x3FFFu) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
-}
-
-// Instruction descriptor, kind::f16: bf16 A/B, fp32 D; A and B K-major unless flagged.
-__host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool a_mn_major,
-                                                  bool b_mn_major = false) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn_major ? 1u : 0u) << 15) |
-         ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-
-// Byte offset of element (row h, column k) in a [rows x 64] bf16 tile stored
-// K-major with the 128-byte swizzle (the UMMA canonical SW128 K-major layout).
-__device__ __forceinline__ uint32_t sw128_off(int h, int k) {
-  return (uint32_t)((h >> 3) * 1024 + (h & 7) * 128 + ((((k >> 3) ^ (h & 7))) << 4) + (k & 7) * 2);
-}
-
-// Bounded mbarrier wait.  `spin` polls without letting the hardware suspend the thread
-// (for the latency-critical MMA issuer); otherwise try_wait may suspend it briefly.
-struct Waiter {
-  volatile uint32_t* abort_flag;
-  uint32_t* err;
-  uint64_t limit;  // cycles
-  bool spin = false;
-  __device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) const {
-    return spin ? ptx::mbar_test_wait(bar, parity) : ptx::mbar_try_wait(bar, parity);
-  }
-  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) const {
-    if (poll(bar, parity)) return true;
-    const uint64_t t0 = ptx::cycles();
-    for (uint32_t it = 1;; ++it) {
-      if (poll(bar, parity)) return true;
-      if ((it & 63u) == 0) {
-        if (*abort_flag) return false;
-        if (ptx::cycles() - t0 > limit) {
-          *abort_flag = 1;
-          atomicOr(err, (uint32_t)DSA_DEVERR_TIMEOUT);
-          return false;
-        }
-      }
-    }
-  }
 };
 
 // CTA c owns units [u_begin(c), u_begin(c+1)).
@@ -167,25 +114,6 @@ __global__ void selftest_wait_kernel(uint32_t* err, int64_t timeout_ns) {
 namespace dsa {
 // ====================================================================== host side
 namespace {
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn get_encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, []() {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault,
-                                         &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  });
-  return fn;
-}
 
 constexpr int kMaxDevices = 64;
 
@@ -269,10 +197,6 @@ int device_pairs(int dev) {
   return d.pairs;
 }
 
-bool heads_supported(int heads) {
-  return heads == 16 || heads == 32 || heads == 64 || heads == 128;
-}
-
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 // Workspace layout, fixed for a device so that calls of any shape can share it:
@@ -295,60 +219,6 @@ WsLayout ws_layout(int sms) {
   // one partial slot per cluster pair (a pair occupies two SMs)
   w.total = align_up(w.parts_off + (size_t)((sms + 1) / 2) * kMaxSlotFloats * 4, 256);
   return w;
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-// Encoded tensor maps of recent calls (per host thread): a decode loop reuses its pools and
-// usually its query buffers, and encoding costs microseconds of host time per map.
-struct MapKey {
-  const void* base;
-  int rank;
-  cuuint64_t dims[3], strides[2];
-  cuuint32_t box[3];
-  int swz;
-  bool operator==(const MapKey& o) const { return memcmp(this, &o, sizeof(MapKey)) == 0; }
-};
-struct MapCache {
-  static constexpr int kWays = 16;
-  MapKey key[kWays];
-  CUtensorMap map[kWays];
-  bool used[kWays] = {};
-  int next = 0;
-};
-thread_local MapCache t_maps;
-
-int encode(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims,
-           const cuuint64_t* strides_bytes, const cuuint32_t* box, CUtensorMapSwizzle swz) {
-  MapKey k;
-  memset(&k, 0, sizeof(k));  // padding bytes take part in the comparison
-  k.base = base;
-  k.rank = rank;
-  for (int i = 0; i < rank; ++i) {
-    k.dims[i] = dims[i];
-    k.box[i] = box[i];
-  }
-  for (int i = 0; i + 1 < rank; ++i) k.strides[i] = strides_bytes[i];
-  k.swz = (int)swz;
-  MapCache& c = t_maps;
-  for (int w = 0; w < MapCache::kWays; ++w)
-    if (c.used[w] && c.key[w] == k) {
-      *m = c.map[w];
-      return DSA_OK;
-    }
-  EncodeTiledFn fn = get_encode_fn();
-  if (!fn) return DSA_ERR_DRIVER;
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base),
-                  dims, strides_bytes, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return DSA_ERR_DRIVER;
-  const int w = c.next;
-  c.next = (c.next + 1) % MapCache::kWays;
-  c.key[w] = k;
-  c.map[w] = *m;
-  c.used[w] = true;
-  return DSA_OK;
 }
 
 // Every kernel of a call is launched with programmatic stream serialization: it may be
@@ -526,7 +396,7 @@ int run_plan(const DecodeArgs& a, const Plan& pl, uint8_t* ws, cudaStream_t st) 
   prm.err = reinterpret_cast<uint32_t*>(ws);
   prm.parts = reinterpret_cast<float*>(ws + kPartsOff);
   prm.counters = reinterpret_cast<uint32_t*>(ws + kCountersOff);
-  prm.wait_cycles = g_wait_cycles.load(std::memory_order_relaxed);
+  prm.wait_cycles = wait_limit_cycles();
   prm.pt = a.page_table;
   prm.pt_sb = a.pt_sb;
   prm.pt_cols = a.pt_cols;
@@ -568,6 +438,9 @@ int decode_with_workspace(const DecodeArgs& a, void* workspace, size_t workspace
 }
 
 }  // namespace
+
+uint64_t wait_limit_cycles() { return g_wait_cycles.load(std::memory_order_relaxed); }
+
 }  // namespace dsa
 
 using namespace dsa;

@@ -13,15 +13,9 @@ namespace pipe {
 constexpr int kBlk = 4;                   // 64-wide ckv d-blocks per CTA
 constexpr int kProdWarps = kBlk + 1;      // one gather producer warp per d-block + the kpe half
 constexpr int kMaskAny = 7;               // mask word of a stage: nonzero when any slot is valid
-constexpr uint32_t kSw128 = 2, kSw64 = 4;  // UMMA descriptor layout types
-
-// UMMA shared-memory descriptor (sm_100, version 1): start, leading and stride byte offsets.
-__device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t lbo, uint32_t sbo,
-                                         uint32_t layout) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
-         ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | ((uint64_t)1 << 46) |
-         ((uint64_t)layout << 61);
-}
+using dsa::desc;
+using dsa::kSw128;
+using dsa::kSw64;
 
 // Index entries of tile t of (row, head group) rh for a producer lane's group g: slot
 // ids, or token positions in a paged call; -1 past topk.

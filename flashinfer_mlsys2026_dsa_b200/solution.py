@@ -28,6 +28,8 @@ ENTRY_POINT = "kernel.cu::kernel"
 SOURCE_FILES = (
     ("kernel.cu", os.path.join(_build.CSRC, "kernel.cu")),
     ("dsa_decode.cu", os.path.join(_build.CSRC, "dsa_decode.cu")),
+    ("dsa_common.cuh", os.path.join(_build.CSRC, "dsa_common.cuh")),
+    ("dsa_host.cuh", os.path.join(_build.CSRC, "dsa_host.cuh")),
     ("dsa_pipeline.cuh", os.path.join(_build.CSRC, "dsa_pipeline.cuh")),
     ("dsa_decode_h16.cuh", os.path.join(_build.CSRC, "dsa_decode_h16.cuh")),
     ("dsa_decode_hm.cuh", os.path.join(_build.CSRC, "dsa_decode_hm.cuh")),
