@@ -41,6 +41,28 @@ _PAGED_ARGTYPES = (_DECODE_ARGTYPES[:11]
                       _c.c_void_p, _c.c_int64]                          # positions, stride_b
                    + _DECODE_ARGTYPES[13:])
 
+_I32, _I64, _PTR, _SIZE, _F32 = _c.c_int32, _c.c_int64, _c.c_void_p, _c.c_size_t, _c.c_float
+_Q8_CACHE = [_PTR, _I64, _PTR, _I32, _PTR, _I64, _I64]  # ckv_q8, stride, scale, block, kpe,
+#                                                         stride, num_slots
+_TABLE = [_PTR, _I64, _I32]                             # page_table, stride_b, cols
+_DECODE_Q8_ARGTYPES = (_DECODE_ARGTYPES[:6] + _Q8_CACHE + _TABLE + [_I32]  # page_size
+                       + [_PTR, _I64, _F32]             # indices, stride_b, sm_scale
+                       + _DECODE_ARGTYPES[14:20] + [_PTR, _I64]  # output, lse; weights, stride_b
+                       + [_I64, _I32, _I32]             # num_tokens, num_heads, topk
+                       + [_PTR, _SIZE, _PTR, _PTR])     # scratch, bytes, workspace, stream
+_APPEND_Q8_ARGTYPES = ([_PTR, _I64, _PTR, _I64, _I64]   # ckv, stride_t, kpe, stride_t, num_tokens
+                       + [_PTR, _PTR, _I32]             # row_offsets, starts, num_rows
+                       + _TABLE + [_I32] + _Q8_CACHE + [_PTR, _PTR])
+_ACCUMULATE_ARGTYPES = [_PTR, _I64, _PTR, _I64, _I64, _I32,  # weights, positions, tokens, topk
+                        _PTR, _I64, _I32, _I32, _PTR,        # acc, stride_r, cols, rows, offsets
+                        _PTR, _PTR]
+_EVICT_ARGTYPES = [_PTR, _I64, _PTR, _I64, _I32,             # acc, stride_b, lengths, rows, max_len
+                   _I32, _I32, _I32, _PTR, _I64, _PTR,       # budget, sinks, recent, keep,
+                   #                                           stride_b, new_lengths
+                   _PTR, _I64, _I32, _PTR]                   # new_acc, stride_b, cols, stream
+_COMPACT_Q8_ARGTYPES = ([_PTR, _I64, _I32, _I32] + _TABLE + _TABLE + [_I32] + _Q8_CACHE
+                        + [_PTR, _PTR])
+
 EXPORTED_SYMBOLS = (
     "dsa_sparse_mla_decode",
     "dsa_sparse_mla_decode_paged",
@@ -48,6 +70,12 @@ EXPORTED_SYMBOLS = (
     "dsa_sparse_mla_decode_grouped",
     "dsa_topk_slots",
     "dsa_union_groups",
+    "dsa_sparse_mla_decode_q8",
+    "dsa_q8_scratch_size",
+    "dsa_append_q8",
+    "dsa_accumulate_weights",
+    "dsa_evict_positions",
+    "dsa_compact_q8",
     "dsa_sparse_mla_decode_workspace_size",
     "dsa_read_error_word",
     "dsa_selftest_bounded_wait",
@@ -103,6 +131,15 @@ def load(build_if_missing: bool = True):
             _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int32, _c.c_float,
             _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int64,
             _c.c_int64, _c.c_int32, _c.c_void_p, _c.c_size_t, _c.c_void_p]
+        for name, argtypes in (("dsa_sparse_mla_decode_q8", _DECODE_Q8_ARGTYPES),
+                               ("dsa_append_q8", _APPEND_Q8_ARGTYPES),
+                               ("dsa_accumulate_weights", _ACCUMULATE_ARGTYPES),
+                               ("dsa_evict_positions", _EVICT_ARGTYPES),
+                               ("dsa_compact_q8", _COMPACT_Q8_ARGTYPES)):
+            getattr(lib, name).restype = _c.c_int
+            getattr(lib, name).argtypes = argtypes
+        lib.dsa_q8_scratch_size.restype = _c.c_size_t
+        lib.dsa_q8_scratch_size.argtypes = [_c.c_int64, _c.c_int32, _c.c_int32]
         lib.dsa_sparse_mla_decode_workspace_size.restype = _c.c_size_t
         lib.dsa_sparse_mla_decode_workspace_size.argtypes = [_c.c_int64, _c.c_int32, _c.c_int32,
                                                              _c.c_int32]

@@ -1,0 +1,594 @@
+// The 8-bit latent cache: sparse-MLA decode over it, the append that writes it, the
+// accumulation of attention weights and the compaction that follows an eviction.
+//
+// Cache layout.  A slot's latent row is 512 e4m3 values (1 sign, 4 exponent, 3 mantissa bits;
+// no infinities); every `block` consecutive slots of a page (a power of two that divides the
+// page size) share one fp32 scale, so that
+//     ckv[slot][d] = float(ckv_q8[slot][d]) * ckv_scale[slot / block].
+// The 64 rope key values of a slot stay bf16: they are an eighth of the values, take no part in the
+// output, and carry the positions' phases, which 3 mantissa bits would blur.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <atomic>
+#include <utility>
+
+#include "dsa_b200.h"
+#include "dsa_common.cuh"
+#include "dsa_host.cuh"
+#include "sm100_ptx.cuh"
+
+namespace dsa {
+namespace q8 {
+
+// A cache as the kernels see it.
+struct Cache {
+  uint8_t* ckv;
+  int64_t ckv_ss;  // bytes between slots
+  float* scale;    // one per block, consecutive
+  __nv_bfloat16* kpe;
+  int64_t kpe_ss;  // elements between slots
+  int64_t num_slots;
+  int32_t block_shift;  // log2(tokens per scale)
+};
+
+// A row-major int32 table of pool pages.
+struct PageTable {
+  const int32_t* pt;
+  int64_t sb;
+  int32_t cols;
+  int32_t shift;  // log2(page size)
+};
+
+// The slot of token position `pos` of a row; -1 when the table has none for it or it lies
+// outside the pool.
+__device__ __forceinline__ int slot_at(const PageTable& t, int64_t row, int pos,
+                                       int64_t num_slots) {
+  const int pg = pos >> t.shift;
+  if (pos < 0 || pg >= t.cols) return -1;
+  const int32_t page = __ldg(t.pt + row * t.sb + pg);
+  if (page < 0) return -1;
+  const int64_t slot = ((int64_t)page << t.shift) | (int64_t)(pos & ((1 << t.shift) - 1));
+  return slot < num_slots ? (int)slot : -1;
+}
+
+// Two floats rounded to e4m3 (nearest, ties to even; past 448 to 448; NaN stays NaN).
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Two e4m3 values (exact in fp16).
+__device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)v));
+  return __half22float2(*reinterpret_cast<__half2*>(&h));
+}
+
+// Sixteen e4m3 values times `ratio`, rounded to e4m3 again.
+__device__ __forceinline__ uint4 rescale16(uint4 v, float ratio) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 a = from_e4m3x2(w[i] & 0xFFFFu), b = from_e4m3x2(w[i] >> 16);
+    w[i] = to_e4m3x2(a.x * ratio, a.y * ratio) | (to_e4m3x2(b.x * ratio, b.y * ratio) << 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The smallest power of two s with amax <= 448 s, at least 2^-126 (so that 1 / s is finite).
+// 448 = 1.75 * 2^8: with amax = m 2^e (1 <= m < 2), s = 2^(e - 8) when m <= 1.75, else 2^(e - 7).
+__device__ __forceinline__ float scale_for(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  const int e = (int)(u >> 23) - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);  // biased
+  return __uint_as_float((uint32_t)(e < 1 ? 1 : e) << 23);
+}
+
+}  // namespace q8
+}  // namespace dsa
+
+#include "dsa_q8_attend.cuh"
+
+namespace dsa {
+namespace q8 {
+
+// ------------------------------------------------------------------------------- append
+//
+// Row r's new tokens [offsets[r], offsets[r + 1]) take the positions starts[r], starts[r] + 1,
+// ... of its sequence.  The unit of work is one block of the cache that the call writes to
+// (a job): its scale becomes the smallest power of two that holds every new token of the
+// block, or the block's earlier scale if that is larger and the block has earlier tokens; if
+// the scale grew, the earlier tokens are re-expressed in it (times old / new, an exact shift
+// of the exponent for powers of two, except where a value becomes subnormal).  One CTA owns a
+// job, so that the amax, the earlier tokens and the scale need no other CTA; a warp moves one
+// token at a time, a lane 16 of its values.  Jobs are found from the tokens: CTA c looks at
+// tokens [c * chunk, (c + 1) * chunk) and runs the jobs whose first token lies there.
+
+constexpr int kAppendThreads = 256;
+constexpr int kAppendWarps = kAppendThreads / 32;
+
+struct AppendParams {
+  const __nv_bfloat16* ckv;
+  int64_t ckv_sb;
+  const __nv_bfloat16* kpe;
+  int64_t kpe_sb;
+  const int32_t* offsets;
+  const int32_t* starts;
+  int32_t rows;
+  int32_t tokens;
+  int32_t chunk;
+  PageTable table;
+  Cache cache;
+  uint32_t* err;
+};
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a <= 3.402823466e38f ? a : 0.f;  // infinities and NaN take no part in the scale
+}
+
+// Eight bf16 values (16 bytes) as floats; infinities become NaN, as e4m3 has none.
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
+  __shared__ uint32_t amax_s;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int block = 1 << p.cache.block_shift;
+  ptx::grid_dep_wait();
+  ptx::launch_dependents();
+  const int last = min(p.tokens, max(0, __ldg(p.offsets + p.rows)));
+  int t = (int)blockIdx.x * p.chunk;
+  const int t_end = min(t + p.chunk, last);
+  if (t >= t_end) return;
+  // the row of token t: offsets are ascending, so it is how many of offsets[1..rows] are <= t
+  int row = 0;
+  for (int i0 = 0; i0 < p.rows; i0 += kAppendThreads) {
+    const int i = i0 + (int)threadIdx.x;
+    row += __syncthreads_count(i < p.rows && __ldg(p.offsets + i + 1) <= t);
+  }
+  for (; t < t_end;) {
+    while (row < p.rows && __ldg(p.offsets + row + 1) <= t) ++row;
+    if (row >= p.rows) return;
+    const int lo = __ldg(p.offsets + row), hi = min(__ldg(p.offsets + row + 1), last);
+    if (t < lo) {  // tokens before the first row
+      t = min(lo, t_end);
+      continue;
+    }
+    const int64_t start = __ldg(p.starts + row);
+    const int64_t pos64 = start + (t - lo);
+    if (start < 0 || pos64 + block > INT32_MAX) {  // the row has no such positions
+      if (threadIdx.x == 0) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
+      t = hi;
+      continue;
+    }
+    const int pos = (int)pos64;
+    const int in_block = pos & (block - 1);
+    const int n = min(block - in_block, hi - t);  // tokens of this row left in the block
+    if (t > lo && in_block != 0) {                // not a job's first token
+      t += n;
+      continue;
+    }
+    const int slot0 = slot_at(p.table, row, pos, p.cache.num_slots);
+    if (slot0 < 0) {
+      if (threadIdx.x == 0) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
+      t += n;
+      continue;
+    }
+    if (threadIdx.x == 0) amax_s = 0u;
+    __syncthreads();
+    float a = 0.f;
+    for (int i = warp; i < n; i += kAppendWarps) {
+      const uint4* src = reinterpret_cast<const uint4*>(p.ckv + (int64_t)(t + i) * p.ckv_sb) + 2 * lane;
+      float f[8];
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        unpack8(__ldg(src + v), f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_abs(f[j]));
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+    if (lane == 0) atomicMax(&amax_s, __float_as_uint(a));  // non-negative floats order as bits
+    const float before = in_block != 0 ? p.cache.scale[slot0 >> p.cache.block_shift] : 0.f;
+    __syncthreads();
+    const float need = scale_for(__uint_as_float(amax_s));
+    const float scale = fmaxf(need, before);
+    if (scale != before) {
+      const float ratio = before / scale;
+      for (int i = warp; i < in_block; i += kAppendWarps) {
+        uint4* q = reinterpret_cast<uint4*>(p.cache.ckv + (int64_t)(slot0 - in_block + i) * p.cache.ckv_ss) + lane;
+        *q = rescale16(*q, ratio);
+      }
+      if (threadIdx.x == 0) p.cache.scale[slot0 >> p.cache.block_shift] = scale;
+    }
+    // 1 / scale is exact for a power of two; a caller's other scales take the division
+    const bool pow2 = (__float_as_uint(scale) & 0x7FFFFFu) == 0u;
+    const float inv = 1.f / scale;
+    for (int i = warp; i < n; i += kAppendWarps) {
+      const uint4* src = reinterpret_cast<const uint4*>(p.ckv + (int64_t)(t + i) * p.ckv_sb) + 2 * lane;
+      uint32_t w[4];
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        float f[8];
+        unpack8(__ldg(src + v), f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (isinf(f[j])) f[j] = NAN;
+          f[j] = pow2 ? f[j] * inv : f[j] / scale;
+        }
+        w[2 * v] = to_e4m3x2(f[0], f[1]) | (to_e4m3x2(f[2], f[3]) << 16);
+        w[2 * v + 1] = to_e4m3x2(f[4], f[5]) | (to_e4m3x2(f[6], f[7]) << 16);
+      }
+      const int64_t slot = slot0 + i;
+      reinterpret_cast<uint4*>(p.cache.ckv + slot * p.cache.ckv_ss)[lane] =
+          make_uint4(w[0], w[1], w[2], w[3]);
+      if (lane < 8)
+        reinterpret_cast<uint4*>(p.cache.kpe + slot * p.cache.kpe_ss)[lane] =
+            __ldg(reinterpret_cast<const uint4*>(p.kpe + (int64_t)(t + i) * p.kpe_sb) + lane);
+    }
+    t += n;
+    __syncthreads();  // amax_s is rewritten by the next job
+  }
+}
+
+// --------------------------------------------------------------------------- accumulate
+//
+// acc[r][positions[t][k]] += weights[t][k] for the tokens t of row r.  Tokens of one row may
+// name the same position, so one CTA adds a row's tokens in order, a barrier between them;
+// with one token per row the entries are independent and spread over CTAs of 256.  The adds
+// are fire-and-forget reductions, also right when a token names a position twice.
+
+struct AccumulateParams {
+  const float* weights;
+  int64_t w_sb;
+  const int32_t* positions;
+  int64_t pos_sb;
+  float* acc;
+  int64_t acc_sb;
+  const int32_t* offsets;  // nullptr: token r is row r
+  int32_t tokens;
+  int32_t topk;
+  int32_t acc_cols;
+  uint32_t* err;
+};
+
+__device__ __forceinline__ void accumulate_entry(const AccumulateParams& p, float* row, int64_t t,
+                                                 int k) {
+  const int pos = __ldg(p.positions + t * p.pos_sb + k);
+  const float w = __ldg(p.weights + t * p.w_sb + k);
+  if (pos >= 0 && pos < p.acc_cols)
+    atomicAdd(row + pos, w);
+  else if (pos != -1)
+    atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
+}
+
+__global__ void __launch_bounds__(256) accumulate_kernel(const AccumulateParams p) {
+  ptx::grid_dep_wait();
+  ptx::launch_dependents();
+  const int64_t t = blockIdx.x;
+  const int k = (int)(blockIdx.y * 256 + threadIdx.x);
+  if (k < p.topk) accumulate_entry(p, p.acc + t * p.acc_sb, t, k);
+}
+
+__global__ void __launch_bounds__(1024) accumulate_tokens_kernel(const AccumulateParams p) {
+  ptx::grid_dep_wait();
+  ptx::launch_dependents();
+  const int64_t r = blockIdx.x;
+  const int lo = max(0, __ldg(p.offsets + r)), hi = min(p.tokens, __ldg(p.offsets + r + 1));
+  for (int t = lo; t < hi; ++t) {
+    for (int k = threadIdx.x; k < p.topk; k += 1024)
+      accumulate_entry(p, p.acc + r * p.acc_sb, t, k);
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------------------ compact
+//
+// Entry j of row r (keep[r][j], a position of the row's sequence; -1: none) moves from the
+// slot of that position in the row's pages to slot j of its new pages.  The scale of a new
+// block is the largest scale among the tokens that move into it, and every token is
+// re-expressed in it, as in the append.  A CTA owns 64 consecutive entries of a row (or one
+// block, if that is larger), which are whole blocks of the new pages.
+
+constexpr int kCompactThreads = 256;
+constexpr int kCompactWarps = kCompactThreads / 32;
+constexpr int kCompactSpan = 64;
+constexpr int kMaxBlock = 256;  // tokens per scale
+
+struct CompactParams {
+  const int32_t* keep;
+  int64_t keep_sb;
+  int32_t cols;
+  int32_t span;  // entries per CTA
+  PageTable from, to;
+  Cache cache;
+  uint32_t* err;
+};
+
+__global__ void __launch_bounds__(kCompactThreads) compact_kernel(const CompactParams p) {
+  __shared__ int src_s[kMaxBlock], dst_s[kMaxBlock];
+  __shared__ float old_s[kMaxBlock], new_s[kMaxBlock];  // scales per entry
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  ptx::grid_dep_wait();
+  ptx::launch_dependents();
+  const int64_t row = blockIdx.x;
+  const int j0 = (int)blockIdx.y * p.span;
+  const int n = min(p.span, p.cols - j0);
+  const int block = 1 << p.cache.block_shift;
+  for (int i = threadIdx.x; i < n; i += kCompactThreads) {
+    const int pos = __ldg(p.keep + row * p.keep_sb + j0 + i);
+    int src = -1, dst = -1;
+    if (pos != -1) {
+      src = slot_at(p.from, row, pos, p.cache.num_slots);
+      dst = slot_at(p.to, row, j0 + i, p.cache.num_slots);
+      if (src < 0 || dst < 0) {
+        atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
+        src = -1;
+      }
+    }
+    src_s[i] = src;
+    dst_s[i] = dst;
+    old_s[i] = src >= 0 ? __ldg(p.cache.scale + (src >> p.cache.block_shift)) : 0.f;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kCompactThreads) {
+    const int b0 = i & ~(block - 1);
+    float big = 0.f;
+    for (int e = b0; e < min(b0 + block, n); ++e) big = fmaxf(big, old_s[e]);
+    new_s[i] = big;
+    // the first entry of the block that moves writes the block's scale
+    if (src_s[i] >= 0) {
+      bool first = true;
+      for (int e = b0; e < i; ++e) first = first && src_s[e] < 0;
+      if (first) p.cache.scale[dst_s[i] >> p.cache.block_shift] = big;
+    }
+  }
+  __syncthreads();
+  for (int i = warp; i < n; i += kCompactWarps) {
+    const int src = src_s[i], dst = dst_s[i];
+    if (src < 0) continue;
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.cache.ckv + (int64_t)src * p.cache.ckv_ss) + lane);
+    uint4 pe = make_uint4(0u, 0u, 0u, 0u);
+    if (lane < 8)
+      pe = __ldg(reinterpret_cast<const uint4*>(p.cache.kpe + (int64_t)src * p.cache.kpe_ss) + lane);
+    const float ratio = new_s[i] > 0.f ? old_s[i] / new_s[i] : 0.f;
+    reinterpret_cast<uint4*>(p.cache.ckv + (int64_t)dst * p.cache.ckv_ss)[lane] =
+        ratio == 1.f ? v : rescale16(v, ratio);
+    if (lane < 8)
+      reinterpret_cast<uint4*>(p.cache.kpe + (int64_t)dst * p.cache.kpe_ss)[lane] = pe;
+  }
+}
+
+// ====================================================================== host side
+namespace {
+
+cudaLaunchAttribute pdl_attr() {
+  cudaLaunchAttribute a;
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return a;
+}
+
+// Launched so that the grid may be scheduled while the stream's previous one drains; every
+// kernel here waits for it (griddepcontrol.wait) before it touches global memory.
+template <typename P>
+int launch(void (*kern)(P), dim3 grid, unsigned threads, cudaStream_t st, const P& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1] = {pdl_attr()};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
+}
+
+bool power_of_two(int32_t v) { return v > 0 && (v & (v - 1)) == 0; }
+int32_t log2_of(int32_t v) {
+  int32_t s = 0;
+  while ((1 << s) < v) ++s;
+  return s;
+}
+
+int check_cache(const void* ckv, int64_t ckv_ss, const float* scale, const void* kpe,
+                int64_t kpe_ss, int64_t num_slots, int32_t block) {
+  if (!ckv || !scale || !kpe || ckv_ss < kDCkv || kpe_ss < kDKpe || num_slots < 1 ||
+      num_slots > INT32_MAX || !power_of_two(block) || block > kMaxBlock)
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (!aligned16(ckv) || !aligned16(kpe) || ckv_ss % 16 || (kpe_ss * 2) % 16)
+    return DSA_ERR_MISALIGNED;
+  return DSA_OK;
+}
+
+int check_table(const int32_t* pt, int64_t sb, int32_t cols, int32_t page_size, int32_t block) {
+  if (!pt || cols < 1 || sb < 0 || !power_of_two(page_size) || page_size > (1 << 20) ||
+      page_size < block || (int64_t)cols * page_size > INT32_MAX)
+    return DSA_ERR_INVALID_ARGUMENT;
+  return DSA_OK;
+}
+
+Cache cache_of(void* ckv, int64_t ckv_ss, float* scale, void* kpe, int64_t kpe_ss,
+               int64_t num_slots, int32_t block) {
+  return Cache{static_cast<uint8_t*>(ckv), ckv_ss, scale, static_cast<__nv_bfloat16*>(kpe),
+               kpe_ss, num_slots, log2_of(block)};
+}
+
+}  // namespace
+}  // namespace q8
+}  // namespace dsa
+
+using namespace dsa;
+
+extern "C" int dsa_append_q8(const void* ckv, int64_t ckv_stride_t, const void* kpe,
+                             int64_t kpe_stride_t, int64_t num_tokens,
+                             const int32_t* row_offsets, const int32_t* starts, int32_t num_rows,
+                             const int32_t* page_table, int64_t page_table_stride_b,
+                             int32_t page_table_cols, int32_t page_size, void* ckv_q8,
+                             int64_t ckv_slot_stride, float* ckv_scale, int32_t block,
+                             void* kpe_cache, int64_t kpe_slot_stride, int64_t num_slots,
+                             void* workspace, void* stream) {
+  if (num_tokens < 0 || num_tokens > INT32_MAX || num_rows < 0) return DSA_ERR_INVALID_ARGUMENT;
+  if (num_tokens == 0 || num_rows == 0) return DSA_OK;
+  if (!ckv || !kpe || !row_offsets || !starts || ckv_stride_t < 0 || kpe_stride_t < 0)
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (!workspace) return DSA_ERR_WORKSPACE;
+  int rc = q8::check_cache(ckv_q8, ckv_slot_stride, ckv_scale, kpe_cache, kpe_slot_stride,
+                           num_slots, block);
+  if (rc == DSA_OK)
+    rc = q8::check_table(page_table, page_table_stride_b, page_table_cols, page_size, block);
+  if (rc != DSA_OK) return rc;
+  if (!aligned16(ckv) || !aligned16(kpe) || (ckv_stride_t * 2) % 16 || (kpe_stride_t * 2) % 16)
+    return DSA_ERR_MISALIGNED;
+  q8::AppendParams p;
+  p.ckv = static_cast<const __nv_bfloat16*>(ckv);
+  p.ckv_sb = ckv_stride_t;
+  p.kpe = static_cast<const __nv_bfloat16*>(kpe);
+  p.kpe_sb = kpe_stride_t;
+  p.offsets = row_offsets;
+  p.starts = starts;
+  p.rows = num_rows;
+  p.tokens = (int32_t)num_tokens;
+  // about eight CTAs per SM of a B200, one token each while the call is small
+  p.chunk = (int32_t)((num_tokens + 1183) / 1184);
+  p.table = q8::PageTable{page_table, page_table_stride_b, page_table_cols, q8::log2_of(page_size)};
+  p.cache = q8::cache_of(ckv_q8, ckv_slot_stride, ckv_scale, kpe_cache, kpe_slot_stride, num_slots,
+                         block);
+  p.err = static_cast<uint32_t*>(workspace);
+  return q8::launch(q8::append_kernel, dim3((unsigned)((num_tokens + p.chunk - 1) / p.chunk)),
+                    q8::kAppendThreads, static_cast<cudaStream_t>(stream), p);
+}
+
+extern "C" int dsa_accumulate_weights(const float* weights, int64_t weights_stride_t,
+                                      const int32_t* positions, int64_t positions_stride_t,
+                                      int64_t num_tokens, int32_t topk, float* acc,
+                                      int64_t acc_stride_r, int32_t acc_cols, int32_t num_rows,
+                                      const int32_t* row_offsets, void* workspace, void* stream) {
+  if (num_tokens < 0 || num_tokens > INT32_MAX || num_rows < 0 || topk < 1 || acc_cols < 0)
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (num_tokens == 0 || num_rows == 0) return DSA_OK;
+  if (!weights || !positions || !acc || weights_stride_t < 0 || positions_stride_t < 0 ||
+      (num_rows > 1 && acc_stride_r < acc_cols) || (!row_offsets && num_rows != num_tokens) || topk > 65535 * 256)
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (!workspace) return DSA_ERR_WORKSPACE;
+  const q8::AccumulateParams p{weights,  weights_stride_t, positions,           positions_stride_t,
+                               acc,      acc_stride_r,     row_offsets,         (int32_t)num_tokens,
+                               topk,     acc_cols,         static_cast<uint32_t*>(workspace)};
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (row_offsets)
+    return q8::launch(q8::accumulate_tokens_kernel, dim3((unsigned)num_rows), 1024, st, p);
+  return q8::launch(q8::accumulate_kernel,
+                    dim3((unsigned)num_tokens, (unsigned)((topk + 255) / 256)), 256, st, p);
+}
+
+extern "C" int dsa_compact_q8(const int32_t* keep, int64_t keep_stride_b, int32_t num_rows,
+                              int32_t keep_cols, const int32_t* page_table,
+                              int64_t page_table_stride_b, int32_t page_table_cols,
+                              const int32_t* new_page_table, int64_t new_page_table_stride_b,
+                              int32_t new_page_table_cols, int32_t page_size, void* ckv_q8,
+                              int64_t ckv_slot_stride, float* ckv_scale, int32_t block,
+                              void* kpe_cache, int64_t kpe_slot_stride, int64_t num_slots,
+                              void* workspace, void* stream) {
+  if (num_rows < 0 || keep_cols < 0) return DSA_ERR_INVALID_ARGUMENT;
+  if (num_rows == 0 || keep_cols == 0) return DSA_OK;
+  if (!keep || keep_stride_b < 0) return DSA_ERR_INVALID_ARGUMENT;
+  if (!workspace) return DSA_ERR_WORKSPACE;
+  int rc = q8::check_cache(ckv_q8, ckv_slot_stride, ckv_scale, kpe_cache, kpe_slot_stride,
+                           num_slots, block);
+  if (rc == DSA_OK)
+    rc = q8::check_table(page_table, page_table_stride_b, page_table_cols, page_size, block);
+  if (rc == DSA_OK)
+    rc = q8::check_table(new_page_table, new_page_table_stride_b, new_page_table_cols, page_size,
+                         block);
+  if (rc != DSA_OK) return rc;
+  q8::CompactParams p;
+  p.keep = keep;
+  p.keep_sb = keep_stride_b;
+  p.cols = keep_cols;
+  p.span = block > q8::kCompactSpan ? block : q8::kCompactSpan;
+  const int shift = q8::log2_of(page_size);
+  p.from = q8::PageTable{page_table, page_table_stride_b, page_table_cols, shift};
+  p.to = q8::PageTable{new_page_table, new_page_table_stride_b, new_page_table_cols, shift};
+  p.cache = q8::cache_of(ckv_q8, ckv_slot_stride, ckv_scale, kpe_cache, kpe_slot_stride, num_slots,
+                         block);
+  p.err = static_cast<uint32_t*>(workspace);
+  const int64_t spans = ((int64_t)keep_cols + p.span - 1) / p.span;
+  if (spans > 65535) return DSA_ERR_INVALID_ARGUMENT;
+  return q8::launch(q8::compact_kernel, dim3((unsigned)num_rows, (unsigned)spans),
+                    q8::kCompactThreads, static_cast<cudaStream_t>(stream), p);
+}
+
+extern "C" size_t dsa_q8_scratch_size(int64_t num_tokens, int32_t num_heads, int32_t topk) {
+  if (num_tokens < 0 || topk < 1 || !heads_supported(num_heads)) return 0;
+  return (size_t)num_tokens * (size_t)topk * 4;
+}
+
+extern "C" int dsa_sparse_mla_decode_q8(
+    const void* q_nope, int64_t q_nope_stride_b, int64_t q_nope_stride_h, const void* q_pe,
+    int64_t q_pe_stride_b, int64_t q_pe_stride_h, const void* ckv_q8, int64_t ckv_slot_stride,
+    const float* ckv_scale, int32_t block, const void* kpe_cache, int64_t kpe_slot_stride,
+    int64_t num_slots, const int32_t* page_table, int64_t page_table_stride_b,
+    int32_t page_table_cols, int32_t page_size, const int32_t* indices, int64_t indices_stride_b,
+    float sm_scale, void* output, int64_t output_stride_b, int64_t output_stride_h, float* lse,
+    int64_t lse_stride_b, int64_t lse_stride_h, float* weights, int64_t weights_stride_b,
+    int64_t num_tokens, int32_t num_heads, int32_t topk, void* scratch, size_t scratch_bytes,
+    void* workspace, void* stream) {
+  if (num_tokens < 0 || num_tokens > INT32_MAX || topk < 1) return DSA_ERR_INVALID_ARGUMENT;
+  if (!heads_supported(num_heads)) return DSA_ERR_UNSUPPORTED;
+  if (num_tokens == 0) return DSA_OK;
+  if (!q_nope || !q_pe || !indices || !output || !lse || q_nope_stride_h < 0 ||
+      q_pe_stride_h < 0 || q_nope_stride_b < 0 || q_pe_stride_b < 0 || indices_stride_b < 0)
+    return DSA_ERR_INVALID_ARGUMENT;
+  int rc = q8::check_cache(ckv_q8, ckv_slot_stride, ckv_scale, kpe_cache, kpe_slot_stride,
+                           num_slots, block);
+  if (rc == DSA_OK && page_table != nullptr)
+    rc = q8::check_table(page_table, page_table_stride_b, page_table_cols, page_size, block);
+  if (rc != DSA_OK) return rc;
+  if (!aligned16(q_nope) || !aligned16(q_pe) || (q_nope_stride_b * 2) % 16 ||
+      (q_nope_stride_h * 2) % 16 || (q_pe_stride_b * 2) % 16 || (q_pe_stride_h * 2) % 16)
+    return DSA_ERR_MISALIGNED;
+  if (!workspace) return DSA_ERR_WORKSPACE;
+  if (weights != nullptr) {
+    if (num_tokens > 1 && weights_stride_b < topk) return DSA_ERR_INVALID_ARGUMENT;
+    if (!scratch || scratch_bytes < dsa_q8_scratch_size(num_tokens, num_heads, topk))
+      return DSA_ERR_WORKSPACE;
+  }
+  q8::AttendParams p;
+  p.qn = static_cast<const __nv_bfloat16*>(q_nope);
+  p.qn_sb = q_nope_stride_b;
+  p.qn_sh = q_nope_stride_h;
+  p.qp = static_cast<const __nv_bfloat16*>(q_pe);
+  p.qp_sb = q_pe_stride_b;
+  p.qp_sh = q_pe_stride_h;
+  p.cache = q8::cache_of(const_cast<void*>(ckv_q8), ckv_slot_stride, const_cast<float*>(ckv_scale),
+                         const_cast<void*>(kpe_cache), kpe_slot_stride, num_slots, block);
+  p.idx = indices;
+  p.idx_sb = indices_stride_b;
+  p.table = q8::PageTable{page_table, page_table_stride_b, page_table_cols,
+                          page_table != nullptr ? q8::log2_of(page_size) : 0};
+  p.out = static_cast<__nv_bfloat16*>(output);
+  p.out_sb = output_stride_b;
+  p.out_sh = output_stride_h;
+  p.lse = lse;
+  p.lse_sb = lse_stride_b;
+  p.lse_sh = lse_stride_h;
+  p.weights = weights;
+  p.w_sb = weights_stride_b;
+  p.scratch = static_cast<float*>(scratch);
+  p.heads = num_heads;
+  p.topk = topk;
+  p.scale_log2 = sm_scale * kLog2e;
+  p.err = static_cast<uint32_t*>(workspace);
+  return q8::launch(q8::attend_kernel, dim3((unsigned)num_tokens), 256,
+                    static_cast<cudaStream_t>(stream), p);
+}

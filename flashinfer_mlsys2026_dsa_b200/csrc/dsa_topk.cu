@@ -63,6 +63,13 @@ struct Params {
   int32_t k;
   int32_t* slots;
   int64_t slots_sb;
+  // evictions only: positions below `sinks` and the row's last `recent` are always taken
+  int32_t sinks;
+  int32_t recent;
+  int32_t* new_lengths;
+  float* new_scores;  // the taken positions' scores, then zeros (nullptr: not wanted)
+  int64_t new_scores_sb;
+  int32_t new_cols;
 };
 
 // Order-preserving key: a larger float has a larger key; NaN maps below every number.
@@ -250,7 +257,12 @@ __device__ __forceinline__ uint4 ld_peer_v4(const uint32_t* local, uint32_t rank
 // distributed shared memory after a cluster barrier, so that both CTAs pick the same bin and
 // end with the same T; rank 1's compaction then starts after rank 0's keys.  The output is
 // the same array as with one CTA per row.
-template <bool kCached, int kParts>
+//
+// kEvict: the selection of an eviction.  The scores are a row's accumulated attention weights,
+// the page table is absent, and the key of a protected position is the largest there is, so
+// that the same select takes it first; the row's new length and its taken scores are written
+// beside the positions.
+template <bool kCached, int kParts, bool kEvict>
 __global__ void __launch_bounds__(kThreads, 1) topk_slots_kernel(const Params p) {
   static_assert(kParts == 1 || kParts == 2, "one or two CTAs per row");
   extern __shared__ uint32_t skey[];         // kCached: the keys of this CTA's positions
@@ -275,10 +287,24 @@ __global__ void __launch_bounds__(kThreads, 1) topk_slots_kernel(const Params p)
   int L = __ldg(p.lengths + row);
   L = L < 0 ? 0 : (L > p.max_len ? p.max_len : L);
   const int k = p.k;
+  float* new_scores = nullptr;
+  if constexpr (kEvict) {
+    if (p.new_scores != nullptr) {
+      new_scores = p.new_scores + (int64_t)row * p.new_scores_sb;
+      for (int i = min(L, k) + (int)part * kThreads + threadIdx.x; i < p.new_cols;
+           i += kParts * kThreads)
+        new_scores[i] = 0.f;
+    }
+    if (part == 0 && threadIdx.x == 0) p.new_lengths[row] = min(L, k);
+  }
 
   if (L <= k) {  // every position, in order, then padding (both CTAs return here together)
-    for (int i = (int)part * kThreads + threadIdx.x; i < k; i += kParts * kThreads)
+    for (int i = (int)part * kThreads + threadIdx.x; i < k; i += kParts * kThreads) {
       out[i] = i < L ? slot_of(p, pr, i) : -1;
+      if constexpr (kEvict) {
+        if (new_scores != nullptr && i < L) new_scores[i] = __ldg(sr + i);
+      }
+    }
     return;
   }
 
@@ -289,9 +315,15 @@ __global__ void __launch_bounds__(kThreads, 1) topk_slots_kernel(const Params p)
   const float* sl = sr + lo;
 
   constexpr bool cached = kCached;
-  auto key_at = [&](int j) -> uint32_t {  // j: index into [lo, hi)
+  auto key_of = [&](int j, float f) -> uint32_t {  // j: index into [lo, hi), f: its score
+    if constexpr (kEvict) {
+      if (lo + j < p.sinks || lo + j >= L - p.recent) return 0xFFFFFFFFu;
+    }
+    return score_key(f);
+  };
+  auto key_at = [&](int j) -> uint32_t {
     if constexpr (kCached) return skey[j];
-    else return score_key(__ldg(sl + j));
+    else return key_of(j, __ldg(sl + j));
   };
 
   // ---- radix select of the k-th largest key: the top byte (bits 31..24), then bits 23..12,
@@ -307,8 +339,8 @@ __global__ void __launch_bounds__(kThreads, 1) topk_slots_kernel(const Params p)
 #pragma unroll 2
     for (int v = threadIdx.x; v < nv; v += kThreads) {
       const float4 f = __ldg(sr4 + v);
-      const uint32_t k0 = score_key(f.x), k1 = score_key(f.y), k2 = score_key(f.z),
-                     k3 = score_key(f.w);
+      const uint32_t k0 = key_of(4 * v, f.x), k1 = key_of(4 * v + 1, f.y),
+                     k2 = key_of(4 * v + 2, f.z), k3 = key_of(4 * v + 3, f.w);
       if constexpr (cached) reinterpret_cast<uint4*>(skey)[v] = make_uint4(k0, k1, k2, k3);
       atomicAdd(&wh[k0 >> 24], 1u);
       atomicAdd(&wh[k1 >> 24], 1u);
@@ -316,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1) topk_slots_kernel(const Params p)
       atomicAdd(&wh[k3 >> 24], 1u);
     }
     for (int i = 4 * nv + threadIdx.x; i < n; i += kThreads) {
-      const uint32_t key = score_key(__ldg(sl + i));
+      const uint32_t key = key_of(i, __ldg(sl + i));
       if constexpr (cached) skey[i] = key;
       atomicAdd(&wh[key >> 24], 1u);
     }
@@ -456,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1) topk_slots_kernel(const Params p)
   // ---- positions to slot ids: a separate pass over the entries this CTA wrote, so that
   // the page-table loads of a thread's entries are in flight together instead of one per
   // compaction step
-  if (pr != nullptr) {
+  if (pr != nullptr || (kEvict && new_scores != nullptr)) {
     int j0 = 0, j1 = k;
     if constexpr (kParts == 2) {
       // rank 0 wrote [0, m0), rank 1 [m0, k), m0 = rank 0's keys > T and taken keys == T
@@ -465,7 +497,10 @@ __global__ void __launch_bounds__(kThreads, 1) topk_slots_kernel(const Params p)
     }
     __syncthreads();
 #pragma unroll 4
-    for (int j = j0 + threadIdx.x; j < j1; j += kThreads) out[j] = slot_of(p, pr, out[j]);
+    for (int j = j0 + threadIdx.x; j < j1; j += kThreads) {
+      if constexpr (kEvict) new_scores[j] = __ldg(sr + out[j]);
+      else out[j] = slot_of(p, pr, out[j]);
+    }
   }
   if constexpr (kParts == 2) cluster_wait();
 }
@@ -573,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1) union_groups_kernel(const UnionPa
 
 // Launch with kParts CTAs per row (a cluster of that size), as a programmatic dependent of
 // the stream's previous grid.
-template <bool kCached, int kParts>
+template <bool kCached, int kParts, bool kEvict>
 int launch(const Params& p, int64_t rows, size_t smem, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * kParts));
@@ -589,8 +624,47 @@ int launch(const Params& p, int64_t rows, size_t smem, cudaStream_t st) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = kParts > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, topk_slots_kernel<kCached, kParts>, p) == cudaSuccess ? DSA_OK
-                                                                                         : DSA_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, topk_slots_kernel<kCached, kParts, kEvict>, p) == cudaSuccess
+             ? DSA_OK
+             : DSA_ERR_CUDA;
+}
+
+template <bool kEvict>
+int run(const Params& p, int64_t num_rows, cudaStream_t st) {
+  // Two CTAs per row (a cluster) when the call has at most half as many rows as the GPU has
+  // SMs and rows longer than kPartsMinLen.  When every row's keys fit (kCapKeys per CTA)
+  // they stay in dynamic shared memory, a per-device function attribute of the cached
+  // instances, set once per device (not inside a stream capture when the first call ran
+  // eagerly).
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return DSA_ERR_CUDA;
+  static std::atomic<int> sm_count[64];
+  static std::atomic<bool> attr_set[64];
+  int sms = sm_count[dev].load(std::memory_order_acquire);
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1)
+      return DSA_ERR_CUDA;
+    sm_count[dev].store(sms, std::memory_order_release);
+  }
+  if (!attr_set[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(topk_slots_kernel<true, 1, kEvict>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kCapKeys * 4) != cudaSuccess ||
+        cudaFuncSetAttribute(topk_slots_kernel<true, 2, kEvict>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kCapKeysPart * 4) != cudaSuccess)
+      return DSA_ERR_CUDA;
+    attr_set[dev].store(true, std::memory_order_release);
+  }
+  if (num_rows * 2 <= sms && p.max_len > kPartsMinLen) {
+    const int per_cta = (p.max_len >> 1) + 4;  // the larger half of a row, rounded up
+    return per_cta <= kCapKeysPart
+               ? launch<true, 2, kEvict>(p, num_rows, (size_t)per_cta * 4, st)
+               : launch<false, 2, kEvict>(p, num_rows, 0, st);
+  }
+  return p.max_len <= kCapKeys
+             ? launch<true, 1, kEvict>(p, num_rows, (size_t)p.max_len * 4, st)
+             : launch<false, 1, kEvict>(p, num_rows, 0, st);
 }
 
 }  // namespace topk
@@ -622,41 +696,50 @@ extern "C" int dsa_topk_slots(const float* scores, int64_t scores_stride_b, cons
   p.k = k;
   p.slots = slots;
   p.slots_sb = slots_stride_b;
-  // Two CTAs per row (a cluster) when the call has at most half as many rows as the GPU has
-  // SMs and rows longer than kPartsMinLen.  When every row's keys fit (kCapKeys per CTA)
-  // they stay in dynamic shared memory, a per-device function attribute of the cached
-  // instances, set once per device (not inside a stream capture when the first call ran
-  // eagerly).
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return DSA_ERR_CUDA;
-  static std::atomic<int> sm_count[64];
-  static std::atomic<bool> attr_set[64];
-  int sms = sm_count[dev].load(std::memory_order_acquire);
-  if (sms == 0) {
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1)
-      return DSA_ERR_CUDA;
-    sm_count[dev].store(sms, std::memory_order_release);
-  }
-  if (!attr_set[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(dsa::topk::topk_slots_kernel<true, 1>,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             dsa::topk::kCapKeys * 4) != cudaSuccess ||
-        cudaFuncSetAttribute(dsa::topk::topk_slots_kernel<true, 2>,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             dsa::topk::kCapKeysPart * 4) != cudaSuccess)
-      return DSA_ERR_CUDA;
-    attr_set[dev].store(true, std::memory_order_release);
-  }
-  if (num_rows * 2 <= sms && max_len > dsa::topk::kPartsMinLen) {
-    const int per_cta = (max_len >> 1) + 4;  // the larger half of a row, rounded up
-    return per_cta <= dsa::topk::kCapKeysPart
-               ? dsa::topk::launch<true, 2>(p, num_rows, (size_t)per_cta * 4, st)
-               : dsa::topk::launch<false, 2>(p, num_rows, 0, st);
-  }
-  return max_len <= dsa::topk::kCapKeys
-             ? dsa::topk::launch<true, 1>(p, num_rows, (size_t)max_len * 4, st)
-             : dsa::topk::launch<false, 1>(p, num_rows, 0, st);
+  p.sinks = p.recent = 0;
+  p.new_lengths = nullptr;
+  p.new_scores = nullptr;
+  p.new_scores_sb = 0;
+  p.new_cols = 0;
+  return dsa::topk::run<false>(p, num_rows, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int dsa_evict_positions(const float* acc, int64_t acc_stride_b, const int32_t* lengths,
+                                   int64_t num_rows, int32_t max_len, int32_t budget,
+                                   int32_t sinks, int32_t recent, int32_t* keep,
+                                   int64_t keep_stride_b, int32_t* new_lengths, float* new_acc,
+                                   int64_t new_acc_stride_b, int32_t new_acc_cols,
+                                   void* stream) {
+  if (num_rows < 0 || num_rows > INT32_MAX || max_len < 0 || budget < 1 || sinks < 0 ||
+      recent < 0 || (int64_t)sinks + recent > budget)
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (num_rows == 0) return DSA_OK;
+  if ((!acc && max_len > 0) || !lengths || !keep || !new_lengths || acc_stride_b < 0 ||
+      (num_rows > 1 && keep_stride_b < budget))
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (new_acc != nullptr &&
+      (new_acc == acc || new_acc_cols < budget ||
+       (num_rows > 1 && new_acc_stride_b < new_acc_cols)))
+    return DSA_ERR_INVALID_ARGUMENT;
+  dsa::topk::Params p;
+  p.scores = acc;
+  p.scores_sb = acc_stride_b;
+  p.lengths = lengths;
+  p.pt = nullptr;
+  p.pt_sb = 0;
+  p.pt_cols = 0;
+  p.pg_shift = 0;
+  p.max_len = max_len;
+  p.k = budget;
+  p.slots = keep;
+  p.slots_sb = keep_stride_b;
+  p.sinks = sinks;
+  p.recent = recent;
+  p.new_lengths = new_lengths;
+  p.new_scores = new_acc;
+  p.new_scores_sb = new_acc_stride_b;
+  p.new_cols = new_acc_cols;
+  return dsa::topk::run<true>(p, num_rows, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int dsa_union_groups(const int32_t* positions, int64_t positions_stride_b,

@@ -194,6 +194,106 @@ int dsa_sparse_mla_decode_grouped(
     void* stream);
 
 /*
+ * The 8-bit latent cache.  No counterpart in the reference, whose pools are bf16
+ * (fused.py:155-156); the decode is baseline.py:17-45 on the values that the cache stands for.
+ *
+ *   ckv_q8    [num_slots, 512] e4m3 (one byte each), row stride ckv_slot_stride bytes
+ *   ckv_scale [num_slots / block] fp32: the latent value of a slot is
+ *             float(ckv_q8[slot][d]) * ckv_scale[slot / block].  `block` consecutive slots of a
+ *             page share a scale; a power of two, at most 256, that divides the page size
+ *   kpe_cache [num_slots, 64] bf16, row stride kpe_slot_stride elements (not quantised)
+ *
+ * Pools, bf16 inputs and their row strides are 16-byte aligned.  `workspace` is the decode's
+ * (only its error word is used: an entry that names no slot, position or page of the call sets
+ * DSA_DEVERR_BAD_INDEX and is left out).  Scales are expected to be finite and >= 0.
+ *
+ * dsa_sparse_mla_decode_q8: dsa_sparse_mla_decode() over this cache.  With page_table NULL
+ * `indices` holds flat slot ids, otherwise token positions that are translated as in
+ * dsa_sparse_mla_decode_paged().  -1 is padding; a row of padding alone gets output 0 and lse
+ * -inf.  `weights` (optional, NULL: not wanted) [num_tokens, topk] fp32, row stride
+ * weights_stride_b: the probability that each entry received, summed over the heads; 0 for
+ * padding.  It needs `scratch`, a device buffer of dsa_q8_scratch_size() bytes for this call
+ * alone (calls that may overlap on the GPU need one each); without weights scratch is unused.
+ */
+int dsa_sparse_mla_decode_q8(
+    const void* q_nope, int64_t q_nope_stride_b, int64_t q_nope_stride_h, const void* q_pe,
+    int64_t q_pe_stride_b, int64_t q_pe_stride_h, const void* ckv_q8, int64_t ckv_slot_stride,
+    const float* ckv_scale, int32_t block, const void* kpe_cache, int64_t kpe_slot_stride,
+    int64_t num_slots, const int32_t* page_table, int64_t page_table_stride_b,
+    int32_t page_table_cols, int32_t page_size, const int32_t* indices, int64_t indices_stride_b,
+    float sm_scale, void* output, int64_t output_stride_b, int64_t output_stride_h, float* lse,
+    int64_t lse_stride_b, int64_t lse_stride_h, float* weights, int64_t weights_stride_b,
+    int64_t num_tokens, int32_t num_heads, int32_t topk, void* scratch, size_t scratch_bytes,
+    void* workspace, void* stream);
+
+/* Bytes of scratch a decode with weights needs; 0 for an unsupported shape. */
+size_t dsa_q8_scratch_size(int64_t num_tokens, int32_t num_heads, int32_t topk);
+
+/*
+ * Appends tokens to the 8-bit cache.  Row r's new tokens are ckv / kpe rows
+ * [row_offsets[r], row_offsets[r + 1]) (row_offsets: num_rows + 1 ascending int32; tokens
+ * before the first or behind the last offset are not read); they take the positions
+ * starts[r], starts[r] + 1, ... of the row's sequence, whose pages are page_table row r.
+ * The rows' pages are distinct.
+ *
+ * A block's scale becomes the smallest power of two (at least 2^-126) that holds every new
+ * token of the block within +-448; if the block has earlier tokens of the row (positions
+ * before starts[r]) and a larger scale, that scale stays.  When the scale grows, the earlier
+ * tokens are re-expressed in it: value * (old / new), rounded to e4m3 again.  Rounding is to
+ * nearest even; infinities and NaN become NaN and take no part in the scale.  kpe is copied.
+ */
+int dsa_append_q8(const void* ckv, int64_t ckv_stride_t, const void* kpe, int64_t kpe_stride_t,
+                  int64_t num_tokens, const int32_t* row_offsets, const int32_t* starts,
+                  int32_t num_rows, const int32_t* page_table, int64_t page_table_stride_b,
+                  int32_t page_table_cols, int32_t page_size, void* ckv_q8,
+                  int64_t ckv_slot_stride, float* ckv_scale, int32_t block, void* kpe_cache,
+                  int64_t kpe_slot_stride, int64_t num_slots, void* workspace, void* stream);
+
+/*
+ * acc[r][positions[t][k]] += weights[t][k] for every token t of row r and every entry k whose
+ * position is not -1: the running totals of the decode's attention weights.  row_offsets
+ * (num_rows + 1 ascending int32) gives the tokens of each row; NULL: token r is row r.
+ * A row's tokens are added in order, so distinct positions per token give the same bits in
+ * every run; a position that one token names more than once is counted as often, in no fixed
+ * order.
+ */
+int dsa_accumulate_weights(const float* weights, int64_t weights_stride_t,
+                           const int32_t* positions, int64_t positions_stride_t,
+                           int64_t num_tokens, int32_t topk, float* acc, int64_t acc_stride_r,
+                           int32_t acc_cols, int32_t num_rows, const int32_t* row_offsets,
+                           void* workspace, void* stream);
+
+/*
+ * Which positions an eviction keeps.  Row b keeps its first `sinks` and last `recent`
+ * positions and, up to `budget` in all, those with the largest acc (ordered as
+ * dsa_topk_slots orders scores; ties to the smaller positions); a row of at most `budget`
+ * positions keeps them all.  keep [num_rows, >= budget] int32: the kept positions, ascending,
+ * then -1.  new_lengths [num_rows]: how many.  new_acc (optional) [num_rows, >= new_acc_cols],
+ * new_acc_cols >= budget: the kept positions' totals, then zeros; it does not overlap acc.
+ * sinks + recent <= budget.  Lengths past max_len count as max_len.
+ */
+int dsa_evict_positions(const float* acc, int64_t acc_stride_b, const int32_t* lengths,
+                        int64_t num_rows, int32_t max_len, int32_t budget, int32_t sinks,
+                        int32_t recent, int32_t* keep, int64_t keep_stride_b,
+                        int32_t* new_lengths, float* new_acc, int64_t new_acc_stride_b,
+                        int32_t new_acc_cols, void* stream);
+
+/*
+ * Moves the kept tokens of an 8-bit cache to new pages: position keep[r][j] of row r (page_table
+ * row r) becomes position j of new_page_table row r; -1 entries are left out.  A new block
+ * gets the largest scale among the tokens that move into it, and each token is re-expressed in
+ * that scale as in dsa_append_q8.  The new pages are distinct from each other and from every
+ * page that the call reads; what no entry moves to in them is left as it was.
+ */
+int dsa_compact_q8(const int32_t* keep, int64_t keep_stride_b, int32_t num_rows,
+                   int32_t keep_cols, const int32_t* page_table, int64_t page_table_stride_b,
+                   int32_t page_table_cols, const int32_t* new_page_table,
+                   int64_t new_page_table_stride_b, int32_t new_page_table_cols,
+                   int32_t page_size, void* ckv_q8, int64_t ckv_slot_stride, float* ckv_scale,
+                   int32_t block, void* kpe_cache, int64_t kpe_slot_stride, int64_t num_slots,
+                   void* workspace, void* stream);
+
+/*
  * Bytes of workspace dsa_sparse_mla_decode() needs for this problem on
  * `device` (split-K partials and the error word; the size depends only on
  * the device's SM count, so one workspace serves every shape).
