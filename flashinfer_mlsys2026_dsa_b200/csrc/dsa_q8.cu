@@ -68,6 +68,16 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
   return __half22float2(*reinterpret_cast<__half2*>(&h));
 }
 
+// Eight bf16 values (16 bytes) as floats.
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+
 // Sixteen e4m3 values times `ratio`, rounded to e4m3 again.
 __device__ __forceinline__ uint4 rescale16(uint4 v, float ratio) {
   uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -128,16 +138,6 @@ struct AppendParams {
 __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);
   return a <= 3.402823466e38f ? a : 0.f;  // infinities and NaN take no part in the scale
-}
-
-// Eight bf16 values (16 bytes) as floats; infinities become NaN, as e4m3 has none.
-__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-  }
 }
 
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
         unpack8(__ldg(src + v), f);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (isinf(f[j])) f[j] = NAN;
+          if (isinf(f[j])) f[j] = NAN;  // e4m3 has no infinities
           f[j] = pow2 ? f[j] * inv : f[j] / scale;
         }
         w[2 * v] = to_e4m3x2(f[0], f[1]) | (to_e4m3x2(f[2], f[3]) << 16);
@@ -528,9 +528,56 @@ extern "C" int dsa_compact_q8(const int32_t* keep, int64_t keep_stride_b, int32_
                     q8::kCompactThreads, static_cast<cudaStream_t>(stream), p);
 }
 
+namespace dsa {
+namespace q8 {
+namespace {
+
+using AttendFn = void (*)(CUtensorMap, CUtensorMap, AttendParams);
+
+int group_heads(int heads) { return heads == 16 ? 16 : 32; }
+
+// SMs of the current device, with the attend kernels' shared-memory limit raised on it.
+int prepare_device() {
+  static std::atomic<int> sms[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  int n = sms[dev].load(std::memory_order_acquire);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+        cudaFuncSetAttribute(attend_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Cfg<16>::SMEM_BYTES) != cudaSuccess ||
+        cudaFuncSetAttribute(attend_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Cfg<32>::SMEM_BYTES) != cudaSuccess)
+      return 0;
+    sms[dev].store(n, std::memory_order_release);
+  }
+  return n;
+}
+
+// CTAs per (row, head group).
+int choose_splits(int64_t units, int groups, int ntiles, int sms) {
+  int best = 1;
+  double best_cost = 0;
+  for (int s = 1; s * groups <= kMaxCluster; s *= 2) {
+    const int64_t waves = (units * s + sms - 1) / sms;
+    const double cost = (double)waves * (2.5 + (s > 1 ? 1.5 : 0.0) + 1.4 * ((ntiles + s - 1) / s));
+    if (s == 1 || cost < best_cost) {
+      best = s;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+
+}  // namespace
+}  // namespace q8
+}  // namespace dsa
+
 extern "C" size_t dsa_q8_scratch_size(int64_t num_tokens, int32_t num_heads, int32_t topk) {
   if (num_tokens < 0 || topk < 1 || !heads_supported(num_heads)) return 0;
-  return (size_t)num_tokens * (size_t)topk * 4;
+  const size_t tiles = ((size_t)topk + q8::kTS - 1) / q8::kTS;
+  const size_t groups = (size_t)(num_heads / q8::group_heads(num_heads));
+  return (size_t)num_tokens * tiles * ((size_t)num_heads * q8::kTS + groups) * 4;
 }
 
 extern "C" int dsa_sparse_mla_decode_q8(
@@ -584,11 +631,51 @@ extern "C" int dsa_sparse_mla_decode_q8(
   p.lse_sh = lse_stride_h;
   p.weights = weights;
   p.w_sb = weights_stride_b;
-  p.scratch = static_cast<float*>(scratch);
-  p.heads = num_heads;
+  const int nh = q8::group_heads(num_heads);
   p.topk = topk;
+  p.ntiles = (int32_t)(((int64_t)topk + q8::kTS - 1) / q8::kTS);
+  p.groups = num_heads / nh;
+  p.scores = static_cast<float*>(scratch);
+  p.tiles = weights == nullptr ? nullptr
+                               : reinterpret_cast<int32_t*>(
+                                     p.scores + num_tokens * p.ntiles * num_heads * q8::kTS);
   p.scale_log2 = sm_scale * kLog2e;
+  p.wait_cycles = wait_limit_cycles();
   p.err = static_cast<uint32_t*>(workspace);
-  return q8::launch(q8::attend_kernel, dim3((unsigned)num_tokens), 256,
-                    static_cast<cudaStream_t>(stream), p);
+  const int sms = q8::prepare_device();
+  if (sms <= 0) return DSA_ERR_CUDA;
+  const int64_t units = num_tokens * p.groups;
+  p.splits = q8::choose_splits(units, p.groups, p.ntiles, sms);
+  const int64_t grid = units * p.splits;
+  if (grid > INT32_MAX) return DSA_ERR_INVALID_ARGUMENT;
+  // gathers of single slots: 128-byte boxes of one row
+  CUtensorMap m_ckv, m_kpe;
+  {
+    cuuint64_t dims[2] = {(cuuint64_t)kDCkv, (cuuint64_t)num_slots};
+    cuuint64_t str[1] = {(cuuint64_t)ckv_slot_stride};
+    cuuint32_t box[2] = {128, 1};
+    rc = encode(&m_ckv, ckv_q8, 2, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_DATA_TYPE_UINT8);
+  }
+  if (rc == DSA_OK) {
+    cuuint64_t dims[2] = {(cuuint64_t)kDKpe, (cuuint64_t)num_slots};
+    cuuint64_t str[1] = {(cuuint64_t)kpe_slot_stride * 2};
+    cuuint32_t box[2] = {64, 1};
+    rc = encode(&m_kpe, kpe_cache, 2, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  }
+  if (rc != DSA_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(q8::kThreads);
+  cfg.dynamicSmemBytes = (size_t)(nh == 16 ? q8::Cfg<16>::SMEM_BYTES : q8::Cfg<32>::SMEM_BYTES);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2] = {q8::pdl_attr(), {}};
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)(p.splits * p.groups);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const q8::AttendFn fn = nh == 16 ? q8::attend_kernel<16> : q8::attend_kernel<32>;
+  return cudaLaunchKernelEx(&cfg, fn, m_ckv, m_kpe, p) == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
 }

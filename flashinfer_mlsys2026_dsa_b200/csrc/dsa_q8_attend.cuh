@@ -5,8 +5,36 @@
 //     out[b,h] = bf16(sum_k softmax(z)[h,k] v[k])
 //     weights[b,k] = sum_h softmax(z)[h,k]          (optional)
 //
-// One CTA per row, one head at a time, one warp per slot: the plain arrangement that the
-// tests pin down first.
+// The e4m3 rows go to the tensor cores as they lie in memory (tcgen05 kind::f8f6f4, exact
+// products, fp32 accumulation), so nothing is converted on the way:
+//   * a slot's scale is constant along its row, so it factors out of the score and moves from
+//     the value into the probability: out = sum_k (p[k] scale[k]) ckv_q8[k];
+//   * a query row times a power of two (its largest value then lies in [128, 256)) is split into
+//     two e4m3 terms, q = hi + lo / 16: a bf16 value has 8 significant bits and a term holds 4,
+//     so the split is exact down to 2^-14 of the row's largest value and off by at most
+//     2^-21 of that below;
+//   * p scale / u is split the same way, where u is the largest scale seen so far (a running
+//     maximum like that of the scores, so that scales of any size fit).  Two terms round to 8
+//     significant bits (2^-8 at most, as a bf16 probability does); the running maximum is
+//     kept within 2^2 of the true one and P scaled by 2^6, which puts the first term's ceiling at
+//     2^8 < 448 and the smallest step of the second at 2^-19 of the largest probability.
+// The terms are extra columns of the same MMA (N = 2 NH): an M = 128 MMA costs about the same
+// from N = 16 to N = 64, so they are nearly free.
+//
+// A CTA takes one group of NH heads (16, or 32 for rows of more) of one row, or a 1/S share of
+// that group's tiles.  Tile: 96 slots (rows of the score MMA; a multiple of the PV's K = 32),
+// gathered by TMA into one of three stages of 96 x (512 + 128) bytes; whole slots fit, where
+// the bf16 pools need two CTAs for a row.  The CTAs of a row (S splits x G head groups) form a
+// cluster: splits are merged through distributed shared memory, so that no partial result
+// touches global memory, calls share no state and the sums have one order.
+//
+// Per CTA (384 threads):
+//   warp 0       gather producer: lane g fetches slots 4g .. 4g + 3 of a tile (five gather4
+//                copies), their scales and their validity; tiles without a valid entry are skipped
+//   warp 1       score issuer: S^T[96 slots x (hi, lo, pe)], 16 f8 + 4 bf16 MMAs
+//   warp 2       PV issuer: O^T[512 x (hi, lo)] += V^T P^T, 12 f8 MMAs (V^T read in place)
+//   warp 3       finds the row's last entry that is not padding, so that warp 0 can stop there
+//   warps 4-11   softmax: warp w reads TMEM lanes 32 (w % 4) .. (slots) and half of the heads
 #pragma once
 
 namespace dsa {
@@ -27,98 +55,761 @@ struct AttendParams {
   int64_t lse_sb, lse_sh;
   float* weights;
   int64_t w_sb;
-  float* scratch;
-  int32_t heads;
+  float* scores;    // weights only: every tile's scores, [row][group][tile][NH][kTS]
+  int32_t* tiles;   // weights only: the tiles a CTA ran, in the places of its scores
   int32_t topk;
+  int32_t ntiles;
+  int32_t splits;   // S
+  int32_t groups;   // G
   float scale_log2;
   uint32_t* err;
+  uint64_t wait_cycles;
 };
 
-// The slot of entry k of row b; -1 for padding and, flagged, for what names no slot.
-__device__ __forceinline__ int entry_slot(const AttendParams& p, int64_t b, int k) {
-  const int e = __ldg(p.idx + b * p.idx_sb + k);
-  if (e == -1) return -1;
-  const int slot = p.table.pt != nullptr ? slot_at(p.table, b, e, p.cache.num_slots)
-                   : (e >= 0 && e < p.cache.num_slots) ? e : -1;
-  if (slot < 0) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
-  return slot;
+constexpr int kTS = 96;               // slots per tile
+constexpr int kBlocks = 5;            // 128-byte column blocks of a slot: four of ckv, one of kpe
+constexpr int kRB = kTS * 128;        // one block's region of a stage
+constexpr int kStageB = kBlocks * kRB;
+constexpr int kStages = 3;
+constexpr int kLanes = kTS / 4;       // producer lanes, four slots each
+constexpr int kThreads = 384;
+constexpr int kProducer = 0, kScore = 1, kPv = 2, kScout = 3, kSm0 = 4;
+constexpr int kSmWarps = 8, kSmThreads = 256;
+constexpr uint32_t kSmBar = 1, kQBar = 2;
+constexpr float kTauQ8 = 2.f;         // log2: how far a score may pass the running maximum
+constexpr float kPScale = 64.f;       // 2^6: P <= 2^(6 + 2) = 256 < 448
+constexpr int kMaxCluster = 8;
+
+template <int NH>
+struct Cfg {
+  static_assert(NH == 16 || NH == 32, "head group width");
+  static constexpr int kHT = NH / 2;               // heads per softmax thread
+  static constexpr int kPBufs = NH == 16 ? 2 : 1;  // two do not fit beside 32 heads' Q
+  static constexpr int kQBlk = 2 * NH * 128;       // one 128-wide block of Q, hi rows then lo rows
+  static constexpr int kPB = 2 * NH * 128;         // P^T [2 NH x 96 slots], rows of 128 bytes
+  static constexpr int OFF_Q = kStages * kStageB;
+  static constexpr int OFF_QP = OFF_Q + 4 * kQBlk;
+  static constexpr int OFF_P = OFF_QP + NH * 128;
+  static constexpr int OFF_BAR = OFF_P + kPBufs * kPB;
+  static constexpr int OFF_MISC = OFF_BAR + 128;   // [0] TMEM base, [2] abort, [3] drain, [4] end tile
+  static constexpr int OFF_CMD = OFF_MISC + 32;    // [stage][4]: three validity words, the tile (-1: end)
+  static constexpr int OFF_SMAX = OFF_CMD + kStages * 16;  // [stage] largest scale of the tile
+  static constexpr int OFF_QS = OFF_SMAX + 16;     // [NH] score units per query row
+  static constexpr int OFF_SC = OFF_QS + NH * 4;   // [stage][96] scales; at the end m, L, lse
+  static constexpr int OFF_RED = OFF_SC + kStages * kTS * 4;  // [half][quadrant][kHT]
+  static constexpr int SMEM_USED = OFF_RED + 8 * kHT * 4;
+  static constexpr int SMEM_BYTES = SMEM_USED + 1024;
+  static_assert(SMEM_BYTES <= 232448, "shared memory budget");
+  static_assert(3 * NH * 4 <= kStages * kTS * 4, "m, L, lse in the scales' place");
+  static_assert(NH * kDCkv * 4 + kMaxCluster * 2 * NH * 4 <= kStages * kStageB,
+                "merge buffer, and the splits' m and L, in the stages' place");
+  static constexpr int kSCols = 3 * NH;            // a score buffer: hi, lo, pe
+  static constexpr int O_COL = 2 * kSCols;         // four 128-row tiles of O^T, 2 NH columns each
+  static constexpr int TMEM_COLS = NH == 16 ? 256 : 512;
+  static_assert(O_COL + 8 * NH <= TMEM_COLS, "tensor memory");
+};
+
+enum : int {
+  B_KVF = 0,                 // [stage] slots landed
+  B_KVE = B_KVF + kStages,   // [stage] free again: the tile's PV is done
+  B_SF = B_KVE + kStages,    // [2] score written
+  B_SE = B_SF + 2,           // [2] score read
+  B_PF = B_SE + 2,           // [2] P written (and O rescaled)
+  B_PD = B_PF + 2,           // [2] PV done
+  B_DRAIN = B_PD + 2,        // [2] used only when an issuer stops early
+  B_COUNT = B_DRAIN + 2
+};
+static_assert(B_COUNT * 8 <= 128, "barrier block");
+
+// Instruction descriptor, kind::f8f6f4: e4m3 A and B, fp32 D.
+__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N, bool a_mn_major) {
+  return (1u << 4) | ((a_mn_major ? 1u : 0u) << 15) | ((uint32_t)(N >> 3) << 17) |
+         ((uint32_t)(M >> 4) << 24);
 }
 
-__global__ void __launch_bounds__(256) attend_kernel(const AttendParams p) {
-  __shared__ float o_s[8][kDCkv];
-  __shared__ float m_s[8], l_s[8];
-  ptx::grid_dep_wait();
-  ptx::launch_dependents();
-  const int64_t b = blockIdx.x;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (p.weights != nullptr)
-    for (int k = threadIdx.x; k < p.topk; k += 256) p.weights[b * p.w_sb + k] = 0.f;
-  for (int h = 0; h < p.heads; ++h) {
-    float q[16], o[16];
-    const __nv_bfloat16* qn = p.qn + b * p.qn_sb + h * p.qn_sh + 16 * lane;
-    const __nv_bfloat16* qp = p.qp + b * p.qp_sb + h * p.qp_sh + 2 * lane;
-    const float qp0 = __bfloat162float(qp[0]), qp1 = __bfloat162float(qp[1]);
+// Byte b of row r of an operand with 128-byte rows and the 128-byte swizzle.
+__device__ __forceinline__ uint32_t sw128_byte(int r, int b) {
+  return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + (((b >> 4) ^ (r & 7)) << 4) + (b & 15));
+}
+
+// ---------------------------------------------------------------- gather producer (warp 0)
+template <int NH>
+__device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap* tm_ckv,
+                                        const CUtensorMap* tm_kpe, int64_t row, int split, int lane,
+                                        uint32_t sbase, uint8_t* sgen, const Waiter& wait) {
+  using C = Cfg<NH>;
+  const uint32_t bar0 = sbase + (uint32_t)C::OFF_BAR;
+  volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sgen + C::OFF_MISC);
+  volatile int* cmd = reinterpret_cast<volatile int*>(sgen + C::OFF_CMD);
+  volatile float* smax = reinterpret_cast<volatile float*>(sgen + C::OFF_SMAX);
+  float* sc = reinterpret_cast<float*>(sgen + C::OFF_SC);
+  const bool has = lane < kLanes;
+  const int32_t* ir = p.idx + row * p.idx_sb;
+  const uint64_t policy = ptx::policy_evict_first();
+  const bool paged = p.table.pt != nullptr;
+
+  auto load_pos = [&](int t, int (&pos)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t k = (int64_t)t * kTS + 4 * lane + e;
+      pos[e] = has && k < p.topk ? __ldg(ir + k) : -1;
+    }
+  };
+  // -1: padding, -2: names no slot
+  auto load_slot = [&](const int (&pos)[4], int (&slot)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (pos[e] == -1) slot[e] = -1;
+      else if (paged) slot[e] = slot_at(p.table, row, pos[e], p.cache.num_slots);
+      else slot[e] = pos[e] >= 0 && pos[e] < p.cache.num_slots ? pos[e] : -1;
+      if (slot[e] < 0 && pos[e] != -1) slot[e] = -2;
+    }
+  };
+  auto load_scale = [&](const int (&slot)[4], float (&scale)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      scale[e] = slot[e] >= 0 ? __ldg(p.cache.scale + (slot[e] >> p.cache.block_shift)) : 0.f;
+  };
+
+  int pos2[4], slot1[4], slot0[4];
+  float scale0[4];
+  int t = split;
+  {
+    int a[4], b[4];
+    load_pos(t, a);
+    load_pos(t + p.splits, b);
+    load_pos(t + 2 * p.splits, pos2);
+    load_slot(a, slot0);
+    load_slot(b, slot1);
+    load_scale(slot0, scale0);
+  }
+  bool ok = true;
+  int64_t n = 0;  // live tiles
+  int st = 0;
+  uint32_t phase = 0;
+  // misc[4] is the scout's to lower at any time: the lanes agree on one reading
+  for (; t < __shfl_sync(0xffffffffu, (int)misc[4], 0); t += p.splits) {
+    // what the next two iterations need
+    float scale1[4];
+    int slot2[4], pos3[4];
+    load_scale(slot1, scale1);
+    load_slot(pos2, slot2);
+    load_pos(t + 3 * p.splits, pos3);
+
+    uint32_t nib = 0;
+    bool bad = false;
+    float big = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      bad |= slot0[e] == -2;
+      nib |= (slot0[e] >= 0 ? 1u : 0u) << e;
+      big = fmaxf(big, fabsf(scale0[e]));
+    }
+    if (bad) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
+    if (__ballot_sync(0xffffffffu, nib != 0u) != 0u) {
+      const uint32_t sh = nib << (4 * (lane & 7));
+      const uint32_t w0 = __reduce_or_sync(0xffffffffu, (lane >> 3) == 0 ? sh : 0u);
+      const uint32_t w1 = __reduce_or_sync(0xffffffffu, (lane >> 3) == 1 ? sh : 0u);
+      const uint32_t w2 = __reduce_or_sync(0xffffffffu, (lane >> 3) == 2 ? sh : 0u);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+      if (lane == 0) ok = wait(bar0 + 8u * (uint32_t)(B_KVE + st), phase ^ 1u);
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      if (!ok) break;
+      if (has)
+        *reinterpret_cast<float4*>(sc + st * kTS + 4 * lane) =
+            make_float4(scale0[0], scale0[1], scale0[2], scale0[3]);
+      if (lane == 0) {
+        cmd[4 * st] = (int)w0;
+        cmd[4 * st + 1] = (int)w1;
+        cmd[4 * st + 2] = (int)w2;
+        cmd[4 * st + 3] = t;
+        smax[st] = big;
+      }
+      __syncwarp();
+      const uint32_t full = bar0 + 8u * (uint32_t)(B_KVF + st);
+      if (lane == 0) ptx::mbar_arrive_expect_tx(full, (uint32_t)kStageB);
+      __syncwarp();
+      // a row without a slot lies outside the tensor map: the copy fills it with zeros, so
+      // that PV reads 0 * 0 there
+      if (has) {
+        const int4 r = make_int4(slot0[0], slot0[1], slot0[2], slot0[3]);
+        const uint32_t dst = sbase + (uint32_t)(st * kStageB + lane * 512);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ptx::tma_gather4(dst + j * kRB, tm_ckv, 128 * j, r, full, policy);
+        ptx::tma_gather4(dst + 4 * kRB, tm_kpe, 0, r, full, policy);
+      }
+      ++n;
+      if (++st == kStages) {
+        st = 0;
+        phase ^= 1u;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      slot0[e] = slot1[e];
+      scale0[e] = scale1[e];
+      slot1[e] = slot2[e];
+      pos2[e] = pos3[e];
+    }
+  }
+  // the end: one more stage that holds no slots
+  if (lane == 0) {
+    ok = ok && wait(bar0 + 8u * (uint32_t)(B_KVE + st), phase ^ 1u);
+    if (ok) {
+      cmd[4 * st + 3] = -1;
+      ptx::mbar_arrive(bar0 + 8u * (uint32_t)(B_KVF + st));
+    } else {
+      // this warp's copies land before the CTA leaves
+      const Waiter drain{misc + 3, p.err, p.wait_cycles};
+      for (int64_t i = n - 1; i >= 0 && i >= n - kStages; --i)
+        drain(bar0 + 8u * (uint32_t)(B_KVF + (int)(i % kStages)), (uint32_t)((i / kStages) & 1));
+    }
+  }
+  __syncwarp();
+}
+
+// The tile behind the row's last entry that is not padding, found from the end in steps of
+// 512 entries (warp 3).
+template <int NH>
+__device__ __forceinline__ void scout(const AttendParams& p, int64_t row, int lane, uint8_t* sgen) {
+  const int32_t* ir = p.idx + row * p.idx_sb;
+  int end = 0;
+  for (int hi = p.topk; hi > 0 && end == 0; hi -= 512) {
+    int last = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      q[i] = __bfloat162float(qn[i]);
-      o[i] = 0.f;
+      const int k = hi - 512 + 32 * i + lane;
+      if (k >= 0 && __ldg(ir + k) != -1) last = k + 1;
     }
-    float m = -INFINITY, l = 0.f;
-    for (int k = warp; k < p.topk; k += 8) {
-      const int slot = entry_slot(p, b, k);
-      float z = -INFINITY;
-      if (slot >= 0) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(p.cache.ckv + (int64_t)slot * p.cache.ckv_ss) + lane);
-        const float scale = __ldg(p.cache.scale + (slot >> p.cache.block_shift));
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-        float v[16], dot = 0.f;
+    end = __reduce_max_sync(0xffffffffu, last);
+  }
+  if (lane == 0)
+    reinterpret_cast<volatile uint32_t*>(sgen + Cfg<NH>::OFF_MISC)[4] = (uint32_t)((end + kTS - 1) / kTS);
+}
+
+// One query head into shared memory: hi and lo rows of q_nope in e4m3, the q_pe row in bf16.
+// Returns the head's score unit: (hi + lo / 16) * unit is in log2 units.  A row with an
+// infinity or a NaN has the unit NaN, which reaches every one of its scores.
+template <int NH>
+__device__ __forceinline__ float stage_query(const AttendParams& p, int64_t row, int head, int h,
+                                             int lane, uint8_t* sgen) {
+  using C = Cfg<NH>;
+  const uint4* src = reinterpret_cast<const uint4*>(p.qn + row * p.qn_sb + head * p.qn_sh) + 2 * lane;
+  const uint4 raw[2] = {__ldg(src), __ldg(src + 1)};
+  uint4 pe = make_uint4(0u, 0u, 0u, 0u);
+  if (lane < 8) pe = __ldg(reinterpret_cast<const uint4*>(p.qp + row * p.qp_sb + head * p.qp_sh) + lane);
+  float f[16], g[8];
+  unpack8(raw[0], *reinterpret_cast<float(*)[8]>(f));
+  unpack8(raw[1], *reinterpret_cast<float(*)[8]>(f + 8));
+  unpack8(pe, g);
+  float big = 0.f;
+  bool fine = true;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 f = from_e4m3x2((ws[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
-          v[2 * i] = f.x * scale;
-          v[2 * i + 1] = f.y * scale;
-        }
+  for (int i = 0; i < 16; ++i) {
+    big = fmaxf(big, fabsf(f[i]));
+    fine = fine && fabsf(f[i]) <= 3.402823466e38f;
+  }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) dot += q[i] * v[i];
-        const __nv_bfloat16* kp = p.cache.kpe + (int64_t)slot * p.cache.kpe_ss + 2 * lane;
-        dot += qp0 * __bfloat162float(kp[0]) + qp1 * __bfloat162float(kp[1]);
+  for (int i = 0; i < 8; ++i) fine = fine && fabsf(g[i]) <= 3.402823466e38f;
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
-        z = dot * p.scale_log2;
-        const float mn = fmaxf(m, z);
-        const float keep = m == -INFINITY ? 0.f : exp2f(m - mn), e = exp2f(z - mn);
-        l = l * keep + e;
+  for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+  fine = __all_sync(0xffffffffu, fine);
+  // 2^e <= big < 2^(e + 1); times 2^(7 - e), with e kept where both powers are normal
+  int e = (int)(__float_as_uint(big) >> 23) - 127;
+  e = e < -118 ? -118 : e;
+  const float mul = __uint_as_float((uint32_t)(127 + 7 - e) << 23);
+  uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = o[i] * keep + e * v[i];
-        m = mn;
+  for (int i = 0; i < 4; ++i) {
+    hi[i] = lo[i] = 0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float a = f[4 * i + 2 * k] * mul, b = f[4 * i + 2 * k + 1] * mul;
+      const uint32_t t = to_e4m3x2(a, b);
+      const float2 back = from_e4m3x2(t);
+      hi[i] |= t << (16 * k);
+      lo[i] |= to_e4m3x2((a - back.x) * 16.f, (b - back.y) * 16.f) << (16 * k);
+    }
+  }
+  uint8_t* q = sgen + C::OFF_Q + (lane >> 3) * C::kQBlk;
+  *reinterpret_cast<uint4*>(q + sw128_byte(h, 16 * (lane & 7))) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+  *reinterpret_cast<uint4*>(q + sw128_byte(NH + h, 16 * (lane & 7))) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  if (lane < 8) *reinterpret_cast<uint4*>(sgen + C::OFF_QP + sw128_byte(h, 16 * lane)) = pe;
+  return fine ? __uint_as_float((uint32_t)(127 + e - 7) << 23) * p.scale_log2 : NAN;
+}
+
+template <int kN>
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t* r) {
+#pragma unroll
+  for (int c = 0; c < kN; c += 8) ptx::tmem_ld8(addr + (uint32_t)c, r + c);
+}
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int NH>
+__global__ void __launch_bounds__(kThreads, 1)
+    attend_kernel(const __grid_constant__ CUtensorMap tm_ckv,
+                  const __grid_constant__ CUtensorMap tm_kpe, const __grid_constant__ AttendParams p) {
+  using C = Cfg<NH>;
+  constexpr int kHT = C::kHT;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = ptx::smem_u32(smem_raw);
+  const uint32_t sbase = (raw_addr + 1023u) & ~1023u;
+  uint8_t* sgen = smem_raw + (sbase - raw_addr);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sgen + C::OFF_MISC);
+  volatile int* cmd = reinterpret_cast<volatile int*>(sgen + C::OFF_CMD);
+  const uint32_t bar0 = sbase + (uint32_t)C::OFF_BAR;
+  auto bar = [&](int k) { return bar0 + 8u * (uint32_t)k; };
+
+  const int S = p.splits, G = p.groups;
+  const int rank = (int)blockIdx.x % (S * G);
+  const int64_t row = blockIdx.x / (unsigned)(S * G);
+  const int group = rank / S, split = rank % S;
+  const int h0 = group * NH;  // first head of the group
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(bar(B_KVF + s), 1);
+      ptx::mbar_init(bar(B_KVE + s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(bar(B_SF + b), 1);
+      ptx::mbar_init(bar(B_SE + b), kSmWarps);  // one arrive per softmax warp
+      ptx::mbar_init(bar(B_PF + b), kSmWarps);
+      ptx::mbar_init(bar(B_PD + b), 1);
+      ptx::mbar_init(bar(B_DRAIN + b), 1);
+    }
+    misc[2] = 0;
+    misc[3] = 0;
+    misc[4] = (uint32_t)p.ntiles;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(&tm_ckv);
+    ptx::prefetch_tmap(&tm_kpe);
+  }
+  if (warp == kScore) {
+    ptx::tmem_alloc(sbase + (uint32_t)C::OFF_MISC, (uint32_t)C::TMEM_COLS);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = misc[0];
+  ptx::grid_dep_wait();
+  ptx::launch_dependents();
+  const Waiter wait{misc + 2, p.err, p.wait_cycles};
+  const Waiter spin{misc + 2, p.err, p.wait_cycles, true};
+
+  // softmax state, kept past the loop for the merge
+  const int qd = warp & 3;                   // TMEM lane quadrant: slots 32 qd .. 32 qd + 31
+  const int hh = (warp - kSm0) >> 2;         // heads kHT hh .. kHT hh + kHT - 1 of the group
+  const uint32_t lane_base = (uint32_t)(32 * qd) << 16;
+  float m_run[kHT], l_part[kHT];
+  float u = 0.f;                             // the largest scale so far
+  int64_t n = 0;                             // live tiles
+  float* red = reinterpret_cast<float*>(sgen + C::OFF_RED);
+  float* ml = reinterpret_cast<float*>(sgen + C::OFF_SC);  // at the end: m, L, lse
+  bool aborted = false;
+
+  if (warp == kProducer) {
+    produce<NH>(p, &tm_ckv, &tm_kpe, row, split, lane, sbase, sgen, wait);
+  } else {
+    if (warp == kScout) {
+      scout<NH>(p, row, lane, sgen);
+    } else {
+      float* qs = reinterpret_cast<float*>(sgen + C::OFF_QS);
+      for (int h = warp < kScout ? warp - 1 : warp - 2; h < NH; h += kThreads / 32 - 2) {
+        const float unit = stage_query<NH>(p, row, h0 + h, h, lane, sgen);
+        if (lane == 0) qs[h] = unit;
       }
-      if (p.weights != nullptr && lane == 0) p.scratch[b * p.topk + k] = z;
+      ptx::fence_proxy_async_smem();
+      ptx::bar_sync(kQBar, kThreads - 64);
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o_s[warp][16 * lane + i] = o[i];
+  }
+  if (warp == kScore) {
+    // ------------------------------------------------------------------ score issuer
     if (lane == 0) {
-      m_s[warp] = m;
-      l_s[warp] = l;
-    }
-    __syncthreads();
-    float M = -INFINITY, L = 0.f;
-    for (int w = 0; w < 8; ++w) M = fmaxf(M, m_s[w]);
-    // a warp without a score has l = 0; scores that are NaN leave its maximum at -inf, and l NaN
-    for (int w = 0; w < 8; ++w) L += l_s[w] == 0.f ? 0.f : l_s[w] * exp2f(m_s[w] - M);
-    const bool any = L != 0.f;
-    const float lse = any ? M + log2f(L) : -INFINITY;
-    for (int d = threadIdx.x; d < kDCkv; d += 256) {
-      float a = 0.f;
-      for (int w = 0; w < 8; ++w) a += l_s[w] == 0.f ? 0.f : o_s[w][d] * exp2f(m_s[w] - M);
-      p.out[b * p.out_sb + h * p.out_sh + d] = __float2bfloat16_rn(any ? a / L : 0.f);
-    }
-    if (threadIdx.x == 0) p.lse[b * p.lse_sb + h * p.lse_sh] = lse;
-    if (p.weights != nullptr)
-      for (int k = threadIdx.x; k < p.topk; k += 256) {
-        const float z = p.scratch[b * p.topk + k];
-        if (z != -INFINITY) p.weights[b * p.w_sb + k] += exp2f(z - lse);
+      constexpr uint32_t kId = idesc_e4m3(128, 2 * NH, false), kIdPe = idesc_bf16(128, NH, false);
+      const uint64_t dk = desc(sbase, 16, 1024, kSw128);
+      const uint64_t dq = desc(sbase + (uint32_t)C::OFF_Q, 16, 1024, kSw128);
+      const uint64_t dqp = desc(sbase + (uint32_t)C::OFF_QP, 16, 1024, kSw128);
+      bool ok = true;
+      for (int64_t i = 0;; ++i) {
+        const int st = (int)(i % kStages), sb = (int)(i & 1);
+        ok = spin(bar(B_KVF + st), (uint32_t)((i / kStages) & 1));
+        if (!ok || cmd[4 * st + 3] < 0) break;
+        ok = spin(bar(B_SE + sb), (uint32_t)(((i >> 1) & 1) ^ 1));
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(C::kSCols * sb);
+        const uint64_t ko = (uint64_t)((st * kStageB) >> 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            ptx::umma_f8(d, dk + ko + (uint64_t)((j * kRB + ks * 32) >> 4),
+                         dq + (uint64_t)((j * C::kQBlk + ks * 32) >> 4), kId, (j | ks) ? 1u : 0u);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+          ptx::umma_bf16(d + 2 * NH, dk + ko + (uint64_t)((4 * kRB + ks * 32) >> 4),
+                         dqp + (uint64_t)((ks * 32) >> 4), kIdPe, ks ? 1u : 0u);
+        ptx::umma_commit(bar(B_SF + sb));
       }
-    __syncthreads();
+      if (!ok) {
+        const Waiter drain{misc + 3, p.err, p.wait_cycles};
+        ptx::umma_commit(bar(B_DRAIN));
+        drain(bar(B_DRAIN), 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kPv) {
+    // ------------------------------------------------------------------ PV issuer
+    if (lane == 0) {
+      constexpr uint32_t kId = idesc_e4m3(128, 2 * NH, true);
+      const uint64_t dv = desc(sbase, kRB, 1024, kSw128);
+      const uint64_t dp = desc(sbase + (uint32_t)C::OFF_P, 16, 1024, kSw128);
+      bool ok = true;
+      for (int64_t i = 0;; ++i) {
+        const int st = (int)(i % kStages), pb = (int)(i & 1);
+        ok = spin(bar(B_KVF + st), (uint32_t)((i / kStages) & 1));
+        if (!ok || cmd[4 * st + 3] < 0) break;
+        ok = spin(bar(B_PF + pb), (uint32_t)((i >> 1) & 1));
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const uint64_t vo = (uint64_t)((st * kStageB) >> 4);
+        const uint64_t po = (uint64_t)(((int)(i % C::kPBufs) * C::kPB) >> 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int ks = 0; ks < kTS / 32; ++ks)
+            ptx::umma_f8(tmem + (uint32_t)(C::O_COL + 2 * NH * j),
+                         dv + vo + (uint64_t)((j * kRB + ks * 4096) >> 4),
+                         dp + po + (uint64_t)((ks * 32) >> 4), kId, (i > 0 || ks > 0) ? 1u : 0u);
+        ptx::umma_commit(bar(B_KVE + st));
+        ptx::umma_commit(bar(B_PD + pb));
+      }
+      if (!ok) {
+        const Waiter drain{misc + 3, p.err, p.wait_cycles};
+        ptx::umma_commit(bar(B_DRAIN + 1));
+        drain(bar(B_DRAIN + 1), 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= kSm0) {
+    // ------------------------------------------------------------------ softmax
+    const int slot = 32 * qd + lane;
+    const bool slot_ok = slot < kTS;  // quadrant 3 holds no slots; its lanes are rows of O
+    const float* sc = reinterpret_cast<const float*>(sgen + C::OFF_SC);
+    const volatile float* smax = reinterpret_cast<const volatile float*>(sgen + C::OFF_SMAX);
+    const float* qs = reinterpret_cast<const float*>(sgen + C::OFF_QS) + kHT * hh;
+    const int sm_tid = (int)threadIdx.x - 32 * kSm0;
+    // entries of tiles that turn out to hold nothing get no other value (group g's CTA writes
+    // the row's tiles with (tile / S) % G == g, here and at the end)
+    if (p.weights != nullptr)
+      for (int t = split + S * group; t < p.ntiles; t += S * G) {
+        const int64_t k = (int64_t)t * kTS + sm_tid;
+        if (sm_tid < kTS && k < p.topk) p.weights[row * p.w_sb + k] = 0.f;
+      }
+#pragma unroll
+    for (int h = 0; h < kHT; ++h) {
+      m_run[h] = -INFINITY;
+      l_part[h] = 0.f;
+    }
+    for (;; ++n) {
+      const int st = (int)(n % kStages), sb = (int)(n & 1);
+      bool ok = wait(bar(B_KVF + st), (uint32_t)((n / kStages) & 1));
+      const int tile = cmd[4 * st + 3];
+      const bool end = ok && tile < 0;
+      if (!end) ok = ok && wait(bar(B_SF + sb), (uint32_t)((n >> 1) & 1));
+      float x[kHT];
+      float scale = 0.f;
+      bool valid = false;
+      if (slot_ok && __all_sync(0xffffffffu, ok && !end)) {  // warp-uniform
+        ptx::tc_fence_after();
+        uint32_t hi[kHT], lo[kHT], pe[kHT];
+        const uint32_t ta = tmem + lane_base + (uint32_t)(C::kSCols * sb + kHT * hh);
+        tmem_ld<kHT>(ta, hi);
+        tmem_ld<kHT>(ta + NH, lo);
+        tmem_ld<kHT>(ta + 2 * NH, pe);
+        scale = sc[st * kTS + slot];
+        valid = ((uint32_t)cmd[4 * st + qd] >> lane) & 1u;
+        ptx::tmem_wait_ld();
+        ptx::tc_fence_before();
+#pragma unroll
+        for (int h = 0; h < kHT; ++h) {
+          const float q = fmaf(__uint_as_float(lo[h]), 0.0625f, __uint_as_float(hi[h]));
+          x[h] = valid ? fmaf(q * scale, qs[h], __uint_as_float(pe[h]) * p.scale_log2) : -INFINITY;
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < kHT; ++h) x[h] = -INFINITY;
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(B_SE + sb));
+      const float u_tile = smax[st];
+      bool need = u_tile > u || end;
+#pragma unroll
+      for (int h = 0; h < kHT; ++h) need |= x[h] > m_run[h] + kTauQ8;
+      if (ptx::bar_red_or(kSmBar, kSmThreads, need || !ok || aborted)) {
+        if (ptx::bar_red_or(kSmBar, kSmThreads, !ok || aborted)) {
+          aborted = true;
+          break;
+        }
+        if (end) break;  // every thread has seen it: none voted that a wait failed
+        // raise the running maxima (scores per head, scale) and bring O and l to them
+#pragma unroll
+        for (int h = 0; h < kHT; ++h) {
+          float v = x[h];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+          if (lane == 0) red[(hh * 4 + qd) * kHT + h] = v;
+        }
+        ptx::bar_sync(kSmBar, kSmThreads);
+        const float un = fmaxf(u, u_tile);
+        const float beta = u > 0.f ? u / un : 0.f;
+        u = un;
+        float alpha[kHT];
+#pragma unroll
+        for (int h = 0; h < kHT; ++h) {
+          const float* r4 = red + hh * 4 * kHT + h;
+          const float mn = fmaxf(m_run[h], fmaxf(r4[0], fmaxf(r4[kHT], r4[2 * kHT])));
+          const float a = m_run[h] == -INFINITY ? 0.f : ptx::ex2(m_run[h] - mn);
+          // l that is NaN while no score was a number stays so
+          l_part[h] = m_run[h] == -INFINITY ? l_part[h] : l_part[h] * a;
+          m_run[h] = mn;
+          alpha[h] = a * beta;
+        }
+        if (n > 0) {
+          const bool wok = wait(bar(B_PD + (int)((n - 1) & 1)), (uint32_t)(((n - 1) >> 1) & 1));
+          if (!__all_sync(0xffffffffu, wok)) {
+            aborted = true;
+          } else {
+            ptx::tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {  // four tiles of O, hi and lo
+              const uint32_t ta = tmem + lane_base + (uint32_t)(C::O_COL + NH * c + kHT * hh);
+              uint32_t r[kHT];
+              tmem_ld<kHT>(ta, r);
+              ptx::tmem_wait_ld();
+#pragma unroll
+              for (int h = 0; h < kHT; ++h)
+                r[h] = __float_as_uint(alpha[h] == 0.f ? 0.f : __uint_as_float(r[h]) * alpha[h]);
+#pragma unroll
+              for (int b = 0; b < kHT; b += 8) ptx::tmem_st8(ta + (uint32_t)b, r + b);
+            }
+            ptx::tmem_wait_st();
+          }
+        }
+      }
+      // P[n % kPBufs] was last read by the PV of tile n - kPBufs
+      if (n >= C::kPBufs && !aborted) {
+        const int64_t j = n - C::kPBufs;
+        const bool wok = wait(bar(B_PD + (int)(j & 1)), (uint32_t)((j >> 1) & 1));
+        if (!__all_sync(0xffffffffu, wok)) aborted = true;
+      }
+      if (aborted) continue;  // the next vote ends the loop for every thread
+      if (slot_ok) {
+        uint8_t* pb = sgen + C::OFF_P + (int)(n % C::kPBufs) * C::kPB;
+        const float ratio = u > 0.f ? scale / u * kPScale : 0.f;
+#pragma unroll
+        for (int h = 0; h < kHT; h += 2) {
+          float e[2], v[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float mr = m_run[h + k] == -INFINITY ? 0.f : m_run[h + k];
+            e[k] = ptx::ex2(x[h + k] - mr);
+            l_part[h + k] += e[k];
+            v[k] = valid ? e[k] * ratio : 0.f;
+          }
+          const uint32_t hi = to_e4m3x2(v[0], v[1]);
+          const float2 back = from_e4m3x2(hi);
+          const uint32_t lo = to_e4m3x2((v[0] - back.x) * 16.f, (v[1] - back.y) * 16.f);
+          const int r = kHT * hh + h;
+          pb[sw128_byte(r, slot)] = (uint8_t)hi;
+          pb[sw128_byte(r + 1, slot)] = (uint8_t)(hi >> 8);
+          pb[sw128_byte(NH + r, slot)] = (uint8_t)lo;
+          pb[sw128_byte(NH + r + 1, slot)] = (uint8_t)(lo >> 8);
+        }
+        if (p.weights != nullptr) {
+          const int64_t at = (row * G + group) * p.ntiles + split + n * S;
+          float* s = p.scores + (at * NH + kHT * hh) * kTS + slot;
+#pragma unroll
+          for (int h = 0; h < kHT; ++h) s[h * kTS] = x[h];
+          if (threadIdx.x == 32 * kSm0) p.tiles[at] = tile;
+        }
+      }
+      ptx::fence_proxy_async_smem();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(B_PF + sb));
+    }
+    // ------------------------------------------------------------------ this CTA's m and L
+    // PD of tile n - 3 (two P buffers) or n - 2 was waited for above, on the same barrier or
+    // before, so this wait is exact
+    bool ok = !aborted;
+    if (ok && n > 0) ok = wait(bar(B_PD + (int)((n - 1) & 1)), (uint32_t)(((n - 1) >> 1) & 1));
+    aborted = ptx::bar_red_or(kSmBar, kSmThreads, !ok);
+    ptx::tc_fence_after();
+#pragma unroll
+    for (int h = 0; h < kHT; ++h) {
+      float v = l_part[h];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == 0) red[(hh * 4 + qd) * kHT + h] = v;
+    }
+    ptx::bar_sync(kSmBar, kSmThreads);
+    if (qd == 0 && lane == 0) {
+#pragma unroll
+      for (int h = 0; h < kHT; ++h) {
+        const float* r4 = red + hh * 4 * kHT + h;
+        ml[kHT * hh + h] = m_run[h];
+        ml[NH + kHT * hh + h] = (r4[0] + r4[kHT]) + r4[2 * kHT];
+      }
+    }
+    ptx::bar_sync(kSmBar, kSmThreads);
+  }
+  __syncwarp();
+
+  // -------------------------------------------------------------------- merge of the splits
+  // Every CTA of the cluster is past its loop after this barrier: its stages are free for the
+  // partial outputs of the others, and its m and L can be read.
+  if (S * G > 1) ptx::cluster_sync();
+  bool lost = false;  // a wait ran out somewhere in the cluster: the row is written as NaN
+  if (warp >= kSm0) {
+    const int sm_tid = (int)threadIdx.x - 32 * kSm0;
+    // the splits' m and L, [split][m, L][head], behind the merge buffer
+    float* all = reinterpret_cast<float*>(sgen + kStages * kStageB - kMaxCluster * 2 * NH * 4);
+    for (int e = sm_tid; e < S * 2 * NH; e += kSmThreads) {
+      const uint32_t at = sbase + (uint32_t)C::OFF_SC + 4u * (uint32_t)(e % (2 * NH));
+      all[e] = ld_cluster(ptx::mapa(at, (uint32_t)(group * S + e / (2 * NH))));
+    }
+    if (sm_tid < S * G)
+      lost = __float_as_uint(ld_cluster(
+                 ptx::mapa(sbase + (uint32_t)C::OFF_MISC + 8u, (uint32_t)sm_tid))) != 0u;
+    lost = ptx::bar_red_or(kSmBar, kSmThreads, lost);
+    float f[kHT];  // this CTA's weight in each head, with what P was scaled by
+    float lse_h[kHT];
+#pragma unroll
+    for (int h = 0; h < kHT; ++h) {
+      const float* a = all + kHT * hh + h;
+      float M = -INFINITY, L = 0.f, mine = 0.f;
+      for (int s = 0; s < S; ++s) M = fmaxf(M, a[s * 2 * NH]);
+      for (int s = 0; s < S; ++s) {
+        const float ls = a[s * 2 * NH + NH];
+        const float w = ls == 0.f ? 0.f : ptx::ex2(a[s * 2 * NH] - M);
+        L += ls == 0.f ? 0.f : ls * w;
+        if (s == split) mine = w;
+      }
+      lse_h[h] = lost ? NAN : L == 0.f ? -INFINITY : M + ptx::lg2(L);
+      f[h] = lost ? NAN : L == 0.f || mine == 0.f ? 0.f : mine / L * (u * (1.f / kPScale));
+    }
+    if (split == 0 && qd == 0 && lane == 0) {
+#pragma unroll
+      for (int h = 0; h < kHT; ++h)
+        p.lse[row * p.lse_sb + (int64_t)(h0 + kHT * hh + h) * p.lse_sh] = lse_h[h];
+    }
+    // O^T to the output, or each head's part to the CTA that owns the head's sum
+    const int per = NH / S;  // heads each CTA of the row sums and writes
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t hi[kHT], lo[kHT];
+      const uint32_t ta = tmem + lane_base + (uint32_t)(C::O_COL + 2 * NH * j + kHT * hh);
+      tmem_ld<kHT>(ta, hi);
+      tmem_ld<kHT>(ta + NH, lo);
+      ptx::tmem_wait_ld();
+      const int d = 128 * j + 32 * qd + lane;
+#pragma unroll
+      for (int h = 0; h < kHT; ++h) {
+        const int hl = kHT * hh + h;
+        // a CTA without tiles has nothing in its O
+        const float o = f[h] == 0.f ? 0.f
+                        : lost ? NAN
+                               : fmaf(__uint_as_float(lo[h]), 0.0625f, __uint_as_float(hi[h])) * f[h];
+        if (S == 1) {
+          p.out[row * p.out_sb + (int64_t)(h0 + hl) * p.out_sh + d] = __float2bfloat16_rn(o);
+        } else {
+          const uint32_t dst = sbase + 4u * (uint32_t)((split * per + hl % per) * kDCkv + d);
+          ptx::st_cluster_u32(ptx::mapa(dst, (uint32_t)(group * S + hl / per)), __float_as_uint(o));
+        }
+      }
+    }
+    if (qd == 0 && lane == 0) {
+#pragma unroll
+      for (int h = 0; h < kHT; ++h) ml[2 * NH + kHT * hh + h] = lse_h[h];
+    }
+  }
+  __syncwarp();
+  if (S > 1) ptx::cluster_sync();
+  if (warp >= kSm0) {
+    const int sm_tid = (int)threadIdx.x - 32 * kSm0;
+    if (S > 1) {
+      const int per = NH / S;
+      const float* part = reinterpret_cast<const float*>(sgen);
+      for (int e = sm_tid; e < per * kDCkv; e += kSmThreads) {
+        float o = 0.f;
+        for (int s = 0; s < S; ++s) o += part[s * per * kDCkv + e];
+        const int hl = split * per + e / kDCkv;
+        p.out[row * p.out_sb + (int64_t)(h0 + hl) * p.out_sh + e % kDCkv] = __float2bfloat16_rn(o);
+      }
+    }
+    if (p.weights != nullptr && lost) {
+      for (int t = split + S * group; t < p.ntiles; t += S * G) {
+        const int64_t k = (int64_t)t * kTS + sm_tid;
+        if (sm_tid < kTS && k < p.topk) p.weights[row * p.w_sb + k] = NAN;
+      }
+    } else if (p.weights != nullptr) {
+      // ---------------------------------------------------------------- weights
+      ptx::bar_sync(kSmBar, kSmThreads);  // lse in ml; every tile's scores (S == 1)
+      const float* lse_s = ml + 2 * NH;
+      const int64_t first = (row * G + group) * p.ntiles + split;
+      for (int64_t e = sm_tid; e < n * kTS; e += kSmThreads) {
+        const int64_t at = first + e / kTS * S;
+        const int slot = (int)(e % kTS);
+        float* s = p.scores + at * NH * kTS + slot;
+        float w = 0.f;
+        for (int h = 0; h < NH; ++h) {
+          const float x = s[h * kTS];
+          w += x == -INFINITY ? 0.f : ptx::ex2(x - lse_s[h]);
+        }
+        if (G == 1) {
+          const int64_t k = (int64_t)p.tiles[at] * kTS + slot;
+          if (k < p.topk) p.weights[row * p.w_sb + k] = w;
+        } else {
+          s[0] = w;  // this group's sum, in the place of its first head's score
+        }
+      }
+    }
+  }
+  if (G > 1 && p.weights != nullptr) {
+    __syncwarp();
+    ptx::cluster_sync();
+    if (warp >= kSm0 && !lost) {
+      // the groups ran the same tiles; each adds up the tiles it owns, group by group
+      const int sm_tid = (int)threadIdx.x - 32 * kSm0;
+      const int64_t first = row * G * p.ntiles + split;
+      for (int64_t e = sm_tid; e < n * kTS; e += kSmThreads) {
+        const int64_t at = first + e / kTS * S;
+        const int tile = __ldcg(p.tiles + at + (int64_t)group * p.ntiles);
+        const int slot = (int)(e % kTS);
+        const int64_t k = (int64_t)tile * kTS + slot;
+        if ((tile / S) % G != group || k >= p.topk) continue;
+        float w = 0.f;
+        for (int g = 0; g < G; ++g)
+          w += __ldcg(p.scores + (at + (int64_t)g * p.ntiles) * NH * kTS + slot);
+        p.weights[row * p.w_sb + k] = w;
+      }
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == kScore) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, (uint32_t)C::TMEM_COLS);
   }
 }
 
