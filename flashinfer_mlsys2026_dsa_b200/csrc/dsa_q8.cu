@@ -626,6 +626,8 @@ extern "C" int dsa_sparse_mla_decode_q8(
   p.out = static_cast<__nv_bfloat16*>(output);
   p.out_sb = output_stride_b;
   p.out_sh = output_stride_h;
+  p.out8 = (reinterpret_cast<uintptr_t>(output) & 7u) == 0 && output_stride_b % 4 == 0 &&
+           output_stride_h % 4 == 0;
   p.lse = lse;
   p.lse_sb = lse_stride_b;
   p.lse_sh = lse_stride_h;

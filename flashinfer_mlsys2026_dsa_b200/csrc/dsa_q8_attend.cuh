@@ -16,8 +16,8 @@
 //   * p scale / u is split the same way, where u is the largest scale seen so far (a running
 //     maximum like that of the scores, so that scales of any size fit).  Two terms round to 8
 //     significant bits (2^-8 at most, as a bf16 probability does); the running maximum is
-//     kept within 2^2 of the true one and P scaled by 2^6, which puts the first term's ceiling at
-//     2^8 < 448 and the smallest step of the second at 2^-19 of the largest probability.
+//     kept within 2^3 of the true one and P scaled by 56, so that P reaches e4m3's largest value,
+//     448, and the second term's smallest step is 2^-18.8 of the largest probability.
 // The terms are extra columns of the same MMA (N = 2 NH): an M = 128 MMA costs about the same
 // from N = 16 to N = 64, so they are nearly free.
 //
@@ -28,13 +28,13 @@
 // cluster: splits are merged through distributed shared memory, so that no partial result
 // touches global memory, calls share no state and the sums have one order.
 //
-// Per CTA (384 threads):
-//   warp 0       gather producer: lane g fetches slots 4g .. 4g + 3 of a tile (five gather4
-//                copies), their scales and their validity; tiles without a valid entry are skipped
-//   warp 1       score issuer: S^T[96 slots x (hi, lo, pe)], 16 f8 + 4 bf16 MMAs
-//   warp 2       PV issuer: O^T[512 x (hi, lo)] += V^T P^T, 12 f8 MMAs (V^T read in place)
-//   warp 3       finds the row's last entry that is not padding, so that warp 0 can stop there
-//   warps 4-11   softmax: warp w reads TMEM lanes 32 (w % 4) .. (slots) and half of the heads
+// Per CTA (512 threads):
+//   warps 0-4    gather producers, one per 128-byte column block of the slots; lane g fetches
+//                slots 4g .. 4g + 3 of a tile; tiles without a valid entry are skipped
+//   warp 5       score issuer: S^T[96 slots x (hi, lo, pe)], 16 f8 + 4 bf16 MMAs
+//   warp 6       PV issuer: O^T[512 x (hi, lo)] += V^T P^T, 12 f8 MMAs (V^T read in place)
+//   warp 7       finds the row's last entry that is not padding, so that the producers can stop there
+//   warps 8-15   softmax: warp w reads TMEM lanes 32 (w % 4) .. (slots) and half of the heads
 #pragma once
 
 namespace dsa {
@@ -61,6 +61,7 @@ struct AttendParams {
   int32_t ntiles;
   int32_t splits;   // S
   int32_t groups;   // G
+  bool out8;        // output rows are 8-byte aligned
   float scale_log2;
   uint32_t* err;
   uint64_t wait_cycles;
@@ -72,12 +73,12 @@ constexpr int kRB = kTS * 128;        // one block's region of a stage
 constexpr int kStageB = kBlocks * kRB;
 constexpr int kStages = 3;
 constexpr int kLanes = kTS / 4;       // producer lanes, four slots each
-constexpr int kThreads = 384;
-constexpr int kProducer = 0, kScore = 1, kPv = 2, kScout = 3, kSm0 = 4;
+constexpr int kThreads = 512;
+constexpr int kScore = 5, kPv = 6, kScout = 7, kSm0 = 8;  // warps 0 .. 4: producers
 constexpr int kSmWarps = 8, kSmThreads = 256;
 constexpr uint32_t kSmBar = 1, kQBar = 2;
-constexpr float kTauQ8 = 2.f;         // log2: how far a score may pass the running maximum
-constexpr float kPScale = 64.f;       // 2^6: P <= 2^(6 + 2) = 256 < 448
+constexpr float kTauQ8 = 3.f;         // log2: how far a score may pass the running maximum
+constexpr float kPScale = 56.f;       // P <= 56 * 2^3 = 448, the largest e4m3 value
 constexpr int kMaxCluster = 8;
 
 template <int NH>
@@ -95,14 +96,18 @@ struct Cfg {
   static constexpr int OFF_CMD = OFF_MISC + 32;    // [stage][4]: three validity words, the tile (-1: end)
   static constexpr int OFF_SMAX = OFF_CMD + kStages * 16;  // [stage] largest scale of the tile
   static constexpr int OFF_QS = OFF_SMAX + 16;     // [NH] score units per query row
-  static constexpr int OFF_SC = OFF_QS + NH * 4;   // [stage][96] scales; at the end m, L, lse
+  static constexpr int OFF_SC = OFF_QS + NH * 4;   // [stage][96] scales; at the end kMl floats
+  static constexpr int kMl = 2 * NH + 1;           // a CTA's m, L and u, for the merge
   static constexpr int OFF_RED = OFF_SC + kStages * kTS * 4;  // [half][quadrant][kHT]
   static constexpr int SMEM_USED = OFF_RED + 8 * kHT * 4;
   static constexpr int SMEM_BYTES = SMEM_USED + 1024;
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
-  static_assert(3 * NH * 4 <= kStages * kTS * 4, "m, L, lse in the scales' place");
-  static_assert(NH * kDCkv * 4 + kMaxCluster * 2 * NH * 4 <= kStages * kStageB,
-                "merge buffer, and the splits' m and L, in the stages' place");
+  static_assert(kMl <= kStages * kTS, "m, L and u in the scales' place");
+  // after the last tile, in the stages' place: this CTA's O, then the merge's tables
+  static constexpr int OFF_O = 0;
+  static constexpr int OFF_ALL = NH * kDCkv * 4;                  // [split][kMl]
+  static constexpr int OFF_COEF = OFF_ALL + kMaxCluster * kMl * 4;  // [split][NH], then lse [NH]
+  static_assert(OFF_COEF + (kMaxCluster + 1) * NH * 4 <= kStages * kStageB, "merge tables");
   static constexpr int kSCols = 3 * NH;            // a score buffer: hi, lo, pe
   static constexpr int O_COL = 2 * kSCols;         // four 128-row tiles of O^T, 2 NH columns each
   static constexpr int TMEM_COLS = NH == 16 ? 256 : 512;
@@ -132,11 +137,16 @@ __device__ __forceinline__ uint32_t sw128_byte(int r, int b) {
   return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + (((b >> 4) ^ (r & 7)) << 4) + (b & 15));
 }
 
-// ---------------------------------------------------------------- gather producer (warp 0)
+// ---------------------------------------------------------------- gather producers
+//
+// Warp j < 5 fetches column block j of every slot.  Five warps, because a lane's gather takes
+// about 67 cycles to issue from one warp (8,000 cycles for a tile's 120) while the copy engine
+// takes one in 21.  They look at the same entries and so agree on the live tiles; warp 0 also
+// provides the scales, the validity words and the tile number.
 template <int NH>
-__device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap* tm_ckv,
-                                        const CUtensorMap* tm_kpe, int64_t row, int split, int lane,
-                                        uint32_t sbase, uint8_t* sgen, const Waiter& wait) {
+__device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap* map, int blk,
+                                        int64_t row, int split, int lane, uint32_t sbase,
+                                        uint8_t* sgen, const Waiter& wait) {
   using C = Cfg<NH>;
   const uint32_t bar0 = sbase + (uint32_t)C::OFF_BAR;
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sgen + C::OFF_MISC);
@@ -147,11 +157,12 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
   const int32_t* ir = p.idx + row * p.idx_sb;
   const uint64_t policy = ptx::policy_evict_first();
   const bool paged = p.table.pt != nullptr;
+  const int col = blk < 4 ? 128 * blk : 0;
 
-  auto load_pos = [&](int t, int (&pos)[4]) {
+  auto load_pos = [&](int64_t t, int (&pos)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int64_t k = (int64_t)t * kTS + 4 * lane + e;
+      const int64_t k = t * kTS + 4 * lane + e;
       pos[e] = has && k < p.topk ? __ldg(ir + k) : -1;
     }
   };
@@ -165,15 +176,10 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
       if (slot[e] < 0 && pos[e] != -1) slot[e] = -2;
     }
   };
-  auto load_scale = [&](const int (&slot)[4], float (&scale)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      scale[e] = slot[e] >= 0 ? __ldg(p.cache.scale + (slot[e] >> p.cache.block_shift)) : 0.f;
-  };
 
+  // slots of this iteration and the next, entries of the one after
   int pos2[4], slot1[4], slot0[4];
-  float scale0[4];
-  int t = split;
+  int64_t t = split;
   {
     int a[4], b[4];
     load_pos(t, a);
@@ -181,7 +187,6 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
     load_pos(t + 2 * p.splits, pos2);
     load_slot(a, slot0);
     load_slot(b, slot1);
-    load_scale(slot0, scale0);
   }
   bool ok = true;
   int64_t n = 0;  // live tiles
@@ -189,56 +194,54 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
   uint32_t phase = 0;
   // misc[4] is the scout's to lower at any time: the lanes agree on one reading
   for (; t < __shfl_sync(0xffffffffu, (int)misc[4], 0); t += p.splits) {
-    // what the next two iterations need
-    float scale1[4];
+    uint32_t nib = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) nib |= (slot0[e] >= 0 ? 1u : 0u) << e;
+    const bool live = __ballot_sync(0xffffffffu, nib != 0u) != 0u;
+    float scale[4];
+    if (blk == 0) {
+      bool bad = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        bad |= slot0[e] == -2;
+        scale[e] = slot0[e] >= 0 ? __ldg(p.cache.scale + (slot0[e] >> p.cache.block_shift)) : 0.f;
+      }
+      if (bad) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
+    }
     int slot2[4], pos3[4];
-    load_scale(slot1, scale1);
     load_slot(pos2, slot2);
     load_pos(t + 3 * p.splits, pos3);
-
-    uint32_t nib = 0;
-    bool bad = false;
-    float big = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      bad |= slot0[e] == -2;
-      nib |= (slot0[e] >= 0 ? 1u : 0u) << e;
-      big = fmaxf(big, fabsf(scale0[e]));
-    }
-    if (bad) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
-    if (__ballot_sync(0xffffffffu, nib != 0u) != 0u) {
-      const uint32_t sh = nib << (4 * (lane & 7));
-      const uint32_t w0 = __reduce_or_sync(0xffffffffu, (lane >> 3) == 0 ? sh : 0u);
-      const uint32_t w1 = __reduce_or_sync(0xffffffffu, (lane >> 3) == 1 ? sh : 0u);
-      const uint32_t w2 = __reduce_or_sync(0xffffffffu, (lane >> 3) == 2 ? sh : 0u);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+    if (live) {
       if (lane == 0) ok = wait(bar0 + 8u * (uint32_t)(B_KVE + st), phase ^ 1u);
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       if (!ok) break;
-      if (has)
-        *reinterpret_cast<float4*>(sc + st * kTS + 4 * lane) =
-            make_float4(scale0[0], scale0[1], scale0[2], scale0[3]);
-      if (lane == 0) {
-        cmd[4 * st] = (int)w0;
-        cmd[4 * st + 1] = (int)w1;
-        cmd[4 * st + 2] = (int)w2;
-        cmd[4 * st + 3] = t;
-        smax[st] = big;
-      }
-      __syncwarp();
       const uint32_t full = bar0 + 8u * (uint32_t)(B_KVF + st);
-      if (lane == 0) ptx::mbar_arrive_expect_tx(full, (uint32_t)kStageB);
-      __syncwarp();
       // a row without a slot lies outside the tensor map: the copy fills it with zeros, so
       // that PV reads 0 * 0 there
-      if (has) {
-        const int4 r = make_int4(slot0[0], slot0[1], slot0[2], slot0[3]);
-        const uint32_t dst = sbase + (uint32_t)(st * kStageB + lane * 512);
+      if (has)
+        ptx::tma_gather4(sbase + (uint32_t)(st * kStageB + blk * kRB + lane * 512), map, col,
+                         make_int4(slot0[0], slot0[1], slot0[2], slot0[3]), full, policy);
+      if (blk == 0) {
+        if (has)
+          *reinterpret_cast<float4*>(sc + st * kTS + 4 * lane) =
+              make_float4(scale[0], scale[1], scale[2], scale[3]);
+        float big = fmaxf(fmaxf(fabsf(scale[0]), fabsf(scale[1])), fmaxf(fabsf(scale[2]), fabsf(scale[3])));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ptx::tma_gather4(dst + j * kRB, tm_ckv, 128 * j, r, full, policy);
-        ptx::tma_gather4(dst + 4 * kRB, tm_kpe, 0, r, full, policy);
+        for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+        const uint32_t sh = nib << (4 * (lane & 7));
+        const uint32_t w0 = __reduce_or_sync(0xffffffffu, (lane >> 3) == 0 ? sh : 0u);
+        const uint32_t w1 = __reduce_or_sync(0xffffffffu, (lane >> 3) == 1 ? sh : 0u);
+        const uint32_t w2 = __reduce_or_sync(0xffffffffu, (lane >> 3) == 2 ? sh : 0u);
+        if (lane == 0) {
+          cmd[4 * st] = (int)w0;
+          cmd[4 * st + 1] = (int)w1;
+          cmd[4 * st + 2] = (int)w2;
+          cmd[4 * st + 3] = (int)t;
+          smax[st] = big;
+        }
       }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_expect_tx(full, (uint32_t)kRB);
       ++n;
       if (++st == kStages) {
         st = 0;
@@ -248,7 +251,6 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       slot0[e] = slot1[e];
-      scale0[e] = scale1[e];
       slot1[e] = slot2[e];
       pos2[e] = pos3[e];
     }
@@ -257,7 +259,7 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
   if (lane == 0) {
     ok = ok && wait(bar0 + 8u * (uint32_t)(B_KVE + st), phase ^ 1u);
     if (ok) {
-      cmd[4 * st + 3] = -1;
+      if (blk == 0) cmd[4 * st + 3] = -1;
       ptx::mbar_arrive(bar0 + 8u * (uint32_t)(B_KVF + st));
     } else {
       // this warp's copies land before the CTA leaves
@@ -351,6 +353,15 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
 template <int NH>
 __global__ void __launch_bounds__(kThreads, 1)
     attend_kernel(const __grid_constant__ CUtensorMap tm_ckv,
@@ -375,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      ptx::mbar_init(bar(B_KVF + s), 1);
+      ptx::mbar_init(bar(B_KVF + s), kBlocks);  // one arrive per producer warp
       ptx::mbar_init(bar(B_KVE + s), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -413,23 +424,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   float u = 0.f;                             // the largest scale so far
   int64_t n = 0;                             // live tiles
   float* red = reinterpret_cast<float*>(sgen + C::OFF_RED);
-  float* ml = reinterpret_cast<float*>(sgen + C::OFF_SC);  // at the end: m, L, lse
+  float* ml = reinterpret_cast<float*>(sgen + C::OFF_SC);
   bool aborted = false;
 
-  if (warp == kProducer) {
-    produce<NH>(p, &tm_ckv, &tm_kpe, row, split, lane, sbase, sgen, wait);
+  if (warp < kBlocks) {
+    produce<NH>(p, warp < 4 ? &tm_ckv : &tm_kpe, warp, row, split, lane, sbase, sgen, wait);
+  } else if (warp == kScout) {
+    scout<NH>(p, row, lane, sgen);
   } else {
-    if (warp == kScout) {
-      scout<NH>(p, row, lane, sgen);
-    } else {
-      float* qs = reinterpret_cast<float*>(sgen + C::OFF_QS);
-      for (int h = warp < kScout ? warp - 1 : warp - 2; h < NH; h += kThreads / 32 - 2) {
-        const float unit = stage_query<NH>(p, row, h0 + h, h, lane, sgen);
-        if (lane == 0) qs[h] = unit;
-      }
-      ptx::fence_proxy_async_smem();
-      ptx::bar_sync(kQBar, kThreads - 64);
+    constexpr int kQWarps = kThreads / 32 - kBlocks - 1;
+    float* qs = reinterpret_cast<float*>(sgen + C::OFF_QS);
+    for (int h = warp < kScout ? warp - kBlocks : warp - kBlocks - 1; h < NH; h += kQWarps) {
+      const float unit = stage_query<NH>(p, row, h0 + h, h, lane, sgen);
+      if (lane == 0) qs[h] = unit;
     }
+    ptx::fence_proxy_async_smem();
+    ptx::bar_sync(kQBar, 32 * kQWarps);
   }
   if (warp == kScore) {
     // ------------------------------------------------------------------ score issuer
@@ -590,17 +600,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             aborted = true;
           } else {
             ptx::tc_fence_after();
+            // four tiles of O, hi and lo: kC loads in flight at a time
+            constexpr int kC = NH == 16 ? 4 : 2;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {  // four tiles of O, hi and lo
+            for (int c = 0; c < 8; c += kC) {
               const uint32_t ta = tmem + lane_base + (uint32_t)(C::O_COL + NH * c + kHT * hh);
-              uint32_t r[kHT];
-              tmem_ld<kHT>(ta, r);
+              uint32_t r[kC][kHT];
+#pragma unroll
+              for (int b = 0; b < kC; ++b) tmem_ld<kHT>(ta + (uint32_t)(NH * b), r[b]);
               ptx::tmem_wait_ld();
 #pragma unroll
-              for (int h = 0; h < kHT; ++h)
-                r[h] = __float_as_uint(alpha[h] == 0.f ? 0.f : __uint_as_float(r[h]) * alpha[h]);
+              for (int b = 0; b < kC; ++b) {
 #pragma unroll
-              for (int b = 0; b < kHT; b += 8) ptx::tmem_st8(ta + (uint32_t)b, r + b);
+                for (int h = 0; h < kHT; ++h)
+                  r[b][h] = alpha[h] == 0.f ? 0u : __float_as_uint(__uint_as_float(r[b][h]) * alpha[h]);
+#pragma unroll
+                for (int k = 0; k < kHT; k += 8) ptx::tmem_st8(ta + (uint32_t)(NH * b + k), r[b] + k);
+              }
             }
             ptx::tmem_wait_st();
           }
@@ -670,51 +686,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         ml[kHT * hh + h] = m_run[h];
         ml[NH + kHT * hh + h] = (r4[0] + r4[kHT]) + r4[2 * kHT];
       }
+      ml[2 * NH] = u;
     }
-    ptx::bar_sync(kSmBar, kSmThreads);
-  }
-  __syncwarp();
-
-  // -------------------------------------------------------------------- merge of the splits
-  // Every CTA of the cluster is past its loop after this barrier: its stages are free for the
-  // partial outputs of the others, and its m and L can be read.
-  if (S * G > 1) ptx::cluster_sync();
-  bool lost = false;  // a wait ran out somewhere in the cluster: the row is written as NaN
-  if (warp >= kSm0) {
-    const int sm_tid = (int)threadIdx.x - 32 * kSm0;
-    // the splits' m and L, [split][m, L][head], behind the merge buffer
-    float* all = reinterpret_cast<float*>(sgen + kStages * kStageB - kMaxCluster * 2 * NH * 4);
-    for (int e = sm_tid; e < S * 2 * NH; e += kSmThreads) {
-      const uint32_t at = sbase + (uint32_t)C::OFF_SC + 4u * (uint32_t)(e % (2 * NH));
-      all[e] = ld_cluster(ptx::mapa(at, (uint32_t)(group * S + e / (2 * NH))));
-    }
-    if (sm_tid < S * G)
-      lost = __float_as_uint(ld_cluster(
-                 ptx::mapa(sbase + (uint32_t)C::OFF_MISC + 8u, (uint32_t)sm_tid))) != 0u;
-    lost = ptx::bar_red_or(kSmBar, kSmThreads, lost);
-    float f[kHT];  // this CTA's weight in each head, with what P was scaled by
-    float lse_h[kHT];
-#pragma unroll
-    for (int h = 0; h < kHT; ++h) {
-      const float* a = all + kHT * hh + h;
-      float M = -INFINITY, L = 0.f, mine = 0.f;
-      for (int s = 0; s < S; ++s) M = fmaxf(M, a[s * 2 * NH]);
-      for (int s = 0; s < S; ++s) {
-        const float ls = a[s * 2 * NH + NH];
-        const float w = ls == 0.f ? 0.f : ptx::ex2(a[s * 2 * NH] - M);
-        L += ls == 0.f ? 0.f : ls * w;
-        if (s == split) mine = w;
-      }
-      lse_h[h] = lost ? NAN : L == 0.f ? -INFINITY : M + ptx::lg2(L);
-      f[h] = lost ? NAN : L == 0.f || mine == 0.f ? 0.f : mine / L * (u * (1.f / kPScale));
-    }
-    if (split == 0 && qd == 0 && lane == 0) {
-#pragma unroll
-      for (int h = 0; h < kHT; ++h)
-        p.lse[row * p.lse_sb + (int64_t)(h0 + kHT * hh + h) * p.lse_sh] = lse_h[h];
-    }
-    // O^T to the output, or each head's part to the CTA that owns the head's sum
-    const int per = NH / S;  // heads each CTA of the row sums and writes
+    // O to shared memory, [head][512] (nothing was ever written to it without a live tile)
+    float* o_s = reinterpret_cast<float*>(sgen + C::OFF_O);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t hi[kHT], lo[kHT];
@@ -722,39 +697,77 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld<kHT>(ta, hi);
       tmem_ld<kHT>(ta + NH, lo);
       ptx::tmem_wait_ld();
-      const int d = 128 * j + 32 * qd + lane;
 #pragma unroll
-      for (int h = 0; h < kHT; ++h) {
-        const int hl = kHT * hh + h;
-        // a CTA without tiles has nothing in its O
-        const float o = f[h] == 0.f ? 0.f
-                        : lost ? NAN
-                               : fmaf(__uint_as_float(lo[h]), 0.0625f, __uint_as_float(hi[h])) * f[h];
-        if (S == 1) {
-          p.out[row * p.out_sb + (int64_t)(h0 + hl) * p.out_sh + d] = __float2bfloat16_rn(o);
-        } else {
-          const uint32_t dst = sbase + 4u * (uint32_t)((split * per + hl % per) * kDCkv + d);
-          ptx::st_cluster_u32(ptx::mapa(dst, (uint32_t)(group * S + hl / per)), __float_as_uint(o));
-        }
-      }
-    }
-    if (qd == 0 && lane == 0) {
-#pragma unroll
-      for (int h = 0; h < kHT; ++h) ml[2 * NH + kHT * hh + h] = lse_h[h];
+      for (int h = 0; h < kHT; ++h)
+        o_s[(kHT * hh + h) * kDCkv + 128 * j + 32 * qd + lane] =
+            n > 0 ? fmaf(__uint_as_float(lo[h]), 0.0625f, __uint_as_float(hi[h])) : 0.f;
     }
   }
   __syncwarp();
-  if (S > 1) ptx::cluster_sync();
+
+  // -------------------------------------------------------------------- merge of the splits
+  // Behind this barrier every CTA of the cluster has its m, L, u and O in shared memory.
+  if (S * G > 1) ptx::cluster_sync();
+  bool lost = false;  // a wait ran out somewhere in the cluster: the row is written as NaN
   if (warp >= kSm0) {
     const int sm_tid = (int)threadIdx.x - 32 * kSm0;
-    if (S > 1) {
-      const int per = NH / S;
-      const float* part = reinterpret_cast<const float*>(sgen);
-      for (int e = sm_tid; e < per * kDCkv; e += kSmThreads) {
-        float o = 0.f;
-        for (int s = 0; s < S; ++s) o += part[s * per * kDCkv + e];
-        const int hl = split * per + e / kDCkv;
-        p.out[row * p.out_sb + (int64_t)(h0 + hl) * p.out_sh + e % kDCkv] = __float2bfloat16_rn(o);
+    float* all = reinterpret_cast<float*>(sgen + C::OFF_ALL);
+    float* coef = reinterpret_cast<float*>(sgen + C::OFF_COEF);
+    float* lse_s = coef + S * NH;
+    const int rank0 = group * S;  // the rank of split 0 of this group
+    if (S == 1) ptx::bar_sync(kSmBar, kSmThreads);
+    for (int e = sm_tid; e < S * C::kMl; e += kSmThreads)
+      all[e] = ld_cluster(ptx::mapa(sbase + (uint32_t)C::OFF_SC + 4u * (uint32_t)(e % C::kMl),
+                                    (uint32_t)(rank0 + e / C::kMl)));
+    if (sm_tid < S * G)
+      lost = __float_as_uint(ld_cluster(
+                 ptx::mapa(sbase + (uint32_t)C::OFF_MISC + 8u, (uint32_t)sm_tid))) != 0u;
+    lost = ptx::bar_red_or(kSmBar, kSmThreads, lost);
+    if (sm_tid < NH) {
+      // a head's lse, and what a value of split s in O counts for in its output
+      float M = -INFINITY, L = 0.f;
+      for (int s = 0; s < S; ++s) M = fmaxf(M, all[s * C::kMl + sm_tid]);
+      for (int s = 0; s < S; ++s) {
+        const float ls = all[s * C::kMl + NH + sm_tid];
+        const float w = ls == 0.f ? 0.f : ptx::ex2(all[s * C::kMl + sm_tid] - M);
+        L += ls == 0.f ? 0.f : ls * w;
+        coef[s * NH + sm_tid] = w;
+      }
+      for (int s = 0; s < S; ++s)
+        if (coef[s * NH + sm_tid] != 0.f)
+          coef[s * NH + sm_tid] = coef[s * NH + sm_tid] / L * (all[s * C::kMl + 2 * NH] * (1.f / kPScale));
+      lse_s[sm_tid] = lost ? NAN : L == 0.f ? -INFINITY : M + ptx::lg2(L);
+      if (split == 0)
+        p.lse[row * p.lse_sb + (int64_t)(h0 + sm_tid) * p.lse_sh] = lse_s[sm_tid];
+    }
+    ptx::bar_sync(kSmBar, kSmThreads);
+    // split s sums and writes the heads [s NH / S, (s + 1) NH / S), four values a thread
+    const int per = NH / S;
+    for (int e = sm_tid; e < per * (kDCkv / 4); e += kSmThreads) {
+      const int hl = split * per + e / (kDCkv / 4), d = 4 * (e % (kDCkv / 4));
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int s = 0; s < S; ++s) {
+        const float c = coef[s * NH + hl];
+        const float4 v = ld_cluster4(
+            ptx::mapa(sbase + (uint32_t)(C::OFF_O + 4 * (hl * kDCkv + d)), (uint32_t)(rank0 + s)));
+        if (c != 0.f) {  // 0: no weight, whatever the values
+          o.x = fmaf(v.x, c, o.x);
+          o.y = fmaf(v.y, c, o.y);
+          o.z = fmaf(v.z, c, o.z);
+          o.w = fmaf(v.w, c, o.w);
+        }
+      }
+      if (lost) o = make_float4(NAN, NAN, NAN, NAN);
+      __nv_bfloat16* dst = p.out + row * p.out_sb + (int64_t)(h0 + hl) * p.out_sh + d;
+      const __nv_bfloat162 a = __floats2bfloat162_rn(o.x, o.y), b = __floats2bfloat162_rn(o.z, o.w);
+      if (p.out8) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a),
+                                                    *reinterpret_cast<const uint32_t*>(&b));
+      } else {
+        dst[0] = a.x;
+        dst[1] = a.y;
+        dst[2] = b.x;
+        dst[3] = b.y;
       }
     }
     if (p.weights != nullptr && lost) {
@@ -764,8 +777,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (p.weights != nullptr) {
       // ---------------------------------------------------------------- weights
-      ptx::bar_sync(kSmBar, kSmThreads);  // lse in ml; every tile's scores (S == 1)
-      const float* lse_s = ml + 2 * NH;
+      // every tile's scores are behind the barriers above
       const int64_t first = (row * G + group) * p.ntiles + split;
       for (int64_t e = sm_tid; e < n * kTS; e += kSmThreads) {
         const int64_t at = first + e / kTS * S;
@@ -807,6 +819,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   ptx::tc_fence_before();
   __syncthreads();
+  // no CTA leaves while another may still read its shared memory
+  if (S > 1) ptx::cluster_sync();
   if (warp == kScore) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, (uint32_t)C::TMEM_COLS);
