@@ -13,13 +13,15 @@
 //     two e4m3 terms, q = hi + lo / 16: a bf16 value has 8 significant bits and a term holds 4,
 //     so the split is exact down to 2^-14 of the row's largest value and off by at most
 //     2^-21 of that below;
-//   * p scale / u is split the same way, where u is the largest scale seen so far (a running
-//     maximum like that of the scores, so that scales of any size fit).  Two terms round to 8
-//     significant bits (2^-8 at most, as a bf16 probability does); the running maximum is
-//     kept within 2^3 of the true one and P scaled by 56, so that P reaches e4m3's largest value,
-//     448, and the second term's smallest step is 2^-18.8 of the largest probability.
-// The terms are extra columns of the same MMA (N = 2 NH): an M = 128 MMA costs about the same
-// from N = 16 to N = 64, so they are nearly free.
+//   * p scale / u is split into three terms, P = t0 + t1 / 16 + t2 / 256, where u, the unit, is
+//     the largest scale of the first tile (raised when a later one passes it 16-fold, so that
+//     scales of any size fit).  P is 3.5 2^(x + log2(scale / u) - m) with a running maximum m
+//     that a value may pass by 2^7 before it is raised, so that P stays within e4m3's 448 and
+//     O is hardly ever rescaled.  Three terms round to 12 significant bits, and the third's
+//     smallest step is 2^-18.8 of a weight at m.  (Two terms, which allow 2^3, rescaled O in
+//     about half of the tiles.)
+// The terms are extra columns of the same MMA (N = 2 NH and 3 NH): an M = 128 MMA costs about
+// the same from N = 16 to N = 64, so they are nearly free.
 //
 // A CTA takes one group of NH heads (16, or 32 for rows of more) of one row, or a 1/S share of
 // that group's tiles.  Tile: 96 slots (rows of the score MMA; a multiple of the PV's K = 32),
@@ -29,10 +31,10 @@
 // touches global memory, calls share no state and the sums have one order.
 //
 // Per CTA (512 threads):
-//   warps 0-4    gather producers, one per 128-byte column block of the slots; lane g fetches
-//                slots 4g .. 4g + 3 of a tile; tiles without a valid entry are skipped
+//   warps 0-4    gather producers, one per 128-byte column block of the slots; tiles without a
+//                valid entry are skipped
 //   warp 5       score issuer: S^T[96 slots x (hi, lo, pe)], 16 f8 + 4 bf16 MMAs
-//   warp 6       PV issuer: O^T[512 x (hi, lo)] += V^T P^T, 12 f8 MMAs (V^T read in place)
+//   warp 6       PV issuer: O^T[512 x 3 terms] += V^T P^T, 12 f8 MMAs (V^T read in place)
 //   warp 7       finds the row's last entry that is not padding, so that the producers can stop there
 //   warps 8-15   softmax: warp w reads TMEM lanes 32 (w % 4) .. (slots) and half of the heads
 #pragma once
@@ -72,14 +74,18 @@ constexpr int kBlocks = 5;            // 128-byte column blocks of a slot: four 
 constexpr int kRB = kTS * 128;        // one block's region of a stage
 constexpr int kStageB = kBlocks * kRB;
 constexpr int kStages = 3;
-constexpr int kLanes = kTS / 4;       // producer lanes, four slots each
 constexpr int kThreads = 512;
-constexpr int kScore = 5, kPv = 6, kScout = 7, kSm0 = 8;  // warps 0 .. 4: producers
+constexpr int kProdWarps = 5;
+constexpr int kScore = 5, kPv = 6, kScout = 7, kSm0 = 8;
 constexpr int kSmWarps = 8, kSmThreads = 256;
 constexpr uint32_t kSmBar = 1, kQBar = 2;
-constexpr float kTauQ8 = 3.f;         // log2: how far a score may pass the running maximum
-constexpr float kPScale = 56.f;       // P <= 56 * 2^3 = 448, the largest e4m3 value
+constexpr float kTauQ8 = 7.f;         // log2: how far a weighted score may pass the running maximum
+constexpr float kTauL = 60.f;         // the same for a score alone: its exponential stays finite
+constexpr float kTauU = 16.f;         // how far a scale may pass the unit
+constexpr float kPScale = 3.5f;       // P <= 3.5 * 2^7 = 448, the largest e4m3 value
 constexpr int kMaxCluster = 8;
+constexpr uint32_t kRise = 1u, kFailed = 2u;  // vote words
+constexpr uint32_t kSw32 = 6;         // UMMA descriptor layout type: 32-byte swizzle
 
 template <int NH>
 struct Cfg {
@@ -87,35 +93,35 @@ struct Cfg {
   static constexpr int kHT = NH / 2;               // heads per softmax thread
   static constexpr int kPBufs = NH == 16 ? 2 : 1;  // two do not fit beside 32 heads' Q
   static constexpr int kQBlk = 2 * NH * 128;       // one 128-wide block of Q, hi rows then lo rows
-  static constexpr int kPB = 2 * NH * 128;         // P^T [2 NH x 96 slots], rows of 128 bytes
+  static constexpr int kPK = 3 * NH * 32;          // P^T, 32 slots of it: rows of 32 bytes
+  static constexpr int kPB = kTS / 32 * kPK;
   static constexpr int OFF_Q = kStages * kStageB;
   static constexpr int OFF_QP = OFF_Q + 4 * kQBlk;
   static constexpr int OFF_P = OFF_QP + NH * 128;
   static constexpr int OFF_BAR = OFF_P + kPBufs * kPB;
-  static constexpr int OFF_MISC = OFF_BAR + 128;   // [0] TMEM base, [2] abort, [3] drain, [4] end tile
+  static constexpr int OFF_MISC = OFF_BAR + 256;   // [0] TMEM base, [2] abort, [3] drain, [4] end tile
   static constexpr int OFF_CMD = OFF_MISC + 32;    // [stage][4]: three validity words, the tile (-1: end)
   static constexpr int OFF_SMAX = OFF_CMD + kStages * 16;  // [stage] largest scale of the tile
   static constexpr int OFF_QS = OFF_SMAX + 16;     // [NH] score units per query row
   static constexpr int OFF_SC = OFF_QS + NH * 4;   // [stage][96] scales; at the end kMl floats
   static constexpr int kMl = 2 * NH + 1;           // a CTA's m, L and u, for the merge
-  static constexpr int OFF_RED = OFF_SC + kStages * kTS * 4;  // [half][quadrant][kHT]
-  static constexpr int SMEM_USED = OFF_RED + 8 * kHT * 4;
-  static constexpr int SMEM_BYTES = SMEM_USED + 1024;
+  static constexpr int OFF_RED = OFF_SC + kStages * kTS * 4;  // [half][2 buffers][4 warps] votes
+  static constexpr int SMEM_BYTES = OFF_RED + 16 * 4;
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
   static_assert(kMl <= kStages * kTS, "m, L and u in the scales' place");
-  // after the last tile, in the stages' place: this CTA's O, then the merge's tables
+  // after the last tile, in the stages' place: this CTA's O, then the merge's table
   static constexpr int OFF_O = 0;
-  static constexpr int OFF_ALL = NH * kDCkv * 4;                  // [split][kMl]
-  static constexpr int OFF_COEF = OFF_ALL + kMaxCluster * kMl * 4;  // [split][NH], then lse [NH]
-  static_assert(OFF_COEF + (kMaxCluster + 1) * NH * 4 <= kStages * kStageB, "merge tables");
+  static constexpr int OFF_COEF = NH * kDCkv * 4;  // [split][NH], then lse [NH]
+  static_assert(OFF_COEF + (kMaxCluster + 1) * NH * 4 <= kStages * kStageB, "merge table");
   static constexpr int kSCols = 3 * NH;            // a score buffer: hi, lo, pe
-  static constexpr int O_COL = 2 * kSCols;         // four 128-row tiles of O^T, 2 NH columns each
-  static constexpr int TMEM_COLS = NH == 16 ? 256 : 512;
-  static_assert(O_COL + 8 * NH <= TMEM_COLS, "tensor memory");
+  static constexpr int kSBufs = NH == 16 ? 2 : 1;  // as many as fit beside O
+  static constexpr int O_COL = kSBufs * kSCols;    // four 128-row tiles of O^T, 3 NH columns each
+  static constexpr int TMEM_COLS = 512;
+  static_assert(O_COL + 12 * NH <= TMEM_COLS, "tensor memory");
 };
 
 enum : int {
-  B_KVF = 0,                 // [stage] slots landed
+  B_KVF = 0,                 // [stage] slots landed, scales, validity and tile number written
   B_KVE = B_KVF + kStages,   // [stage] free again: the tile's PV is done
   B_SF = B_KVE + kStages,    // [2] score written
   B_SE = B_SF + 2,           // [2] score read
@@ -124,12 +130,30 @@ enum : int {
   B_DRAIN = B_PD + 2,        // [2] used only when an issuer stops early
   B_COUNT = B_DRAIN + 2
 };
-static_assert(B_COUNT * 8 <= 128, "barrier block");
+static_assert(B_COUNT * 8 <= 256, "barrier block");
+
+// Byte b of row r of an operand with 32-byte rows and the 32-byte swizzle.
+__device__ __forceinline__ uint32_t sw32_byte(int r, int b) {
+  return (uint32_t)(r * 32 + ((((b >> 4) ^ (r >> 2)) & 1) << 4) + (b & 15));
+}
 
 // Instruction descriptor, kind::f8f6f4: e4m3 A and B, fp32 D.
 __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N, bool a_mn_major) {
   return (1u << 4) | ((a_mn_major ? 1u : 0u) << 15) | ((uint32_t)(N >> 3) << 17) |
          ((uint32_t)(M >> 4) << 24);
+}
+
+// Read-only loads that are issued where they stand (the compiler sinks plain ones past the
+// gathers, to where the value is used).
+__device__ __forceinline__ int ldg_now(const int* p) {
+  int v;
+  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ldg_now(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
 }
 
 // Byte b of row r of an operand with 128-byte rows and the 128-byte swizzle.
@@ -139,37 +163,41 @@ __device__ __forceinline__ uint32_t sw128_byte(int r, int b) {
 
 // ---------------------------------------------------------------- gather producers
 //
-// Warp j < 5 fetches column block j of every slot.  Five warps, because a lane's gather takes
-// about 67 cycles to issue from one warp (8,000 cycles for a tile's 120) while the copy engine
-// takes one in 21.  They look at the same entries and so agree on the live tiles; warp 0 also
-// provides the scales, the validity words and the tile number.
+// Warp j < 5 gathers column block j of every slot of a tile, lane g < 24 that of the slots 4g ..
+// 4g + 3.  Five warps, because a lane's gather takes about 67 cycles to issue from one warp
+// (8,000 cycles for a tile's 120) while the copy engine takes one in about 20.  The warps look
+// at the same entries, lane l at those of slots l, l + 32 and l + 64, and so agree on the live
+// tiles; warp 0 also provides the scales, the validity words and the tile number.
 template <int NH>
-__device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap* map, int blk,
-                                        int64_t row, int split, int lane, uint32_t sbase,
-                                        uint8_t* sgen, const Waiter& wait) {
+__device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap* tm_ckv,
+                                        const CUtensorMap* tm_kpe, int pw, int64_t row, int split,
+                                        int lane, uint32_t sbase, uint8_t* sgen, const Waiter& wait) {
   using C = Cfg<NH>;
+  constexpr int kE = kTS / 32;
   const uint32_t bar0 = sbase + (uint32_t)C::OFF_BAR;
+  auto bar = [&](int k) { return bar0 + 8u * (uint32_t)k; };
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sgen + C::OFF_MISC);
   volatile int* cmd = reinterpret_cast<volatile int*>(sgen + C::OFF_CMD);
   volatile float* smax = reinterpret_cast<volatile float*>(sgen + C::OFF_SMAX);
   float* sc = reinterpret_cast<float*>(sgen + C::OFF_SC);
-  const bool has = lane < kLanes;
   const int32_t* ir = p.idx + row * p.idx_sb;
-  const uint64_t policy = ptx::policy_evict_first();
   const bool paged = p.table.pt != nullptr;
-  const int col = blk < 4 ? 128 * blk : 0;
+  const CUtensorMap* map = pw < 4 ? tm_ckv : tm_kpe;
+  const int col = pw < 4 ? 128 * pw : 0;
+  const uint32_t off = (uint32_t)(pw * kRB + lane * 512);
+  const uint64_t policy = ptx::policy_evict_first();
 
-  auto load_pos = [&](int64_t t, int (&pos)[4]) {
+  auto load_pos = [&](int64_t t, int (&pos)[kE]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t k = t * kTS + 4 * lane + e;
-      pos[e] = has && k < p.topk ? __ldg(ir + k) : -1;
+    for (int e = 0; e < kE; ++e) {
+      const int64_t k = t * kTS + 32 * e + lane;
+      pos[e] = k < p.topk ? ldg_now(ir + k) : -1;
     }
   };
   // -1: padding, -2: names no slot
-  auto load_slot = [&](const int (&pos)[4], int (&slot)[4]) {
+  auto load_slot = [&](const int (&pos)[kE], int (&slot)[kE]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < kE; ++e) {
       if (pos[e] == -1) slot[e] = -1;
       else if (paged) slot[e] = slot_at(p.table, row, pos[e], p.cache.num_slots);
       else slot[e] = pos[e] >= 0 && pos[e] < p.cache.num_slots ? pos[e] : -1;
@@ -178,10 +206,10 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
   };
 
   // slots of this iteration and the next, entries of the one after
-  int pos2[4], slot1[4], slot0[4];
+  int pos2[kE], slot1[kE], slot0[kE];
   int64_t t = split;
   {
-    int a[4], b[4];
+    int a[kE], b[kE];
     load_pos(t, a);
     load_pos(t + p.splits, b);
     load_pos(t + 2 * p.splits, pos2);
@@ -194,53 +222,60 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
   uint32_t phase = 0;
   // misc[4] is the scout's to lower at any time: the lanes agree on one reading
   for (; t < __shfl_sync(0xffffffffu, (int)misc[4], 0); t += p.splits) {
-    uint32_t nib = 0;
+    uint32_t w[kE], any = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) nib |= (slot0[e] >= 0 ? 1u : 0u) << e;
-    const bool live = __ballot_sync(0xffffffffu, nib != 0u) != 0u;
-    float scale[4];
-    if (blk == 0) {
+    for (int e = 0; e < kE; ++e) {
+      w[e] = __ballot_sync(0xffffffffu, slot0[e] >= 0);
+      any |= w[e];
+    }
+    float scale[kE];
+    if (pw == 0) {
       bool bad = false;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < kE; ++e) {
         bad |= slot0[e] == -2;
-        scale[e] = slot0[e] >= 0 ? __ldg(p.cache.scale + (slot0[e] >> p.cache.block_shift)) : 0.f;
+        scale[e] = slot0[e] >= 0 ? ldg_now(p.cache.scale + (slot0[e] >> p.cache.block_shift)) : 0.f;
       }
       if (bad) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
     }
-    int slot2[4], pos3[4];
+    int slot2[kE], pos3[kE];
     load_slot(pos2, slot2);
     load_pos(t + 3 * p.splits, pos3);
-    if (live) {
-      if (lane == 0) ok = wait(bar0 + 8u * (uint32_t)(B_KVE + st), phase ^ 1u);
+    if (any != 0u) {
+      // The four slots of lane g are entries of lanes 4 (g % 8) .. + 3, register g / 8.  A slot
+      // that is none lies outside the tensor map: the copy fills its row with zeros, so that PV
+      // reads 0 * 0 there.
+      int r[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int from = 4 * (lane & 7) + e;
+        const int a = __shfl_sync(0xffffffffu, slot0[0], from), b = __shfl_sync(0xffffffffu, slot0[1], from),
+                  c = __shfl_sync(0xffffffffu, slot0[2], from);
+        r[e] = lane < 8 ? a : lane < 16 ? b : c;
+      }
+      if (lane == 0) ok = wait(bar(B_KVE + st), phase ^ 1u);
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       if (!ok) break;
-      const uint32_t full = bar0 + 8u * (uint32_t)(B_KVF + st);
-      // a row without a slot lies outside the tensor map: the copy fills it with zeros, so
-      // that PV reads 0 * 0 there
-      if (has)
-        ptx::tma_gather4(sbase + (uint32_t)(st * kStageB + blk * kRB + lane * 512), map, col,
-                         make_int4(slot0[0], slot0[1], slot0[2], slot0[3]), full, policy);
-      if (blk == 0) {
-        if (has)
-          *reinterpret_cast<float4*>(sc + st * kTS + 4 * lane) =
-              make_float4(scale[0], scale[1], scale[2], scale[3]);
-        float big = fmaxf(fmaxf(fabsf(scale[0]), fabsf(scale[1])), fmaxf(fabsf(scale[2]), fabsf(scale[3])));
+      const uint32_t full = bar(B_KVF + st);
+      if (lane < kTS / 4)
+        ptx::tma_gather4(sbase + (uint32_t)(st * kStageB) + off, map, col,
+                         make_int4(r[0], r[1], r[2], r[3]), full, policy);
+      if (pw == 0) {
+        float big = 0.f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-        const uint32_t sh = nib << (4 * (lane & 7));
-        const uint32_t w0 = __reduce_or_sync(0xffffffffu, (lane >> 3) == 0 ? sh : 0u);
-        const uint32_t w1 = __reduce_or_sync(0xffffffffu, (lane >> 3) == 1 ? sh : 0u);
-        const uint32_t w2 = __reduce_or_sync(0xffffffffu, (lane >> 3) == 2 ? sh : 0u);
+        for (int e = 0; e < kE; ++e) {
+          sc[st * kTS + 32 * e + lane] = scale[e];
+          big = fmaxf(big, fabsf(scale[e]));
+        }
+        big = ptx::warp_max(big);
         if (lane == 0) {
-          cmd[4 * st] = (int)w0;
-          cmd[4 * st + 1] = (int)w1;
-          cmd[4 * st + 2] = (int)w2;
+#pragma unroll
+          for (int e = 0; e < kE; ++e) cmd[4 * st + e] = (int)w[e];
           cmd[4 * st + 3] = (int)t;
           smax[st] = big;
         }
+        __syncwarp();
       }
-      __syncwarp();
       if (lane == 0) ptx::mbar_arrive_expect_tx(full, (uint32_t)kRB);
       ++n;
       if (++st == kStages) {
@@ -249,23 +284,23 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
       }
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < kE; ++e) {
       slot0[e] = slot1[e];
       slot1[e] = slot2[e];
       pos2[e] = pos3[e];
     }
   }
-  // the end: one more stage that holds no slots
+  // the end: one more stage, without slots
   if (lane == 0) {
-    ok = ok && wait(bar0 + 8u * (uint32_t)(B_KVE + st), phase ^ 1u);
+    ok = ok && wait(bar(B_KVE + st), phase ^ 1u);
     if (ok) {
-      if (blk == 0) cmd[4 * st + 3] = -1;
-      ptx::mbar_arrive(bar0 + 8u * (uint32_t)(B_KVF + st));
+      if (pw == 0) cmd[4 * st + 3] = -1;
+      ptx::mbar_arrive(bar(B_KVF + st));
     } else {
       // this warp's copies land before the CTA leaves
       const Waiter drain{misc + 3, p.err, p.wait_cycles};
       for (int64_t i = n - 1; i >= 0 && i >= n - kStages; --i)
-        drain(bar0 + 8u * (uint32_t)(B_KVF + (int)(i % kStages)), (uint32_t)((i / kStages) & 1));
+        drain(bar(B_KVF + (int)(i % kStages)), (uint32_t)((i / kStages) & 1));
     }
   }
   __syncwarp();
@@ -368,10 +403,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const __grid_constant__ CUtensorMap tm_kpe, const __grid_constant__ AttendParams p) {
   using C = Cfg<NH>;
   constexpr int kHT = C::kHT;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw_addr = ptx::smem_u32(smem_raw);
-  const uint32_t sbase = (raw_addr + 1023u) & ~1023u;
-  uint8_t* sgen = smem_raw + (sbase - raw_addr);
+  extern __shared__ __align__(1024) uint8_t smem_raw[];  // swizzle atoms are 1024 bytes
+  const uint32_t sbase = ptx::smem_u32(smem_raw);
+  uint8_t* sgen = smem_raw;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sgen + C::OFF_MISC);
   volatile int* cmd = reinterpret_cast<volatile int*>(sgen + C::OFF_CMD);
@@ -386,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      ptx::mbar_init(bar(B_KVF + s), kBlocks);  // one arrive per producer warp
+      ptx::mbar_init(bar(B_KVF + s), kProdWarps);  // one arrive, with its bytes, per warp
       ptx::mbar_init(bar(B_KVE + s), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -423,18 +457,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   float m_run[kHT], l_part[kHT];
   float u = 0.f;                             // the largest scale so far
   int64_t n = 0;                             // live tiles
-  float* red = reinterpret_cast<float*>(sgen + C::OFF_RED);
   float* ml = reinterpret_cast<float*>(sgen + C::OFF_SC);
   bool aborted = false;
 
-  if (warp < kBlocks) {
-    produce<NH>(p, warp < 4 ? &tm_ckv : &tm_kpe, warp, row, split, lane, sbase, sgen, wait);
+  if (warp < kProdWarps) {
+    produce<NH>(p, &tm_ckv, &tm_kpe, warp, row, split, lane, sbase, sgen, wait);
   } else if (warp == kScout) {
     scout<NH>(p, row, lane, sgen);
   } else {
-    constexpr int kQWarps = kThreads / 32 - kBlocks - 1;
+    constexpr int kQWarps = kSmWarps + 2;
     float* qs = reinterpret_cast<float*>(sgen + C::OFF_QS);
-    for (int h = warp < kScout ? warp - kBlocks : warp - kBlocks - 1; h < NH; h += kQWarps) {
+    for (int h = warp < kSm0 ? kSmWarps + warp - kScore : warp - kSm0; h < NH; h += kQWarps) {
       const float unit = stage_query<NH>(p, row, h0 + h, h, lane, sgen);
       if (lane == 0) qs[h] = unit;
     }
@@ -450,10 +483,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t dqp = desc(sbase + (uint32_t)C::OFF_QP, 16, 1024, kSw128);
       bool ok = true;
       for (int64_t i = 0;; ++i) {
-        const int st = (int)(i % kStages), sb = (int)(i & 1);
+        const int st = (int)(i % kStages), sb = (int)(i % C::kSBufs);
         ok = spin(bar(B_KVF + st), (uint32_t)((i / kStages) & 1));
         if (!ok || cmd[4 * st + 3] < 0) break;
-        ok = spin(bar(B_SE + sb), (uint32_t)(((i >> 1) & 1) ^ 1));
+        ok = spin(bar(B_SE + sb), (uint32_t)(((i / C::kSBufs) & 1) ^ 1));
         if (!ok) break;
         ptx::tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(C::kSCols * sb);
@@ -480,9 +513,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kPv) {
     // ------------------------------------------------------------------ PV issuer
     if (lane == 0) {
-      constexpr uint32_t kId = idesc_e4m3(128, 2 * NH, true);
+      constexpr uint32_t kId = idesc_e4m3(128, 3 * NH, true);
       const uint64_t dv = desc(sbase, kRB, 1024, kSw128);
-      const uint64_t dp = desc(sbase + (uint32_t)C::OFF_P, 16, 1024, kSw128);
+      const uint64_t dp = desc(sbase + (uint32_t)C::OFF_P, 16, 256, kSw32);
       bool ok = true;
       for (int64_t i = 0;; ++i) {
         const int st = (int)(i % kStages), pb = (int)(i & 1);
@@ -497,9 +530,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int ks = 0; ks < kTS / 32; ++ks)
-            ptx::umma_f8(tmem + (uint32_t)(C::O_COL + 2 * NH * j),
+            ptx::umma_f8(tmem + (uint32_t)(C::O_COL + 3 * NH * j),
                          dv + vo + (uint64_t)((j * kRB + ks * 4096) >> 4),
-                         dp + po + (uint64_t)((ks * 32) >> 4), kId, (i > 0 || ks > 0) ? 1u : 0u);
+                         dp + po + (uint64_t)((ks * C::kPK) >> 4), kId, (i > 0 || ks > 0) ? 1u : 0u);
         ptx::umma_commit(bar(B_KVE + st));
         ptx::umma_commit(bar(B_PD + pb));
       }
@@ -516,7 +549,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool slot_ok = slot < kTS;  // quadrant 3 holds no slots; its lanes are rows of O
     const float* sc = reinterpret_cast<const float*>(sgen + C::OFF_SC);
     const volatile float* smax = reinterpret_cast<const volatile float*>(sgen + C::OFF_SMAX);
-    const float* qs = reinterpret_cast<const float*>(sgen + C::OFF_QS) + kHT * hh;
     const int sm_tid = (int)threadIdx.x - 32 * kSm0;
     // entries of tiles that turn out to hold nothing get no other value (group g's CTA writes
     // the row's tiles with (tile / S) % G == g, here and at the end)
@@ -530,15 +562,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       m_run[h] = -INFINITY;
       l_part[h] = 0.f;
     }
+    const float* unit = reinterpret_cast<const float*>(sgen + C::OFF_QS) + kHT * hh;
+    float qs[kHT];
+#pragma unroll
+    for (int h = 0; h < kHT; ++h) qs[h] = unit[h];
     for (;; ++n) {
-      const int st = (int)(n % kStages), sb = (int)(n & 1);
+      const int st = (int)(n % kStages), sb = (int)(n % C::kSBufs), pb = (int)(n & 1);
       bool ok = wait(bar(B_KVF + st), (uint32_t)((n / kStages) & 1));
       const int tile = cmd[4 * st + 3];
       const bool end = ok && tile < 0;
-      if (!end) ok = ok && wait(bar(B_SF + sb), (uint32_t)((n >> 1) & 1));
+      if (!end) ok = ok && wait(bar(B_SF + sb), (uint32_t)((n / C::kSBufs) & 1));
+      if (n == 0) {  // the unit of the scales, the same in every thread
+        const float first = smax[st];
+        u = first > 0.f ? first : 1.f;
+      }
       float x[kHT];
-      float scale = 0.f;
+      float ratio = 0.f;  // scale in units, lr its log2
+      float lr = -INFINITY;
       bool valid = false;
+      const bool grow = !end && smax[st] > kTauU * u;
       if (slot_ok && __all_sync(0xffffffffu, ok && !end)) {  // warp-uniform
         ptx::tc_fence_after();
         uint32_t hi[kHT], lo[kHT], pe[kHT];
@@ -546,8 +588,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld<kHT>(ta, hi);
         tmem_ld<kHT>(ta + NH, lo);
         tmem_ld<kHT>(ta + 2 * NH, pe);
-        scale = sc[st * kTS + slot];
+        const float scale = sc[st * kTS + slot];
         valid = ((uint32_t)cmd[4 * st + qd] >> lane) & 1u;
+        ratio = scale / u;
+        lr = ptx::lg2(fabsf(ratio));
         ptx::tmem_wait_ld();
         ptx::tc_fence_before();
 #pragma unroll
@@ -561,65 +605,84 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar(B_SE + sb));
-      const float u_tile = smax[st];
-      bool need = u_tile > u || end;
+      // Whether a running maximum or the unit has to rise, or a wait failed, through one barrier
+      // of the four warps that share the heads.  Their decisions are the same, as they read
+      // the same words; the words are written again two tiles later, behind the next tile's
+      // barrier.
+      const float tau = fminf(kTauQ8 - lr, kTauL);  // P = 2^(x + lr - m) and l's 2^(x - m) in range
+      uint32_t vote = ok && !aborted ? 0u : kFailed;
 #pragma unroll
-      for (int h = 0; h < kHT; ++h) need |= x[h] > m_run[h] + kTauQ8;
-      if (ptx::bar_red_or(kSmBar, kSmThreads, need || !ok || aborted)) {
-        if (ptx::bar_red_or(kSmBar, kSmThreads, !ok || aborted)) {
-          aborted = true;
-          break;
+      for (int h = 0; h < kHT; ++h) vote |= x[h] > m_run[h] + tau ? kRise : 0u;
+      vote = __reduce_or_sync(0xffffffffu, vote);
+      uint32_t* words = reinterpret_cast<uint32_t*>(sgen + C::OFF_RED) + (hh * 2 + pb) * 4;
+      if (lane == 0) words[qd] = vote;
+      ptx::bar_sync(kSmBar + 2 + hh, kSmThreads / 2);
+      {
+        const uint4 v = *reinterpret_cast<const uint4*>(words);
+        vote = v.x | v.y | v.z | v.w;
+      }
+      if (vote & kFailed) {
+        aborted = true;
+        break;
+      }
+      if (end) break;
+      if (vote != 0u || grow) {
+        // Rare past the first tile: raise the maxima to this tile's, the unit to its largest
+        // scale, and bring l and O to them.
+        if (n > 0) {
+          const bool wok = wait(bar(B_PD + (int)((n - 1) & 1)), (uint32_t)(((n - 1) >> 1) & 1));
+          if (!__all_sync(0xffffffffu, wok)) aborted = true;
+          ptx::tc_fence_after();
         }
-        if (end) break;  // every thread has seen it: none voted that a wait failed
-        // raise the running maxima (scores per head, scale) and bring O and l to them
+        float beta = 1.f;
+        if (grow) {
+          const float un = smax[st];
+          beta = u / un;
+          lr += ptx::lg2(beta);
+          ratio *= beta;
+          u = un;
+        }
+        // the maxima go through this tile's P buffer, whose last reader (PV) is done
+        // (in the first term's rows of these heads, which only these warps write)
+        float* tops = reinterpret_cast<float*>(sgen + C::OFF_P + (int)(n % C::kPBufs) * C::kPB + hh * kHT * 32);
+        const float over = fmaxf(lr, 8.f - kTauL);
 #pragma unroll
         for (int h = 0; h < kHT; ++h) {
-          float v = x[h];
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-          if (lane == 0) red[(hh * 4 + qd) * kHT + h] = v;
+          const float v = ptx::warp_max(x[h] + over);
+          if (slot_ok && lane == 0) tops[qd * kHT + h] = v;
         }
-        ptx::bar_sync(kSmBar, kSmThreads);
-        const float un = fmaxf(u, u_tile);
-        const float beta = u > 0.f ? u / un : 0.f;
-        u = un;
+        ptx::bar_sync(kSmBar + 2 + hh, kSmThreads / 2);
         float alpha[kHT];
 #pragma unroll
         for (int h = 0; h < kHT; ++h) {
-          const float* r4 = red + hh * 4 * kHT + h;
-          const float mn = fmaxf(m_run[h], fmaxf(r4[0], fmaxf(r4[kHT], r4[2 * kHT])));
+          const float mn = fmaxf(m_run[h], fmaxf(tops[h], fmaxf(tops[kHT + h], tops[2 * kHT + h])));
           const float a = m_run[h] == -INFINITY ? 0.f : ptx::ex2(m_run[h] - mn);
           // l that is NaN while no score was a number stays so
           l_part[h] = m_run[h] == -INFINITY ? l_part[h] : l_part[h] * a;
           m_run[h] = mn;
           alpha[h] = a * beta;
         }
-        if (n > 0) {
-          const bool wok = wait(bar(B_PD + (int)((n - 1) & 1)), (uint32_t)(((n - 1) >> 1) & 1));
-          if (!__all_sync(0xffffffffu, wok)) {
-            aborted = true;
-          } else {
-            ptx::tc_fence_after();
-            // four tiles of O, hi and lo: kC loads in flight at a time
-            constexpr int kC = NH == 16 ? 4 : 2;
+        ptx::bar_sync(kSmBar + 2 + hh, kSmThreads / 2);  // the buffer is P's again
+        if (n > 0 && !aborted) {
+          // four tiles of O, three terms: kC loads in flight at a time
+          constexpr int kC = NH == 16 ? 4 : 2;
+#pragma unroll 1
+          for (int c = 0; c < 12; c += kC) {
+            const uint32_t ta = tmem + lane_base + (uint32_t)(C::O_COL + NH * c + kHT * hh);
+            uint32_t r[kC][kHT];
 #pragma unroll
-            for (int c = 0; c < 8; c += kC) {
-              const uint32_t ta = tmem + lane_base + (uint32_t)(C::O_COL + NH * c + kHT * hh);
-              uint32_t r[kC][kHT];
+            for (int b = 0; b < kC; ++b) tmem_ld<kHT>(ta + (uint32_t)(NH * b), r[b]);
+            ptx::tmem_wait_ld();
 #pragma unroll
-              for (int b = 0; b < kC; ++b) tmem_ld<kHT>(ta + (uint32_t)(NH * b), r[b]);
-              ptx::tmem_wait_ld();
+            for (int b = 0; b < kC; ++b) {
 #pragma unroll
-              for (int b = 0; b < kC; ++b) {
+              for (int h = 0; h < kHT; ++h)
+                r[b][h] = alpha[h] == 0.f ? 0u : __float_as_uint(__uint_as_float(r[b][h]) * alpha[h]);
 #pragma unroll
-                for (int h = 0; h < kHT; ++h)
-                  r[b][h] = alpha[h] == 0.f ? 0u : __float_as_uint(__uint_as_float(r[b][h]) * alpha[h]);
-#pragma unroll
-                for (int k = 0; k < kHT; k += 8) ptx::tmem_st8(ta + (uint32_t)(NH * b + k), r[b] + k);
-              }
+              for (int k = 0; k < kHT; k += 8) ptx::tmem_st8(ta + (uint32_t)(NH * b + k), r[b] + k);
             }
-            ptx::tmem_wait_st();
           }
+          ptx::tmem_wait_st();
         }
       }
       // P[n % kPBufs] was last read by the PV of tile n - kPBufs
@@ -630,26 +693,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (aborted) continue;  // the next vote ends the loop for every thread
       if (slot_ok) {
-        uint8_t* pb = sgen + C::OFF_P + (int)(n % C::kPBufs) * C::kPB;
-        const float ratio = u > 0.f ? scale / u * kPScale : 0.f;
+        // byte (row r, slot) of P: 32-slot planes of 32-byte rows, 32-byte swizzle
+        uint8_t* pbuf = sgen + C::OFF_P + (int)(n % C::kPBufs) * C::kPB + qd * C::kPK;
+        const float scaled = valid ? ratio * kPScale : 0.f;
 #pragma unroll
         for (int h = 0; h < kHT; h += 2) {
-          float e[2], v[2];
+          float v[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const float mr = m_run[h + k] == -INFINITY ? 0.f : m_run[h + k];
-            e[k] = ptx::ex2(x[h + k] - mr);
-            l_part[h + k] += e[k];
-            v[k] = valid ? e[k] * ratio : 0.f;
+            const float e = ptx::ex2(x[h + k] - mr);
+            l_part[h + k] += e;
+            v[k] = valid ? e * scaled : 0.f;
           }
-          const uint32_t hi = to_e4m3x2(v[0], v[1]);
-          const float2 back = from_e4m3x2(hi);
-          const uint32_t lo = to_e4m3x2((v[0] - back.x) * 16.f, (v[1] - back.y) * 16.f);
           const int r = kHT * hh + h;
-          pb[sw128_byte(r, slot)] = (uint8_t)hi;
-          pb[sw128_byte(r + 1, slot)] = (uint8_t)(hi >> 8);
-          pb[sw128_byte(NH + r, slot)] = (uint8_t)lo;
-          pb[sw128_byte(NH + r + 1, slot)] = (uint8_t)(lo >> 8);
+#pragma unroll
+          for (int term = 0; term < 3; ++term) {
+            const uint32_t b = to_e4m3x2(v[0], v[1]);
+            const float2 back = from_e4m3x2(b);
+            v[0] = (v[0] - back.x) * 16.f;
+            v[1] = (v[1] - back.y) * 16.f;
+            pbuf[sw32_byte(term * NH + r, lane)] = (uint8_t)b;
+            pbuf[sw32_byte(term * NH + r + 1, lane)] = (uint8_t)(b >> 8);
+          }
         }
         if (p.weights != nullptr) {
           const int64_t at = (row * G + group) * p.ntiles + split + n * S;
@@ -662,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::fence_proxy_async_smem();
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar(B_PF + sb));
+      if (lane == 0) ptx::mbar_arrive(bar(B_PF + pb));
     }
     // ------------------------------------------------------------------ this CTA's m and L
     // PD of tile n - 3 (two P buffers) or n - 2 was waited for above, on the same barrier or
@@ -671,20 +737,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && n > 0) ok = wait(bar(B_PD + (int)((n - 1) & 1)), (uint32_t)(((n - 1) >> 1) & 1));
     aborted = ptx::bar_red_or(kSmBar, kSmThreads, !ok);
     ptx::tc_fence_after();
+    float* red = reinterpret_cast<float*>(sgen + C::OFF_P);  // [half][quadrant][kHT]
 #pragma unroll
     for (int h = 0; h < kHT; ++h) {
       float v = l_part[h];
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == 0) red[(hh * 4 + qd) * kHT + h] = v;
+      if (lane == 0 && slot_ok) red[(hh * 3 + qd) * kHT + h] = v;
     }
     ptx::bar_sync(kSmBar, kSmThreads);
     if (qd == 0 && lane == 0) {
 #pragma unroll
       for (int h = 0; h < kHT; ++h) {
-        const float* r4 = red + hh * 4 * kHT + h;
+        const float* r3 = red + hh * 3 * kHT + h;
         ml[kHT * hh + h] = m_run[h];
-        ml[NH + kHT * hh + h] = (r4[0] + r4[kHT]) + r4[2 * kHT];
+        ml[NH + kHT * hh + h] = (r3[0] + r3[kHT]) + r3[2 * kHT];
       }
       ml[2 * NH] = u;
     }
@@ -692,15 +759,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* o_s = reinterpret_cast<float*>(sgen + C::OFF_O);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      uint32_t hi[kHT], lo[kHT];
-      const uint32_t ta = tmem + lane_base + (uint32_t)(C::O_COL + 2 * NH * j + kHT * hh);
-      tmem_ld<kHT>(ta, hi);
-      tmem_ld<kHT>(ta + NH, lo);
+      uint32_t r[3][kHT];
+#pragma unroll
+      for (int c = 0; c < 3; ++c)
+        tmem_ld<kHT>(tmem + lane_base + (uint32_t)(C::O_COL + NH * (3 * j + c) + kHT * hh), r[c]);
       ptx::tmem_wait_ld();
 #pragma unroll
-      for (int h = 0; h < kHT; ++h)
-        o_s[(kHT * hh + h) * kDCkv + 128 * j + 32 * qd + lane] =
-            n > 0 ? fmaf(__uint_as_float(lo[h]), 0.0625f, __uint_as_float(hi[h])) : 0.f;
+      for (int h = 0; h < kHT; ++h) {
+        const float o = fmaf(fmaf(__uint_as_float(r[2][h]), 0.0625f, __uint_as_float(r[1][h])), 0.0625f,
+                             __uint_as_float(r[0][h]));
+        o_s[(kHT * hh + h) * kDCkv + 128 * j + 32 * qd + lane] = n > 0 ? o : 0.f;
+      }
     }
   }
   __syncwarp();
@@ -711,52 +780,58 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool lost = false;  // a wait ran out somewhere in the cluster: the row is written as NaN
   if (warp >= kSm0) {
     const int sm_tid = (int)threadIdx.x - 32 * kSm0;
-    float* all = reinterpret_cast<float*>(sgen + C::OFF_ALL);
     float* coef = reinterpret_cast<float*>(sgen + C::OFF_COEF);
     float* lse_s = coef + S * NH;
     const int rank0 = group * S;  // the rank of split 0 of this group
     if (S == 1) ptx::bar_sync(kSmBar, kSmThreads);
-    for (int e = sm_tid; e < S * C::kMl; e += kSmThreads)
-      all[e] = ld_cluster(ptx::mapa(sbase + (uint32_t)C::OFF_SC + 4u * (uint32_t)(e % C::kMl),
-                                    (uint32_t)(rank0 + e / C::kMl)));
     if (sm_tid < S * G)
       lost = __float_as_uint(ld_cluster(
                  ptx::mapa(sbase + (uint32_t)C::OFF_MISC + 8u, (uint32_t)sm_tid))) != 0u;
+    // split s sums and writes the heads [s NH / S, (s + 1) NH / S), four values a thread at a
+    // time: NH / 2 reads whatever S, under way while the coefficients are computed
+    const int ss = __ffs(S) - 1;  // S is a power of two
+    const int per = NH >> ss;
+    float4 part[NH / 2];
+#pragma unroll
+    for (int i = 0; i < NH / 2; ++i) {
+      const int e = sm_tid + kSmThreads * (i >> ss);  // value 4 e of the heads of this split
+      part[i] = ld_cluster4(ptx::mapa(sbase + (uint32_t)(C::OFF_O + 4 * (split * per * kDCkv + 4 * e)),
+                                      (uint32_t)(rank0 + (i & (S - 1)))));
+    }
     lost = ptx::bar_red_or(kSmBar, kSmThreads, lost);
-    if (sm_tid < NH) {
-      // a head's lse, and what a value of split s in O counts for in its output
-      float M = -INFINITY, L = 0.f;
-      for (int s = 0; s < S; ++s) M = fmaxf(M, all[s * C::kMl + sm_tid]);
-      for (int s = 0; s < S; ++s) {
-        const float ls = all[s * C::kMl + NH + sm_tid];
-        const float w = ls == 0.f ? 0.f : ptx::ex2(all[s * C::kMl + sm_tid] - M);
-        L += ls == 0.f ? 0.f : ls * w;
-        coef[s * NH + sm_tid] = w;
+    for (int e = sm_tid; e < NH * S; e += kSmThreads) {
+      // thread (head, split): the head's lse, and what a value of the split's O counts for in
+      // its output; the S threads of a head are neighbours in a warp
+      const int h = e >> ss, s = e & (S - 1);
+      const uint32_t at = ptx::mapa(sbase + (uint32_t)C::OFF_SC, (uint32_t)(rank0 + s));
+      const float ms = ld_cluster(at + 4u * (uint32_t)h), ls = ld_cluster(at + 4u * (uint32_t)(NH + h));
+      const float us = ld_cluster(at + 8u * NH);
+      float M = ms;
+      for (int k = 1; k < S; k <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+      const float w = ls == 0.f ? 0.f : ptx::ex2(ms - M);
+      float L = ls == 0.f ? 0.f : ls * w;
+      for (int k = 1; k < S; k <<= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
+      coef[s * NH + h] = w == 0.f ? 0.f : w / L * (us * (1.f / kPScale));
+      const float lse = lost ? NAN : L == 0.f ? -INFINITY : M + ptx::lg2(L);
+      if (s == 0) {
+        lse_s[h] = lse;
+        if (split == 0) p.lse[row * p.lse_sb + (int64_t)(h0 + h) * p.lse_sh] = lse;
       }
-      for (int s = 0; s < S; ++s)
-        if (coef[s * NH + sm_tid] != 0.f)
-          coef[s * NH + sm_tid] = coef[s * NH + sm_tid] / L * (all[s * C::kMl + 2 * NH] * (1.f / kPScale));
-      lse_s[sm_tid] = lost ? NAN : L == 0.f ? -INFINITY : M + ptx::lg2(L);
-      if (split == 0)
-        p.lse[row * p.lse_sb + (int64_t)(h0 + sm_tid) * p.lse_sh] = lse_s[sm_tid];
     }
     ptx::bar_sync(kSmBar, kSmThreads);
-    // split s sums and writes the heads [s NH / S, (s + 1) NH / S), four values a thread
-    const int per = NH / S;
-    for (int e = sm_tid; e < per * (kDCkv / 4); e += kSmThreads) {
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NH / 2; ++i) {
+      const int e = sm_tid + kSmThreads * (i >> ss);
       const int hl = split * per + e / (kDCkv / 4), d = 4 * (e % (kDCkv / 4));
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int s = 0; s < S; ++s) {
-        const float c = coef[s * NH + hl];
-        const float4 v = ld_cluster4(
-            ptx::mapa(sbase + (uint32_t)(C::OFF_O + 4 * (hl * kDCkv + d)), (uint32_t)(rank0 + s)));
-        if (c != 0.f) {  // 0: no weight, whatever the values
-          o.x = fmaf(v.x, c, o.x);
-          o.y = fmaf(v.y, c, o.y);
-          o.z = fmaf(v.z, c, o.z);
-          o.w = fmaf(v.w, c, o.w);
-        }
+      const float c = coef[(i & (S - 1)) * NH + hl];
+      if (c != 0.f) {  // 0: no weight, whatever the values
+        o.x = fmaf(part[i].x, c, o.x);
+        o.y = fmaf(part[i].y, c, o.y);
+        o.z = fmaf(part[i].z, c, o.z);
+        o.w = fmaf(part[i].w, c, o.w);
       }
+      if ((i & (S - 1)) != S - 1) continue;
       if (lost) o = make_float4(NAN, NAN, NAN, NAN);
       __nv_bfloat16* dst = p.out + row * p.out_sb + (int64_t)(h0 + hl) * p.out_sh + d;
       const __nv_bfloat162 a = __floats2bfloat162_rn(o.x, o.y), b = __floats2bfloat162_rn(o.z, o.w);
@@ -769,6 +844,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         dst[2] = b.x;
         dst[3] = b.y;
       }
+      o = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     if (p.weights != nullptr && lost) {
       for (int t = split + S * group; t < p.ntiles; t += S * G) {
