@@ -35,7 +35,7 @@
 //                valid entry are skipped
 //   warp 5       score issuer: S^T[96 slots x (hi, lo, pe)], 16 f8 + 4 bf16 MMAs
 //   warp 6       PV issuer: O^T[512 x 3 terms] += V^T P^T, 12 f8 MMAs (V^T read in place)
-//   warp 7       finds the row's last entry that is not padding, so that the producers can stop there
+//   warp 7       keeper: the tiles' scales, validity and numbers, and where the row's padding begins
 //   warps 8-15   softmax: warp w reads TMEM lanes 32 (w % 4) .. (slots) and half of the heads
 #pragma once
 
@@ -76,7 +76,7 @@ constexpr int kStageB = kBlocks * kRB;
 constexpr int kStages = 3;
 constexpr int kThreads = 512;
 constexpr int kProdWarps = 5;
-constexpr int kScore = 5, kPv = 6, kScout = 7, kSm0 = 8;
+constexpr int kScore = 5, kPv = 6, kKeeper = 7, kSm0 = 8;
 constexpr int kSmWarps = 8, kSmThreads = 256;
 constexpr uint32_t kSmBar = 1, kQBar = 2;
 constexpr float kTauQ8 = 7.f;         // log2: how far a weighted score may pass the running maximum
@@ -161,140 +161,117 @@ __device__ __forceinline__ uint32_t sw128_byte(int r, int b) {
   return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + (((b >> 4) ^ (r & 7)) << 4) + (b & 15));
 }
 
-// ---------------------------------------------------------------- gather producers
+// ---------------------------------------------------------------- index entries
 //
-// Warp j < 5 gathers column block j of every slot of a tile, lane g < 24 that of the slots 4g ..
-// 4g + 3.  Five warps, because a lane's gather takes about 67 cycles to issue from one warp
-// (8,000 cycles for a tile's 120) while the copy engine takes one in about 20.  The warps look
-// at the same entries, lane l at those of slots l, l + 32 and l + 64, and so agree on the live
-// tiles; warp 0 also provides the scales, the validity words and the tile number.
-template <int NH>
-__device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap* tm_ckv,
-                                        const CUtensorMap* tm_kpe, int pw, int64_t row, int split,
-                                        int lane, uint32_t sbase, uint8_t* sgen, const Waiter& wait) {
-  using C = Cfg<NH>;
-  constexpr int kE = kTS / 32;
-  const uint32_t bar0 = sbase + (uint32_t)C::OFF_BAR;
-  auto bar = [&](int k) { return bar0 + 8u * (uint32_t)k; };
-  volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sgen + C::OFF_MISC);
-  volatile int* cmd = reinterpret_cast<volatile int*>(sgen + C::OFF_CMD);
-  volatile float* smax = reinterpret_cast<volatile float*>(sgen + C::OFF_SMAX);
-  float* sc = reinterpret_cast<float*>(sgen + C::OFF_SC);
-  const int32_t* ir = p.idx + row * p.idx_sb;
-  const bool paged = p.table.pt != nullptr;
-  const CUtensorMap* map = pw < 4 ? tm_ckv : tm_kpe;
-  const int col = pw < 4 ? 128 * pw : 0;
-  const uint32_t off = (uint32_t)(pw * kRB + lane * 512);
-  const uint64_t policy = ptx::policy_evict_first();
+// The slots that a lane's kN entries of a tile name, fetched ahead: entries three tiles, pages (of
+// a paged call) two.  -1: padding, -2: names no slot.
+template <int kN>
+struct Entries {
+  const AttendParams& p;
+  const int32_t* ir;
+  int64_t row;
+  int first, step;  // this lane: entries first + step e of a tile
+  int pos2[kN], slot1[kN], slot0[kN];
 
-  auto load_pos = [&](int64_t t, int (&pos)[kE]) {
+  __device__ __forceinline__ void load(int64_t t, int (&pos)[kN], bool has) const {
 #pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      const int64_t k = t * kTS + 32 * e + lane;
-      pos[e] = k < p.topk ? ldg_now(ir + k) : -1;
+    for (int e = 0; e < kN; ++e) {
+      const int64_t k = t * kTS + first + step * e;
+      pos[e] = has && k < p.topk ? ldg_now(ir + k) : -1;
     }
-  };
-  // -1: padding, -2: names no slot
-  auto load_slot = [&](const int (&pos)[kE], int (&slot)[kE]) {
+  }
+  __device__ __forceinline__ void translate(const int (&pos)[kN], int (&slot)[kN]) const {
 #pragma unroll
-    for (int e = 0; e < kE; ++e) {
+    for (int e = 0; e < kN; ++e) {
       if (pos[e] == -1) slot[e] = -1;
-      else if (paged) slot[e] = slot_at(p.table, row, pos[e], p.cache.num_slots);
+      else if (p.table.pt != nullptr) slot[e] = slot_at(p.table, row, pos[e], p.cache.num_slots);
       else slot[e] = pos[e] >= 0 && pos[e] < p.cache.num_slots ? pos[e] : -1;
       if (slot[e] < 0 && pos[e] != -1) slot[e] = -2;
     }
-  };
-
-  // slots of this iteration and the next, entries of the one after
-  int pos2[kE], slot1[kE], slot0[kE];
-  int64_t t = split;
-  {
-    int a[kE], b[kE];
-    load_pos(t, a);
-    load_pos(t + p.splits, b);
-    load_pos(t + 2 * p.splits, pos2);
-    load_slot(a, slot0);
-    load_slot(b, slot1);
   }
+  __device__ __forceinline__ void start(int64_t t, bool has) {
+    int a[kN], b[kN];
+    load(t, a, has);
+    load(t + p.splits, b, has);
+    load(t + 2 * p.splits, pos2, has);
+    translate(a, slot0);
+    translate(b, slot1);
+  }
+  // What tile t + 2 S and t + 3 S need, to be in slot0 two and three advances from now.
+  int slot2[kN], pos3[kN];
+  __device__ __forceinline__ void prefetch(int64_t t, bool has) {
+    translate(pos2, slot2);
+    load(t + 3 * p.splits, pos3, has);
+  }
+  __device__ __forceinline__ void advance() {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      slot0[e] = slot1[e];
+      slot1[e] = slot2[e];
+      pos2[e] = pos3[e];
+    }
+  }
+};
+
+// ---------------------------------------------------------------- gather producers
+//
+// Warp j < 5 gathers column block j of every slot of a tile, four slots a copy, lane g < 24
+// holding the slots 4g .. 4g + 3.  One elected thread issues the copies of a warp-uniform loop:
+// 1,650 cycles a tile for the five warps, against 2,200 when each lane issues its own (and
+// 8,000 from one warp), so that HBM and not the issue is the limit.  They do nothing else: the
+// keeper (warp 7) looks at the same entries and provides the scales, the validity words and
+// the tile number, so all agree on the live tiles.
+template <int NH>
+__device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap* map, int blk,
+                                        int64_t row, int split, int lane, uint32_t sbase,
+                                        uint8_t* sgen, const Waiter& wait) {
+  using C = Cfg<NH>;
+  const uint32_t bar0 = sbase + (uint32_t)C::OFF_BAR;
+  auto bar = [&](int k) { return bar0 + 8u * (uint32_t)k; };
+  volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sgen + C::OFF_MISC);
+  const bool has = lane < kTS / 4;
+  const int col = blk < 4 ? 128 * blk : 0;
+  const bool el = ptx::elect_one();
+  const uint64_t policy = ptx::policy_evict_first();
+  Entries<4> in{p, p.idx + row * p.idx_sb, row, 4 * lane, 1};
+  int64_t t = split;
+  in.start(t, has);
   bool ok = true;
   int64_t n = 0;  // live tiles
   int st = 0;
   uint32_t phase = 0;
-  // misc[4] is the scout's to lower at any time: the lanes agree on one reading
+  // misc[4] is the keeper's to lower at any time: the lanes agree on one reading
   for (; t < __shfl_sync(0xffffffffu, (int)misc[4], 0); t += p.splits) {
-    uint32_t w[kE], any = 0;
-#pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      w[e] = __ballot_sync(0xffffffffu, slot0[e] >= 0);
-      any |= w[e];
-    }
-    float scale[kE];
-    if (pw == 0) {
-      bool bad = false;
-#pragma unroll
-      for (int e = 0; e < kE; ++e) {
-        bad |= slot0[e] == -2;
-        scale[e] = slot0[e] >= 0 ? ldg_now(p.cache.scale + (slot0[e] >> p.cache.block_shift)) : 0.f;
-      }
-      if (bad) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
-    }
-    int slot2[kE], pos3[kE];
-    load_slot(pos2, slot2);
-    load_pos(t + 3 * p.splits, pos3);
-    if (any != 0u) {
-      // The four slots of lane g are entries of lanes 4 (g % 8) .. + 3, register g / 8.  A slot
-      // that is none lies outside the tensor map: the copy fills its row with zeros, so that PV
-      // reads 0 * 0 there.
-      int r[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int from = 4 * (lane & 7) + e;
-        const int a = __shfl_sync(0xffffffffu, slot0[0], from), b = __shfl_sync(0xffffffffu, slot0[1], from),
-                  c = __shfl_sync(0xffffffffu, slot0[2], from);
-        r[e] = lane < 8 ? a : lane < 16 ? b : c;
-      }
-      if (lane == 0) ok = wait(bar(B_KVE + st), phase ^ 1u);
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+    const int4 r = make_int4(in.slot0[0], in.slot0[1], in.slot0[2], in.slot0[3]);
+    const bool live = __any_sync(0xffffffffu, r.x >= 0 || r.y >= 0 || r.z >= 0 || r.w >= 0);
+    in.prefetch(t, has);
+    if (live) {
+      ok = __all_sync(0xffffffffu, wait(bar(B_KVE + st), phase ^ 1u));
       if (!ok) break;
       const uint32_t full = bar(B_KVF + st);
-      if (lane < kTS / 4)
-        ptx::tma_gather4(sbase + (uint32_t)(st * kStageB) + off, map, col,
-                         make_int4(r[0], r[1], r[2], r[3]), full, policy);
-      if (pw == 0) {
-        float big = 0.f;
+      const uint32_t dst = sbase + (uint32_t)(st * kStageB + blk * kRB);
+      if (el) ptx::mbar_arrive_expect_tx(full, (uint32_t)kRB);
+      // a slot that is none lies outside the tensor map: the copy fills its row with zeros, so
+      // that PV reads 0 * 0 there
 #pragma unroll
-        for (int e = 0; e < kE; ++e) {
-          sc[st * kTS + 32 * e + lane] = scale[e];
-          big = fmaxf(big, fabsf(scale[e]));
-        }
-        big = ptx::warp_max(big);
-        if (lane == 0) {
-#pragma unroll
-          for (int e = 0; e < kE; ++e) cmd[4 * st + e] = (int)w[e];
-          cmd[4 * st + 3] = (int)t;
-          smax[st] = big;
-        }
-        __syncwarp();
+      for (int g = 0; g < kTS / 4; ++g) {
+        const int4 s = make_int4(__shfl_sync(0xffffffffu, r.x, g), __shfl_sync(0xffffffffu, r.y, g),
+                                 __shfl_sync(0xffffffffu, r.z, g), __shfl_sync(0xffffffffu, r.w, g));
+        if (el) ptx::tma_gather4(dst + (uint32_t)(g * 512), map, col, s, full, policy);
       }
-      if (lane == 0) ptx::mbar_arrive_expect_tx(full, (uint32_t)kRB);
+      __syncwarp();
       ++n;
       if (++st == kStages) {
         st = 0;
         phase ^= 1u;
       }
     }
-#pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      slot0[e] = slot1[e];
-      slot1[e] = slot2[e];
-      pos2[e] = pos3[e];
-    }
+    in.advance();
   }
   // the end: one more stage, without slots
-  if (lane == 0) {
+  if (el) {
     ok = ok && wait(bar(B_KVE + st), phase ^ 1u);
     if (ok) {
-      if (pw == 0) cmd[4 * st + 3] = -1;
       ptx::mbar_arrive(bar(B_KVF + st));
     } else {
       // this warp's copies land before the CTA leaves
@@ -306,23 +283,82 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
   __syncwarp();
 }
 
-// The tile behind the row's last entry that is not padding, found from the end in steps of
-// 512 entries (warp 3).
+// The keeper (warp 7).  First the tile behind the row's last entry that is not padding, found
+// from the end in steps of 512 entries, so that nobody walks a short row's padding; then,
+// tile by tile, lane l the entries l, l + 32 and l + 64: scales, validity, the tile's number.
 template <int NH>
-__device__ __forceinline__ void scout(const AttendParams& p, int64_t row, int lane, uint8_t* sgen) {
-  const int32_t* ir = p.idx + row * p.idx_sb;
+__device__ __forceinline__ void keep_books(const AttendParams& p, int64_t row, int split, int lane,
+                                           uint32_t sbase, uint8_t* sgen, const Waiter& wait) {
+  using C = Cfg<NH>;
+  constexpr int kE = kTS / 32;
+  const uint32_t bar0 = sbase + (uint32_t)C::OFF_BAR;
+  auto bar = [&](int k) { return bar0 + 8u * (uint32_t)k; };
+  volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sgen + C::OFF_MISC);
+  volatile int* cmd = reinterpret_cast<volatile int*>(sgen + C::OFF_CMD);
+  volatile float* smax = reinterpret_cast<volatile float*>(sgen + C::OFF_SMAX);
+  float* sc = reinterpret_cast<float*>(sgen + C::OFF_SC);
+  Entries<kE> in{p, p.idx + row * p.idx_sb, row, lane, 32};
+  int64_t t = split;
+  in.start(t, true);
   int end = 0;
   for (int hi = p.topk; hi > 0 && end == 0; hi -= 512) {
     int last = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int k = hi - 512 + 32 * i + lane;
-      if (k >= 0 && __ldg(ir + k) != -1) last = k + 1;
+      if (k >= 0 && __ldg(in.ir + k) != -1) last = k + 1;
     }
     end = __reduce_max_sync(0xffffffffu, last);
   }
-  if (lane == 0)
-    reinterpret_cast<volatile uint32_t*>(sgen + Cfg<NH>::OFF_MISC)[4] = (uint32_t)((end + kTS - 1) / kTS);
+  end = (end + kTS - 1) / kTS;
+  if (lane == 0) misc[4] = (uint32_t)end;
+  bool ok = true;
+  int st = 0;
+  uint32_t phase = 0;
+  for (; t < end; t += p.splits) {
+    uint32_t w[kE], any = 0;
+    float scale[kE], big = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) {
+      const int slot = in.slot0[e];
+      w[e] = __ballot_sync(0xffffffffu, slot >= 0);
+      any |= w[e];
+      bad |= slot == -2;
+      scale[e] = slot >= 0 ? ldg_now(p.cache.scale + (slot >> p.cache.block_shift)) : 0.f;
+    }
+    if (bad) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
+    in.prefetch(t, true);
+    if (any != 0u) {
+      if (lane == 0) ok = wait(bar(B_KVE + st), phase ^ 1u);
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      if (!ok) break;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+        sc[st * kTS + 32 * e + lane] = scale[e];
+        big = fmaxf(big, fabsf(scale[e]));
+      }
+      big = ptx::warp_max(big);
+      if (lane == 0) {
+#pragma unroll
+        for (int e = 0; e < kE; ++e) cmd[4 * st + e] = (int)w[e];
+        cmd[4 * st + 3] = (int)t;
+        smax[st] = big;
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(B_KVF + st));
+      if (++st == kStages) {
+        st = 0;
+        phase ^= 1u;
+      }
+    }
+    in.advance();
+  }
+  if (lane == 0 && ok && wait(bar(B_KVE + st), phase ^ 1u)) {
+    cmd[4 * st + 3] = -1;
+    ptx::mbar_arrive(bar(B_KVF + st));
+  }
+  __syncwarp();
 }
 
 // One query head into shared memory: hi and lo rows of q_nope in e4m3, the q_pe row in bf16.
@@ -420,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      ptx::mbar_init(bar(B_KVF + s), kProdWarps);  // one arrive, with its bytes, per warp
+      ptx::mbar_init(bar(B_KVF + s), kProdWarps + 1);  // the gatherers (with their bytes) and the keeper
       ptx::mbar_init(bar(B_KVE + s), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -461,9 +497,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool aborted = false;
 
   if (warp < kProdWarps) {
-    produce<NH>(p, &tm_ckv, &tm_kpe, warp, row, split, lane, sbase, sgen, wait);
-  } else if (warp == kScout) {
-    scout<NH>(p, row, lane, sgen);
+    produce<NH>(p, warp < 4 ? &tm_ckv : &tm_kpe, warp, row, split, lane, sbase, sgen, wait);
+  } else if (warp == kKeeper) {
+    keep_books<NH>(p, row, split, lane, sbase, sgen, wait);
   } else {
     constexpr int kQWarps = kSmWarps + 2;
     float* qs = reinterpret_cast<float*>(sgen + C::OFF_QS);
@@ -476,21 +512,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (warp == kScore) {
     // ------------------------------------------------------------------ score issuer
-    if (lane == 0) {
-      constexpr uint32_t kId = idesc_e4m3(128, 2 * NH, false), kIdPe = idesc_bf16(128, NH, false);
-      const uint64_t dk = desc(sbase, 16, 1024, kSw128);
-      const uint64_t dq = desc(sbase + (uint32_t)C::OFF_Q, 16, 1024, kSw128);
-      const uint64_t dqp = desc(sbase + (uint32_t)C::OFF_QP, 16, 1024, kSw128);
-      bool ok = true;
-      for (int64_t i = 0;; ++i) {
-        const int st = (int)(i % kStages), sb = (int)(i % C::kSBufs);
-        ok = spin(bar(B_KVF + st), (uint32_t)((i / kStages) & 1));
-        if (!ok || cmd[4 * st + 3] < 0) break;
-        ok = spin(bar(B_SE + sb), (uint32_t)(((i / C::kSBufs) & 1) ^ 1));
-        if (!ok) break;
-        ptx::tc_fence_after();
-        const uint32_t d = tmem + (uint32_t)(C::kSCols * sb);
-        const uint64_t ko = (uint64_t)((st * kStageB) >> 4);
+    constexpr uint32_t kId = idesc_e4m3(128, 2 * NH, false), kIdPe = idesc_bf16(128, NH, false);
+    const uint64_t dk = desc(sbase, 16, 1024, kSw128);
+    const uint64_t dq = desc(sbase + (uint32_t)C::OFF_Q, 16, 1024, kSw128);
+    const uint64_t dqp = desc(sbase + (uint32_t)C::OFF_QP, 16, 1024, kSw128);
+    const bool el = ptx::elect_one();  // warp-uniform loops around one issuing thread
+    bool ok = true;
+    for (int64_t i = 0;; ++i) {
+      const int st = (int)(i % kStages), sb = (int)(i % C::kSBufs);
+      ok = __all_sync(0xffffffffu, spin(bar(B_KVF + st), (uint32_t)((i / kStages) & 1)));
+      if (!ok || __any_sync(0xffffffffu, cmd[4 * st + 3] < 0)) break;
+      ok = __all_sync(0xffffffffu, spin(bar(B_SE + sb), (uint32_t)(((i / C::kSBufs) & 1) ^ 1)));
+      if (!ok) break;
+      ptx::tc_fence_after();
+      const uint32_t d = tmem + (uint32_t)(C::kSCols * sb);
+      const uint64_t ko = (uint64_t)((st * kStageB) >> 4);
+      if (el) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -503,29 +540,31 @@ __global__ void __launch_bounds__(kThreads, 1)
                          dqp + (uint64_t)((ks * 32) >> 4), kIdPe, ks ? 1u : 0u);
         ptx::umma_commit(bar(B_SF + sb));
       }
-      if (!ok) {
-        const Waiter drain{misc + 3, p.err, p.wait_cycles};
-        ptx::umma_commit(bar(B_DRAIN));
-        drain(bar(B_DRAIN), 0);
-      }
+      __syncwarp();
+    }
+    if (!ok && el) {
+      const Waiter drain{misc + 3, p.err, p.wait_cycles};
+      ptx::umma_commit(bar(B_DRAIN));
+      drain(bar(B_DRAIN), 0);
     }
     __syncwarp();
   } else if (warp == kPv) {
     // ------------------------------------------------------------------ PV issuer
-    if (lane == 0) {
-      constexpr uint32_t kId = idesc_e4m3(128, 3 * NH, true);
-      const uint64_t dv = desc(sbase, kRB, 1024, kSw128);
-      const uint64_t dp = desc(sbase + (uint32_t)C::OFF_P, 16, 256, kSw32);
-      bool ok = true;
-      for (int64_t i = 0;; ++i) {
-        const int st = (int)(i % kStages), pb = (int)(i & 1);
-        ok = spin(bar(B_KVF + st), (uint32_t)((i / kStages) & 1));
-        if (!ok || cmd[4 * st + 3] < 0) break;
-        ok = spin(bar(B_PF + pb), (uint32_t)((i >> 1) & 1));
-        if (!ok) break;
-        ptx::tc_fence_after();
-        const uint64_t vo = (uint64_t)((st * kStageB) >> 4);
-        const uint64_t po = (uint64_t)(((int)(i % C::kPBufs) * C::kPB) >> 4);
+    constexpr uint32_t kId = idesc_e4m3(128, 3 * NH, true);
+    const uint64_t dv = desc(sbase, kRB, 1024, kSw128);
+    const uint64_t dp = desc(sbase + (uint32_t)C::OFF_P, 16, 256, kSw32);
+    const bool el = ptx::elect_one();
+    bool ok = true;
+    for (int64_t i = 0;; ++i) {
+      const int st = (int)(i % kStages), pb = (int)(i & 1);
+      ok = __all_sync(0xffffffffu, spin(bar(B_KVF + st), (uint32_t)((i / kStages) & 1)));
+      if (!ok || __any_sync(0xffffffffu, cmd[4 * st + 3] < 0)) break;
+      ok = __all_sync(0xffffffffu, spin(bar(B_PF + pb), (uint32_t)((i >> 1) & 1)));
+      if (!ok) break;
+      ptx::tc_fence_after();
+      const uint64_t vo = (uint64_t)((st * kStageB) >> 4);
+      const uint64_t po = (uint64_t)(((int)(i % C::kPBufs) * C::kPB) >> 4);
+      if (el) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -536,11 +575,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::umma_commit(bar(B_KVE + st));
         ptx::umma_commit(bar(B_PD + pb));
       }
-      if (!ok) {
-        const Waiter drain{misc + 3, p.err, p.wait_cycles};
-        ptx::umma_commit(bar(B_DRAIN + 1));
-        drain(bar(B_DRAIN + 1), 0);
-      }
+      __syncwarp();
+    }
+    if (!ok && el) {
+      const Waiter drain{misc + 3, p.err, p.wait_cycles};
+      ptx::umma_commit(bar(B_DRAIN + 1));
+      drain(bar(B_DRAIN + 1), 0);
     }
     __syncwarp();
   } else if (warp >= kSm0) {

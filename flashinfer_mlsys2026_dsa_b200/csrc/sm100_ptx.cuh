@@ -59,6 +59,18 @@ __device__ __forceinline__ uint64_t cycles() {
   return t;
 }
 
+// True in one thread of a converged warp, the same one every time.  A branch on it keeps its
+// operands in uniform registers, where tensor-core and copy instructions want them.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // ---------------------------------------------------------------- proxies
 // Generic-proxy writes to shared memory become visible to the async proxy
 // (tensor core operand reads) after this fence.
