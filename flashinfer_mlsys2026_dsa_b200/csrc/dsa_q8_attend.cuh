@@ -82,6 +82,7 @@ constexpr uint32_t kSmBar = 1, kQBar = 2;
 constexpr float kTauQ8 = 7.f;         // log2: how far a weighted score may pass the running maximum
 constexpr float kTauL = 60.f;         // the same for a score alone: its exponential stays finite
 constexpr float kTauU = 16.f;         // how far a scale may pass the unit
+constexpr float kNone = -3e38f;       // running maximum before the first score
 constexpr float kPScale = 3.5f;       // P <= 3.5 * 2^7 = 448, the largest e4m3 value
 constexpr int kMaxCluster = 8;
 constexpr uint32_t kRise = 1u, kFailed = 2u;  // vote words
@@ -418,6 +419,34 @@ __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t* r) {
   for (int c = 0; c < kN; c += 8) ptx::tmem_ld8(addr + (uint32_t)c, r + c);
 }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
+        "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 pair(const uint32_t* r, int i) {
+  return make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -490,8 +519,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int qd = warp & 3;                   // TMEM lane quadrant: slots 32 qd .. 32 qd + 31
   const int hh = (warp - kSm0) >> 2;         // heads kHT hh .. kHT hh + kHT - 1 of the group
   const uint32_t lane_base = (uint32_t)(32 * qd) << 16;
-  float m_run[kHT], l_part[kHT];
-  float u = 0.f;                             // the largest scale so far
+  float2 m_neg[kHT / 2], l_part[kHT / 2];    // per head: minus the running maximum, and its sum
+  float u = 0.f;                             // the unit of the scales
   int64_t n = 0;                             // live tiles
   float* ml = reinterpret_cast<float*>(sgen + C::OFF_SC);
   bool aborted = false;
@@ -597,15 +626,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int64_t k = (int64_t)t * kTS + sm_tid;
         if (sm_tid < kTS && k < p.topk) p.weights[row * p.w_sb + k] = 0.f;
       }
+    float2 qs[kHT / 2];
 #pragma unroll
-    for (int h = 0; h < kHT; ++h) {
-      m_run[h] = -INFINITY;
-      l_part[h] = 0.f;
+    for (int i = 0; i < kHT / 2; ++i) {
+      m_neg[i] = both(-kNone);
+      l_part[i] = both(0.f);
+      qs[i] = reinterpret_cast<const float2*>(sgen + C::OFF_QS)[kHT / 2 * hh + i];
     }
-    const float* unit = reinterpret_cast<const float*>(sgen + C::OFF_QS) + kHT * hh;
-    float qs[kHT];
-#pragma unroll
-    for (int h = 0; h < kHT; ++h) qs[h] = unit[h];
+    float u_inv = 0.f;
     for (;; ++n) {
       const int st = (int)(n % kStages), sb = (int)(n % C::kSBufs), pb = (int)(n & 1);
       bool ok = wait(bar(B_KVF + st), (uint32_t)((n / kStages) & 1));
@@ -614,9 +642,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!end) ok = ok && wait(bar(B_SF + sb), (uint32_t)((n / C::kSBufs) & 1));
       if (n == 0) {  // the unit of the scales, the same in every thread
         const float first = smax[st];
-        u = first > 0.f ? first : 1.f;
+        u = first > 0.f ? fmaxf(first, 1.17549435e-38f) : 1.f;  // 1 / u is finite
+        u_inv = 1.f / u;
       }
-      float x[kHT];
+      float2 x[kHT / 2], d[kHT / 2];  // scores, and over the running maximum
       float ratio = 0.f;  // scale in units, lr its log2
       float lr = -INFINITY;
       bool valid = false;
@@ -630,18 +659,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld<kHT>(ta + 2 * NH, pe);
         const float scale = sc[st * kTS + slot];
         valid = ((uint32_t)cmd[4 * st + qd] >> lane) & 1u;
-        ratio = scale / u;
+        ratio = scale * u_inv;
         lr = ptx::lg2(fabsf(ratio));
         ptx::tmem_wait_ld();
         ptx::tc_fence_before();
 #pragma unroll
-        for (int h = 0; h < kHT; ++h) {
-          const float q = fmaf(__uint_as_float(lo[h]), 0.0625f, __uint_as_float(hi[h]));
-          x[h] = valid ? fmaf(q * scale, qs[h], __uint_as_float(pe[h]) * p.scale_log2) : -INFINITY;
+        for (int i = 0; i < kHT / 2; ++i) {
+          const float2 q = fma2(pair(lo, i), both(0.0625f), pair(hi, i));
+          x[i] = fma2(mul2(q, both(scale)), qs[i], mul2(pair(pe, i), both(p.scale_log2)));
+        }
+        if (!valid) {
+#pragma unroll
+          for (int i = 0; i < kHT / 2; ++i) x[i] = both(-INFINITY);
         }
       } else {
 #pragma unroll
-        for (int h = 0; h < kHT; ++h) x[h] = -INFINITY;
+        for (int i = 0; i < kHT / 2; ++i) x[i] = both(-INFINITY);
       }
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar(B_SE + sb));
@@ -650,10 +683,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the same words; the words are written again two tiles later, behind the next tile's
       // barrier.
       const float tau = fminf(kTauQ8 - lr, kTauL);  // P = 2^(x + lr - m) and l's 2^(x - m) in range
-      uint32_t vote = ok && !aborted ? 0u : kFailed;
+      float top = kNone;
 #pragma unroll
-      for (int h = 0; h < kHT; ++h) vote |= x[h] > m_run[h] + tau ? kRise : 0u;
-      vote = __reduce_or_sync(0xffffffffu, vote);
+      for (int i = 0; i < kHT / 2; ++i) {
+        d[i] = add2(x[i], m_neg[i]);
+        top = fmaxf(top, fmaxf(d[i].x, d[i].y));
+      }
+      uint32_t vote = __reduce_or_sync(0xffffffffu, (ok && !aborted ? 0u : kFailed) | (top > tau ? kRise : 0u));
       uint32_t* words = reinterpret_cast<uint32_t*>(sgen + C::OFF_RED) + (hh * 2 + pb) * 4;
       if (lane == 0) words[qd] = vote;
       ptx::bar_sync(kSmBar + 2 + hh, kSmThreads / 2);
@@ -679,8 +715,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float un = smax[st];
           beta = u / un;
           lr += ptx::lg2(beta);
-          ratio *= beta;
           u = un;
+          u_inv = 1.f / u;
+          ratio *= beta;
         }
         // the maxima go through this tile's P buffer, whose last reader (PV) is done
         // (in the first term's rows of these heads, which only these warps write)
@@ -688,19 +725,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float over = fmaxf(lr, 8.f - kTauL);
 #pragma unroll
         for (int h = 0; h < kHT; ++h) {
-          const float v = ptx::warp_max(x[h] + over);
+          const float v = ptx::warp_max(((h & 1) ? x[h / 2].y : x[h / 2].x) + over);
           if (slot_ok && lane == 0) tops[qd * kHT + h] = v;
         }
         ptx::bar_sync(kSmBar + 2 + hh, kSmThreads / 2);
-        float alpha[kHT];
+        float2 alpha[kHT / 2];
 #pragma unroll
-        for (int h = 0; h < kHT; ++h) {
-          const float mn = fmaxf(m_run[h], fmaxf(tops[h], fmaxf(tops[kHT + h], tops[2 * kHT + h])));
-          const float a = m_run[h] == -INFINITY ? 0.f : ptx::ex2(m_run[h] - mn);
-          // l that is NaN while no score was a number stays so
-          l_part[h] = m_run[h] == -INFINITY ? l_part[h] : l_part[h] * a;
-          m_run[h] = mn;
-          alpha[h] = a * beta;
+        for (int i = 0; i < kHT / 2; ++i) {
+          const float2* t2 = reinterpret_cast<const float2*>(tops) + i;
+          const float2 a = t2[0], b = t2[kHT / 2], c = t2[kHT];
+          const float2 mn = make_float2(fmaxf(-m_neg[i].x, fmaxf(a.x, fmaxf(b.x, c.x))),
+                                        fmaxf(-m_neg[i].y, fmaxf(a.y, fmaxf(b.y, c.y))));
+          alpha[i] = make_float2(ptx::ex2(-m_neg[i].x - mn.x), ptx::ex2(-m_neg[i].y - mn.y));
+          l_part[i] = mul2(l_part[i], alpha[i]);
+          m_neg[i] = make_float2(-mn.x, -mn.y);
+          d[i] = add2(x[i], m_neg[i]);
+          alpha[i] = mul2(alpha[i], both(beta));
         }
         ptx::bar_sync(kSmBar + 2 + hh, kSmThreads / 2);  // the buffer is P's again
         if (n > 0 && !aborted) {
@@ -717,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int b = 0; b < kC; ++b) {
 #pragma unroll
               for (int h = 0; h < kHT; ++h)
-                r[b][h] = alpha[h] == 0.f ? 0u : __float_as_uint(__uint_as_float(r[b][h]) * alpha[h]);
+                r[b][h] = __float_as_uint(__uint_as_float(r[b][h]) * ((h & 1) ? alpha[h / 2].y : alpha[h / 2].x));
 #pragma unroll
               for (int k = 0; k < kHT; k += 8) ptx::tmem_st8(ta + (uint32_t)(NH * b + k), r[b] + k);
             }
@@ -735,24 +775,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (slot_ok) {
         // byte (row r, slot) of P: 32-slot planes of 32-byte rows, 32-byte swizzle
         uint8_t* pbuf = sgen + C::OFF_P + (int)(n % C::kPBufs) * C::kPB + qd * C::kPK;
-        const float scaled = valid ? ratio * kPScale : 0.f;
+        const float2 scaled = both(ratio * kPScale);
 #pragma unroll
-        for (int h = 0; h < kHT; h += 2) {
-          float v[2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float mr = m_run[h + k] == -INFINITY ? 0.f : m_run[h + k];
-            const float e = ptx::ex2(x[h + k] - mr);
-            l_part[h + k] += e;
-            v[k] = valid ? e * scaled : 0.f;
-          }
-          const int r = kHT * hh + h;
+        for (int i = 0; i < kHT / 2; ++i) {
+          const float2 e = make_float2(ptx::ex2(d[i].x), ptx::ex2(d[i].y));
+          l_part[i] = add2(l_part[i], e);
+          float2 v = mul2(e, scaled);
+          const int r = kHT * hh + 2 * i;
 #pragma unroll
           for (int term = 0; term < 3; ++term) {
-            const uint32_t b = to_e4m3x2(v[0], v[1]);
-            const float2 back = from_e4m3x2(b);
-            v[0] = (v[0] - back.x) * 16.f;
-            v[1] = (v[1] - back.y) * 16.f;
+            const uint32_t b = to_e4m3x2(v.x, v.y);
+            if (term < 2) v = fma2(from_e4m3x2(b), both(-16.f), mul2(v, both(16.f)));
             pbuf[sw32_byte(term * NH + r, lane)] = (uint8_t)b;
             pbuf[sw32_byte(term * NH + r + 1, lane)] = (uint8_t)(b >> 8);
           }
@@ -761,7 +794,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int64_t at = (row * G + group) * p.ntiles + split + n * S;
           float* s = p.scores + (at * NH + kHT * hh) * kTS + slot;
 #pragma unroll
-          for (int h = 0; h < kHT; ++h) s[h * kTS] = x[h];
+          for (int i = 0; i < kHT / 2; ++i) {
+            s[2 * i * kTS] = x[i].x;
+            s[(2 * i + 1) * kTS] = x[i].y;
+          }
           if (threadIdx.x == 32 * kSm0) p.tiles[at] = tile;
         }
       }
@@ -780,7 +816,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* red = reinterpret_cast<float*>(sgen + C::OFF_P);  // [half][quadrant][kHT]
 #pragma unroll
     for (int h = 0; h < kHT; ++h) {
-      float v = l_part[h];
+      float v = (h & 1) ? l_part[h / 2].y : l_part[h / 2].x;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
       if (lane == 0 && slot_ok) red[(hh * 3 + qd) * kHT + h] = v;
@@ -790,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int h = 0; h < kHT; ++h) {
         const float* r3 = red + hh * 3 * kHT + h;
-        ml[kHT * hh + h] = m_run[h];
+        ml[kHT * hh + h] = -((h & 1) ? m_neg[h / 2].y : m_neg[h / 2].x);
         ml[NH + kHT * hh + h] = (r3[0] + r3[kHT]) + r3[2 * kHT];
       }
       ml[2 * NH] = u;
