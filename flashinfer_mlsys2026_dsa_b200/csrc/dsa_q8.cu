@@ -554,13 +554,16 @@ int prepare_device() {
   return n;
 }
 
-// CTAs per (row, head group).
-int choose_splits(int64_t units, int groups, int ntiles, int sms) {
+// CTAs per (row, head group).  Per CTA about 7 us are spent outside the tiles (first gather, merge)
+// and 1.4 us (16 heads) or 1.75 us (32) per tile; a call whose units do not fill the SMs splits
+// them while that shortens the longest CTA.
+int choose_splits(int64_t units, int nh, int groups, int ntiles, int sms) {
+  const double tile = nh == 16 ? 1.4 : 1.75;
   int best = 1;
   double best_cost = 0;
   for (int s = 1; s * groups <= kMaxCluster; s *= 2) {
     const int64_t waves = (units * s + sms - 1) / sms;
-    const double cost = (double)waves * (2.5 + (s > 1 ? 1.5 : 0.0) + 1.4 * ((ntiles + s - 1) / s));
+    const double cost = (double)waves * ((s > 1 ? 8.0 : 7.0) + tile * ((ntiles + s - 1) / s));
     if (s == 1 || cost < best_cost) {
       best = s;
       best_cost = cost;
@@ -646,9 +649,13 @@ extern "C" int dsa_sparse_mla_decode_q8(
   p.err = static_cast<uint32_t*>(workspace);
   const int sms = q8::prepare_device();
   if (sms <= 0) return DSA_ERR_CUDA;
-  const int64_t units = num_tokens * p.groups;
-  p.splits = q8::choose_splits(units, p.groups, p.ntiles, sms);
-  const int64_t grid = units * p.splits;
+  p.units = num_tokens * p.groups;
+  p.splits = q8::choose_splits(p.units, nh, p.groups, p.ntiles, sms);
+  // The CTAs of a row form a cluster where they have something to add up: a unit's splits, or
+  // the groups' weights.  Otherwise at most one CTA per SM takes unit after unit.
+  p.clustered = p.splits > 1 || (weights != nullptr && p.groups > 1);
+  const int cluster = p.clustered ? p.splits * p.groups : 1;
+  const int64_t grid = p.clustered ? p.units * p.splits : (p.units < sms ? p.units : sms);
   if (grid > INT32_MAX) return DSA_ERR_INVALID_ARGUMENT;
   // gathers of single slots: 128-byte boxes of one row
   CUtensorMap m_ckv, m_kpe;
@@ -673,7 +680,7 @@ extern "C" int dsa_sparse_mla_decode_q8(
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[2] = {q8::pdl_attr(), {}};
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)(p.splits * p.groups);
+  attr[1].val.clusterDim.x = (unsigned)cluster;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;

@@ -61,8 +61,11 @@ struct AttendParams {
   int32_t* tiles;   // weights only: the tiles a CTA ran, in the places of its scores
   int32_t topk;
   int32_t ntiles;
+  int64_t units;    // rows x G
   int32_t splits;   // S
-  int32_t groups;   // G
+  int32_t groups;   // G, a power of two
+  int32_t clustered;  // one unit per CTA, the S G CTAs of a row in a cluster; else CTA c takes
+                      // the units c, c + grid, ...
   bool out8;        // output rows are 8-byte aligned
   float scale_log2;
   uint32_t* err;
@@ -78,7 +81,7 @@ constexpr int kThreads = 512;
 constexpr int kProdWarps = 5;
 constexpr int kScore = 5, kPv = 6, kKeeper = 7, kSm0 = 8;
 constexpr int kSmWarps = 8, kSmThreads = 256;
-constexpr uint32_t kSmBar = 1, kQBar = 2;
+constexpr uint32_t kSmBar = 1;  // all softmax warps; + 2 + half: those of a half of the heads
 constexpr float kTauQ8 = 7.f;         // log2: how far a weighted score may pass the running maximum
 constexpr float kTauL = 60.f;         // the same for a score alone: its exponential stays finite
 constexpr float kTauU = 16.f;         // how far a scale may pass the unit
@@ -100,14 +103,16 @@ struct Cfg {
   static constexpr int OFF_QP = OFF_Q + 4 * kQBlk;
   static constexpr int OFF_P = OFF_QP + NH * 128;
   static constexpr int OFF_BAR = OFF_P + kPBufs * kPB;
-  static constexpr int OFF_MISC = OFF_BAR + 256;   // [0] TMEM base, [2] abort, [3] drain, [4] end tile
-  static constexpr int OFF_CMD = OFF_MISC + 32;    // [stage][4]: three validity words, the tile (-1: end)
+  static constexpr int OFF_MISC = OFF_BAR + 256;   // [0] TMEM base, [2] abort, [3] drain, [8..15] end
+                                                   // tiles of the units in flight
+  static constexpr int OFF_CMD = OFF_MISC + 64;    // [stage][4]: three validity words, the tile (-1: end)
   static constexpr int OFF_SMAX = OFF_CMD + kStages * 16;  // [stage] largest scale of the tile
   static constexpr int OFF_QS = OFF_SMAX + 16;     // [NH] score units per query row
   static constexpr int OFF_SC = OFF_QS + NH * 4;   // [stage][96] scales; at the end kMl floats
   static constexpr int kMl = 2 * NH + 1;           // a CTA's m, L and u, for the merge
   static constexpr int OFF_RED = OFF_SC + kStages * kTS * 4;  // [half][2 buffers][4 warps] votes
-  static constexpr int SMEM_BYTES = OFF_RED + 16 * 4;
+  static constexpr int OFF_LSE = OFF_RED + 16 * 4;  // [NH], for the weights
+  static constexpr int SMEM_BYTES = OFF_LSE + NH * 4;
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
   static_assert(kMl <= kStages * kTS, "m, L and u in the scales' place");
   // after the last tile, in the stages' place: this CTA's O, then the merge's table
@@ -123,12 +128,13 @@ struct Cfg {
 
 enum : int {
   B_KVF = 0,                 // [stage] slots landed, scales, validity and tile number written
-  B_KVE = B_KVF + kStages,   // [stage] free again: the tile's PV is done
+  B_KVE = B_KVF + kStages,   // [stage] free again: PV done, and its words read by score and softmax
   B_SF = B_KVE + kStages,    // [2] score written
   B_SE = B_SF + 2,           // [2] score read
   B_PF = B_SE + 2,           // [2] P written (and O rescaled)
   B_PD = B_PF + 2,           // [2] PV done
-  B_DRAIN = B_PD + 2,        // [2] used only when an issuer stops early
+  B_QF = B_PD + 2,           // a unit's queries staged
+  B_DRAIN = B_QF + 1,        // [2] used only when an issuer stops early
   B_COUNT = B_DRAIN + 2
 };
 static_assert(B_COUNT * 8 <= 256, "barrier block");
@@ -161,6 +167,19 @@ __device__ __forceinline__ float ldg_now(const float* p) {
 __device__ __forceinline__ uint32_t sw128_byte(int r, int b) {
   return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + (((b >> 4) ^ (r & 7)) << 4) + (b & 15));
 }
+
+// The units, (row, head group) pairs, of this CTA.
+struct Units {
+  int64_t first, step;
+  int shift;  // log2(G)
+  __device__ __forceinline__ explicit Units(const AttendParams& p) {
+    shift = __ffs(p.groups) - 1;
+    const unsigned per = (unsigned)(p.splits * p.groups);
+    first = p.clustered ? (int64_t)(blockIdx.x / per) * p.groups + blockIdx.x % per / (unsigned)p.splits
+                        : (int64_t)blockIdx.x;
+    step = p.clustered ? p.units : (int64_t)gridDim.x;
+  }
+};
 
 // ---------------------------------------------------------------- index entries
 //
@@ -224,7 +243,7 @@ struct Entries {
 // the tile number, so all agree on the live tiles.
 template <int NH>
 __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap* map, int blk,
-                                        int64_t row, int split, int lane, uint32_t sbase,
+                                        const Units& units, int split, int lane, uint32_t sbase,
                                         uint8_t* sgen, const Waiter& wait) {
   using C = Cfg<NH>;
   const uint32_t bar0 = sbase + (uint32_t)C::OFF_BAR;
@@ -234,62 +253,72 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
   const int col = blk < 4 ? 128 * blk : 0;
   const bool el = ptx::elect_one();
   const uint64_t policy = ptx::policy_evict_first();
-  Entries<4> in{p, p.idx + row * p.idx_sb, row, 4 * lane, 1};
-  int64_t t = split;
-  in.start(t, has);
   bool ok = true;
-  int64_t n = 0;  // live tiles
+  int64_t n = 0;  // stages filled
   int st = 0;
   uint32_t phase = 0;
-  // misc[4] is the keeper's to lower at any time: the lanes agree on one reading
-  for (; t < __shfl_sync(0xffffffffu, (int)misc[4], 0); t += p.splits) {
-    const int4 r = make_int4(in.slot0[0], in.slot0[1], in.slot0[2], in.slot0[3]);
-    const bool live = __any_sync(0xffffffffu, r.x >= 0 || r.y >= 0 || r.z >= 0 || r.w >= 0);
-    in.prefetch(t, has);
-    if (live) {
-      ok = __all_sync(0xffffffffu, wait(bar(B_KVE + st), phase ^ 1u));
-      if (!ok) break;
-      const uint32_t full = bar(B_KVF + st);
-      const uint32_t dst = sbase + (uint32_t)(st * kStageB + blk * kRB);
-      if (el) ptx::mbar_arrive_expect_tx(full, (uint32_t)kRB);
-      // a slot that is none lies outside the tensor map: the copy fills its row with zeros, so
-      // that PV reads 0 * 0 there
+  int k = 0;
+  for (int64_t un = units.first; ok && un < p.units; un += units.step, ++k) {
+    const int64_t row = un >> units.shift;
+    Entries<4> in{p, p.idx + row * p.idx_sb, row, 4 * lane, 1};
+    in.start(split, has);
+    // the end tile is the keeper's to lower at any time: the lanes agree on one reading
+    for (int64_t t = split; t < __shfl_sync(0xffffffffu, (int)misc[8 + (k & 7)], 0); t += p.splits) {
+      const int4 r = make_int4(in.slot0[0], in.slot0[1], in.slot0[2], in.slot0[3]);
+      const bool live = __any_sync(0xffffffffu, r.x >= 0 || r.y >= 0 || r.z >= 0 || r.w >= 0);
+      in.prefetch(t, has);
+      if (live) {
+        ok = __all_sync(0xffffffffu, wait(bar(B_KVE + st), phase ^ 1u));
+        if (!ok) break;
+        const uint32_t full = bar(B_KVF + st);
+        const uint32_t dst = sbase + (uint32_t)(st * kStageB + blk * kRB);
+        if (el) ptx::mbar_arrive_expect_tx(full, (uint32_t)kRB);
+        // a slot that is none lies outside the tensor map: the copy fills its row with zeros, so
+        // that PV reads 0 * 0 there
 #pragma unroll
-      for (int g = 0; g < kTS / 4; ++g) {
-        const int4 s = make_int4(__shfl_sync(0xffffffffu, r.x, g), __shfl_sync(0xffffffffu, r.y, g),
-                                 __shfl_sync(0xffffffffu, r.z, g), __shfl_sync(0xffffffffu, r.w, g));
-        if (el) ptx::tma_gather4(dst + (uint32_t)(g * 512), map, col, s, full, policy);
+        for (int g = 0; g < kTS / 4; ++g) {
+          const int4 s = make_int4(__shfl_sync(0xffffffffu, r.x, g), __shfl_sync(0xffffffffu, r.y, g),
+                                   __shfl_sync(0xffffffffu, r.z, g), __shfl_sync(0xffffffffu, r.w, g));
+          if (el) ptx::tma_gather4(dst + (uint32_t)(g * 512), map, col, s, full, policy);
+        }
+        __syncwarp();
+        ++n;
+        if (++st == kStages) {
+          st = 0;
+          phase ^= 1u;
+        }
       }
-      __syncwarp();
-      ++n;
-      if (++st == kStages) {
-        st = 0;
-        phase ^= 1u;
-      }
+      in.advance();
     }
-    in.advance();
+    if (!ok) break;
+    // the unit's end: a stage without slots
+    ok = __all_sync(0xffffffffu, wait(bar(B_KVE + st), phase ^ 1u));
+    if (!ok) break;
+    if (el) ptx::mbar_arrive(bar(B_KVF + st));
+    ++n;
+    if (++st == kStages) {
+      st = 0;
+      phase ^= 1u;
+    }
   }
-  // the end: one more stage, without slots
-  if (el) {
-    ok = ok && wait(bar(B_KVE + st), phase ^ 1u);
-    if (ok) {
-      ptx::mbar_arrive(bar(B_KVF + st));
-    } else {
-      // this warp's copies land before the CTA leaves
-      const Waiter drain{misc + 3, p.err, p.wait_cycles};
-      for (int64_t i = n - 1; i >= 0 && i >= n - kStages; --i)
-        drain(bar(B_KVF + (int)(i % kStages)), (uint32_t)((i / kStages) & 1));
-    }
+  if (!ok && el) {
+    // this warp's copies land before the CTA leaves
+    const Waiter drain{misc + 3, p.err, p.wait_cycles};
+    for (int64_t i = n - 1; i >= 0 && i >= n - kStages; --i)
+      drain(bar(B_KVF + (int)(i % kStages)), (uint32_t)((i / kStages) & 1));
   }
   __syncwarp();
 }
 
-// The keeper (warp 7).  First the tile behind the row's last entry that is not padding, found
-// from the end in steps of 512 entries, so that nobody walks a short row's padding; then,
-// tile by tile, lane l the entries l, l + 32 and l + 64: scales, validity, the tile's number.
+// The keeper (warp 7).  Per unit first the tile behind the row's last entry that is not
+// padding, found from the end in steps of 512 entries, so that nobody walks a short row's padding;
+// then, tile by tile, lane l the entries l, l + 32 and l + 64: scales, validity, the tile's
+// number.  The end tiles have eight places; the gatherers are at most three stages, so at most
+// three units, ahead of the keeper, which opens a unit's place four units before it.
 template <int NH>
-__device__ __forceinline__ void keep_books(const AttendParams& p, int64_t row, int split, int lane,
-                                           uint32_t sbase, uint8_t* sgen, const Waiter& wait) {
+__device__ __forceinline__ void keep_books(const AttendParams& p, const Units& units, int split,
+                                           int lane, uint32_t sbase, uint8_t* sgen,
+                                           const Waiter& wait) {
   using C = Cfg<NH>;
   constexpr int kE = kTS / 32;
   const uint32_t bar0 = sbase + (uint32_t)C::OFF_BAR;
@@ -298,66 +327,75 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, int64_t row, i
   volatile int* cmd = reinterpret_cast<volatile int*>(sgen + C::OFF_CMD);
   volatile float* smax = reinterpret_cast<volatile float*>(sgen + C::OFF_SMAX);
   float* sc = reinterpret_cast<float*>(sgen + C::OFF_SC);
-  Entries<kE> in{p, p.idx + row * p.idx_sb, row, lane, 32};
-  int64_t t = split;
-  in.start(t, true);
-  int end = 0;
-  for (int hi = p.topk; hi > 0 && end == 0; hi -= 512) {
-    int last = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int k = hi - 512 + 32 * i + lane;
-      if (k >= 0 && __ldg(in.ir + k) != -1) last = k + 1;
-    }
-    end = __reduce_max_sync(0xffffffffu, last);
-  }
-  end = (end + kTS - 1) / kTS;
-  if (lane == 0) misc[4] = (uint32_t)end;
   bool ok = true;
   int st = 0;
   uint32_t phase = 0;
-  for (; t < end; t += p.splits) {
-    uint32_t w[kE], any = 0;
-    float scale[kE], big = 0.f;
-    bool bad = false;
+  int unit = 0;
+  for (int64_t un = units.first; ok && un < p.units; un += units.step, ++unit) {
+    const int64_t row = un >> units.shift;
+    Entries<kE> in{p, p.idx + row * p.idx_sb, row, lane, 32};
+    if (lane == 0) misc[8 + ((unit + 4) & 7)] = (uint32_t)p.ntiles;
+    in.start(split, true);
+    int end = 0;
+    for (int hi = p.topk; hi > 0 && end == 0; hi -= 512) {
+      int last = 0;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      const int slot = in.slot0[e];
-      w[e] = __ballot_sync(0xffffffffu, slot >= 0);
-      any |= w[e];
-      bad |= slot == -2;
-      scale[e] = slot >= 0 ? ldg_now(p.cache.scale + (slot >> p.cache.block_shift)) : 0.f;
+      for (int i = 0; i < 16; ++i) {
+        const int k = hi - 512 + 32 * i + lane;
+        if (k >= 0 && __ldg(in.ir + k) != -1) last = k + 1;
+      }
+      end = __reduce_max_sync(0xffffffffu, last);
     }
-    if (bad) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
-    in.prefetch(t, true);
-    if (any != 0u) {
-      if (lane == 0) ok = wait(bar(B_KVE + st), phase ^ 1u);
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-      if (!ok) break;
+    end = (end + kTS - 1) / kTS;
+    if (lane == 0) misc[8 + (unit & 7)] = (uint32_t)end;
+    for (int64_t t = split; t < end; t += p.splits) {
+      uint32_t w[kE], any = 0;
+      float scale[kE], big = 0.f;
+      bool bad = false;
 #pragma unroll
       for (int e = 0; e < kE; ++e) {
-        sc[st * kTS + 32 * e + lane] = scale[e];
-        big = fmaxf(big, fabsf(scale[e]));
+        const int slot = in.slot0[e];
+        w[e] = __ballot_sync(0xffffffffu, slot >= 0);
+        any |= w[e];
+        bad |= slot == -2;
+        scale[e] = slot >= 0 ? ldg_now(p.cache.scale + (slot >> p.cache.block_shift)) : 0.f;
       }
-      big = ptx::warp_max(big);
-      if (lane == 0) {
+      if (bad) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
+      in.prefetch(t, true);
+      if (any != 0u) {
+        ok = __all_sync(0xffffffffu, wait(bar(B_KVE + st), phase ^ 1u));
+        if (!ok) break;
 #pragma unroll
-        for (int e = 0; e < kE; ++e) cmd[4 * st + e] = (int)w[e];
-        cmd[4 * st + 3] = (int)t;
-        smax[st] = big;
+        for (int e = 0; e < kE; ++e) {
+          sc[st * kTS + 32 * e + lane] = scale[e];
+          big = fmaxf(big, fabsf(scale[e]));
+        }
+        big = ptx::warp_max(big);
+        if (lane == 0) {
+#pragma unroll
+          for (int e = 0; e < kE; ++e) cmd[4 * st + e] = (int)w[e];
+          cmd[4 * st + 3] = (int)t;
+          smax[st] = big;
+        }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(B_KVF + st));
+        if (++st == kStages) {
+          st = 0;
+          phase ^= 1u;
+        }
       }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar(B_KVF + st));
-      if (++st == kStages) {
-        st = 0;
-        phase ^= 1u;
-      }
+      in.advance();
     }
-    in.advance();
-  }
-  if (lane == 0 && ok && wait(bar(B_KVE + st), phase ^ 1u)) {
-    cmd[4 * st + 3] = -1;
-    ptx::mbar_arrive(bar(B_KVF + st));
+    if (!ok) break;
+    ok = __all_sync(0xffffffffu, wait(bar(B_KVE + st), phase ^ 1u));
+    if (ok && lane == 0) {
+      cmd[4 * st + 3] = -1;
+      ptx::mbar_arrive(bar(B_KVF + st));
+    }
+    if (++st == kStages) {
+      st = 0;
+      phase ^= 1u;
+    }
   }
   __syncwarp();
 }
@@ -447,6 +485,18 @@ __device__ __forceinline__ float2 pair(const uint32_t* r, int i) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
+// An entry's probability summed over the heads, from its scores (kTS apart) and their lse.
+template <int NH>
+__device__ __forceinline__ float head_sum(const float* scores, const float* lse) {
+  float w = 0.f;
+#pragma unroll 8
+  for (int h = 0; h < NH; ++h) {
+    const float x = scores[h * kTS];
+    w += x == -INFINITY ? 0.f : ptx::ex2(x - lse[h]);
+  }
+  return w;
+}
+
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -478,15 +528,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto bar = [&](int k) { return bar0 + 8u * (uint32_t)k; };
 
   const int S = p.splits, G = p.groups;
-  const int rank = (int)blockIdx.x % (S * G);
-  const int64_t row = blockIdx.x / (unsigned)(S * G);
-  const int group = rank / S, split = rank % S;
-  const int h0 = group * NH;  // first head of the group
+  const Units units(p);
+  const int split = p.clustered ? (int)(blockIdx.x % (unsigned)S) : 0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       ptx::mbar_init(bar(B_KVF + s), kProdWarps + 1);  // the gatherers (with their bytes) and the keeper
-      ptx::mbar_init(bar(B_KVE + s), 1);
+      ptx::mbar_init(bar(B_KVE + s), 3);  // PV, score issuer, softmax
     }
     for (int b = 0; b < 2; ++b) {
       ptx::mbar_init(bar(B_SF + b), 1);
@@ -497,7 +545,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     misc[2] = 0;
     misc[3] = 0;
-    misc[4] = (uint32_t)p.ntiles;
+    for (int i = 0; i < 8; ++i) misc[8 + i] = (uint32_t)p.ntiles;
+    ptx::mbar_init(bar(B_QF), kSmWarps);
     ptx::fence_mbar_init();
     ptx::prefetch_tmap(&tm_ckv);
     ptx::prefetch_tmap(&tm_kpe);
@@ -515,30 +564,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Waiter wait{misc + 2, p.err, p.wait_cycles};
   const Waiter spin{misc + 2, p.err, p.wait_cycles, true};
 
-  // softmax state, kept past the loop for the merge
+  // softmax state, kept past the loop for the merge of a clustered call's single unit
   const int qd = warp & 3;                   // TMEM lane quadrant: slots 32 qd .. 32 qd + 31
   const int hh = (warp - kSm0) >> 2;         // heads kHT hh .. kHT hh + kHT - 1 of the group
   const uint32_t lane_base = (uint32_t)(32 * qd) << 16;
   float2 m_neg[kHT / 2], l_part[kHT / 2];    // per head: minus the running maximum, and its sum
   float u = 0.f;                             // the unit of the scales
-  int64_t n = 0;                             // live tiles
+  int64_t row = 0;
+  int group = 0;
+  int live = 0;                              // the unit's tiles
   float* ml = reinterpret_cast<float*>(sgen + C::OFF_SC);
   bool aborted = false;
 
-  if (warp < kProdWarps) {
-    produce<NH>(p, warp < 4 ? &tm_ckv : &tm_kpe, warp, row, split, lane, sbase, sgen, wait);
-  } else if (warp == kKeeper) {
-    keep_books<NH>(p, row, split, lane, sbase, sgen, wait);
-  } else {
-    constexpr int kQWarps = kSmWarps + 2;
-    float* qs = reinterpret_cast<float*>(sgen + C::OFF_QS);
-    for (int h = warp < kSm0 ? kSmWarps + warp - kScore : warp - kSm0; h < NH; h += kQWarps) {
-      const float unit = stage_query<NH>(p, row, h0 + h, h, lane, sgen);
-      if (lane == 0) qs[h] = unit;
-    }
-    ptx::fence_proxy_async_smem();
-    ptx::bar_sync(kQBar, 32 * kQWarps);
-  }
+  if (warp < kProdWarps)
+    produce<NH>(p, warp < 4 ? &tm_ckv : &tm_kpe, warp, units, split, lane, sbase, sgen, wait);
+  else if (warp == kKeeper)
+    keep_books<NH>(p, units, split, lane, sbase, sgen, wait);
   if (warp == kScore) {
     // ------------------------------------------------------------------ score issuer
     constexpr uint32_t kId = idesc_e4m3(128, 2 * NH, false), kIdPe = idesc_bf16(128, NH, false);
@@ -547,29 +588,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t dqp = desc(sbase + (uint32_t)C::OFF_QP, 16, 1024, kSw128);
     const bool el = ptx::elect_one();  // warp-uniform loops around one issuing thread
     bool ok = true;
-    for (int64_t i = 0;; ++i) {
-      const int st = (int)(i % kStages), sb = (int)(i % C::kSBufs);
-      ok = __all_sync(0xffffffffu, spin(bar(B_KVF + st), (uint32_t)((i / kStages) & 1)));
-      if (!ok || __any_sync(0xffffffffu, cmd[4 * st + 3] < 0)) break;
-      ok = __all_sync(0xffffffffu, spin(bar(B_SE + sb), (uint32_t)(((i / C::kSBufs) & 1) ^ 1)));
-      if (!ok) break;
-      ptx::tc_fence_after();
-      const uint32_t d = tmem + (uint32_t)(C::kSCols * sb);
-      const uint64_t ko = (uint64_t)((st * kStageB) >> 4);
-      if (el) {
+    int64_t c = 0, i = 0;  // stages, tiles
+    for (int64_t un = units.first, k = 0; ok && un < p.units; un += units.step, ++k) {
+      ok = __all_sync(0xffffffffu, spin(bar(B_QF), (uint32_t)(k & 1)));
+      for (; ok; ++i) {
+        const int st = (int)(c % kStages), sb = (int)(i % C::kSBufs);
+        ok = __all_sync(0xffffffffu, spin(bar(B_KVF + st), (uint32_t)((c / kStages) & 1)));
+        if (!ok) break;
+        const bool end = __any_sync(0xffffffffu, cmd[4 * st + 3] < 0);
+        if (el) ptx::mbar_arrive(bar(B_KVE + st));
+        ++c;
+        if (end) break;
+        ok = __all_sync(0xffffffffu, spin(bar(B_SE + sb), (uint32_t)(((i / C::kSBufs) & 1) ^ 1)));
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(C::kSCols * sb);
+        const uint64_t ko = (uint64_t)((st * kStageB) >> 4);
+        if (el) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              ptx::umma_f8(d, dk + ko + (uint64_t)((j * kRB + ks * 32) >> 4),
+                           dq + (uint64_t)((j * C::kQBlk + ks * 32) >> 4), kId, (j | ks) ? 1u : 0u);
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
-            ptx::umma_f8(d, dk + ko + (uint64_t)((j * kRB + ks * 32) >> 4),
-                         dq + (uint64_t)((j * C::kQBlk + ks * 32) >> 4), kId, (j | ks) ? 1u : 0u);
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-          ptx::umma_bf16(d + 2 * NH, dk + ko + (uint64_t)((4 * kRB + ks * 32) >> 4),
-                         dqp + (uint64_t)((ks * 32) >> 4), kIdPe, ks ? 1u : 0u);
-        ptx::umma_commit(bar(B_SF + sb));
+            ptx::umma_bf16(d + 2 * NH, dk + ko + (uint64_t)((4 * kRB + ks * 32) >> 4),
+                           dqp + (uint64_t)((ks * 32) >> 4), kIdPe, ks ? 1u : 0u);
+          ptx::umma_commit(bar(B_SF + sb));
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
     if (!ok && el) {
       const Waiter drain{misc + 3, p.err, p.wait_cycles};
@@ -584,27 +633,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t dp = desc(sbase + (uint32_t)C::OFF_P, 16, 256, kSw32);
     const bool el = ptx::elect_one();
     bool ok = true;
-    for (int64_t i = 0;; ++i) {
-      const int st = (int)(i % kStages), pb = (int)(i & 1);
-      ok = __all_sync(0xffffffffu, spin(bar(B_KVF + st), (uint32_t)((i / kStages) & 1)));
-      if (!ok || __any_sync(0xffffffffu, cmd[4 * st + 3] < 0)) break;
-      ok = __all_sync(0xffffffffu, spin(bar(B_PF + pb), (uint32_t)((i >> 1) & 1)));
-      if (!ok) break;
-      ptx::tc_fence_after();
-      const uint64_t vo = (uint64_t)((st * kStageB) >> 4);
-      const uint64_t po = (uint64_t)(((int)(i % C::kPBufs) * C::kPB) >> 4);
-      if (el) {
+    int64_t c = 0, i = 0;  // stages, tiles
+    for (int64_t un = units.first; ok && un < p.units; un += units.step) {
+      for (bool first = true; ok; ++i, first = false) {
+        const int st = (int)(c % kStages), pb = (int)(i & 1);
+        ok = __all_sync(0xffffffffu, spin(bar(B_KVF + st), (uint32_t)((c / kStages) & 1)));
+        if (!ok) break;
+        ++c;
+        if (__any_sync(0xffffffffu, cmd[4 * st + 3] < 0)) {
+          if (el) ptx::mbar_arrive(bar(B_KVE + st));
+          break;
+        }
+        ok = __all_sync(0xffffffffu, spin(bar(B_PF + pb), (uint32_t)((i >> 1) & 1)));
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const uint64_t vo = (uint64_t)((st * kStageB) >> 4);
+        const uint64_t po = (uint64_t)(((int)(i % C::kPBufs) * C::kPB) >> 4);
+        if (el) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int ks = 0; ks < kTS / 32; ++ks)
-            ptx::umma_f8(tmem + (uint32_t)(C::O_COL + 3 * NH * j),
-                         dv + vo + (uint64_t)((j * kRB + ks * 4096) >> 4),
-                         dp + po + (uint64_t)((ks * C::kPK) >> 4), kId, (i > 0 || ks > 0) ? 1u : 0u);
-        ptx::umma_commit(bar(B_KVE + st));
-        ptx::umma_commit(bar(B_PD + pb));
+            for (int ks = 0; ks < kTS / 32; ++ks)
+              ptx::umma_f8(tmem + (uint32_t)(C::O_COL + 3 * NH * j),
+                           dv + vo + (uint64_t)((j * kRB + ks * 4096) >> 4),
+                           dp + po + (uint64_t)((ks * C::kPK) >> 4), kId, (!first || ks > 0) ? 1u : 0u);
+          ptx::umma_commit(bar(B_KVE + st));
+          ptx::umma_commit(bar(B_PD + pb));
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
     if (!ok && el) {
       const Waiter drain{misc + 3, p.err, p.wait_cycles};
@@ -619,232 +676,310 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float* sc = reinterpret_cast<const float*>(sgen + C::OFF_SC);
     const volatile float* smax = reinterpret_cast<const volatile float*>(sgen + C::OFF_SMAX);
     const int sm_tid = (int)threadIdx.x - 32 * kSm0;
-    // entries of tiles that turn out to hold nothing get no other value (group g's CTA writes
-    // the row's tiles with (tile / S) % G == g, here and at the end)
-    if (p.weights != nullptr)
-      for (int t = split + S * group; t < p.ntiles; t += S * G) {
-        const int64_t k = (int64_t)t * kTS + sm_tid;
-        if (sm_tid < kTS && k < p.topk) p.weights[row * p.w_sb + k] = 0.f;
-      }
-    float2 qs[kHT / 2];
-#pragma unroll
-    for (int i = 0; i < kHT / 2; ++i) {
-      m_neg[i] = both(-kNone);
-      l_part[i] = both(0.f);
-      qs[i] = reinterpret_cast<const float2*>(sgen + C::OFF_QS)[kHT / 2 * hh + i];
-    }
-    float u_inv = 0.f;
-    for (;; ++n) {
-      const int st = (int)(n % kStages), sb = (int)(n % C::kSBufs), pb = (int)(n & 1);
-      bool ok = wait(bar(B_KVF + st), (uint32_t)((n / kStages) & 1));
-      const int tile = cmd[4 * st + 3];
-      const bool end = ok && tile < 0;
-      if (!end) ok = ok && wait(bar(B_SF + sb), (uint32_t)((n / C::kSBufs) & 1));
-      if (n == 0) {  // the unit of the scales, the same in every thread
-        const float first = smax[st];
-        u = first > 0.f ? fmaxf(first, 1.17549435e-38f) : 1.f;  // 1 / u is finite
-        u_inv = 1.f / u;
-      }
-      float2 x[kHT / 2], d[kHT / 2];  // scores, and over the running maximum
-      float ratio = 0.f;  // scale in units, lr its log2
-      float lr = -INFINITY;
-      bool valid = false;
-      const bool grow = !end && smax[st] > kTauU * u;
-      if (slot_ok && __all_sync(0xffffffffu, ok && !end)) {  // warp-uniform
-        ptx::tc_fence_after();
-        uint32_t hi[kHT], lo[kHT], pe[kHT];
-        const uint32_t ta = tmem + lane_base + (uint32_t)(C::kSCols * sb + kHT * hh);
-        tmem_ld<kHT>(ta, hi);
-        tmem_ld<kHT>(ta + NH, lo);
-        tmem_ld<kHT>(ta + 2 * NH, pe);
-        const float scale = sc[st * kTS + slot];
-        valid = ((uint32_t)cmd[4 * st + qd] >> lane) & 1u;
-        ratio = scale * u_inv;
-        lr = ptx::lg2(fabsf(ratio));
-        ptx::tmem_wait_ld();
-        ptx::tc_fence_before();
-#pragma unroll
-        for (int i = 0; i < kHT / 2; ++i) {
-          const float2 q = fma2(pair(lo, i), both(0.0625f), pair(hi, i));
-          x[i] = fma2(mul2(q, both(scale)), qs[i], mul2(pair(pe, i), both(p.scale_log2)));
-        }
-        if (!valid) {
-#pragma unroll
-          for (int i = 0; i < kHT / 2; ++i) x[i] = both(-INFINITY);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kHT / 2; ++i) x[i] = both(-INFINITY);
-      }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar(B_SE + sb));
-      // Whether a running maximum or the unit has to rise, or a wait failed, through one barrier
-      // of the four warps that share the heads.  Their decisions are the same, as they read
-      // the same words; the words are written again two tiles later, behind the next tile's
-      // barrier.
-      const float tau = fminf(kTauQ8 - lr, kTauL);  // P = 2^(x + lr - m) and l's 2^(x - m) in range
-      float top = kNone;
-#pragma unroll
-      for (int i = 0; i < kHT / 2; ++i) {
-        d[i] = add2(x[i], m_neg[i]);
-        top = fmaxf(top, fmaxf(d[i].x, d[i].y));
-      }
-      uint32_t vote = __reduce_or_sync(0xffffffffu, (ok && !aborted ? 0u : kFailed) | (top > tau ? kRise : 0u));
-      uint32_t* words = reinterpret_cast<uint32_t*>(sgen + C::OFF_RED) + (hh * 2 + pb) * 4;
-      if (lane == 0) words[qd] = vote;
-      ptx::bar_sync(kSmBar + 2 + hh, kSmThreads / 2);
-      {
-        const uint4 v = *reinterpret_cast<const uint4*>(words);
-        vote = v.x | v.y | v.z | v.w;
-      }
-      if (vote & kFailed) {
-        aborted = true;
-        break;
-      }
-      if (end) break;
-      if (vote != 0u || grow) {
-        // Rare past the first tile: raise the maxima to this tile's, the unit to its largest
-        // scale, and bring l and O to them.
-        if (n > 0) {
-          const bool wok = wait(bar(B_PD + (int)((n - 1) & 1)), (uint32_t)(((n - 1) >> 1) & 1));
-          if (!__all_sync(0xffffffffu, wok)) aborted = true;
-          ptx::tc_fence_after();
-        }
-        float beta = 1.f;
-        if (grow) {
-          const float un = smax[st];
-          beta = u / un;
-          lr += ptx::lg2(beta);
-          u = un;
-          u_inv = 1.f / u;
-          ratio *= beta;
-        }
-        // the maxima go through this tile's P buffer, whose last reader (PV) is done
-        // (in the first term's rows of these heads, which only these warps write)
-        float* tops = reinterpret_cast<float*>(sgen + C::OFF_P + (int)(n % C::kPBufs) * C::kPB + hh * kHT * 32);
-        const float over = fmaxf(lr, 8.f - kTauL);
-#pragma unroll
-        for (int h = 0; h < kHT; ++h) {
-          const float v = ptx::warp_max(((h & 1) ? x[h / 2].y : x[h / 2].x) + over);
-          if (slot_ok && lane == 0) tops[qd * kHT + h] = v;
-        }
-        ptx::bar_sync(kSmBar + 2 + hh, kSmThreads / 2);
-        float2 alpha[kHT / 2];
-#pragma unroll
-        for (int i = 0; i < kHT / 2; ++i) {
-          const float2* t2 = reinterpret_cast<const float2*>(tops) + i;
-          const float2 a = t2[0], b = t2[kHT / 2], c = t2[kHT];
-          const float2 mn = make_float2(fmaxf(-m_neg[i].x, fmaxf(a.x, fmaxf(b.x, c.x))),
-                                        fmaxf(-m_neg[i].y, fmaxf(a.y, fmaxf(b.y, c.y))));
-          alpha[i] = make_float2(ptx::ex2(-m_neg[i].x - mn.x), ptx::ex2(-m_neg[i].y - mn.y));
-          l_part[i] = mul2(l_part[i], alpha[i]);
-          m_neg[i] = make_float2(-mn.x, -mn.y);
-          d[i] = add2(x[i], m_neg[i]);
-          alpha[i] = mul2(alpha[i], both(beta));
-        }
-        ptx::bar_sync(kSmBar + 2 + hh, kSmThreads / 2);  // the buffer is P's again
-        if (n > 0 && !aborted) {
-          // four tiles of O, three terms: kC loads in flight at a time
-          constexpr int kC = NH == 16 ? 4 : 2;
-#pragma unroll 1
-          for (int c = 0; c < 12; c += kC) {
-            const uint32_t ta = tmem + lane_base + (uint32_t)(C::O_COL + NH * c + kHT * hh);
-            uint32_t r[kC][kHT];
-#pragma unroll
-            for (int b = 0; b < kC; ++b) tmem_ld<kHT>(ta + (uint32_t)(NH * b), r[b]);
-            ptx::tmem_wait_ld();
-#pragma unroll
-            for (int b = 0; b < kC; ++b) {
-#pragma unroll
-              for (int h = 0; h < kHT; ++h)
-                r[b][h] = __float_as_uint(__uint_as_float(r[b][h]) * ((h & 1) ? alpha[h / 2].y : alpha[h / 2].x));
-#pragma unroll
-              for (int k = 0; k < kHT; k += 8) ptx::tmem_st8(ta + (uint32_t)(NH * b + k), r[b] + k);
-            }
-          }
-          ptx::tmem_wait_st();
-        }
-      }
-      // P[n % kPBufs] was last read by the PV of tile n - kPBufs
-      if (n >= C::kPBufs && !aborted) {
-        const int64_t j = n - C::kPBufs;
-        const bool wok = wait(bar(B_PD + (int)(j & 1)), (uint32_t)((j >> 1) & 1));
-        if (!__all_sync(0xffffffffu, wok)) aborted = true;
-      }
-      if (aborted) continue;  // the next vote ends the loop for every thread
-      if (slot_ok) {
-        // byte (row r, slot) of P: 32-slot planes of 32-byte rows, 32-byte swizzle
-        uint8_t* pbuf = sgen + C::OFF_P + (int)(n % C::kPBufs) * C::kPB + qd * C::kPK;
-        const float2 scaled = both(ratio * kPScale);
-#pragma unroll
-        for (int i = 0; i < kHT / 2; ++i) {
-          const float2 e = make_float2(ptx::ex2(d[i].x), ptx::ex2(d[i].y));
-          l_part[i] = add2(l_part[i], e);
-          float2 v = mul2(e, scaled);
-          const int r = kHT * hh + 2 * i;
-#pragma unroll
-          for (int term = 0; term < 3; ++term) {
-            const uint32_t b = to_e4m3x2(v.x, v.y);
-            if (term < 2) v = fma2(from_e4m3x2(b), both(-16.f), mul2(v, both(16.f)));
-            pbuf[sw32_byte(term * NH + r, lane)] = (uint8_t)b;
-            pbuf[sw32_byte(term * NH + r + 1, lane)] = (uint8_t)(b >> 8);
-          }
-        }
-        if (p.weights != nullptr) {
-          const int64_t at = (row * G + group) * p.ntiles + split + n * S;
-          float* s = p.scores + (at * NH + kHT * hh) * kTS + slot;
-#pragma unroll
-          for (int i = 0; i < kHT / 2; ++i) {
-            s[2 * i * kTS] = x[i].x;
-            s[(2 * i + 1) * kTS] = x[i].y;
-          }
-          if (threadIdx.x == 32 * kSm0) p.tiles[at] = tile;
-        }
+    int64_t c = 0, n = 0;  // stages, tiles
+    for (int64_t un = units.first; un < p.units; un += units.step) {
+      row = un >> units.shift;
+      group = (int)(un & (G - 1));
+      const int h0 = group * NH;  // first head of the group
+      // The score issuer has passed the unit before (also one without tiles, whose queries it
+      // never used) once the end's stage is free.
+      bool go = !aborted;
+      if (go && c > 0) go = wait(bar(B_KVE + (int)((c - 1) % kStages)), (uint32_t)(((c - 1) / kStages) & 1));
+      // The queries, into a buffer whose last reader, the previous unit's last score, is done.
+      float* units_s = reinterpret_cast<float*>(sgen + C::OFF_QS);
+      for (int h = warp - kSm0; h < NH; h += kSmWarps) {
+        const float unit = stage_query<NH>(p, row, h0 + h, h, lane, sgen);
+        if (lane == 0) units_s[h] = unit;
       }
       ptx::fence_proxy_async_smem();
-      ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar(B_PF + pb));
-    }
-    // ------------------------------------------------------------------ this CTA's m and L
-    // PD of tile n - 3 (two P buffers) or n - 2 was waited for above, on the same barrier or
-    // before, so this wait is exact
-    bool ok = !aborted;
-    if (ok && n > 0) ok = wait(bar(B_PD + (int)((n - 1) & 1)), (uint32_t)(((n - 1) >> 1) & 1));
-    aborted = ptx::bar_red_or(kSmBar, kSmThreads, !ok);
-    ptx::tc_fence_after();
-    float* red = reinterpret_cast<float*>(sgen + C::OFF_P);  // [half][quadrant][kHT]
+      if (lane == 0) ptx::mbar_arrive(bar(B_QF));
+      aborted = ptx::bar_red_or(kSmBar, kSmThreads, !go);
+      // entries of tiles that turn out to hold nothing get no other weight (of a clustered row,
+      // group g's CTA writes the tiles with (tile / S) % G == g, here and at the end)
+      if (p.weights != nullptr)
+        for (int64_t t = p.clustered ? split + S * group : 0; t < p.ntiles; t += p.clustered ? S * G : 1) {
+          const int64_t at = t * kTS + sm_tid;
+          if (sm_tid < kTS && at < p.topk) p.weights[row * p.w_sb + at] = 0.f;
+        }
+      float2 qs[kHT / 2];
 #pragma unroll
-    for (int h = 0; h < kHT; ++h) {
-      float v = (h & 1) ? l_part[h / 2].y : l_part[h / 2].x;
+      for (int j = 0; j < kHT / 2; ++j) {
+        m_neg[j] = both(-kNone);
+        l_part[j] = both(0.f);
+        qs[j] = reinterpret_cast<const float2*>(units_s)[kHT / 2 * hh + j];
+      }
+      float u_inv = 0.f;
+      u = 0.f;
+      bool failed = false;  // a wait of this warp ran out: the next vote ends the loop for every thread
+      for (live = 0; !aborted; ++live, ++n) {
+        const int st = (int)(c % kStages), sb = (int)(n % C::kSBufs), pb = (int)(n & 1);
+        bool ok = wait(bar(B_KVF + st), (uint32_t)((c / kStages) & 1));
+        const int tile = cmd[4 * st + 3];
+        const bool end = ok && tile < 0;
+        if (!end) ok = ok && wait(bar(B_SF + sb), (uint32_t)((n / C::kSBufs) & 1));
+        ++c;
+        if (live == 0) {  // the unit of the scales, the same in every thread
+          const float first = smax[st];
+          u = first > 0.f ? fmaxf(first, 1.17549435e-38f) : 1.f;  // 1 / u is finite
+          u_inv = 1.f / u;
+        }
+        float2 x[kHT / 2], d[kHT / 2];  // scores, and over the running maximum
+        float ratio = 0.f;  // scale in units, lr its log2
+        float lr = -INFINITY;
+        bool valid = false;
+        const bool grow = !end && smax[st] > kTauU * u;
+        if (slot_ok && __all_sync(0xffffffffu, ok && !end)) {  // warp-uniform
+          ptx::tc_fence_after();
+          uint32_t hi[kHT], lo[kHT], pe[kHT];
+          const uint32_t ta = tmem + lane_base + (uint32_t)(C::kSCols * sb + kHT * hh);
+          tmem_ld<kHT>(ta, hi);
+          tmem_ld<kHT>(ta + NH, lo);
+          tmem_ld<kHT>(ta + 2 * NH, pe);
+          const float scale = sc[st * kTS + slot];
+          valid = ((uint32_t)cmd[4 * st + qd] >> lane) & 1u;
+          ratio = scale * u_inv;
+          lr = ptx::lg2(fabsf(ratio));
+          ptx::tmem_wait_ld();
+          ptx::tc_fence_before();
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == 0 && slot_ok) red[(hh * 3 + qd) * kHT + h] = v;
-    }
-    ptx::bar_sync(kSmBar, kSmThreads);
-    if (qd == 0 && lane == 0) {
+          for (int j = 0; j < kHT / 2; ++j) {
+            const float2 q = fma2(pair(lo, j), both(0.0625f), pair(hi, j));
+            x[j] = fma2(mul2(q, both(scale)), qs[j], mul2(pair(pe, j), both(p.scale_log2)));
+          }
+          if (!valid) {
+#pragma unroll
+            for (int j = 0; j < kHT / 2; ++j) x[j] = both(-INFINITY);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kHT / 2; ++j) x[j] = both(-INFINITY);
+        }
+        __syncwarp();
+        if (lane == 0 && !end) ptx::mbar_arrive(bar(B_SE + sb));
+        // Whether a running maximum or the unit has to rise, or a wait failed, through one barrier
+        // of the four warps that share the heads.  Their decisions are the same, as they read
+        // the same words; the words are written again two tiles later, behind the next tile's
+        // barrier.
+        const float tau = fminf(kTauQ8 - lr, kTauL);  // P = 2^(x + lr - m) and l's 2^(x - m) in range
+        float top = kNone;
+#pragma unroll
+        for (int j = 0; j < kHT / 2; ++j) {
+          d[j] = add2(x[j], m_neg[j]);
+          top = fmaxf(top, fmaxf(d[j].x, d[j].y));
+        }
+        uint32_t vote = __reduce_or_sync(0xffffffffu, (ok && !failed ? 0u : kFailed) | (top > tau ? kRise : 0u));
+        uint32_t* words = reinterpret_cast<uint32_t*>(sgen + C::OFF_RED) + (hh * 2 + pb) * 4;
+        if (lane == 0) words[qd] = vote;
+        ptx::bar_sync(kSmBar + 2 + hh, kSmThreads / 2);
+        {
+          const uint4 v = *reinterpret_cast<const uint4*>(words);
+          vote = v.x | v.y | v.z | v.w;
+        }
+        if (vote & kFailed) {
+          aborted = true;
+          break;
+        }
+        if (end) break;
+        if (vote != 0u || grow) {
+          // Rare past the first tile: raise the maxima to this tile's, the unit to its largest
+          // scale, and bring l and O to them.
+          if (live > 0) {
+            const bool wok = wait(bar(B_PD + (int)((n - 1) & 1)), (uint32_t)(((n - 1) >> 1) & 1));
+            if (!__all_sync(0xffffffffu, wok)) failed = true;
+            ptx::tc_fence_after();
+          }
+          float beta = 1.f;
+          if (grow) {
+            const float un = smax[st];
+            beta = u / un;
+            lr += ptx::lg2(beta);
+            u = un;
+            u_inv = 1.f / u;
+            ratio *= beta;
+          }
+          // the maxima go through this tile's P buffer, whose last reader (PV) is done
+          // (in the first term's rows of these heads, which only these warps write)
+          float* tops = reinterpret_cast<float*>(sgen + C::OFF_P + (int)(n % C::kPBufs) * C::kPB + hh * kHT * 32);
+          const float over = fmaxf(lr, 8.f - kTauL);
+#pragma unroll
+          for (int h = 0; h < kHT; ++h) {
+            const float v = ptx::warp_max(((h & 1) ? x[h / 2].y : x[h / 2].x) + over);
+            if (slot_ok && lane == 0) tops[qd * kHT + h] = v;
+          }
+          ptx::bar_sync(kSmBar + 2 + hh, kSmThreads / 2);
+          float2 alpha[kHT / 2];
+#pragma unroll
+          for (int j = 0; j < kHT / 2; ++j) {
+            const float2* t2 = reinterpret_cast<const float2*>(tops) + j;
+            const float2 a = t2[0], b = t2[kHT / 2], c = t2[kHT];
+            const float2 mn = make_float2(fmaxf(-m_neg[j].x, fmaxf(a.x, fmaxf(b.x, c.x))),
+                                          fmaxf(-m_neg[j].y, fmaxf(a.y, fmaxf(b.y, c.y))));
+            alpha[j] = make_float2(ptx::ex2(-m_neg[j].x - mn.x), ptx::ex2(-m_neg[j].y - mn.y));
+            l_part[j] = mul2(l_part[j], alpha[j]);
+            m_neg[j] = make_float2(-mn.x, -mn.y);
+            d[j] = add2(x[j], m_neg[j]);
+            alpha[j] = mul2(alpha[j], both(beta));
+          }
+          ptx::bar_sync(kSmBar + 2 + hh, kSmThreads / 2);  // the buffer is P's again
+          if (live > 0 && !failed) {
+            // four tiles of O, three terms: kC loads in flight at a time
+            constexpr int kC = NH == 16 ? 4 : 2;
+#pragma unroll 1
+            for (int c = 0; c < 12; c += kC) {
+              const uint32_t ta = tmem + lane_base + (uint32_t)(C::O_COL + NH * c + kHT * hh);
+              uint32_t r[kC][kHT];
+#pragma unroll
+              for (int b = 0; b < kC; ++b) tmem_ld<kHT>(ta + (uint32_t)(NH * b), r[b]);
+              ptx::tmem_wait_ld();
+#pragma unroll
+              for (int b = 0; b < kC; ++b) {
+#pragma unroll
+                for (int h = 0; h < kHT; ++h)
+                  r[b][h] = __float_as_uint(__uint_as_float(r[b][h]) * ((h & 1) ? alpha[h / 2].y : alpha[h / 2].x));
+#pragma unroll
+                for (int k = 0; k < kHT; k += 8) ptx::tmem_st8(ta + (uint32_t)(NH * b + k), r[b] + k);
+              }
+            }
+            ptx::tmem_wait_st();
+          }
+        }
+        // P[n % kPBufs] was last read by the PV of tile n - kPBufs
+        if (n >= C::kPBufs && !failed) {
+          const int64_t j = n - C::kPBufs;
+          const bool wok = wait(bar(B_PD + (int)(j & 1)), (uint32_t)((j >> 1) & 1));
+          if (!__all_sync(0xffffffffu, wok)) failed = true;
+        }
+        if (failed) continue;
+        if (slot_ok) {
+          // byte (row r, slot) of P: 32-slot planes of 32-byte rows, 32-byte swizzle
+          uint8_t* pbuf = sgen + C::OFF_P + (int)(n % C::kPBufs) * C::kPB + qd * C::kPK;
+          const float2 scaled = both(ratio * kPScale);
+#pragma unroll
+          for (int j = 0; j < kHT / 2; ++j) {
+            const float2 e = make_float2(ptx::ex2(d[j].x), ptx::ex2(d[j].y));
+            l_part[j] = add2(l_part[j], e);
+            float2 v = mul2(e, scaled);
+            const int r = kHT * hh + 2 * j;
+#pragma unroll
+            for (int term = 0; term < 3; ++term) {
+              const uint32_t b = to_e4m3x2(v.x, v.y);
+              if (term < 2) v = fma2(from_e4m3x2(b), both(-16.f), mul2(v, both(16.f)));
+              pbuf[sw32_byte(term * NH + r, lane)] = (uint8_t)b;
+              pbuf[sw32_byte(term * NH + r + 1, lane)] = (uint8_t)(b >> 8);
+            }
+          }
+          if (p.weights != nullptr) {
+            const int64_t at = un * p.ntiles + split + (int64_t)live * S;
+            float* s = p.scores + (at * NH + kHT * hh) * kTS + slot;
+#pragma unroll
+            for (int j = 0; j < kHT / 2; ++j) {
+              s[2 * j * kTS] = x[j].x;
+              s[(2 * j + 1) * kTS] = x[j].y;
+            }
+            if (threadIdx.x == 32 * kSm0) p.tiles[at] = tile;
+          }
+        }
+        ptx::fence_proxy_async_smem();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (warp == kSm0) ptx::mbar_arrive(bar(B_KVE + st));
+          ptx::mbar_arrive(bar(B_PF + pb));
+        }
+      }
+      // ------------------------------------------------------------------ the unit's end
+      // PD of tile n - 3 (two P buffers) or n - 2 was waited for above, on the same barrier or
+      // before, so this wait is exact
+      bool ok = !aborted;
+      if (ok && live > 0) ok = wait(bar(B_PD + (int)((n - 1) & 1)), (uint32_t)(((n - 1) >> 1) & 1));
+      aborted = ptx::bar_red_or(kSmBar, kSmThreads, !ok);
+      // every warp has read the end's words
+      if (!aborted && threadIdx.x == 32 * kSm0) ptx::mbar_arrive(bar(B_KVE + (int)((c - 1) % kStages)));
+      ptx::tc_fence_after();
+      float* red = reinterpret_cast<float*>(sgen + C::OFF_P);  // [half][quadrant][kHT]
+#pragma unroll
+      for (int h = 0; h < kHT; ++h) {
+        float v = (h & 1) ? l_part[h / 2].y : l_part[h / 2].x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == 0 && slot_ok) red[(hh * 3 + qd) * kHT + h] = v;
+      }
+      ptx::bar_sync(kSmBar, kSmThreads);
+      if (p.clustered) break;
+      // A unit of its own: O^T / L from tensor memory to the output.  The next unit's first PV
+      // comes after these reads, as it needs this warp's P.
+      float coef[kHT];
+      float* lse_s = reinterpret_cast<float*>(sgen + C::OFF_LSE);
 #pragma unroll
       for (int h = 0; h < kHT; ++h) {
         const float* r3 = red + hh * 3 * kHT + h;
-        ml[kHT * hh + h] = -((h & 1) ? m_neg[h / 2].y : m_neg[h / 2].x);
-        ml[NH + kHT * hh + h] = (r3[0] + r3[kHT]) + r3[2 * kHT];
+        const float L = (r3[0] + r3[kHT]) + r3[2 * kHT];
+        coef[h] = aborted ? NAN : L == 0.f ? 0.f : 1.f / L * (u * (1.f / kPScale));  // as the merge rounds it
+        if (qd == 0 && lane == 0) {
+          const float m = -((h & 1) ? m_neg[h / 2].y : m_neg[h / 2].x);
+          const float lse = aborted ? NAN : L == 0.f ? -INFINITY : m + ptx::lg2(L);
+          lse_s[kHT * hh + h] = lse;
+          p.lse[row * p.lse_sb + (int64_t)(h0 + kHT * hh + h) * p.lse_sh] = lse;
+        }
       }
-      ml[2 * NH] = u;
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j) {
+        uint32_t r[3][kHT];
+#pragma unroll
+        for (int t = 0; t < 3; ++t)
+          tmem_ld<kHT>(tmem + lane_base + (uint32_t)(C::O_COL + NH * (3 * j + t) + kHT * hh), r[t]);
+        ptx::tmem_wait_ld();
+        __nv_bfloat16* dst = p.out + row * p.out_sb + (int64_t)(h0 + kHT * hh) * p.out_sh + 128 * j + 32 * qd + lane;
+#pragma unroll
+        for (int h = 0; h < kHT; ++h) {
+          const float o = fmaf(fmaf(__uint_as_float(r[2][h]), 0.0625f, __uint_as_float(r[1][h])), 0.0625f,
+                               __uint_as_float(r[0][h]));
+          // 0: no weight, whatever O holds (nothing was written to it without a live tile)
+          dst[(int64_t)h * p.out_sh] = __float2bfloat16_rn(coef[h] == 0.f ? 0.f : o * coef[h]);
+        }
+      }
+      ptx::tc_fence_before();
+      if (p.weights != nullptr) {
+        ptx::bar_sync(kSmBar, kSmThreads);  // lse; every tile's scores are behind the barriers above
+        if (aborted) {
+          for (int k2 = sm_tid; k2 < p.topk; k2 += kSmThreads) p.weights[row * p.w_sb + k2] = NAN;
+        } else {
+          for (int64_t e = sm_tid; e < (int64_t)live * kTS; e += kSmThreads) {
+            const int64_t at = un * p.ntiles + e / kTS;
+            const int64_t k2 = (int64_t)p.tiles[at] * kTS + e % kTS;
+            if (k2 < p.topk)
+              p.weights[row * p.w_sb + k2] = head_sum<NH>(p.scores + at * NH * kTS + e % kTS, lse_s);
+          }
+        }
+      }
     }
-    // O to shared memory, [head][512] (nothing was ever written to it without a live tile)
-    float* o_s = reinterpret_cast<float*>(sgen + C::OFF_O);
+    if (p.clustered) {
+      const float* red = reinterpret_cast<const float*>(sgen + C::OFF_P);
+      if (qd == 0 && lane == 0) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t r[3][kHT];
+        for (int h = 0; h < kHT; ++h) {
+          const float* r3 = red + hh * 3 * kHT + h;
+          ml[kHT * hh + h] = -((h & 1) ? m_neg[h / 2].y : m_neg[h / 2].x);
+          ml[NH + kHT * hh + h] = (r3[0] + r3[kHT]) + r3[2 * kHT];
+        }
+        ml[2 * NH] = u;
+      }
+      // O to shared memory, [head][512] (nothing was ever written to it without a live tile)
+      float* o_s = reinterpret_cast<float*>(sgen + C::OFF_O);
 #pragma unroll
-      for (int c = 0; c < 3; ++c)
-        tmem_ld<kHT>(tmem + lane_base + (uint32_t)(C::O_COL + NH * (3 * j + c) + kHT * hh), r[c]);
-      ptx::tmem_wait_ld();
+      for (int j = 0; j < 4; ++j) {
+        uint32_t r[3][kHT];
 #pragma unroll
-      for (int h = 0; h < kHT; ++h) {
-        const float o = fmaf(fmaf(__uint_as_float(r[2][h]), 0.0625f, __uint_as_float(r[1][h])), 0.0625f,
-                             __uint_as_float(r[0][h]));
-        o_s[(kHT * hh + h) * kDCkv + 128 * j + 32 * qd + lane] = n > 0 ? o : 0.f;
+        for (int c = 0; c < 3; ++c)
+          tmem_ld<kHT>(tmem + lane_base + (uint32_t)(C::O_COL + NH * (3 * j + c) + kHT * hh), r[c]);
+        ptx::tmem_wait_ld();
+#pragma unroll
+        for (int h = 0; h < kHT; ++h) {
+          const float o = fmaf(fmaf(__uint_as_float(r[2][h]), 0.0625f, __uint_as_float(r[1][h])), 0.0625f,
+                               __uint_as_float(r[0][h]));
+          o_s[(kHT * hh + h) * kDCkv + 128 * j + 32 * qd + lane] = live > 0 ? o : 0.f;
+        }
       }
     }
   }
@@ -852,14 +987,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // -------------------------------------------------------------------- merge of the splits
   // Behind this barrier every CTA of the cluster has its m, L, u and O in shared memory.
-  if (S * G > 1) ptx::cluster_sync();
+  if (p.clustered) ptx::cluster_sync();
   bool lost = false;  // a wait ran out somewhere in the cluster: the row is written as NaN
-  if (warp >= kSm0) {
+  if (p.clustered && warp >= kSm0) {
+    const int h0 = group * NH;
     const int sm_tid = (int)threadIdx.x - 32 * kSm0;
     float* coef = reinterpret_cast<float*>(sgen + C::OFF_COEF);
     float* lse_s = coef + S * NH;
     const int rank0 = group * S;  // the rank of split 0 of this group
-    if (S == 1) ptx::bar_sync(kSmBar, kSmThreads);
     if (sm_tid < S * G)
       lost = __float_as_uint(ld_cluster(
                  ptx::mapa(sbase + (uint32_t)C::OFF_MISC + 8u, (uint32_t)sm_tid))) != 0u;
@@ -931,15 +1066,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---------------------------------------------------------------- weights
       // every tile's scores are behind the barriers above
       const int64_t first = (row * G + group) * p.ntiles + split;
-      for (int64_t e = sm_tid; e < n * kTS; e += kSmThreads) {
+      for (int64_t e = sm_tid; e < (int64_t)live * kTS; e += kSmThreads) {
         const int64_t at = first + e / kTS * S;
         const int slot = (int)(e % kTS);
         float* s = p.scores + at * NH * kTS + slot;
-        float w = 0.f;
-        for (int h = 0; h < NH; ++h) {
-          const float x = s[h * kTS];
-          w += x == -INFINITY ? 0.f : ptx::ex2(x - lse_s[h]);
-        }
+        const float w = head_sum<NH>(s, lse_s);
         if (G == 1) {
           const int64_t k = (int64_t)p.tiles[at] * kTS + slot;
           if (k < p.topk) p.weights[row * p.w_sb + k] = w;
@@ -949,14 +1080,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   }
-  if (G > 1 && p.weights != nullptr) {
+  if (p.clustered && G > 1 && p.weights != nullptr) {
     __syncwarp();
     ptx::cluster_sync();
     if (warp >= kSm0 && !lost) {
       // the groups ran the same tiles; each adds up the tiles it owns, group by group
       const int sm_tid = (int)threadIdx.x - 32 * kSm0;
       const int64_t first = row * G * p.ntiles + split;
-      for (int64_t e = sm_tid; e < n * kTS; e += kSmThreads) {
+      for (int64_t e = sm_tid; e < (int64_t)live * kTS; e += kSmThreads) {
         const int64_t at = first + e / kTS * S;
         const int tile = __ldcg(p.tiles + at + (int64_t)group * p.ntiles);
         const int slot = (int)(e % kTS);

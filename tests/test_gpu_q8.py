@@ -107,6 +107,7 @@ def test_attend_row_counts(rows, heads, topk):
     cache = ref.pools(80, 64, 64, rows)
     q, idx = queries(rows, heads, rows), selection(rows, topk, 80 * 64, rows)
     check(run(q, cache, idx), q, cache, idx)
+    check(run(q, cache, idx, weights=False), q, cache, idx)
 
 
 def test_attend_repeated_slots_and_long_selections():
