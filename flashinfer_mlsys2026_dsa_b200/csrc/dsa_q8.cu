@@ -535,6 +535,7 @@ namespace {
 using AttendFn = void (*)(CUtensorMap, CUtensorMap, AttendParams);
 
 int group_heads(int heads) { return heads == 16 ? 16 : 32; }
+int tile_slots(int nh) { return nh == 16 ? Cfg<16>::kTS : Cfg<32>::kTS; }
 
 // SMs of the current device, with the attend kernels' shared-memory limit raised on it.
 int prepare_device() {
@@ -578,9 +579,9 @@ int choose_splits(int64_t units, int nh, int groups, int ntiles, int sms) {
 
 extern "C" size_t dsa_q8_scratch_size(int64_t num_tokens, int32_t num_heads, int32_t topk) {
   if (num_tokens < 0 || topk < 1 || !heads_supported(num_heads)) return 0;
-  const size_t tiles = ((size_t)topk + q8::kTS - 1) / q8::kTS;
-  const size_t groups = (size_t)(num_heads / q8::group_heads(num_heads));
-  return (size_t)num_tokens * tiles * ((size_t)num_heads * q8::kTS + groups) * 4;
+  const int nh = q8::group_heads(num_heads);
+  const size_t ts = (size_t)q8::tile_slots(nh), tiles = ((size_t)topk + ts - 1) / ts;
+  return (size_t)num_tokens * tiles * ((size_t)num_heads * ts + (size_t)(num_heads / nh)) * 4;
 }
 
 extern "C" int dsa_sparse_mla_decode_q8(
@@ -638,12 +639,13 @@ extern "C" int dsa_sparse_mla_decode_q8(
   p.w_sb = weights_stride_b;
   const int nh = q8::group_heads(num_heads);
   p.topk = topk;
-  p.ntiles = (int32_t)(((int64_t)topk + q8::kTS - 1) / q8::kTS);
+  const int ts = q8::tile_slots(nh);
+  p.ntiles = (int32_t)(((int64_t)topk + ts - 1) / ts);
   p.groups = num_heads / nh;
   p.scores = static_cast<float*>(scratch);
   p.tiles = weights == nullptr ? nullptr
                                : reinterpret_cast<int32_t*>(
-                                     p.scores + num_tokens * p.ntiles * num_heads * q8::kTS);
+                                     p.scores + num_tokens * p.ntiles * num_heads * ts);
   p.scale_log2 = sm_scale * kLog2e;
   p.wait_cycles = wait_limit_cycles();
   p.err = static_cast<uint32_t*>(workspace);

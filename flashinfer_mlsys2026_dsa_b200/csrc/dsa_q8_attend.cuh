@@ -72,11 +72,8 @@ struct AttendParams {
   uint64_t wait_cycles;
 };
 
-constexpr int kTS = 96;               // slots per tile
 constexpr int kBlocks = 5;            // 128-byte column blocks of a slot: four of ckv, one of kpe
-constexpr int kRB = kTS * 128;        // one block's region of a stage
-constexpr int kStageB = kBlocks * kRB;
-constexpr int kStages = 3;
+constexpr int kMaxStages = 3;
 constexpr int kThreads = 512;
 constexpr int kProdWarps = 5;
 constexpr int kScore = 5, kPv = 6, kKeeper = 7, kSm0 = 8;
@@ -94,8 +91,13 @@ constexpr uint32_t kSw32 = 6;         // UMMA descriptor layout type: 32-byte sw
 template <int NH>
 struct Cfg {
   static_assert(NH == 16 || NH == 32, "head group width");
+  static constexpr int kTS = NH == 16 ? 96 : 128;  // slots per tile
+  static constexpr int kStages = NH == 16 ? 3 : 2;
+  static constexpr int kQuads = kTS / 32;          // TMEM lane quadrants that hold slots
+  static constexpr int kRB = kTS * 128;            // one block's region of a stage
+  static constexpr int kStageB = kBlocks * kRB;
   static constexpr int kHT = NH / 2;               // heads per softmax thread
-  static constexpr int kPBufs = NH == 16 ? 2 : 1;  // two do not fit beside 32 heads' Q
+  static constexpr int kPBufs = 2;
   static constexpr int kQBlk = 2 * NH * 128;       // one 128-wide block of Q, hi rows then lo rows
   static constexpr int kPK = 3 * NH * 32;          // P^T, 32 slots of it: rows of 32 bytes
   static constexpr int kPB = kTS / 32 * kPK;
@@ -105,8 +107,8 @@ struct Cfg {
   static constexpr int OFF_BAR = OFF_P + kPBufs * kPB;
   static constexpr int OFF_MISC = OFF_BAR + 256;   // [0] TMEM base, [2] abort, [3] drain, [8..15] end
                                                    // tiles of the units in flight
-  static constexpr int OFF_CMD = OFF_MISC + 64;    // [stage][4]: three validity words, the tile (-1: end)
-  static constexpr int OFF_SMAX = OFF_CMD + kStages * 16;  // [stage] largest scale of the tile
+  static constexpr int OFF_CMD = OFF_MISC + 64;    // [stage][8]: validity words; [4] the tile (-1: end)
+  static constexpr int OFF_SMAX = OFF_CMD + kStages * 32;  // [stage] largest scale of the tile
   static constexpr int OFF_QS = OFF_SMAX + 16;     // [NH] score units per query row
   static constexpr int OFF_SC = OFF_QS + NH * 4;   // [stage][96] scales; at the end kMl floats
   static constexpr int kMl = 2 * NH + 1;           // a CTA's m, L and u, for the merge
@@ -128,8 +130,8 @@ struct Cfg {
 
 enum : int {
   B_KVF = 0,                 // [stage] slots landed, scales, validity and tile number written
-  B_KVE = B_KVF + kStages,   // [stage] free again: PV done, and its words read by score and softmax
-  B_SF = B_KVE + kStages,    // [2] score written
+  B_KVE = B_KVF + kMaxStages,   // [stage] free again: PV done, and its words read by score and softmax
+  B_SF = B_KVE + kMaxStages,    // [2] score written
   B_SE = B_SF + 2,           // [2] score read
   B_PF = B_SE + 2,           // [2] P written (and O rescaled)
   B_PD = B_PF + 2,           // [2] PV done
@@ -185,7 +187,7 @@ struct Units {
 //
 // The slots that a lane's kN entries of a tile name, fetched ahead: entries three tiles, pages (of
 // a paged call) two.  -1: padding, -2: names no slot.
-template <int kN>
+template <int kN, int kTS>
 struct Entries {
   const AttendParams& p;
   const int32_t* ir;
@@ -246,6 +248,7 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
                                         const Units& units, int split, int lane, uint32_t sbase,
                                         uint8_t* sgen, const Waiter& wait) {
   using C = Cfg<NH>;
+  constexpr int kTS = C::kTS, kStages = C::kStages, kRB = C::kRB, kStageB = C::kStageB;
   const uint32_t bar0 = sbase + (uint32_t)C::OFF_BAR;
   auto bar = [&](int k) { return bar0 + 8u * (uint32_t)k; };
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sgen + C::OFF_MISC);
@@ -260,7 +263,7 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
   int k = 0;
   for (int64_t un = units.first; ok && un < p.units; un += units.step, ++k) {
     const int64_t row = un >> units.shift;
-    Entries<4> in{p, p.idx + row * p.idx_sb, row, 4 * lane, 1};
+    Entries<4, kTS> in{p, p.idx + row * p.idx_sb, row, 4 * lane, 1};
     in.start(split, has);
     // the end tile is the keeper's to lower at any time: the lanes agree on one reading
     for (int64_t t = split; t < __shfl_sync(0xffffffffu, (int)misc[8 + (k & 7)], 0); t += p.splits) {
@@ -320,7 +323,7 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
                                            int lane, uint32_t sbase, uint8_t* sgen,
                                            const Waiter& wait) {
   using C = Cfg<NH>;
-  constexpr int kE = kTS / 32;
+  constexpr int kTS = C::kTS, kStages = C::kStages, kE = C::kQuads;
   const uint32_t bar0 = sbase + (uint32_t)C::OFF_BAR;
   auto bar = [&](int k) { return bar0 + 8u * (uint32_t)k; };
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sgen + C::OFF_MISC);
@@ -333,7 +336,7 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
   int unit = 0;
   for (int64_t un = units.first; ok && un < p.units; un += units.step, ++unit) {
     const int64_t row = un >> units.shift;
-    Entries<kE> in{p, p.idx + row * p.idx_sb, row, lane, 32};
+    Entries<kE, kTS> in{p, p.idx + row * p.idx_sb, row, lane, 32};
     if (lane == 0) misc[8 + ((unit + 4) & 7)] = (uint32_t)p.ntiles;
     in.start(split, true);
     int end = 0;
@@ -373,8 +376,8 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
         big = ptx::warp_max(big);
         if (lane == 0) {
 #pragma unroll
-          for (int e = 0; e < kE; ++e) cmd[4 * st + e] = (int)w[e];
-          cmd[4 * st + 3] = (int)t;
+          for (int e = 0; e < kE; ++e) cmd[8 * st + e] = (int)w[e];
+          cmd[8 * st + 4] = (int)t;
           smax[st] = big;
         }
         __syncwarp();
@@ -389,7 +392,7 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
     if (!ok) break;
     ok = __all_sync(0xffffffffu, wait(bar(B_KVE + st), phase ^ 1u));
     if (ok && lane == 0) {
-      cmd[4 * st + 3] = -1;
+      cmd[8 * st + 4] = -1;
       ptx::mbar_arrive(bar(B_KVF + st));
     }
     if (++st == kStages) {
@@ -483,6 +486,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 __device__ __forceinline__ float2 pair(const uint32_t* r, int i) {
   return make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
 }
+__device__ __forceinline__ float2 lds2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // An entry's probability summed over the heads, from its scores (kTS apart) and their lse.
@@ -491,7 +499,7 @@ __device__ __forceinline__ float head_sum(const float* scores, const float* lse)
   float w = 0.f;
 #pragma unroll 8
   for (int h = 0; h < NH; ++h) {
-    const float x = scores[h * kTS];
+    const float x = scores[h * Cfg<NH>::kTS];
     w += x == -INFINITY ? 0.f : ptx::ex2(x - lse[h]);
   }
   return w;
@@ -517,7 +525,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     attend_kernel(const __grid_constant__ CUtensorMap tm_ckv,
                   const __grid_constant__ CUtensorMap tm_kpe, const __grid_constant__ AttendParams p) {
   using C = Cfg<NH>;
-  constexpr int kHT = C::kHT;
+  constexpr int kHT = C::kHT, kQuads = C::kQuads;
+  constexpr int kTS = C::kTS, kStages = C::kStages, kRB = C::kRB, kStageB = C::kStageB;
   extern __shared__ __align__(1024) uint8_t smem_raw[];  // swizzle atoms are 1024 bytes
   const uint32_t sbase = ptx::smem_u32(smem_raw);
   uint8_t* sgen = smem_raw;
@@ -595,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int st = (int)(c % kStages), sb = (int)(i % C::kSBufs);
         ok = __all_sync(0xffffffffu, spin(bar(B_KVF + st), (uint32_t)((c / kStages) & 1)));
         if (!ok) break;
-        const bool end = __any_sync(0xffffffffu, cmd[4 * st + 3] < 0);
+        const bool end = __any_sync(0xffffffffu, cmd[8 * st + 4] < 0);
         if (el) ptx::mbar_arrive(bar(B_KVE + st));
         ++c;
         if (end) break;
@@ -640,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, spin(bar(B_KVF + st), (uint32_t)((c / kStages) & 1)));
         if (!ok) break;
         ++c;
-        if (__any_sync(0xffffffffu, cmd[4 * st + 3] < 0)) {
+        if (__any_sync(0xffffffffu, cmd[8 * st + 4] < 0)) {
           if (el) ptx::mbar_arrive(bar(B_KVE + st));
           break;
         }
@@ -672,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp >= kSm0) {
     // ------------------------------------------------------------------ softmax
     const int slot = 32 * qd + lane;
-    const bool slot_ok = slot < kTS;  // quadrant 3 holds no slots; its lanes are rows of O
+    const bool slot_ok = slot < kTS;  // the other quadrants' lanes are only rows of O
     const float* sc = reinterpret_cast<const float*>(sgen + C::OFF_SC);
     const volatile float* smax = reinterpret_cast<const volatile float*>(sgen + C::OFF_SMAX);
     const int sm_tid = (int)threadIdx.x - 32 * kSm0;
@@ -702,12 +711,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int64_t at = t * kTS + sm_tid;
           if (sm_tid < kTS && at < p.topk) p.weights[row * p.w_sb + at] = 0.f;
         }
+      // the heads' score units: in registers, or (32 heads) read from shared memory tile by tile
+      const uint32_t qs_s = sbase + (uint32_t)(C::OFF_QS + 4 * kHT * hh);
       float2 qs[kHT / 2];
 #pragma unroll
       for (int j = 0; j < kHT / 2; ++j) {
         m_neg[j] = both(-kNone);
         l_part[j] = both(0.f);
-        qs[j] = reinterpret_cast<const float2*>(units_s)[kHT / 2 * hh + j];
+        if (NH == 16) qs[j] = lds2(qs_s + 8u * (uint32_t)j);
       }
       float u_inv = 0.f;
       u = 0.f;
@@ -715,7 +726,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (live = 0; !aborted; ++live, ++n) {
         const int st = (int)(c % kStages), sb = (int)(n % C::kSBufs), pb = (int)(n & 1);
         bool ok = wait(bar(B_KVF + st), (uint32_t)((c / kStages) & 1));
-        const int tile = cmd[4 * st + 3];
+        const int tile = cmd[8 * st + 4];
         const bool end = ok && tile < 0;
         if (!end) ok = ok && wait(bar(B_SF + sb), (uint32_t)((n / C::kSBufs) & 1));
         ++c;
@@ -737,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld<kHT>(ta + NH, lo);
           tmem_ld<kHT>(ta + 2 * NH, pe);
           const float scale = sc[st * kTS + slot];
-          valid = ((uint32_t)cmd[4 * st + qd] >> lane) & 1u;
+          valid = ((uint32_t)cmd[8 * st + qd] >> lane) & 1u;
           ratio = scale * u_inv;
           lr = ptx::lg2(fabsf(ratio));
           ptx::tmem_wait_ld();
@@ -745,7 +756,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < kHT / 2; ++j) {
             const float2 q = fma2(pair(lo, j), both(0.0625f), pair(hi, j));
-            x[j] = fma2(mul2(q, both(scale)), qs[j], mul2(pair(pe, j), both(p.scale_log2)));
+            x[j] = fma2(mul2(q, both(scale)), NH == 16 ? qs[j] : lds2(qs_s + 8u * (uint32_t)j),
+                        mul2(pair(pe, j), both(p.scale_log2)));
           }
           if (!valid) {
 #pragma unroll
@@ -812,9 +824,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < kHT / 2; ++j) {
             const float2* t2 = reinterpret_cast<const float2*>(tops) + j;
-            const float2 a = t2[0], b = t2[kHT / 2], c = t2[kHT];
-            const float2 mn = make_float2(fmaxf(-m_neg[j].x, fmaxf(a.x, fmaxf(b.x, c.x))),
-                                          fmaxf(-m_neg[j].y, fmaxf(a.y, fmaxf(b.y, c.y))));
+            float2 mn = make_float2(-m_neg[j].x, -m_neg[j].y);
+#pragma unroll
+            for (int q = 0; q < kQuads; ++q) {
+              const float2 t = t2[q * kHT / 2];
+              mn = make_float2(fmaxf(mn.x, t.x), fmaxf(mn.y, t.y));
+            }
             alpha[j] = make_float2(ptx::ex2(-m_neg[j].x - mn.x), ptx::ex2(-m_neg[j].y - mn.y));
             l_part[j] = mul2(l_part[j], alpha[j]);
             m_neg[j] = make_float2(-mn.x, -mn.y);
@@ -903,7 +918,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float v = (h & 1) ? l_part[h / 2].y : l_part[h / 2].x;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == 0 && slot_ok) red[(hh * 3 + qd) * kHT + h] = v;
+        if (lane == 0 && slot_ok) red[(hh * kQuads + qd) * kHT + h] = v;
       }
       ptx::bar_sync(kSmBar, kSmThreads);
       if (p.clustered) break;
@@ -913,8 +928,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       float* lse_s = reinterpret_cast<float*>(sgen + C::OFF_LSE);
 #pragma unroll
       for (int h = 0; h < kHT; ++h) {
-        const float* r3 = red + hh * 3 * kHT + h;
-        const float L = (r3[0] + r3[kHT]) + r3[2 * kHT];
+        const float* sums = red + hh * kQuads * kHT + h;
+        float L = sums[0];
+#pragma unroll
+        for (int q = 1; q < kQuads; ++q) L += sums[q * kHT];
         coef[h] = aborted ? NAN : L == 0.f ? 0.f : 1.f / L * (u * (1.f / kPScale));  // as the merge rounds it
         if (qd == 0 && lane == 0) {
           const float m = -((h & 1) ? m_neg[h / 2].y : m_neg[h / 2].x);
@@ -959,9 +976,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (qd == 0 && lane == 0) {
 #pragma unroll
         for (int h = 0; h < kHT; ++h) {
-          const float* r3 = red + hh * 3 * kHT + h;
+          const float* sums = red + hh * kQuads * kHT + h;
           ml[kHT * hh + h] = -((h & 1) ? m_neg[h / 2].y : m_neg[h / 2].x);
-          ml[NH + kHT * hh + h] = (r3[0] + r3[kHT]) + r3[2 * kHT];
+          float L = sums[0];
+#pragma unroll
+          for (int q = 1; q < kQuads; ++q) L += sums[q * kHT];
+          ml[NH + kHT * hh + h] = L;
         }
         ml[2 * NH] = u;
       }
