@@ -269,7 +269,6 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
     for (int64_t t = split; t < __shfl_sync(0xffffffffu, (int)misc[8 + (k & 7)], 0); t += p.splits) {
       const int4 r = make_int4(in.slot0[0], in.slot0[1], in.slot0[2], in.slot0[3]);
       const bool live = __any_sync(0xffffffffu, r.x >= 0 || r.y >= 0 || r.z >= 0 || r.w >= 0);
-      in.prefetch(t, has);
       if (live) {
         ok = __all_sync(0xffffffffu, wait(bar(B_KVE + st), phase ^ 1u));
         if (!ok) break;
@@ -291,6 +290,7 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
           phase ^= 1u;
         }
       }
+      in.prefetch(t, has);  // two and three tiles ahead, so the copies go first
       in.advance();
     }
     if (!ok) break;
@@ -313,11 +313,28 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
   __syncwarp();
 }
 
-// The keeper (warp 7).  Per unit first the tile behind the row's last entry that is not
-// padding, found from the end in steps of 512 entries, so that nobody walks a short row's padding;
-// then, tile by tile, lane l the entries l, l + 32 and l + 64: scales, validity, the tile's
-// number.  The end tiles have eight places; the gatherers are at most three stages, so at most
-// three units, ahead of the keeper, which opens a unit's place four units before it.
+// The tile behind a row's last entry that is not padding, found from the end in steps of 512
+// entries.
+template <int kTS>
+__device__ __forceinline__ int end_tile(const int32_t* ir, int topk, int lane) {
+  int end = 0;
+  for (int hi = topk; hi > 0 && end == 0; hi -= 512) {
+    int last = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int k = hi - 512 + 32 * i + lane;
+      if (k >= 0 && __ldg(ir + k) != -1) last = k + 1;
+    }
+    end = __reduce_max_sync(0xffffffffu, last);
+  }
+  return (end + kTS - 1) / kTS;
+}
+
+// The keeper (warp 7).  Tile by tile, lane l the entries l, l + 32, ...: scales, validity, the
+// tile's number; at a unit's first tile without entries also where the row's padding begins, so
+// that nobody walks a short row's padding.  The end tiles have eight places; the gatherers are at most three
+// stages, so at most three units, ahead of the keeper, which opens a unit's place four units
+// before it.
 template <int NH>
 __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& units, int split,
                                            int lane, uint32_t sbase, uint8_t* sgen,
@@ -339,18 +356,8 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
     Entries<kE, kTS> in{p, p.idx + row * p.idx_sb, row, lane, 32};
     if (lane == 0) misc[8 + ((unit + 4) & 7)] = (uint32_t)p.ntiles;
     in.start(split, true);
-    int end = 0;
-    for (int hi = p.topk; hi > 0 && end == 0; hi -= 512) {
-      int last = 0;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int k = hi - 512 + 32 * i + lane;
-        if (k >= 0 && __ldg(in.ir + k) != -1) last = k + 1;
-      }
-      end = __reduce_max_sync(0xffffffffu, last);
-    }
-    end = (end + kTS - 1) / kTS;
-    if (lane == 0) misc[8 + (unit & 7)] = (uint32_t)end;
+    int end = p.ntiles;
+    bool scanned = false;
     for (int64_t t = split; t < end; t += p.splits) {
       uint32_t w[kE], any = 0;
       float scale[kE], big = 0.f;
@@ -386,6 +393,11 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
           st = 0;
           phase ^= 1u;
         }
+      }
+      if (any == 0u && !scanned) {
+        scanned = true;
+        end = end_tile<kTS>(in.ir, p.topk, lane);
+        if (lane == 0) misc[8 + (unit & 7)] = (uint32_t)end;
       }
       in.advance();
     }
@@ -1029,14 +1041,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       part[i] = ld_cluster4(ptx::mapa(sbase + (uint32_t)(C::OFF_O + 4 * (split * per * kDCkv + 4 * e)),
                                       (uint32_t)(rank0 + (i & (S - 1)))));
     }
-    lost = ptx::bar_red_or(kSmBar, kSmThreads, lost);
-    for (int e = sm_tid; e < NH * S; e += kSmThreads) {
-      // thread (head, split): the head's lse, and what a value of the split's O counts for in
-      // its output; the S threads of a head are neighbours in a warp
-      const int h = e >> ss, s = e & (S - 1);
+    // thread (head, split): the head's lse, and what a value of the split's O counts for in its
+    // output; the S threads of a head are neighbours in a warp
+    static_assert(NH * kMaxCluster <= kSmThreads, "a thread per head and split");
+    const int h = sm_tid >> ss, s = sm_tid & (S - 1);
+    float ms = 0.f, ls = 0.f, us = 0.f;
+    if (sm_tid < NH * S) {
       const uint32_t at = ptx::mapa(sbase + (uint32_t)C::OFF_SC, (uint32_t)(rank0 + s));
-      const float ms = ld_cluster(at + 4u * (uint32_t)h), ls = ld_cluster(at + 4u * (uint32_t)(NH + h));
-      const float us = ld_cluster(at + 8u * NH);
+      ms = ld_cluster(at + 4u * (uint32_t)h);
+      ls = ld_cluster(at + 4u * (uint32_t)(NH + h));
+      us = ld_cluster(at + 8u * NH);
+    }
+    lost = ptx::bar_red_or(kSmBar, kSmThreads, lost);
+    if (sm_tid < NH * S) {
       float M = ms;
       for (int k = 1; k < S; k <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
       const float w = ls == 0.f ? 0.f : ptx::ex2(ms - M);
