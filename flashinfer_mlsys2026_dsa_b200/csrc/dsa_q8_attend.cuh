@@ -192,7 +192,7 @@ struct Entries {
   const AttendParams& p;
   const int32_t* ir;
   int64_t row;
-  int first, step;  // this lane: entries first + step e of a tile
+  const int first, step;  // this lane: entries first + step e of a tile
   int pos2[kN], slot1[kN], slot0[kN];
 
   __device__ __forceinline__ void load(int64_t t, int (&pos)[kN], bool has) const {
@@ -211,7 +211,11 @@ struct Entries {
       if (slot[e] < 0 && pos[e] != -1) slot[e] = -2;
     }
   }
-  __device__ __forceinline__ void start(int64_t t, bool has) {
+  __device__ __forceinline__ Entries(const AttendParams& prm, int f, int s)
+      : p(prm), ir(nullptr), row(0), first(f), step(s) {}
+  __device__ __forceinline__ void start(int64_t r, int64_t t, bool has) {
+    row = r;
+    ir = p.idx + r * p.idx_sb;
     int a[kN], b[kN];
     load(t, a, has);
     load(t + p.splits, b, has);
@@ -261,10 +265,9 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
   int st = 0;
   uint32_t phase = 0;
   int k = 0;
+  Entries<4, kTS> in(p, 4 * lane, 1);
+  in.start(units.first >> units.shift, split, has);
   for (int64_t un = units.first; ok && un < p.units; un += units.step, ++k) {
-    const int64_t row = un >> units.shift;
-    Entries<4, kTS> in{p, p.idx + row * p.idx_sb, row, 4 * lane, 1};
-    in.start(split, has);
     // the end tile is the keeper's to lower at any time: the lanes agree on one reading
     for (int64_t t = split; t < __shfl_sync(0xffffffffu, (int)misc[8 + (k & 7)], 0); t += p.splits) {
       const int4 r = make_int4(in.slot0[0], in.slot0[1], in.slot0[2], in.slot0[3]);
@@ -294,6 +297,7 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
       in.advance();
     }
     if (!ok) break;
+    if (un + units.step < p.units) in.start((un + units.step) >> units.shift, split, has);
     // the unit's end: a stage without slots
     ok = __all_sync(0xffffffffu, wait(bar(B_KVE + st), phase ^ 1u));
     if (!ok) break;
@@ -313,22 +317,37 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
   __syncwarp();
 }
 
-// The tile behind a row's last entry that is not padding, found from the end in steps of 512
-// entries.
-template <int kTS>
-__device__ __forceinline__ int end_tile(const int32_t* ir, int topk, int lane) {
-  int end = 0;
-  for (int hi = topk; hi > 0 && end == 0; hi -= 512) {
-    int last = 0;
+// Where a row's padding begins: behind its last entry that is not -1.  The last 512 entries
+// are fetched ahead of their use; a row that is padding there is searched towards its front,
+// 2048 entries a step.
+struct Tail {
+  const int topk, lane;
+  int last[16];
+  __device__ __forceinline__ Tail(const AttendParams& p, int l) : topk(p.topk), lane(l) {}
+  __device__ __forceinline__ void load(const int32_t* ir) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int k = hi - 512 + 32 * i + lane;
-      if (k >= 0 && __ldg(ir + k) != -1) last = k + 1;
+      const int k = topk - 512 + 32 * i + lane;
+      last[i] = k >= 0 ? ldg_now(ir + k) : -1;
     }
-    end = __reduce_max_sync(0xffffffffu, last);
   }
-  return (end + kTS - 1) / kTS;
-}
+  __device__ __forceinline__ int end(const int32_t* ir) const {
+    int e = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (last[i] != -1) e = topk - 512 + 32 * i + lane + 1;
+    e = __reduce_max_sync(0xffffffffu, e);
+    for (int hi = topk - 512; hi > 0 && e == 0; hi -= 2048) {
+#pragma unroll 32
+      for (int i = 0; i < 64; ++i) {
+        const int k = hi - 2048 + 32 * i + lane;
+        if (k >= 0 && __ldg(ir + k) != -1) e = k + 1;
+      }
+      e = __reduce_max_sync(0xffffffffu, e);
+    }
+    return e;
+  }
+};
 
 // The keeper (warp 7).  Tile by tile, lane l the entries l, l + 32, ...: scales, validity, the
 // tile's number; at a unit's first tile without entries also where the row's padding begins, so
@@ -351,11 +370,12 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
   int st = 0;
   uint32_t phase = 0;
   int unit = 0;
+  Entries<kE, kTS> in(p, lane, 32);
+  Tail tail(p, lane);
+  in.start(units.first >> units.shift, split, true);
+  tail.load(in.ir);
   for (int64_t un = units.first; ok && un < p.units; un += units.step, ++unit) {
-    const int64_t row = un >> units.shift;
-    Entries<kE, kTS> in{p, p.idx + row * p.idx_sb, row, lane, 32};
     if (lane == 0) misc[8 + ((unit + 4) & 7)] = (uint32_t)p.ntiles;
-    in.start(split, true);
     int end = p.ntiles;
     bool scanned = false;
     for (int64_t t = split; t < end; t += p.splits) {
@@ -396,12 +416,16 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
       }
       if (any == 0u && !scanned) {
         scanned = true;
-        end = end_tile<kTS>(in.ir, p.topk, lane);
+        end = (tail.end(in.ir) + kTS - 1) / kTS;
         if (lane == 0) misc[8 + (unit & 7)] = (uint32_t)end;
       }
       in.advance();
     }
     if (!ok) break;
+    if (un + units.step < p.units) {
+      in.start((un + units.step) >> units.shift, split, true);
+      tail.load(in.ir);
+    }
     ok = __all_sync(0xffffffffu, wait(bar(B_KVE + st), phase ^ 1u));
     if (ok && lane == 0) {
       cmd[8 * st + 4] = -1;
@@ -418,14 +442,22 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
 // One query head into shared memory: hi and lo rows of q_nope in e4m3, the q_pe row in bf16.
 // Returns the head's score unit: (hi + lo / 16) * unit is in log2 units.  A row with an
 // infinity or a NaN has the unit NaN, which reaches every one of its scores.
+struct Query {
+  uint4 nope[2], pe;  // this lane's sixteen values, and eight (lanes 0 .. 7)
+  __device__ __forceinline__ void load(const AttendParams& p, int64_t row, int head, int lane) {
+    const uint4* src = reinterpret_cast<const uint4*>(p.qn + row * p.qn_sb + head * p.qn_sh) + 2 * lane;
+    nope[0] = __ldg(src);
+    nope[1] = __ldg(src + 1);
+    pe = make_uint4(0u, 0u, 0u, 0u);
+    if (lane < 8) pe = __ldg(reinterpret_cast<const uint4*>(p.qp + row * p.qp_sb + head * p.qp_sh) + lane);
+  }
+};
 template <int NH>
-__device__ __forceinline__ float stage_query(const AttendParams& p, int64_t row, int head, int h,
-                                             int lane, uint8_t* sgen) {
+__device__ __forceinline__ float stage_query(const Query& in, float scale_log2, int h, int lane,
+                                             uint8_t* sgen) {
   using C = Cfg<NH>;
-  const uint4* src = reinterpret_cast<const uint4*>(p.qn + row * p.qn_sb + head * p.qn_sh) + 2 * lane;
-  const uint4 raw[2] = {__ldg(src), __ldg(src + 1)};
-  uint4 pe = make_uint4(0u, 0u, 0u, 0u);
-  if (lane < 8) pe = __ldg(reinterpret_cast<const uint4*>(p.qp + row * p.qp_sb + head * p.qp_sh) + lane);
+  const uint4 (&raw)[2] = in.nope;
+  const uint4 pe = in.pe;
   float f[16], g[8];
   unpack8(raw[0], *reinterpret_cast<float(*)[8]>(f));
   unpack8(raw[1], *reinterpret_cast<float(*)[8]>(f + 8));
@@ -463,7 +495,7 @@ __device__ __forceinline__ float stage_query(const AttendParams& p, int64_t row,
   *reinterpret_cast<uint4*>(q + sw128_byte(h, 16 * (lane & 7))) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
   *reinterpret_cast<uint4*>(q + sw128_byte(NH + h, 16 * (lane & 7))) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   if (lane < 8) *reinterpret_cast<uint4*>(sgen + C::OFF_QP + sw128_byte(h, 16 * lane)) = pe;
-  return fine ? __uint_as_float((uint32_t)(127 + e - 7) << 23) * p.scale_log2 : NAN;
+  return fine ? __uint_as_float((uint32_t)(127 + e - 7) << 23) * scale_log2 : NAN;
 }
 
 template <int kN>
@@ -708,8 +740,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (go && c > 0) go = wait(bar(B_KVE + (int)((c - 1) % kStages)), (uint32_t)(((c - 1) / kStages) & 1));
       // The queries, into a buffer whose last reader, the previous unit's last score, is done.
       float* units_s = reinterpret_cast<float*>(sgen + C::OFF_QS);
-      for (int h = warp - kSm0; h < NH; h += kSmWarps) {
-        const float unit = stage_query<NH>(p, row, h0 + h, h, lane, sgen);
+      constexpr int kQH = NH / kSmWarps;
+      Query query[kQH];
+#pragma unroll
+      for (int j = 0; j < kQH; ++j) query[j].load(p, row, h0 + warp - kSm0 + j * kSmWarps, lane);
+#pragma unroll
+      for (int j = 0; j < kQH; ++j) {
+        const int h = warp - kSm0 + j * kSmWarps;
+        const float unit = stage_query<NH>(query[j], p.scale_log2, h, lane, sgen);
         if (lane == 0) units_s[h] = unit;
       }
       ptx::fence_proxy_async_smem();
@@ -936,22 +974,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (p.clustered) break;
       // A unit of its own: O^T / L from tensor memory to the output.  The next unit's first PV
       // comes after these reads, as it needs this warp's P.
-      float coef[kHT];
+      // Lane h of every warp computes head h's weight 1 / L; quadrant 0's also its lse.
+      float mine = 0.f;
       float* lse_s = reinterpret_cast<float*>(sgen + C::OFF_LSE);
+      if (lane < kHT) {
+        float L = 0.f, m = 0.f;
 #pragma unroll
-      for (int h = 0; h < kHT; ++h) {
-        const float* sums = red + hh * kQuads * kHT + h;
-        float L = sums[0];
+        for (int q = 0; q < kQuads; ++q) L += red[(hh * kQuads + q) * kHT + lane];
+        mine = aborted ? NAN : L == 0.f ? 0.f : 1.f / L * (u * (1.f / kPScale));  // as the merge rounds it
+        if (qd == 0) {
 #pragma unroll
-        for (int q = 1; q < kQuads; ++q) L += sums[q * kHT];
-        coef[h] = aborted ? NAN : L == 0.f ? 0.f : 1.f / L * (u * (1.f / kPScale));  // as the merge rounds it
-        if (qd == 0 && lane == 0) {
-          const float m = -((h & 1) ? m_neg[h / 2].y : m_neg[h / 2].x);
+          for (int h = 0; h < kHT; ++h) m = lane == h ? -((h & 1) ? m_neg[h / 2].y : m_neg[h / 2].x) : m;
           const float lse = aborted ? NAN : L == 0.f ? -INFINITY : m + ptx::lg2(L);
-          lse_s[kHT * hh + h] = lse;
-          p.lse[row * p.lse_sb + (int64_t)(h0 + kHT * hh + h) * p.lse_sh] = lse;
+          lse_s[kHT * hh + lane] = lse;
+          p.lse[row * p.lse_sb + (int64_t)(h0 + kHT * hh + lane) * p.lse_sh] = lse;
         }
       }
+      __syncwarp();
+      float coef[kHT];
+#pragma unroll
+      for (int h = 0; h < kHT; ++h) coef[h] = __shfl_sync(0xffffffffu, mine, h);
 #pragma unroll 1
       for (int j = 0; j < 4; ++j) {
         uint32_t r[3][kHT];
@@ -985,17 +1027,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (p.clustered) {
       const float* red = reinterpret_cast<const float*>(sgen + C::OFF_P);
-      if (qd == 0 && lane == 0) {
+      if (qd == 0 && lane < kHT) {
+        float L = 0.f, m = 0.f;
 #pragma unroll
-        for (int h = 0; h < kHT; ++h) {
-          const float* sums = red + hh * kQuads * kHT + h;
-          ml[kHT * hh + h] = -((h & 1) ? m_neg[h / 2].y : m_neg[h / 2].x);
-          float L = sums[0];
+        for (int q = 0; q < kQuads; ++q) L += red[(hh * kQuads + q) * kHT + lane];
 #pragma unroll
-          for (int q = 1; q < kQuads; ++q) L += sums[q * kHT];
-          ml[NH + kHT * hh + h] = L;
-        }
-        ml[2 * NH] = u;
+        for (int h = 0; h < kHT; ++h) m = lane == h ? -((h & 1) ? m_neg[h / 2].y : m_neg[h / 2].x) : m;
+        ml[kHT * hh + lane] = m;
+        ml[NH + kHT * hh + lane] = L;
+        if (lane == 0) ml[2 * NH] = u;
       }
       // O to shared memory, [head][512] (nothing was ever written to it without a live tile)
       float* o_s = reinterpret_cast<float*>(sgen + C::OFF_O);
