@@ -114,8 +114,12 @@ namespace q8 {
 // the scale grew, the earlier tokens are re-expressed in it (times old / new, an exact shift
 // of the exponent for powers of two, except where a value becomes subnormal).  One CTA owns a
 // job, so that the amax, the earlier tokens and the scale need no other CTA; a warp moves one
-// token at a time, a lane 16 of its values.  Jobs are found from the tokens: CTA c looks at
-// tokens [c * chunk, (c + 1) * chunk) and runs the jobs whose first token lies there.
+// token at a time, a lane 16 of its values.
+//
+// CTA j finds job j by a scan of the rows' job counts, a thread per row; the tokens are then
+// fetched once, while the page is looked up, and stay in registers until the scale is known
+// (blocks up to 64 tokens).  A call is a chain of four dependent loads, so this order is what
+// counts: 17k tokens in blocks of 16 took 11.0 us with the tokens read twice behind the page.
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendWarps = kAppendThreads / 32;
@@ -129,7 +133,6 @@ struct AppendParams {
   const int32_t* starts;
   int32_t rows;
   int32_t tokens;
-  int32_t chunk;
   PageTable table;
   Cache cache;
   uint32_t* err;
@@ -140,114 +143,166 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a <= 3.402823466e38f ? a : 0.f;  // infinities and NaN take no part in the scale
 }
 
+__device__ __forceinline__ float amax16(const uint4 (&v)[2]) {
+  float a = 0.f, f[8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    unpack8(v[h], f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_abs(f[j]));
+  }
+  return a;
+}
+
+// kPer: tokens a warp keeps in registers (kPer * 8 >= block); 0: read again (larger blocks).
+template <int kPer>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
   __shared__ uint32_t amax_s;
+  __shared__ int sums_s[kAppendWarps];
+  __shared__ int job_s[4];  // row, first token, its position, tokens (0: no such job)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int block = 1 << p.cache.block_shift;
+  const int shift = p.cache.block_shift, block = 1 << shift;
+  if (threadIdx.x == 0) {
+    amax_s = 0u;
+    job_s[3] = 0;
+  }
   ptx::grid_dep_wait();
   ptx::launch_dependents();
-  const int last = min(p.tokens, max(0, __ldg(p.offsets + p.rows)));
-  int t = (int)blockIdx.x * p.chunk;
-  const int t_end = min(t + p.chunk, last);
-  if (t >= t_end) return;
-  // the row of token t: offsets are ascending, so it is how many of offsets[1..rows] are <= t
-  int row = 0;
-  for (int i0 = 0; i0 < p.rows; i0 += kAppendThreads) {
-    const int i = i0 + (int)threadIdx.x;
-    row += __syncthreads_count(i < p.rows && __ldg(p.offsets + i + 1) <= t);
+  // ---- the job: the rows' counts of touched blocks, summed in order
+  for (int r0 = 0, before = 0; r0 < p.rows; r0 += kAppendThreads) {
+    const int r = r0 + (int)threadIdx.x;
+    int jobs = 0, lo = 0, n = 0, start = 0;
+    if (r < p.rows) {
+      lo = min(max(__ldg(p.offsets + r), 0), p.tokens);
+      n = min(max(__ldg(p.offsets + r + 1), 0), p.tokens) - lo;
+      start = __ldg(p.starts + r);
+      if (n > 0) {
+        if (start < 0 || start > INT32_MAX - block - n)  // the row has no such positions
+          atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
+        else
+          jobs = ((start + n - 1) >> shift) - (start >> shift) + 1;
+      }
+    }
+    int incl = jobs;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) sums_s[warp] = incl;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < kAppendWarps; ++w) {
+      if (w < warp) incl += sums_s[w];
+      total += sums_s[w];
+    }
+    const int j = (int)blockIdx.x - before - (incl - jobs);  // which of this row's jobs
+    if (j >= 0 && j < jobs) {
+      const int pos = j == 0 ? start : ((start >> shift) + j) << shift;
+      job_s[0] = r;
+      job_s[1] = lo + (pos - start);
+      job_s[2] = pos;
+      job_s[3] = min(block - (pos & (block - 1)), start + n - pos);
+    }
+    __syncthreads();
+    before += total;
+    if (before > (int)blockIdx.x) break;
   }
-  for (; t < t_end;) {
-    while (row < p.rows && __ldg(p.offsets + row + 1) <= t) ++row;
-    if (row >= p.rows) return;
-    const int lo = __ldg(p.offsets + row), hi = min(__ldg(p.offsets + row + 1), last);
-    if (t < lo) {  // tokens before the first row
-      t = min(lo, t_end);
-      continue;
+  const int row = job_s[0], t = job_s[1], pos = job_s[2], n = job_s[3];
+  if (n == 0) return;
+  const int in_block = pos & (block - 1);
+  // ---- the new tokens, on the way while their slots are looked up
+  constexpr int kRegs = kPer > 0 ? kPer : 1;
+  uint4 raw[kRegs][2];
+  auto token = [&](int i) {
+    return reinterpret_cast<const uint4*>(p.ckv + (int64_t)(t + i) * p.ckv_sb) + 2 * lane;
+  };
+  if (kPer > 0) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int i = warp + k * kAppendWarps;
+      if (i < n) {
+        raw[k][0] = __ldg(token(i));
+        raw[k][1] = __ldg(token(i) + 1);
+      }
     }
-    const int64_t start = __ldg(p.starts + row);
-    const int64_t pos64 = start + (t - lo);
-    if (start < 0 || pos64 + block > INT32_MAX) {  // the row has no such positions
-      if (threadIdx.x == 0) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
-      t = hi;
-      continue;
-    }
-    const int pos = (int)pos64;
-    const int in_block = pos & (block - 1);
-    const int n = min(block - in_block, hi - t);  // tokens of this row left in the block
-    if (t > lo && in_block != 0) {                // not a job's first token
-      t += n;
-      continue;
-    }
-    const int slot0 = slot_at(p.table, row, pos, p.cache.num_slots);
-    if (slot0 < 0) {
-      if (threadIdx.x == 0) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
-      t += n;
-      continue;
-    }
-    if (threadIdx.x == 0) amax_s = 0u;
-    __syncthreads();
-    float a = 0.f;
+  }
+  const int slot0 = slot_at(p.table, row, pos, p.cache.num_slots);
+  if (slot0 < 0) {
+    if (threadIdx.x == 0) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
+    return;
+  }
+  const float old = in_block != 0 ? p.cache.scale[slot0 >> shift] : 0.f;
+  float a = 0.f;
+  if (kPer > 0) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      if (warp + k * kAppendWarps < n) a = fmaxf(a, amax16(raw[k]));
+  } else {
     for (int i = warp; i < n; i += kAppendWarps) {
-      const uint4* src = reinterpret_cast<const uint4*>(p.ckv + (int64_t)(t + i) * p.ckv_sb) + 2 * lane;
+      raw[0][0] = __ldg(token(i));
+      raw[0][1] = __ldg(token(i) + 1);
+      a = fmaxf(a, amax16(raw[0]));
+    }
+  }
+  a = ptx::warp_max(a);
+  if (lane == 0) atomicMax(&amax_s, __float_as_uint(a));  // non-negative floats order as bits
+  __syncthreads();
+  const float scale = fmaxf(scale_for(__uint_as_float(amax_s)), old);
+  if (scale != old) {
+    const float ratio = old / scale;
+    for (int i = warp; i < in_block; i += kAppendWarps) {
+      uint4* q = reinterpret_cast<uint4*>(p.cache.ckv + (int64_t)(slot0 - in_block + i) * p.cache.ckv_ss) + lane;
+      *q = rescale16(*q, ratio);
+    }
+    if (threadIdx.x == 0) p.cache.scale[slot0 >> shift] = scale;
+  }
+  // 1 / scale is exact for a power of two; a caller's other scales take the division
+  const bool pow2 = (__float_as_uint(scale) & 0x7FFFFFu) == 0u;
+  const float inv = 1.f / scale;
+  auto put = [&](int i, const uint4 (&v)[2]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
       float f[8];
+      unpack8(v[h], f);
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        unpack8(__ldg(src + v), f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_abs(f[j]));
+      for (int j = 0; j < 8; ++j) {
+        if (isinf(f[j])) f[j] = NAN;  // e4m3 has no infinities
+        f[j] = pow2 ? f[j] * inv : f[j] / scale;
       }
+      w[2 * h] = to_e4m3x2(f[0], f[1]) | (to_e4m3x2(f[2], f[3]) << 16);
+      w[2 * h + 1] = to_e4m3x2(f[4], f[5]) | (to_e4m3x2(f[6], f[7]) << 16);
     }
+    const int64_t slot = slot0 + i;
+    reinterpret_cast<uint4*>(p.cache.ckv + slot * p.cache.ckv_ss)[lane] = make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  // the rope keys: four tokens at a time, eight lanes each
+  for (int i = 4 * warp + (lane >> 3); i < n; i += 4 * kAppendWarps)
+    reinterpret_cast<uint4*>(p.cache.kpe + (int64_t)(slot0 + i) * p.cache.kpe_ss)[lane & 7] =
+        __ldg(reinterpret_cast<const uint4*>(p.kpe + (int64_t)(t + i) * p.kpe_sb) + (lane & 7));
+  if (kPer > 0) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-    if (lane == 0) atomicMax(&amax_s, __float_as_uint(a));  // non-negative floats order as bits
-    const float before = in_block != 0 ? p.cache.scale[slot0 >> p.cache.block_shift] : 0.f;
-    __syncthreads();
-    const float need = scale_for(__uint_as_float(amax_s));
-    const float scale = fmaxf(need, before);
-    if (scale != before) {
-      const float ratio = before / scale;
-      for (int i = warp; i < in_block; i += kAppendWarps) {
-        uint4* q = reinterpret_cast<uint4*>(p.cache.ckv + (int64_t)(slot0 - in_block + i) * p.cache.ckv_ss) + lane;
-        *q = rescale16(*q, ratio);
-      }
-      if (threadIdx.x == 0) p.cache.scale[slot0 >> p.cache.block_shift] = scale;
-    }
-    // 1 / scale is exact for a power of two; a caller's other scales take the division
-    const bool pow2 = (__float_as_uint(scale) & 0x7FFFFFu) == 0u;
-    const float inv = 1.f / scale;
+    for (int k = 0; k < kPer; ++k)
+      if (warp + k * kAppendWarps < n) put(warp + k * kAppendWarps, raw[k]);
+  } else {
     for (int i = warp; i < n; i += kAppendWarps) {
-      const uint4* src = reinterpret_cast<const uint4*>(p.ckv + (int64_t)(t + i) * p.ckv_sb) + 2 * lane;
-      uint32_t w[4];
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        float f[8];
-        unpack8(__ldg(src + v), f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (isinf(f[j])) f[j] = NAN;  // e4m3 has no infinities
-          f[j] = pow2 ? f[j] * inv : f[j] / scale;
-        }
-        w[2 * v] = to_e4m3x2(f[0], f[1]) | (to_e4m3x2(f[2], f[3]) << 16);
-        w[2 * v + 1] = to_e4m3x2(f[4], f[5]) | (to_e4m3x2(f[6], f[7]) << 16);
-      }
-      const int64_t slot = slot0 + i;
-      reinterpret_cast<uint4*>(p.cache.ckv + slot * p.cache.ckv_ss)[lane] =
-          make_uint4(w[0], w[1], w[2], w[3]);
-      if (lane < 8)
-        reinterpret_cast<uint4*>(p.cache.kpe + slot * p.cache.kpe_ss)[lane] =
-            __ldg(reinterpret_cast<const uint4*>(p.kpe + (int64_t)(t + i) * p.kpe_sb) + lane);
+      raw[0][0] = __ldg(token(i));
+      raw[0][1] = __ldg(token(i) + 1);
+      put(i, raw[0]);
     }
-    t += n;
-    __syncthreads();  // amax_s is rewritten by the next job
   }
 }
 
 // --------------------------------------------------------------------------- accumulate
 //
 // acc[r][positions[t][k]] += weights[t][k] for the tokens t of row r.  Tokens of one row may
-// name the same position, so one CTA adds a row's tokens in order, a barrier between them;
-// with one token per row the entries are independent and spread over CTAs of 256.  The adds
-// are fire-and-forget reductions, also right when a token names a position twice.
+// name the same position, so one CTA adds a row's tokens in a fixed order, a barrier between
+// them, with the entries of eight tokens fetched ahead (one at a time, 16 rows of 8 x 1500
+// entries took 8.0 us); with one token per row the entries are independent and spread over CTAs
+// of 256.  The adds are fire-and-forget reductions, also right when a token names a position
+// twice.
 
 struct AccumulateParams {
   const float* weights;
@@ -263,10 +318,8 @@ struct AccumulateParams {
   uint32_t* err;
 };
 
-__device__ __forceinline__ void accumulate_entry(const AccumulateParams& p, float* row, int64_t t,
-                                                 int k) {
-  const int pos = __ldg(p.positions + t * p.pos_sb + k);
-  const float w = __ldg(p.weights + t * p.w_sb + k);
+__device__ __forceinline__ void accumulate_entry(const AccumulateParams& p, float* row, int pos,
+                                                 float w) {
   if (pos >= 0 && pos < p.acc_cols)
     atomicAdd(row + pos, w);
   else if (pos != -1)
@@ -278,18 +331,35 @@ __global__ void __launch_bounds__(256) accumulate_kernel(const AccumulateParams 
   ptx::launch_dependents();
   const int64_t t = blockIdx.x;
   const int k = (int)(blockIdx.y * 256 + threadIdx.x);
-  if (k < p.topk) accumulate_entry(p, p.acc + t * p.acc_sb, t, k);
+  if (k < p.topk)
+    accumulate_entry(p, p.acc + t * p.acc_sb, __ldg(p.positions + t * p.pos_sb + k),
+                     __ldg(p.weights + t * p.w_sb + k));
 }
 
 __global__ void __launch_bounds__(1024) accumulate_tokens_kernel(const AccumulateParams p) {
+  constexpr int kAhead = 8;
   ptx::grid_dep_wait();
   ptx::launch_dependents();
   const int64_t r = blockIdx.x;
   const int lo = max(0, __ldg(p.offsets + r)), hi = min(p.tokens, __ldg(p.offsets + r + 1));
-  for (int t = lo; t < hi; ++t) {
-    for (int k = threadIdx.x; k < p.topk; k += 1024)
-      accumulate_entry(p, p.acc + r * p.acc_sb, t, k);
-    __syncthreads();
+  float* row = p.acc + r * p.acc_sb;
+  for (int k0 = 0; k0 < p.topk; k0 += 1024) {
+    const int k = k0 + (int)threadIdx.x;
+    for (int t0 = lo; t0 < hi; t0 += kAhead) {
+      int pos[kAhead];
+      float w[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const bool has = k < p.topk && t0 + j < hi;
+        pos[j] = has ? __ldg(p.positions + (int64_t)(t0 + j) * p.pos_sb + k) : -1;
+        w[j] = has ? __ldg(p.weights + (int64_t)(t0 + j) * p.w_sb + k) : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        accumulate_entry(p, row, pos[j], w[j]);
+        __syncthreads();
+      }
+    }
   }
 }
 
@@ -355,18 +425,30 @@ __global__ void __launch_bounds__(kCompactThreads) compact_kernel(const CompactP
     }
   }
   __syncthreads();
-  for (int i = warp; i < n; i += kCompactWarps) {
-    const int src = src_s[i], dst = dst_s[i];
-    if (src < 0) continue;
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.cache.ckv + (int64_t)src * p.cache.ckv_ss) + lane);
-    uint4 pe = make_uint4(0u, 0u, 0u, 0u);
-    if (lane < 8)
-      pe = __ldg(reinterpret_cast<const uint4*>(p.cache.kpe + (int64_t)src * p.cache.kpe_ss) + lane);
-    const float ratio = new_s[i] > 0.f ? old_s[i] / new_s[i] : 0.f;
-    reinterpret_cast<uint4*>(p.cache.ckv + (int64_t)dst * p.cache.ckv_ss)[lane] =
-        ratio == 1.f ? v : rescale16(v, ratio);
-    if (lane < 8)
-      reinterpret_cast<uint4*>(p.cache.kpe + (int64_t)dst * p.cache.kpe_ss)[lane] = pe;
+  // four tokens a step, their loads first: a lane 16 bytes of each latent row, and of one of the
+  // four rope rows (eight lanes each)
+  for (int i0 = 4 * warp; i0 < n; i0 += 4 * kCompactWarps) {
+    uint4 v[4], pe = make_uint4(0u, 0u, 0u, 0u);
+    int src[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      src[j] = i0 + j < n ? src_s[i0 + j] : -1;
+      if (src[j] >= 0)
+        v[j] = __ldcs(reinterpret_cast<const uint4*>(p.cache.ckv + (int64_t)src[j] * p.cache.ckv_ss) + lane);
+    }
+    const int ip = i0 + (lane >> 3);
+    const int sp = ip < n ? src_s[ip] : -1;
+    if (sp >= 0)
+      pe = __ldcs(reinterpret_cast<const uint4*>(p.cache.kpe + (int64_t)sp * p.cache.kpe_ss) + (lane & 7));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (src[j] < 0) continue;
+      const float big = new_s[i0 + j], ratio = big > 0.f ? old_s[i0 + j] / big : 0.f;
+      reinterpret_cast<uint4*>(p.cache.ckv + (int64_t)dst_s[i0 + j] * p.cache.ckv_ss)[lane] =
+          ratio == 1.f ? v[j] : rescale16(v[j], ratio);
+    }
+    if (sp >= 0)
+      reinterpret_cast<uint4*>(p.cache.kpe + (int64_t)dst_s[ip] * p.cache.kpe_ss)[lane & 7] = pe;
   }
 }
 
@@ -459,14 +541,19 @@ extern "C" int dsa_append_q8(const void* ckv, int64_t ckv_stride_t, const void* 
   p.starts = starts;
   p.rows = num_rows;
   p.tokens = (int32_t)num_tokens;
-  // about eight CTAs per SM of a B200, one token each while the call is small
-  p.chunk = (int32_t)((num_tokens + 1183) / 1184);
   p.table = q8::PageTable{page_table, page_table_stride_b, page_table_cols, q8::log2_of(page_size)};
   p.cache = q8::cache_of(ckv_q8, ckv_slot_stride, ckv_scale, kpe_cache, kpe_slot_stride, num_slots,
                          block);
   p.err = static_cast<uint32_t*>(workspace);
-  return q8::launch(q8::append_kernel, dim3((unsigned)((num_tokens + p.chunk - 1) / p.chunk)),
-                    q8::kAppendThreads, static_cast<cudaStream_t>(stream), p);
+  // a job has at least one token, and all but a row's first and last fill a block
+  const int64_t bound = num_tokens / block + 2 * (int64_t)num_rows;
+  const dim3 grid((unsigned)(bound < num_tokens ? bound : num_tokens));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (block <= 2 * q8::kAppendWarps)
+    return q8::launch(q8::append_kernel<2>, grid, q8::kAppendThreads, st, p);
+  if (block <= 8 * q8::kAppendWarps)
+    return q8::launch(q8::append_kernel<8>, grid, q8::kAppendThreads, st, p);
+  return q8::launch(q8::append_kernel<0>, grid, q8::kAppendThreads, st, p);
 }
 
 extern "C" int dsa_accumulate_weights(const float* weights, int64_t weights_stride_t,

@@ -253,9 +253,8 @@ int dsa_append_q8(const void* ckv, int64_t ckv_stride_t, const void* kpe, int64_
  * acc[r][positions[t][k]] += weights[t][k] for every token t of row r and every entry k whose
  * position is not -1: the running totals of the decode's attention weights.  row_offsets
  * (num_rows + 1 ascending int32) gives the tokens of each row; NULL: token r is row r.
- * A row's tokens are added in order, so distinct positions per token give the same bits in
- * every run; a position that one token names more than once is counted as often, in no fixed
- * order.
+ * The sums have one order, so distinct positions per token give the same bits in every run; a
+ * position that one token names more than once is counted as often, in no fixed order.
  */
 int dsa_accumulate_weights(const float* weights, int64_t weights_stride_t,
                            const int32_t* positions, int64_t positions_stride_t,
