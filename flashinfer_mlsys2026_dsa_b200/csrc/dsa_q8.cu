@@ -298,11 +298,12 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
 // --------------------------------------------------------------------------- accumulate
 //
 // acc[r][positions[t][k]] += weights[t][k] for the tokens t of row r.  Tokens of one row may
-// name the same position, so one CTA adds a row's tokens in a fixed order, a barrier between
-// them, with the entries of eight tokens fetched ahead (one at a time, 16 rows of 8 x 1500
-// entries took 8.0 us); with one token per row the entries are independent and spread over CTAs
-// of 256.  The adds are fire-and-forget reductions, also right when a token names a position
-// twice.
+// name the same position, so a CTA adds them in a fixed order, a barrier between them, with the
+// entries of eight tokens fetched ahead.  An SM passes on about one scattered reduction per
+// clock, so a row is dealt out to up to eight CTAs by position: each reads all entries and adds
+// those of its own 32-byte sectors, which keeps every position's order.  With one token per row
+// the entries are independent and spread over CTAs of 256.  The adds are fire-and-forget
+// reductions, also right when a token names a position twice.
 
 struct AccumulateParams {
   const float* weights;
@@ -318,12 +319,14 @@ struct AccumulateParams {
   uint32_t* err;
 };
 
+// share of shares: the CTA's part of the row's positions, by sectors of eight
 __device__ __forceinline__ void accumulate_entry(const AccumulateParams& p, float* row, int pos,
-                                                 float w) {
-  if (pos >= 0 && pos < p.acc_cols)
-    atomicAdd(row + pos, w);
-  else if (pos != -1)
+                                                 float w, uint32_t share, uint32_t shares) {
+  if (pos >= 0 && pos < p.acc_cols) {
+    if ((((uint32_t)pos >> 3) & (shares - 1)) == share) atomicAdd(row + pos, w);
+  } else if (pos != -1) {
     atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
+  }
 }
 
 __global__ void __launch_bounds__(256) accumulate_kernel(const AccumulateParams p) {
@@ -333,30 +336,35 @@ __global__ void __launch_bounds__(256) accumulate_kernel(const AccumulateParams 
   const int k = (int)(blockIdx.y * 256 + threadIdx.x);
   if (k < p.topk)
     accumulate_entry(p, p.acc + t * p.acc_sb, __ldg(p.positions + t * p.pos_sb + k),
-                     __ldg(p.weights + t * p.w_sb + k));
+                     __ldg(p.weights + t * p.w_sb + k), 0u, 1u);
 }
 
 __global__ void __launch_bounds__(1024) accumulate_tokens_kernel(const AccumulateParams p) {
-  constexpr int kAhead = 8;
+  constexpr int kAhead = 8, kPer = 2;  // tokens, and entries of each, that a thread fetches at once
   ptx::grid_dep_wait();
   ptx::launch_dependents();
   const int64_t r = blockIdx.x;
   const int lo = max(0, __ldg(p.offsets + r)), hi = min(p.tokens, __ldg(p.offsets + r + 1));
   float* row = p.acc + r * p.acc_sb;
-  for (int k0 = 0; k0 < p.topk; k0 += 1024) {
-    const int k = k0 + (int)threadIdx.x;
+  for (int k0 = 0; k0 < p.topk; k0 += 1024 * kPer) {
     for (int t0 = lo; t0 < hi; t0 += kAhead) {
-      int pos[kAhead];
-      float w[kAhead];
+      int pos[kAhead][kPer];
+      float w[kAhead][kPer];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const bool has = k < p.topk && t0 + j < hi;
-        pos[j] = has ? __ldg(p.positions + (int64_t)(t0 + j) * p.pos_sb + k) : -1;
-        w[j] = has ? __ldg(p.weights + (int64_t)(t0 + j) * p.w_sb + k) : 0.f;
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) {
+          const int k = k0 + c * 1024 + (int)threadIdx.x;
+          const bool has = k < p.topk && t0 + j < hi;
+          pos[j][c] = has ? __ldg(p.positions + (int64_t)(t0 + j) * p.pos_sb + k) : -1;
+          w[j][c] = has ? __ldg(p.weights + (int64_t)(t0 + j) * p.w_sb + k) : 0.f;
+        }
       }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        accumulate_entry(p, row, pos[j], w[j]);
+#pragma unroll
+        for (int c = 0; c < kPer; ++c)
+          accumulate_entry(p, row, pos[j][c], w[j][c], blockIdx.y, gridDim.y);
         __syncthreads();
       }
     }
@@ -369,86 +377,85 @@ __global__ void __launch_bounds__(1024) accumulate_tokens_kernel(const Accumulat
 // slot of that position in the row's pages to slot j of its new pages.  The scale of a new
 // block is the largest scale among the tokens that move into it, and every token is
 // re-expressed in it, as in the append.  A CTA owns 64 consecutive entries of a row (or one
-// block, if that is larger), which are whole blocks of the new pages.
+// block, if that is larger), which are whole blocks of the new pages, and a warp eight of them:
+// it looks their slots up and has all eight tokens on the way before the scales are compared,
+// so that the chain keep -> page -> token is all that a CTA waits for, and an SM holds 32 warps
+// of 5 kB in flight.
 
-constexpr int kCompactThreads = 256;
-constexpr int kCompactWarps = kCompactThreads / 32;
 constexpr int kCompactSpan = 64;
+constexpr int kWarpEntries = 8;
 constexpr int kMaxBlock = 256;  // tokens per scale
 
 struct CompactParams {
   const int32_t* keep;
   int64_t keep_sb;
   int32_t cols;
-  int32_t span;  // entries per CTA
   PageTable from, to;
   Cache cache;
   uint32_t* err;
 };
 
-__global__ void __launch_bounds__(kCompactThreads) compact_kernel(const CompactParams p) {
-  __shared__ int src_s[kMaxBlock], dst_s[kMaxBlock];
-  __shared__ float old_s[kMaxBlock], new_s[kMaxBlock];  // scales per entry
+__global__ void __launch_bounds__(kMaxBlock / kWarpEntries * 32) compact_kernel(const CompactParams p) {
+  __shared__ uint32_t scale_s[kMaxBlock];  // by new block: its scale's bits
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int span = (int)blockDim.x / 32 * kWarpEntries;  // entries per CTA
+  if ((int)threadIdx.x < span) scale_s[threadIdx.x] = 0u;
   ptx::grid_dep_wait();
   ptx::launch_dependents();
   const int64_t row = blockIdx.x;
-  const int j0 = (int)blockIdx.y * p.span;
-  const int n = min(p.span, p.cols - j0);
-  const int block = 1 << p.cache.block_shift;
-  for (int i = threadIdx.x; i < n; i += kCompactThreads) {
-    const int pos = __ldg(p.keep + row * p.keep_sb + j0 + i);
-    int src = -1, dst = -1;
+  const int first = warp * kWarpEntries;  // of the CTA's entries
+  const int j0 = (int)blockIdx.y * span + first;
+  // ---- lane e: entry e
+  int src = -1, dst = -1;
+  if (lane < kWarpEntries && j0 + lane < p.cols) {
+    const int pos = __ldg(p.keep + row * p.keep_sb + j0 + lane);
     if (pos != -1) {
       src = slot_at(p.from, row, pos, p.cache.num_slots);
-      dst = slot_at(p.to, row, j0 + i, p.cache.num_slots);
+      dst = slot_at(p.to, row, j0 + lane, p.cache.num_slots);
       if (src < 0 || dst < 0) {
         atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
         src = -1;
       }
     }
-    src_s[i] = src;
-    dst_s[i] = dst;
-    old_s[i] = src >= 0 ? __ldg(p.cache.scale + (src >> p.cache.block_shift)) : 0.f;
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kCompactThreads) {
-    const int b0 = i & ~(block - 1);
-    float big = 0.f;
-    for (int e = b0; e < min(b0 + block, n); ++e) big = fmaxf(big, old_s[e]);
-    new_s[i] = big;
-    // the first entry of the block that moves writes the block's scale
-    if (src_s[i] >= 0) {
-      bool first = true;
-      for (int e = b0; e < i; ++e) first = first && src_s[e] < 0;
-      if (first) p.cache.scale[dst_s[i] >> p.cache.block_shift] = big;
-    }
+  const float old = src >= 0 ? __ldg(p.cache.scale + (src >> p.cache.block_shift)) : 0.f;
+  // ---- the tokens: a lane 16 bytes of each latent row, and of one of four rope rows at a time
+  uint4 v[kWarpEntries], pe[kWarpEntries / 4];
+#pragma unroll
+  for (int e = 0; e < kWarpEntries; ++e) {
+    const int from = __shfl_sync(0xffffffffu, src, e);
+    if (from >= 0)
+      v[e] = __ldcs(reinterpret_cast<const uint4*>(p.cache.ckv + (int64_t)from * p.cache.ckv_ss) + lane);
   }
+#pragma unroll
+  for (int e = 0; e < kWarpEntries / 4; ++e) {
+    const int from = __shfl_sync(0xffffffffu, src, 4 * e + (lane >> 3));
+    if (from >= 0)
+      pe[e] = __ldcs(reinterpret_cast<const uint4*>(p.cache.kpe + (int64_t)from * p.cache.kpe_ss) + (lane & 7));
+  }
+  // ---- the new blocks' scales (non-negative floats order as bits)
   __syncthreads();
-  // four tokens a step, their loads first: a lane 16 bytes of each latent row, and of one of the
-  // four rope rows (eight lanes each)
-  for (int i0 = 4 * warp; i0 < n; i0 += 4 * kCompactWarps) {
-    uint4 v[4], pe = make_uint4(0u, 0u, 0u, 0u);
-    int src[4];
+  uint32_t* const block_s = scale_s + ((first + (lane & (kWarpEntries - 1))) >> p.cache.block_shift);
+  if (src >= 0) atomicMax(block_s, __float_as_uint(old));
+  __syncthreads();
+  const float big = __uint_as_float(*block_s);
+  const float ratio = big > 0.f ? old / big : 0.f;
+  // every entry that moves into a block writes the same scale
+  if (src >= 0) p.cache.scale[dst >> p.cache.block_shift] = big;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      src[j] = i0 + j < n ? src_s[i0 + j] : -1;
-      if (src[j] >= 0)
-        v[j] = __ldcs(reinterpret_cast<const uint4*>(p.cache.ckv + (int64_t)src[j] * p.cache.ckv_ss) + lane);
-    }
-    const int ip = i0 + (lane >> 3);
-    const int sp = ip < n ? src_s[ip] : -1;
-    if (sp >= 0)
-      pe = __ldcs(reinterpret_cast<const uint4*>(p.cache.kpe + (int64_t)sp * p.cache.kpe_ss) + (lane & 7));
+  for (int e = 0; e < kWarpEntries; ++e) {
+    const int from = __shfl_sync(0xffffffffu, src, e), to = __shfl_sync(0xffffffffu, dst, e);
+    const float r = __shfl_sync(0xffffffffu, ratio, e);
+    if (from >= 0)
+      reinterpret_cast<uint4*>(p.cache.ckv + (int64_t)to * p.cache.ckv_ss)[lane] =
+          r == 1.f ? v[e] : rescale16(v[e], r);
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (src[j] < 0) continue;
-      const float big = new_s[i0 + j], ratio = big > 0.f ? old_s[i0 + j] / big : 0.f;
-      reinterpret_cast<uint4*>(p.cache.ckv + (int64_t)dst_s[i0 + j] * p.cache.ckv_ss)[lane] =
-          ratio == 1.f ? v[j] : rescale16(v[j], ratio);
-    }
-    if (sp >= 0)
-      reinterpret_cast<uint4*>(p.cache.kpe + (int64_t)dst_s[ip] * p.cache.kpe_ss)[lane & 7] = pe;
+  for (int e = 0; e < kWarpEntries / 4; ++e) {
+    const int from = __shfl_sync(0xffffffffu, src, 4 * e + (lane >> 3));
+    const int to = __shfl_sync(0xffffffffu, dst, 4 * e + (lane >> 3));
+    if (from >= 0)
+      reinterpret_cast<uint4*>(p.cache.kpe + (int64_t)to * p.cache.kpe_ss)[lane & 7] = pe[e];
   }
 }
 
@@ -572,8 +579,15 @@ extern "C" int dsa_accumulate_weights(const float* weights, int64_t weights_stri
                                acc,      acc_stride_r,     row_offsets,         (int32_t)num_tokens,
                                topk,     acc_cols,         static_cast<uint32_t*>(workspace)};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (row_offsets)
-    return q8::launch(q8::accumulate_tokens_kernel, dim3((unsigned)num_rows), 1024, st, p);
+  if (row_offsets) {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      return DSA_ERR_CUDA;
+    unsigned shares = 1;
+    while (shares < 8 && 2 * shares * (int64_t)num_rows <= sms) shares *= 2;
+    return q8::launch(q8::accumulate_tokens_kernel, dim3((unsigned)num_rows, shares), 1024, st, p);
+  }
   return q8::launch(q8::accumulate_kernel,
                     dim3((unsigned)num_tokens, (unsigned)((topk + 255) / 256)), 256, st, p);
 }
@@ -602,17 +616,17 @@ extern "C" int dsa_compact_q8(const int32_t* keep, int64_t keep_stride_b, int32_
   p.keep = keep;
   p.keep_sb = keep_stride_b;
   p.cols = keep_cols;
-  p.span = block > q8::kCompactSpan ? block : q8::kCompactSpan;
+  const int span = block > q8::kCompactSpan ? block : q8::kCompactSpan;
   const int shift = q8::log2_of(page_size);
   p.from = q8::PageTable{page_table, page_table_stride_b, page_table_cols, shift};
   p.to = q8::PageTable{new_page_table, new_page_table_stride_b, new_page_table_cols, shift};
   p.cache = q8::cache_of(ckv_q8, ckv_slot_stride, ckv_scale, kpe_cache, kpe_slot_stride, num_slots,
                          block);
   p.err = static_cast<uint32_t*>(workspace);
-  const int64_t spans = ((int64_t)keep_cols + p.span - 1) / p.span;
+  const int64_t spans = ((int64_t)keep_cols + span - 1) / span;
   if (spans > 65535) return DSA_ERR_INVALID_ARGUMENT;
   return q8::launch(q8::compact_kernel, dim3((unsigned)num_rows, (unsigned)spans),
-                    q8::kCompactThreads, static_cast<cudaStream_t>(stream), p);
+                    (unsigned)(span / q8::kWarpEntries * 32), static_cast<cudaStream_t>(stream), p);
 }
 
 namespace dsa {
