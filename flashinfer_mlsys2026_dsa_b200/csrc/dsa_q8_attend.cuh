@@ -24,11 +24,24 @@
 // the same from N = 16 to N = 64, so they are nearly free.
 //
 // A CTA takes one group of NH heads (16, or 32 for rows of more) of one row, or a 1/S share of
-// that group's tiles.  Tile: 96 slots (rows of the score MMA; a multiple of the PV's K = 32),
-// gathered by TMA into one of three stages of 96 x (512 + 128) bytes; whole slots fit, where
-// the bf16 pools need two CTAs for a row.  The CTAs of a row (S splits x G head groups) form a
-// cluster: splits are merged through distributed shared memory, so that no partial result
-// touches global memory, calls share no state and the sums have one order.
+// that group's tiles.  A tile is 96 slots in three stages of 96 x (512 + 128) bytes for 16 heads
+// (64-slot tiles were slower: a tile's fixed latencies are paid more often), and 128 slots in
+// two stages for 32 heads, whose queries and probabilities leave no room for a third; its slots
+// are the rows of the score MMA and a multiple of the PV's K = 32, gathered whole by TMA (the
+// bf16 pools need two CTAs for a row).  Where a call has fewer units (rows x groups) than SMs,
+// the S x G CTAs of a row form a cluster of up to eight: splits are merged through distributed
+// shared memory, so that no partial result touches global memory, calls share no state and the
+// sums have one order.  Otherwise at most one CTA per SM takes unit after unit, the gathers of
+// the next one under the last one's end.
+//
+// What bounds it.  A tile of 16 heads needs 61 kB: 1.40 us a tile at 6.5 TB/s over 148 SMs.
+// Measured: 1.50 us a tile with 16 SMs at work (the life of a stage: 3,900 cycles from the first
+// copy until it has landed, 1,000 score, 1,700 softmax, 1,600 PV and its release, over three
+// stages) and 1.70 us, 5.35 TB/s, with 148 (HBM).  Fixed cost: about 6 us a call, 2 us for each
+// further unit of a CTA.  64 rows of 16 heads and 2048 slots: 28.1 us (3.1 TB/s of the 87 MB
+// that they need; the bf16 kernel 42.5); 256 ragged rows: 90 us (44 tiles on the busiest SM, 28
+// on average); 32 rows of 128 heads: 55 us (each slot is gathered by four groups, three of
+// them from L2; the bf16 kernel 58.4); one row in eight splits: 12 us.
 //
 // Per CTA (512 threads):
 //   warps 0-4    gather producers, one per 128-byte column block of the slots; tiles without a
