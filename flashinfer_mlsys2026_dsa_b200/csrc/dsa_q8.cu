@@ -438,10 +438,10 @@ __global__ void __launch_bounds__(kMaxBlock / kWarpEntries * 32) compact_kernel(
     if (from >= 0)
       pe[e] = __ldcs(reinterpret_cast<const uint4*>(p.cache.kpe + (int64_t)from * p.cache.kpe_ss) + (lane & 7));
   }
-  // ---- the new blocks' scales (non-negative floats order as bits)
+  // ---- the new blocks' scales (non-negative floats order as bits; fabsf: a scale may be -0)
   __syncthreads();
   uint32_t* const block_s = scale_s + ((first + (lane & (kWarpEntries - 1))) >> p.cache.block_shift);
-  if (src >= 0) atomicMax(block_s, __float_as_uint(old));
+  if (src >= 0) atomicMax(block_s, __float_as_uint(fabsf(old)));
   __syncthreads();
   const float big = __uint_as_float(*block_s);
   const float ratio = big > 0.f ? old / big : 0.f;

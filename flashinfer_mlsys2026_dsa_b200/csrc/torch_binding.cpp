@@ -162,7 +162,8 @@ int64_t accumulate_weights(const at::Tensor& weights, const at::Tensor& position
                            int64_t stream) {
   const auto dev = acc.device();
   if (!plain_f32(weights, dev, 2) || !plain_i32(positions, dev, 2) || !plain_f32(acc, dev, 2) ||
-      positions.sizes() != weights.sizes() || ws.device() != dev)
+      positions.sizes() != weights.sizes() || ws.device() != dev || acc.size(1) > INT32_MAX ||
+      weights.size(1) > INT32_MAX)
     return kNotHandled;
   const int64_t T = weights.size(0), R = acc.size(0);
   if (offsets.has_value() ? !plain_i32(*offsets, dev, 1) || offsets->size(0) != R + 1 : R != T)

@@ -295,6 +295,8 @@ def accumulate_weights(weights, positions, acc, row_offsets=None) -> None:
         raise ValueError(f"positions must be {list(weights.shape)}, got {tuple(positions.shape)}")
     tokens, topk = weights.shape
     rows, cols = acc.shape
+    if cols >= 2 ** 31:
+        raise ValueError(f"acc must have less than 2**31 columns, got {cols}")
     if acc.stride(1) != 1 or (rows > 1 and acc.stride(0) < cols):
         raise ValueError(f"acc must have a unit inner stride and rows apart, got strides {acc.stride()}")
     if row_offsets is not None:
@@ -329,8 +331,10 @@ def evict_positions(acc, lengths, budget, sinks=0, recent=0, new_acc=None):
     dev = acc.device
     rows, max_len = acc.shape
     budget, sinks, recent = int(budget), int(sinks), int(recent)
-    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+    if not 1 <= budget < 2 ** 31 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"budget must be >= 1 and hold sinks + recent, got {budget}, {sinks}, {recent}")
+    if max_len >= 2 ** 31:
+        raise ValueError(f"acc must have less than 2**31 columns, got {max_len}")
     keep = torch.empty(rows, budget, dtype=torch.int32, device=dev)
     new_lengths = torch.empty(rows, dtype=torch.int32, device=dev)
     if rows == 0:

@@ -470,7 +470,8 @@ def test_append_many_rows_strides_and_refusals():
 # ------------------------------------------------------------------- accumulate, evict, compact
 
 
-@pytest.mark.parametrize("rows,per,topk,cols", [(1, 1, 1, 1), (5, 1, 700, 900), (3, 4, 257, 300), (2, 9, 1500, 1500)])
+@pytest.mark.parametrize("rows,per,topk,cols", [(1, 1, 1, 1), (5, 1, 700, 900), (3, 4, 257, 300), (2, 9, 1500, 1500),
+                                                (2, 17, 2500, 2600), (30, 8, 1025, 1100), (60, 2, 33, 100), (90, 3, 64, 64)])
 def test_accumulate(rows, per, topk, cols):
     g = torch.Generator().manual_seed(topk)
     n = rows * per
@@ -602,6 +603,75 @@ def test_compact_odd_entries_and_refusals():
     compact_q8(keep.cuda()[:, :0], *args[1:])
     compact_q8(keep.cuda()[:0], table.cuda()[:0], new.cuda()[:0], *cache)
     same_pools(cache, want)
+
+
+def test_compact_scales_of_minus_zero():
+    """A block of scale -0 beside one of a positive scale: the values keep what they stand for."""
+    cache = ref.pools(3, 16, 4, 5)
+    cache[1][0, 0] = -0.0
+    keep = torch.tensor([[1, 5, 9, 2]], dtype=torch.int32)
+    table, new = torch.tensor([[0]], dtype=torch.int32), torch.tensor([[2]], dtype=torch.int32)
+    before = ref.values(*cache[:2])
+    compact_q8(keep.cuda(), table.cuda(), new.cuda(), *cache)
+    after = ref.values(*cache[:2])
+    assert cache[1][2, 0] == cache[1][0, 1:3].max()
+    # one more rounding to e4m3: 2^-4 of the value, or half its smallest step, 2^-10 scales
+    want = before[keep[0].long()]
+    assert ((after[32:36] - want).abs() <= 2.0 ** -4 * want.abs() + 2.0 ** -10 * float(cache[1][2, 0])).all()
+
+
+def test_a_step_in_a_graph_on_another_stream():
+    """Append, decode with weights, accumulate, evict and compact, captured as one graph from a
+    stream that owns none of the tensors, and replayed; the same bits as the eager calls."""
+    rows, page, block, length = 6, 16, 4, 150
+    cols = 16
+    table = tables(rows, 2 * cols, 2 * rows * cols, 9)
+    old, new = table[:, :cols].contiguous().cuda(), table[:, cols:].contiguous().cuda()
+    x, k = (t.cuda() for t in tokens(2 * rows, 77))
+    q = queries(2 * rows, 16, 5)
+    off = (2 * torch.arange(rows + 1)).to(torch.int32).cuda()
+    starts = torch.full((rows,), length, dtype=torch.int32).cuda()
+    lens = starts + 2
+    g = torch.Generator().manual_seed(3)
+    pos = torch.stack([torch.randperm(length + 2, generator=g)[:100] for _ in range(2 * rows)]).to(torch.int32).cuda()
+    per_token = old.repeat_interleave(2, 0)
+
+    def step(cache, acc):
+        out = torch.empty(2 * rows, 16, 512, dtype=torch.bfloat16, device="cuda")
+        lse, w = torch.empty(2 * rows, 16, device="cuda"), torch.empty(2 * rows, 100, device="cuda")
+        new_acc = torch.empty(rows, 64, device="cuda")
+        append_q8(x, k, off, starts, old, *cache)
+        kernel_q8_paged(*q, *cache, per_token, pos, SM, out, lse, weights=w)
+        accumulate_weights(w, pos, acc, off)
+        keep, n = evict_positions(acc, lens, 64, sinks=2, recent=8, new_acc=new_acc)
+        compact_q8(keep, old, new, *cache)
+        return out, lse, w, keep, n, new_acc
+
+    def fresh():
+        return ref.pools(2 * rows * cols, page, block, 21), torch.zeros(rows, 200, device="cuda")
+
+    cache, acc = fresh()
+    want = [t.clone() for t in step(cache, acc)] + [acc] + [t.clone() for t in cache]
+    cache, acc = fresh()
+    start = [t.clone() for t in (*cache, acc)]
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        step(cache, acc)
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            got = step(cache, acc)
+    other = torch.cuda.Stream()
+    for _ in range(3):
+        for t, s in zip((*cache, acc), start):
+            t.view(torch.uint8).copy_(s.view(torch.uint8))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((*got, acc, *cache), want):
+            assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+    assert read_device_errors() == 0
 
 
 # ------------------------------------------------------------------------------ all together
