@@ -119,12 +119,10 @@ namespace q8 {
 // CTA j finds job j by a scan of the rows' job counts, a thread per row; the tokens are then
 // fetched once, while the page is looked up, and stay in registers until the scale is known
 // (blocks up to 64 tokens).  A call is a chain of four dependent loads, so this order is what
-// counts.  Measured: 13.3k tokens of 12 prompts, blocks of 16: 8.8 us, 2.7 TB/s (floor 3.7 us; 11.0 us
-// with the tokens read twice, behind the page); one token for each of 64 rows: 3.2 us, of which an
-// empty launch is about 2.
-
-constexpr int kAppendThreads = 256;
-constexpr int kAppendWarps = kAppendThreads / 32;
+// counts.  Measured: 13.3k tokens of 12 prompts, blocks of 16: 8.2 us, 2.9 TB/s (floor 3.7 us;
+// 8.8 us with CTAs of eight warps, which do not all fit on the GPU at once, and 11.0 us with the
+// tokens read twice, behind the page); one token for each of 64 rows: 3.2 us, of which an empty
+// launch is about 2.
 
 struct AppendParams {
   const __nv_bfloat16* ckv;
@@ -156,11 +154,12 @@ __device__ __forceinline__ float amax16(const uint4 (&v)[2]) {
   return a;
 }
 
-// kPer: tokens a warp keeps in registers (kPer * 8 >= block); 0: read again (larger blocks).
-template <int kPer>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
+// kPer: tokens a warp keeps in registers (kPer * kWarps >= block); 0: read again (larger blocks).
+template <int kWarps, int kPer>
+__global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendParams p) {
+  constexpr int kThreads = 32 * kWarps;
   __shared__ uint32_t amax_s;
-  __shared__ int sums_s[kAppendWarps];
+  __shared__ int sums_s[kWarps];
   __shared__ int job_s[4];  // row, first token, its position, tokens (0: no such job)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int shift = p.cache.block_shift, block = 1 << shift;
@@ -171,7 +170,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
   ptx::grid_dep_wait();
   ptx::launch_dependents();
   // ---- the job: the rows' counts of touched blocks, summed in order
-  for (int r0 = 0, before = 0; r0 < p.rows; r0 += kAppendThreads) {
+  for (int r0 = 0, before = 0; r0 < p.rows; r0 += kThreads) {
     const int r = r0 + (int)threadIdx.x;
     int jobs = 0, lo = 0, n = 0, start = 0;
     if (r < p.rows) {
@@ -195,7 +194,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     __syncthreads();
     int total = 0;
 #pragma unroll
-    for (int w = 0; w < kAppendWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       if (w < warp) incl += sums_s[w];
       total += sums_s[w];
     }
@@ -223,7 +222,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
   if (kPer > 0) {
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      const int i = warp + k * kAppendWarps;
+      const int i = warp + k * kWarps;
       if (i < n) {
         raw[k][0] = __ldg(token(i));
         raw[k][1] = __ldg(token(i) + 1);
@@ -240,9 +239,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
   if (kPer > 0) {
 #pragma unroll
     for (int k = 0; k < kPer; ++k)
-      if (warp + k * kAppendWarps < n) a = fmaxf(a, amax16(raw[k]));
+      if (warp + k * kWarps < n) a = fmaxf(a, amax16(raw[k]));
   } else {
-    for (int i = warp; i < n; i += kAppendWarps) {
+    for (int i = warp; i < n; i += kWarps) {
       raw[0][0] = __ldg(token(i));
       raw[0][1] = __ldg(token(i) + 1);
       a = fmaxf(a, amax16(raw[0]));
@@ -254,7 +253,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
   const float scale = fmaxf(scale_for(__uint_as_float(amax_s)), old);
   if (scale != old) {
     const float ratio = old / scale;
-    for (int i = warp; i < in_block; i += kAppendWarps) {
+    for (int i = warp; i < in_block; i += kWarps) {
       uint4* q = reinterpret_cast<uint4*>(p.cache.ckv + (int64_t)(slot0 - in_block + i) * p.cache.ckv_ss) + lane;
       *q = rescale16(*q, ratio);
     }
@@ -281,15 +280,15 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     reinterpret_cast<uint4*>(p.cache.ckv + slot * p.cache.ckv_ss)[lane] = make_uint4(w[0], w[1], w[2], w[3]);
   };
   // the rope keys: four tokens at a time, eight lanes each
-  for (int i = 4 * warp + (lane >> 3); i < n; i += 4 * kAppendWarps)
+  for (int i = 4 * warp + (lane >> 3); i < n; i += 4 * kWarps)
     reinterpret_cast<uint4*>(p.cache.kpe + (int64_t)(slot0 + i) * p.cache.kpe_ss)[lane & 7] =
         __ldg(reinterpret_cast<const uint4*>(p.kpe + (int64_t)(t + i) * p.kpe_sb) + (lane & 7));
   if (kPer > 0) {
 #pragma unroll
     for (int k = 0; k < kPer; ++k)
-      if (warp + k * kAppendWarps < n) put(warp + k * kAppendWarps, raw[k]);
+      if (warp + k * kWarps < n) put(warp + k * kWarps, raw[k]);
   } else {
-    for (int i = warp; i < n; i += kAppendWarps) {
+    for (int i = warp; i < n; i += kWarps) {
       raw[0][0] = __ldg(token(i));
       raw[0][1] = __ldg(token(i) + 1);
       put(i, raw[0]);
@@ -561,11 +560,9 @@ extern "C" int dsa_append_q8(const void* ckv, int64_t ckv_stride_t, const void* 
   const int64_t bound = num_tokens / block + 2 * (int64_t)num_rows;
   const dim3 grid((unsigned)(bound < num_tokens ? bound : num_tokens));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (block <= 2 * q8::kAppendWarps)
-    return q8::launch(q8::append_kernel<2>, grid, q8::kAppendThreads, st, p);
-  if (block <= 8 * q8::kAppendWarps)
-    return q8::launch(q8::append_kernel<8>, grid, q8::kAppendThreads, st, p);
-  return q8::launch(q8::append_kernel<0>, grid, q8::kAppendThreads, st, p);
+  if (block <= 16) return q8::launch(q8::append_kernel<4, 4>, grid, 128, st, p);
+  if (block <= 64) return q8::launch(q8::append_kernel<8, 8>, grid, 256, st, p);
+  return q8::launch(q8::append_kernel<8, 0>, grid, 256, st, p);
 }
 
 extern "C" int dsa_accumulate_weights(const float* weights, int64_t weights_stride_t,

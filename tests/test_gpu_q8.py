@@ -110,6 +110,24 @@ def test_attend_row_counts(rows, heads, topk):
     check(run(q, cache, idx, weights=False), q, cache, idx)
 
 
+@pytest.mark.parametrize("heads", [16, 64])
+def test_attend_many_rows_most_of_them_empty(heads):
+    """Twenty rows and more per SM, in runs of empty ones (also an SM's first and last)."""
+    rows, topk = 3100, 230
+    cache = ref.pools(8, 64, 16, heads)
+    g = torch.Generator().manual_seed(heads)
+    idx = torch.randint(0, 512, (rows, topk), generator=g, dtype=torch.int32)
+    cut = torch.where(torch.rand(rows, generator=g) < 0.2, torch.randint(0, topk + 1, (rows,), generator=g), 0)
+    cut[:150] = 0
+    cut[-40:] = 0
+    cut[1200:1900] = 0
+    idx[torch.arange(topk)[None] >= cut[:, None]] = -1
+    idx = idx.cuda()
+    q = queries(rows, heads, heads)
+    check(run(q, cache, idx), q, cache, idx)
+    check(run(q, cache, idx, weights=False), q, cache, idx)
+
+
 def test_attend_repeated_slots_and_long_selections():
     """A slot named twice counts twice; topk past the pool, and past 16 bits."""
     cache = ref.pools(4, 64, 32, 9)
