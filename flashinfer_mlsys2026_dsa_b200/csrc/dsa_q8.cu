@@ -664,7 +664,8 @@ int prepare_device() {
 // (* chosen; -: not measured):
 //     1 row, 16 heads, 2048 slots          38.9   23.2     -    12.0*
 //     64 rows, 16 heads, 2048 slots        41.3   28.1*    -      -
-//     256 ragged rows, 16 heads            92.1   90.7*    -      -
+//     256 ragged rows, 16 heads            90.2*  87.5     -      -
+//     256 full rows, 16 heads              87.9* 104.8     -      -
 //     7 rows, 64 heads, 1001 slots         41.0   27.6   20.7*    -
 //     32 rows, 128 heads, 2048 slots       56.8*  95.9     -      -
 int choose_splits(int64_t units, int nh, int groups, int ntiles, int sms) {
