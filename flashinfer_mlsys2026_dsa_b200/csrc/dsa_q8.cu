@@ -13,6 +13,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <atomic>
 #include <utility>
 
@@ -687,8 +688,13 @@ int choose_splits(int64_t units, int nh, int groups, int ntiles, int sms) {
 }  // namespace q8
 }  // namespace dsa
 
+// A decode with weights keeps the scores of at most this many rows at a time: 256 CTAs that take
+// row after row, or launches of 256 rows where a row is a cluster's.
+constexpr int64_t kScoreRows = 256;
+
 extern "C" size_t dsa_q8_scratch_size(int64_t num_tokens, int32_t num_heads, int32_t topk) {
   if (num_tokens < 0 || topk < 1 || !heads_supported(num_heads)) return 0;
+  if (num_tokens > kScoreRows) num_tokens = kScoreRows;
   const int nh = q8::group_heads(num_heads);
   const size_t ts = (size_t)q8::tile_slots(nh), tiles = ((size_t)topk + ts - 1) / ts;
   return (size_t)num_tokens * tiles * ((size_t)num_heads * ts + (size_t)(num_heads / nh)) * 4;
@@ -755,7 +761,7 @@ extern "C" int dsa_sparse_mla_decode_q8(
   p.scores = static_cast<float*>(scratch);
   p.tiles = weights == nullptr ? nullptr
                                : reinterpret_cast<int32_t*>(
-                                     p.scores + num_tokens * p.ntiles * num_heads * ts);
+                                     p.scores + std::min(num_tokens, kScoreRows) * p.ntiles * num_heads * ts);
   p.scale_log2 = sm_scale * kLog2e;
   p.wait_cycles = wait_limit_cycles();
   p.err = static_cast<uint32_t*>(workspace);
@@ -767,8 +773,9 @@ extern "C" int dsa_sparse_mla_decode_q8(
   // the groups' weights.  Otherwise at most one CTA per SM takes unit after unit.
   p.clustered = p.splits > 1 || (weights != nullptr && p.groups > 1);
   const int cluster = p.clustered ? p.splits * p.groups : 1;
-  const int64_t grid = p.clustered ? p.units * p.splits : (p.units < sms ? p.units : sms);
-  if (grid > INT32_MAX) return DSA_ERR_INVALID_ARGUMENT;
+  const int64_t rows = weights != nullptr && p.clustered ? std::min(num_tokens, kScoreRows) : num_tokens;
+  const int64_t ctas = std::min<int64_t>(sms, kScoreRows);
+  if (p.clustered && p.units * p.splits > INT32_MAX) return DSA_ERR_INVALID_ARGUMENT;
   // gathers of single slots: 128-byte boxes of one row
   CUtensorMap m_ckv, m_kpe;
   {
@@ -786,7 +793,6 @@ extern "C" int dsa_sparse_mla_decode_q8(
   }
   if (rc != DSA_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(q8::kThreads);
   cfg.dynamicSmemBytes = (size_t)(nh == 16 ? q8::Cfg<16>::SMEM_BYTES : q8::Cfg<32>::SMEM_BYTES);
   cfg.stream = static_cast<cudaStream_t>(stream);
@@ -798,5 +804,18 @@ extern "C" int dsa_sparse_mla_decode_q8(
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   const q8::AttendFn fn = nh == 16 ? q8::attend_kernel<16> : q8::attend_kernel<32>;
-  return cudaLaunchKernelEx(&cfg, fn, m_ckv, m_kpe, p) == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
+  // one launch, or (clusters with weights) launches of `rows` rows that use the scratch in turn
+  for (int64_t left = num_tokens; left > 0; left -= rows) {
+    p.units = std::min(rows, left) * p.groups;
+    cfg.gridDim = dim3((unsigned)(p.clustered ? p.units * p.splits : std::min(p.units, ctas)));
+    if (cudaLaunchKernelEx(&cfg, fn, m_ckv, m_kpe, p) != cudaSuccess) return DSA_ERR_CUDA;
+    p.qn += rows * p.qn_sb;
+    p.qp += rows * p.qp_sb;
+    p.idx += rows * p.idx_sb;
+    if (p.table.pt != nullptr) p.table.pt += rows * page_table_stride_b;
+    p.out += rows * p.out_sb;
+    p.lse += rows * p.lse_sb;
+    if (p.weights != nullptr) p.weights += rows * p.w_sb;
+  }
+  return DSA_OK;
 }

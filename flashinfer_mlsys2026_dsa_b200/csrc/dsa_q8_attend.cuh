@@ -70,7 +70,8 @@ struct AttendParams {
   int64_t lse_sb, lse_sh;
   float* weights;
   int64_t w_sb;
-  float* scores;    // weights only: every tile's scores, [row][group][tile][NH][kTS]
+  float* scores;    // weights only: every tile's scores, [place][tile][NH][kTS]; a unit's place is
+                    // its number if clustered, else its CTA's
   int32_t* tiles;   // weights only: the tiles a CTA ran, in the places of its scores
   int32_t topk;
   int32_t ntiles;
@@ -948,7 +949,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           if (p.weights != nullptr) {
-            const int64_t at = un * p.ntiles + split + (int64_t)live * S;
+            const int64_t at = (p.clustered ? un : (int64_t)blockIdx.x) * p.ntiles + split + (int64_t)live * S;
             float* s = p.scores + (at * NH + kHT * hh) * kTS + slot;
 #pragma unroll
             for (int j = 0; j < kHT / 2; ++j) {
@@ -1030,7 +1031,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k2 = sm_tid; k2 < p.topk; k2 += kSmThreads) p.weights[row * p.w_sb + k2] = NAN;
         } else {
           for (int64_t e = sm_tid; e < (int64_t)live * kTS; e += kSmThreads) {
-            const int64_t at = un * p.ntiles + e / kTS;
+            const int64_t at = (int64_t)blockIdx.x * p.ntiles + e / kTS;
             const int64_t k2 = (int64_t)p.tiles[at] * kTS + e % kTS;
             if (k2 < p.topk)
               p.weights[row * p.w_sb + k2] = head_sum<NH>(p.scores + at * NH * kTS + e % kTS, lse_s);

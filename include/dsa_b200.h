@@ -226,7 +226,8 @@ int dsa_sparse_mla_decode_q8(
     int64_t num_tokens, int32_t num_heads, int32_t topk, void* scratch, size_t scratch_bytes,
     void* workspace, void* stream);
 
-/* Bytes of scratch a decode with weights needs; 0 for an unsupported shape. */
+/* Bytes of scratch a decode with weights needs (no more past 256 rows); 0 for an unsupported
+ * shape. */
 size_t dsa_q8_scratch_size(int64_t num_tokens, int32_t num_heads, int32_t topk);
 
 /*

@@ -118,3 +118,14 @@ def test_accumulate_evict_and_compact_arguments():
     assert compact(rows=0) == 0 and compact(cols=0) == 0
     assert compact(cols=-1) == 1 and compact(page=32) == 1 and compact(new=[None, 4, 4]) == 1
     assert compact(ws=None) == 4 and compact(cols=1 << 23) == 1
+
+
+def test_scratch_of_a_decode_with_weights():
+    """Scores of at most 256 rows at a time: [rows, heads, whole tiles] fp32 and a tile number each."""
+    lib = _native.load()
+    size = lib.dsa_q8_scratch_size
+    assert size(1, 16, 1) == (16 * 96 + 1) * 4
+    assert size(256, 16, 2048) == 256 * 22 * (16 * 96 + 1) * 4
+    assert size(1 << 20, 16, 2048) == size(256, 16, 2048)
+    assert size(3, 128, 129) == 3 * 2 * (128 * 128 + 4) * 4
+    assert size(0, 16, 2048) == size(1, 48, 2048) == size(1, 16, 0) == size(-1, 16, 1) == 0
