@@ -88,6 +88,8 @@ struct AttendParams {
 
 constexpr int kBlocks = 5;            // 128-byte column blocks of a slot: four of ckv, one of kpe
 constexpr int kMaxStages = 3;
+constexpr int kLists = 4;             // tiles whose slots the keeper may hand out ahead
+enum : int { kTile, kUnitEnd, kDone };  // what a list stands for
 constexpr int kThreads = 512;
 constexpr int kProdWarps = 5;
 constexpr int kScore = 5, kPv = 6, kKeeper = 7, kSm0 = 8;
@@ -119,16 +121,18 @@ struct Cfg {
   static constexpr int OFF_QP = OFF_Q + 4 * kQBlk;
   static constexpr int OFF_P = OFF_QP + NH * 128;
   static constexpr int OFF_BAR = OFF_P + kPBufs * kPB;
-  static constexpr int OFF_MISC = OFF_BAR + 256;   // [0] TMEM base, [2] abort, [3] drain, [8..15] end
-                                                   // tiles of the units in flight
-  static constexpr int OFF_CMD = OFF_MISC + 64;    // [stage][8]: validity words; [4] the tile (-1: end)
+  static constexpr int OFF_MISC = OFF_BAR + 256;   // [0] TMEM base, [2] abort, [3] drain, [4..7] what
+                                                   // the lists of slots stand for
+  static constexpr int OFF_CMD = OFF_MISC + 32;    // [stage][8]: validity words; [4] the tile (-1: end)
   static constexpr int OFF_SMAX = OFF_CMD + kStages * 32;  // [stage] largest scale of the tile
   static constexpr int OFF_QS = OFF_SMAX + 16;     // [NH] score units per query row
   static constexpr int OFF_SC = OFF_QS + NH * 4;   // [stage][96] scales; at the end kMl floats
   static constexpr int kMl = 2 * NH + 1;           // a CTA's m, L and u, for the merge
   static constexpr int OFF_RED = OFF_SC + kStages * kTS * 4;  // [half][2 buffers][4 warps] votes
   static constexpr int OFF_LSE = OFF_RED + 16 * 4;  // [NH], for the weights
-  static constexpr int SMEM_BYTES = OFF_LSE + NH * 4;
+  static constexpr int OFF_LIST = OFF_LSE + NH * 4;  // [kLists][kTS] the slots to gather
+  static constexpr int SMEM_BYTES = OFF_LIST + kLists * kTS * 4;
+  static_assert(OFF_LIST % 16 == 0, "slots are read four at a time");
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
   static_assert(kMl <= kStages * kTS, "m, L and u in the scales' place");
   // after the last tile, in the stages' place: this CTA's O, then the merge's table
@@ -150,7 +154,9 @@ enum : int {
   B_PF = B_SE + 2,           // [2] P written (and O rescaled)
   B_PD = B_PF + 2,           // [2] PV done
   B_QF = B_PD + 2,           // a unit's queries staged
-  B_DRAIN = B_QF + 1,        // [2] used only when an issuer stops early
+  B_LF = B_QF + 1,           // [kLists] slots listed
+  B_LE = B_LF + kLists,      // [kLists] list read by all gatherers
+  B_DRAIN = B_LE + kLists,   // [2] used only when an issuer stops early
   B_COUNT = B_DRAIN + 2
 };
 static_assert(B_COUNT * 8 <= 256, "barrier block");
@@ -255,68 +261,50 @@ struct Entries {
 
 // ---------------------------------------------------------------- gather producers
 //
-// Warp j < 5 gathers column block j of every slot of a tile, four slots a copy, lane g < 24
-// holding the slots 4g .. 4g + 3.  One elected thread issues the copies of a warp-uniform loop:
-// 1,650 cycles a tile for the five warps, against 2,200 when each lane issues its own (and
-// 8,000 from one warp), so that HBM and not the issue is the limit.  They do nothing else: the
-// keeper (warp 7) looks at the same entries and provides the scales, the validity words and
-// the tile number, so all agree on the live tiles.
+// Warp j < 5 gathers column block j of every slot of a tile, four slots a copy, from the list that
+// the keeper (warp 7) hands out for every tile with a valid entry.  One elected thread issues the
+// copies of a warp-uniform loop: 1,650 cycles a tile for the five warps, against 2,200 when
+// each lane issues its own (and 8,000 from one warp), so that HBM and not the issue is the limit.
 template <int NH>
 __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap* map, int blk,
-                                        const Units& units, int split, int lane, uint32_t sbase,
-                                        uint8_t* sgen, const Waiter& wait) {
+                                        uint32_t sbase, uint8_t* sgen, const Waiter& wait) {
   using C = Cfg<NH>;
   constexpr int kTS = C::kTS, kStages = C::kStages, kRB = C::kRB, kStageB = C::kStageB;
   const uint32_t bar0 = sbase + (uint32_t)C::OFF_BAR;
   auto bar = [&](int k) { return bar0 + 8u * (uint32_t)k; };
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sgen + C::OFF_MISC);
-  const bool has = lane < kTS / 4;
   const int col = blk < 4 ? 128 * blk : 0;
   const bool el = ptx::elect_one();
   const uint64_t policy = ptx::policy_evict_first();
   bool ok = true;
-  int64_t n = 0;  // stages filled
+  int64_t n = 0;  // stages filled, lists read
   int st = 0;
   uint32_t phase = 0;
-  int k = 0;
-  Entries<4, kTS> in(p, 4 * lane, 1);
-  in.start(units.first >> units.shift, split, has);
-  for (int64_t un = units.first; ok && un < p.units; un += units.step, ++k) {
-    // the end tile is the keeper's to lower at any time: the lanes agree on one reading
-    for (int64_t t = split; t < __shfl_sync(0xffffffffu, (int)misc[8 + (k & 7)], 0); t += p.splits) {
-      const int4 r = make_int4(in.slot0[0], in.slot0[1], in.slot0[2], in.slot0[3]);
-      const bool live = __any_sync(0xffffffffu, r.x >= 0 || r.y >= 0 || r.z >= 0 || r.w >= 0);
-      if (live) {
-        ok = __all_sync(0xffffffffu, wait(bar(B_KVE + st), phase ^ 1u));
-        if (!ok) break;
-        const uint32_t full = bar(B_KVF + st);
-        const uint32_t dst = sbase + (uint32_t)(st * kStageB + blk * kRB);
-        if (el) ptx::mbar_arrive_expect_tx(full, (uint32_t)kRB);
-        // a slot that is none lies outside the tensor map: the copy fills its row with zeros, so
-        // that PV reads 0 * 0 there
-#pragma unroll
-        for (int g = 0; g < kTS / 4; ++g) {
-          const int4 s = make_int4(__shfl_sync(0xffffffffu, r.x, g), __shfl_sync(0xffffffffu, r.y, g),
-                                   __shfl_sync(0xffffffffu, r.z, g), __shfl_sync(0xffffffffu, r.w, g));
-          if (el) ptx::tma_gather4(dst + (uint32_t)(g * 512), map, col, s, full, policy);
-        }
-        __syncwarp();
-        ++n;
-        if (++st == kStages) {
-          st = 0;
-          phase ^= 1u;
-        }
-      }
-      in.prefetch(t, has);  // two and three tiles ahead, so the copies go first
-      in.advance();
-    }
+  for (;; ++n) {
+    const int l = (int)(n % kLists);
+    ok = __all_sync(0xffffffffu, wait(bar(B_LF + l), (uint32_t)((n / kLists) & 1)));
     if (!ok) break;
-    if (un + units.step < p.units) in.start((un + units.step) >> units.shift, split, has);
-    // the unit's end: a stage without slots
+    const int what = __shfl_sync(0xffffffffu, (int)misc[4 + l], 0);
+    if (what == kDone) break;
     ok = __all_sync(0xffffffffu, wait(bar(B_KVE + st), phase ^ 1u));
     if (!ok) break;
-    if (el) ptx::mbar_arrive(bar(B_KVF + st));
-    ++n;
+    const uint32_t full = bar(B_KVF + st);
+    if (what == kTile) {
+      const int4* slots = reinterpret_cast<const int4*>(sgen + C::OFF_LIST) + l * (kTS / 4);
+      const uint32_t dst = sbase + (uint32_t)(st * kStageB + blk * kRB);
+      if (el) ptx::mbar_arrive_expect_tx(full, (uint32_t)kRB);
+      // a slot that is none lies outside the tensor map: the copy fills its row with zeros, so
+      // that PV reads 0 * 0 there
+#pragma unroll
+      for (int g = 0; g < kTS / 4; ++g) {
+        const int4 s = slots[g];
+        if (el) ptx::tma_gather4(dst + (uint32_t)(g * 512), map, col, s, full, policy);
+      }
+    } else if (el) {
+      ptx::mbar_arrive(full);  // the unit's end: a stage without slots
+    }
+    __syncwarp();
+    if (el) ptx::mbar_arrive(bar(B_LE + l));
     if (++st == kStages) {
       st = 0;
       phase ^= 1u;
@@ -363,11 +351,10 @@ struct Tail {
   }
 };
 
-// The keeper (warp 7).  Tile by tile, lane l the entries l, l + 32, ...: scales, validity, the
-// tile's number; at a unit's first tile without entries also where the row's padding begins, so
-// that nobody walks a short row's padding.  The end tiles have eight places; the gatherers are at most three
-// stages, so at most three units, ahead of the keeper, which opens a unit's place four units
-// before it.
+// The keeper (warp 7).  Tile by tile, lane l the entries l, l + 32, ...: the slots for the gatherers,
+// scales, validity and the tile's number; tiles without a valid entry are passed over, and at
+// a unit's first of them it looks where the row's padding begins, so that a short row's
+// padding is not walked.
 template <int NH>
 __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& units, int split,
                                            int lane, uint32_t sbase, uint8_t* sgen,
@@ -383,24 +370,44 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
   bool ok = true;
   int st = 0;
   uint32_t phase = 0;
-  int unit = 0;
+  int64_t lists = 0;  // handed out
   Entries<kE, kTS> in(p, lane, 32);
   Tail tail(p, lane);
+  auto hand_out = [&](int what) {
+    const int l = (int)(lists % kLists);
+    ok = __all_sync(0xffffffffu, wait(bar(B_LE + l), (uint32_t)(((lists / kLists) & 1) ^ 1)));
+    if (!ok) return;
+    if (what == kTile) {
+      int* slots = reinterpret_cast<int*>(sgen + C::OFF_LIST) + l * kTS;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) slots[32 * e + lane] = in.slot0[e];
+    }
+    if (lane == 0) misc[4 + l] = (uint32_t)what;
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(bar(B_LF + l));
+    ++lists;
+  };
   in.start(units.first >> units.shift, split, true);
   tail.load(in.ir);
-  for (int64_t un = units.first; ok && un < p.units; un += units.step, ++unit) {
-    if (lane == 0) misc[8 + ((unit + 4) & 7)] = (uint32_t)p.ntiles;
+  for (int64_t un = units.first; ok && un < p.units; un += units.step) {
     int end = p.ntiles;
     bool scanned = false;
     for (int64_t t = split; t < end; t += p.splits) {
       uint32_t w[kE], any = 0;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+        w[e] = __ballot_sync(0xffffffffu, in.slot0[e] >= 0);
+        any |= w[e];
+      }
+      if (any != 0u) {
+        hand_out(kTile);
+        if (!ok) break;
+      }
       float scale[kE], big = 0.f;
       bool bad = false;
 #pragma unroll
       for (int e = 0; e < kE; ++e) {
         const int slot = in.slot0[e];
-        w[e] = __ballot_sync(0xffffffffu, slot >= 0);
-        any |= w[e];
         bad |= slot == -2;
         scale[e] = slot >= 0 ? ldg_now(p.cache.scale + (slot >> p.cache.block_shift)) : 0.f;
       }
@@ -431,7 +438,6 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
       if (any == 0u && !scanned) {
         scanned = true;
         end = (tail.end(in.ir) + kTS - 1) / kTS;
-        if (lane == 0) misc[8 + (unit & 7)] = (uint32_t)end;
       }
       in.advance();
     }
@@ -440,6 +446,8 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
       in.start((un + units.step) >> units.shift, split, true);
       tail.load(in.ir);
     }
+    hand_out(kUnitEnd);
+    if (!ok) break;
     ok = __all_sync(0xffffffffu, wait(bar(B_KVE + st), phase ^ 1u));
     if (ok && lane == 0) {
       cmd[8 * st + 4] = -1;
@@ -450,6 +458,7 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
       phase ^= 1u;
     }
   }
+  if (ok) hand_out(kDone);
   __syncwarp();
 }
 
@@ -612,8 +621,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     misc[2] = 0;
     misc[3] = 0;
-    for (int i = 0; i < 8; ++i) misc[8 + i] = (uint32_t)p.ntiles;
     ptx::mbar_init(bar(B_QF), kSmWarps);
+    for (int l = 0; l < kLists; ++l) {
+      ptx::mbar_init(bar(B_LF + l), 1);
+      ptx::mbar_init(bar(B_LE + l), kProdWarps);
+    }
     ptx::fence_mbar_init();
     ptx::prefetch_tmap(&tm_ckv);
     ptx::prefetch_tmap(&tm_kpe);
@@ -644,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool aborted = false;
 
   if (warp < kProdWarps)
-    produce<NH>(p, warp < 4 ? &tm_ckv : &tm_kpe, warp, units, split, lane, sbase, sgen, wait);
+    produce<NH>(p, warp < 4 ? &tm_ckv : &tm_kpe, warp, sbase, sgen, wait);
   else if (warp == kKeeper)
     keep_books<NH>(p, units, split, lane, sbase, sgen, wait);
   if (warp == kScore) {
@@ -660,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = __all_sync(0xffffffffu, spin(bar(B_QF), (uint32_t)(k & 1)));
       for (; ok; ++i) {
         const int st = (int)(c % kStages), sb = (int)(i % C::kSBufs);
-        ok = __all_sync(0xffffffffu, spin(bar(B_KVF + st), (uint32_t)((c / kStages) & 1)));
+        ok = __all_sync(0xffffffffu, wait(bar(B_KVF + st), (uint32_t)((c / kStages) & 1)));
         if (!ok) break;
         const bool end = __any_sync(0xffffffffu, cmd[8 * st + 4] < 0);
         if (el) ptx::mbar_arrive(bar(B_KVE + st));
