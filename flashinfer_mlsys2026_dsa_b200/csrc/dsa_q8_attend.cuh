@@ -284,7 +284,7 @@ __device__ __forceinline__ void produce(const AttendParams& p, const CUtensorMap
     const int l = (int)(n % kLists);
     ok = __all_sync(0xffffffffu, wait(bar(B_LF + l), (uint32_t)((n / kLists) & 1)));
     if (!ok) break;
-    const int what = __shfl_sync(0xffffffffu, (int)misc[4 + l], 0);
+    const int what = (int)misc[4 + l];
     if (what == kDone) break;
     ok = __all_sync(0xffffffffu, wait(bar(B_KVE + st), phase ^ 1u));
     if (!ok) break;
@@ -388,7 +388,6 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
     ++lists;
   };
   in.start(units.first >> units.shift, split, true);
-  tail.load(in.ir);
   for (int64_t un = units.first; ok && un < p.units; un += units.step) {
     int end = p.ntiles;
     bool scanned = false;
@@ -403,6 +402,8 @@ __device__ __forceinline__ void keep_books(const AttendParams& p, const Units& u
         hand_out(kTile);
         if (!ok) break;
       }
+      // not before the call's first list; a later unit's are on the way before its first tile
+      if (un == units.first && t == split) tail.load(in.ir);
       float scale[kE], big = 0.f;
       bool bad = false;
 #pragma unroll
