@@ -662,13 +662,13 @@ int prepare_device() {
 // CTAs per (row, head group).  Per CTA about 7 us are spent outside the tiles (first gather, end;
 // 8 with the merge) and 1.4 us (16 heads) or 1.75 us (32) per tile; a call whose units do not
 // fill the SMs splits them while that shortens the longest CTA.  Measured, us for S = 1, 2, 4, 8
-// (* chosen; -: not measured):
-//     1 row, 16 heads, 2048 slots          38.9   23.2     -    12.0*
-//     64 rows, 16 heads, 2048 slots        41.3   28.1*    -      -
-//     256 ragged rows, 16 heads            90.2*  87.5     -      -
-//     256 full rows, 16 heads              87.9* 104.8     -      -
-//     7 rows, 64 heads, 1001 slots         41.0   27.6   20.7*    -
-//     32 rows, 128 heads, 2048 slots       56.8*  95.9     -      -
+// (* chosen; -: a cluster of more than eight, or not measured):
+//     1 row, 16 heads, 2048 slots          35.4   21.9   15.5   12.1*
+//     64 rows, 16 heads, 2048 slots        37.9   26.4*  36.8     -
+//     256 ragged rows, 16 heads            77.8*  82.7  125.9     -
+//     256 full rows, 16 heads              78.2*  99.6  139.1     -
+//     7 rows, 64 heads, 1001 slots         28.9   21.2   16.6*    -
+//     32 rows, 128 heads, 2048 slots       50.1*  94.2     -      -
 int choose_splits(int64_t units, int nh, int groups, int ntiles, int sms) {
   const double tile = nh == 16 ? 1.4 : 1.75;
   int best = 1;

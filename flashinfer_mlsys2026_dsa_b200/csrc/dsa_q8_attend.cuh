@@ -34,21 +34,21 @@
 // sums have one order.  Otherwise at most one CTA per SM takes unit after unit, the gathers of
 // the next one under the last one's end.
 //
-// What bounds it.  A tile of 16 heads needs 61 kB: 1.40 us a tile at 6.5 TB/s over 148 SMs.
-// Measured: 1.50 us a tile with 16 SMs at work (the life of a stage: 3,900 cycles from the first
-// copy until it has landed, 1,000 score, 1,700 softmax, 1,600 PV and its release, over three
-// stages) and 1.70 us, 5.35 TB/s, with 148 (HBM).  Fixed cost: about 6 us a call, 2 us for each
-// further unit of a CTA.  64 rows of 16 heads and 2048 slots: 28.1 us (3.1 TB/s of the 87 MB
-// that they need; the bf16 kernel 42.5); 256 ragged rows: 90 us (44 tiles on the busiest SM, 28
-// on average); 32 rows of 128 heads: 55 us (each slot is gathered by four groups, three of
-// them from L2; the bf16 kernel 58.4); one row in eight splits: 12 us.
+// What bounds it.  A tile of 16 heads needs 61 kB: 1.40 us a tile at 6.5 TB/s over 148 SMs, and
+// 120 copies of ~20 cycles of the SM's TMA unit, 1.2 us.  Measured: 1.3 us a tile for a row
+// alone on its SM, 1.54 us, 5.9 TB/s, with 148 SMs at work.  Fixed cost: about 6 us a call, 2
+// us for each further unit of a CTA.  64 rows of 16 heads and 2048 slots: 26.1 us (3.3 TB/s of
+// the 87 MB that they need; the bf16 kernel 42.5); 256 ragged rows: 78 us (44 tiles on the busiest
+// SM, 28 on average); 32 rows of 128 heads: 50 us (each slot is gathered by four groups, three
+// of them from L2; the bf16 kernel 58.4); one row in eight splits: 12 us.
 //
 // Per CTA (512 threads):
-//   warps 0-4    gather producers, one per 128-byte column block of the slots; tiles without a
-//                valid entry are skipped
+//   warps 0-4    gather producers, one per 128-byte column block of the slots
 //   warp 5       score issuer: S^T[96 slots x (hi, lo, pe)], 16 f8 + 4 bf16 MMAs
 //   warp 6       PV issuer: O^T[512 x 3 terms] += V^T P^T, 12 f8 MMAs (V^T read in place)
-//   warp 7       keeper: the tiles' scales, validity and numbers, and where the row's padding begins
+//   warp 7       keeper: the slots of every tile with a valid entry, their scales and validity, and
+//                where the row's padding begins.  (Gatherers that each looked the slots up for
+//                themselves: 256 ragged rows 90.5 us, 64 rows 28.1, 32 rows of 128 heads 54.8.)
 //   warps 8-15   softmax: warp w reads TMEM lanes 32 (w % 4) .. (slots) and half of the heads
 #pragma once
 
