@@ -117,10 +117,11 @@ namespace q8 {
 // job, so that the amax, the earlier tokens and the scale need no other CTA; a warp moves one
 // token at a time, a lane 16 of its values.
 //
-// CTA j finds job j by a scan of the rows' job counts, a thread per row; the tokens are then
-// fetched once, while the page is looked up, and stay in registers until the scale is known
-// (blocks up to 64 tokens).  A call is a chain of four dependent loads, so this order is what
-// counts.  Measured: 13.3k tokens of 12 prompts, blocks of 16: 8.2 us, 2.9 TB/s (floor 3.7 us;
+// A row of n tokens touches at most n / block + 2 blocks, so the CTAs from offset / block + 2 r on
+// are enough for row r (in a call of few tokens: the CTAs from its offset on); a CTA finds its row
+// by a search with as many branches as it has threads.  The tokens are then fetched once, while
+// the page is looked up, and stay in registers until the scale is known (blocks up to 64
+// tokens).  A call is a chain of four dependent loads, so this order is what counts.  Measured: 13.3k tokens of 12 prompts, blocks of 16: 8.2 us, 2.9 TB/s (floor 3.7 us;
 // 8.8 us with CTAs of eight warps, which do not all fit on the GPU at once, and 11.0 us with the
 // tokens read twice, behind the page); one token for each of 64 rows: 3.2 us, of which an empty
 // launch is about 2.
@@ -134,6 +135,7 @@ struct AppendParams {
   const int32_t* starts;
   int32_t rows;
   int32_t tokens;
+  bool by_token;  // a row's CTAs begin at its offset
   PageTable table;
   Cache cache;
   uint32_t* err;
@@ -160,7 +162,6 @@ template <int kWarps, int kPer>
 __global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendParams p) {
   constexpr int kThreads = 32 * kWarps;
   __shared__ uint32_t amax_s;
-  __shared__ int sums_s[kWarps];
   __shared__ int job_s[4];  // row, first token, its position, tokens (0: no such job)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int shift = p.cache.block_shift, block = 1 << shift;
@@ -170,47 +171,39 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendParams 
   }
   ptx::grid_dep_wait();
   ptx::launch_dependents();
-  // ---- the job: the rows' counts of touched blocks, summed in order
-  for (int r0 = 0, before = 0; r0 < p.rows; r0 += kThreads) {
-    const int r = r0 + (int)threadIdx.x;
-    int jobs = 0, lo = 0, n = 0, start = 0;
-    if (r < p.rows) {
-      lo = min(max(__ldg(p.offsets + r), 0), p.tokens);
-      n = min(max(__ldg(p.offsets + r + 1), 0), p.tokens) - lo;
+  // ---- the job: the last row whose places begin at or before this CTA's
+  for (int64_t lo = 0, hi = p.rows;;) {
+    const int64_t step = (hi - lo + kThreads - 1) / kThreads;
+    const int64_t r = lo + threadIdx.x * step;
+    int first = 0, count = 0, start = 0;
+    if (r < hi) {
+      first = min(max(__ldg(p.offsets + r), 0), p.tokens);
+      count = min(max(__ldg(p.offsets + r + 1), 0), p.tokens) - first;
       start = __ldg(p.starts + r);
-      if (n > 0) {
-        if (start < 0 || start > INT32_MAX - block - n)  // the row has no such positions
-          atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
-        else
-          jobs = ((start + n - 1) >> shift) - (start >> shift) + 1;
+    }
+    const int64_t place = p.by_token ? first : (first >> shift) + 2 * r;
+    const int at_or_before = __syncthreads_count(r < hi && place <= (int64_t)blockIdx.x);
+    if (at_or_before == 0) return;
+    if (step > 1) {
+      lo += (at_or_before - 1) * step;
+      hi = min(lo + step, hi);
+      continue;
+    }
+    const int64_t j = (int64_t)blockIdx.x - place;  // which of the row's jobs
+    if ((int)threadIdx.x == at_or_before - 1 && count > 0 && j >= 0) {
+      if (start < 0 || start > INT32_MAX - block - count) {  // the row has no such positions
+        if (j == 0) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
+      } else if (j <= ((start + count - 1) >> shift) - (start >> shift)) {
+        const int pos = j == 0 ? start : ((start >> shift) + (int)j) << shift;
+        job_s[0] = (int)r;
+        job_s[1] = first + (pos - start);
+        job_s[2] = pos;
+        job_s[3] = min(block - (pos & (block - 1)), start + count - pos);
       }
     }
-    int incl = jobs;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (lane == 31) sums_s[warp] = incl;
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) incl += sums_s[w];
-      total += sums_s[w];
-    }
-    const int j = (int)blockIdx.x - before - (incl - jobs);  // which of this row's jobs
-    if (j >= 0 && j < jobs) {
-      const int pos = j == 0 ? start : ((start >> shift) + j) << shift;
-      job_s[0] = r;
-      job_s[1] = lo + (pos - start);
-      job_s[2] = pos;
-      job_s[3] = min(block - (pos & (block - 1)), start + n - pos);
-    }
-    __syncthreads();
-    before += total;
-    if (before > (int)blockIdx.x) break;
+    break;
   }
+  __syncthreads();
   const int row = job_s[0], t = job_s[1], pos = job_s[2], n = job_s[3];
   if (n == 0) return;
   const int in_block = pos & (block - 1);
@@ -557,9 +550,10 @@ extern "C" int dsa_append_q8(const void* ckv, int64_t ckv_stride_t, const void* 
   p.cache = q8::cache_of(ckv_q8, ckv_slot_stride, ckv_scale, kpe_cache, kpe_slot_stride, num_slots,
                          block);
   p.err = static_cast<uint32_t*>(workspace);
-  // a job has at least one token, and all but a row's first and last fill a block
   const int64_t bound = num_tokens / block + 2 * (int64_t)num_rows;
-  const dim3 grid((unsigned)(bound < num_tokens ? bound : num_tokens));
+  p.by_token = num_tokens <= bound;
+  if (!p.by_token && bound > INT32_MAX) return DSA_ERR_INVALID_ARGUMENT;
+  const dim3 grid((unsigned)(p.by_token ? num_tokens : bound));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (block <= 16) return q8::launch(q8::append_kernel<4, 4>, grid, 128, st, p);
   if (block <= 64) return q8::launch(q8::append_kernel<8, 8>, grid, 256, st, p);

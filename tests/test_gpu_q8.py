@@ -485,6 +485,29 @@ def test_append_many_rows_strides_and_refusals():
     same_pools(cache, want)
 
 
+@pytest.mark.parametrize("rows,live,most,block", [(70000, 300, 5, 2), (70000, 300, 5, 16), (400, 380, 29, 16),
+                                                  (1000, 150, 29, 64)])
+def test_append_rows_without_a_token(rows, live, most, block):
+    """Many rows, some or most of them without a new token, the first and the last among them;
+    tokens before the first offset and behind the last."""
+    page, cols = max(16, block), 64 // max(16, block) + 1
+    g = torch.Generator().manual_seed(block)
+    counts = torch.zeros(rows, dtype=torch.long)
+    some = torch.randperm(rows - 2, generator=g)[:live] + 1
+    counts[some] = torch.randint(1, most + 1, (live,), generator=g)
+    off = torch.cat([torch.zeros(1, dtype=torch.long), counts.cumsum(0)]) + 3
+    n = int(off[-1]) + 5
+    table = torch.full((rows, cols), -1, dtype=torch.int32)
+    table[some] = tables(live, cols, live * cols + 9, block)
+    starts = torch.randint(0, 34, (rows,), generator=g, dtype=torch.int32)
+    cache = ref.pools(live * cols + 9, page, block, 4)
+    x, k = tokens(n, 8)
+    want = ref.append(x, k, off.tolist(), starts, table.numpy(), *cache)
+    append_q8(x.cuda(), k.cuda(), off.to(torch.int32).cuda(), starts.cuda(), table.cuda(), *cache)
+    same_pools(cache, want)
+    assert read_device_errors() == 0
+
+
 # ------------------------------------------------------------------- accumulate, evict, compact
 
 
