@@ -564,11 +564,15 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // An entry's probability summed over the heads, from its scores (kTS apart) and their lse.
 template <int NH>
 __device__ __forceinline__ float head_sum(const float* scores, const float* lse) {
+  constexpr int kB = 16;  // scores on the way at a time
   float w = 0.f;
-#pragma unroll 8
-  for (int h = 0; h < NH; ++h) {
-    const float x = scores[h * Cfg<NH>::kTS];
-    w += x == -INFINITY ? 0.f : ptx::ex2(x - lse[h]);
+#pragma unroll
+  for (int h0 = 0; h0 < NH; h0 += kB) {
+    float x[kB];
+#pragma unroll
+    for (int h = 0; h < kB; ++h) x[h] = __ldcg(scores + (h0 + h) * Cfg<NH>::kTS);
+#pragma unroll
+    for (int h = 0; h < kB; ++h) w += x[h] == -INFINITY ? 0.f : ptx::ex2(x[h] - lse[h0 + h]);
   }
   return w;
 }
