@@ -38,7 +38,7 @@
 // 120 copies of ~20 cycles of the SM's TMA unit, 1.2 us.  Measured: 1.3 us a tile for a row
 // alone on its SM, 1.54 us, 5.9 TB/s, with 148 SMs at work.  Fixed cost: about 6 us a call, 2
 // us for each further unit of a CTA.  64 rows of 16 heads and 2048 slots: 26.1 us (3.3 TB/s of
-// the 87 MB that they need; the bf16 kernel 42.5); 256 ragged rows: 78 us (44 tiles on the busiest
+// the 87 MB that they need; the bf16 kernel 42.5); 256 ragged rows: 76 us (44 tiles on the busiest
 // SM, 28 on average); 32 rows of 128 heads: 50 us (each slot is gathered by four groups, three
 // of them from L2; the bf16 kernel 58.4); one row in eight splits: 12 us.
 //
