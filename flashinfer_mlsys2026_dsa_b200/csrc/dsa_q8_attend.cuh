@@ -14,8 +14,8 @@
 //     so the split is exact down to 2^-14 of the row's largest value and off by at most
 //     2^-21 of that below;
 //   * p scale / u is split into three terms, P = t0 + t1 / 16 + t2 / 256, where u, the unit, is
-//     the largest scale of the first tile (raised when a later one passes it 16-fold, so that
-//     scales of any size fit).  P is 3.5 2^(x + log2(scale / u) - m) with a running maximum m
+//     the largest scale of the first tile, but 2^-100 at least (a tile of zero tokens has 2^-126),
+//     raised when a later one passes it 16-fold.  P is 3.5 2^(x + log2(scale / u) - m) with a running maximum m
 //     that a value may pass by 2^7 before it is raised, so that P stays within e4m3's 448 and
 //     O is hardly ever rescaled.  Three terms round to 12 significant bits, and the third's
 //     smallest step is 2^-18.8 of a weight at m.  (Two terms, which allow 2^3, rescaled O in
@@ -98,6 +98,8 @@ constexpr uint32_t kSmBar = 1;  // all softmax warps; + 2 + half: those of a hal
 constexpr float kTauQ8 = 7.f;         // log2: how far a weighted score may pass the running maximum
 constexpr float kTauL = 60.f;         // the same for a score alone: its exponential stays finite
 constexpr float kTauU = 16.f;         // how far a scale may pass the unit
+constexpr float kUnitMin = 7.888609e-31f;  // 2^-100, the smallest unit: its inverse, and an output's
+                                           // weight u / L, are normal numbers
 constexpr float kNone = -3e38f;       // running maximum before the first score
 constexpr float kPScale = 3.5f;       // P <= 3.5 * 2^7 = 448, the largest e4m3 value
 constexpr int kMaxCluster = 8;
@@ -561,6 +563,15 @@ __device__ __forceinline__ float2 lds2(uint32_t addr) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
+// log2(a / b) of positive normal numbers, also where the quotient is not one; a whole number for
+// powers of two.
+__device__ __forceinline__ float log2_ratio(float a, float b) {
+  const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+  const float ma = __uint_as_float((ua & 0x7FFFFFu) | 0x3F800000u);
+  const float mb = __uint_as_float((ub & 0x7FFFFFu) | 0x3F800000u);
+  return (float)((int)(ua >> 23) - (int)(ub >> 23)) + (ptx::lg2(ma) - ptx::lg2(mb));
+}
+
 // An entry's probability summed over the heads, from its scores (kTS apart) and their lse.
 template <int NH>
 __device__ __forceinline__ float head_sum(const float* scores, const float* lse) {
@@ -811,16 +822,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool end = ok && tile < 0;
         if (!end) ok = ok && wait(bar(B_SF + sb), (uint32_t)((n / C::kSBufs) & 1));
         ++c;
-        if (live == 0) {  // the unit of the scales, the same in every thread
-          const float first = smax[st];
-          u = first > 0.f ? fmaxf(first, 1.17549435e-38f) : 1.f;  // 1 / u is finite
+        // The unit of the scales, the same in every thread: the first tile's largest scale, or a
+        // later one's that passes it kTauU-fold.  It rises before a scale is divided by it, so that no
+        // ratio passes kTauU (a scale of 2^30 over a unit of 2^-100 would not be finite).
+        const float largest = smax[st];
+        float grow = 0.f;  // log2(old unit / new unit)
+        if (live == 0) {
+          u = fmaxf(largest, kUnitMin);
+          u_inv = 1.f / u;
+        } else if (!end && largest > kTauU * u) {
+          grow = log2_ratio(u, largest);
+          u = largest;
           u_inv = 1.f / u;
         }
         float2 x[kHT / 2], d[kHT / 2];  // scores, and over the running maximum
         float ratio = 0.f;  // scale in units, lr its log2
         float lr = -INFINITY;
         bool valid = false;
-        const bool grow = !end && smax[st] > kTauU * u;
         if (slot_ok && __all_sync(0xffffffffu, ok && !end)) {  // warp-uniform
           ptx::tc_fence_after();
           uint32_t hi[kHT], lo[kHT], pe[kHT];
@@ -874,22 +892,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         if (end) break;
-        if (vote != 0u || grow) {
+        if (vote != 0u || grow != 0.f) {
           // Rare past the first tile: raise the maxima to this tile's, the unit to its largest
           // scale, and bring l and O to them.
           if (live > 0) {
             const bool wok = wait(bar(B_PD + (int)((n - 1) & 1)), (uint32_t)(((n - 1) >> 1) & 1));
             if (!__all_sync(0xffffffffu, wok)) failed = true;
             ptx::tc_fence_after();
-          }
-          float beta = 1.f;
-          if (grow) {
-            const float un = smax[st];
-            beta = u / un;
-            lr += ptx::lg2(beta);
-            u = un;
-            u_inv = 1.f / u;
-            ratio *= beta;
           }
           // the maxima go through this tile's P buffer, whose last reader (PV) is done
           // (in the first term's rows of these heads, which only these warps write)
@@ -911,11 +920,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float2 t = t2[q * kHT / 2];
               mn = make_float2(fmaxf(mn.x, t.x), fmaxf(mn.y, t.y));
             }
-            alpha[j] = make_float2(ptx::ex2(-m_neg[j].x - mn.x), ptx::ex2(-m_neg[j].y - mn.y));
-            l_part[j] = mul2(l_part[j], alpha[j]);
+            // O is in old units: its factor has the unit's in the exponent, where neither can overflow
+            const float2 fall = make_float2(-m_neg[j].x - mn.x, -m_neg[j].y - mn.y);
+            l_part[j] = mul2(l_part[j], make_float2(ptx::ex2(fall.x), ptx::ex2(fall.y)));
+            alpha[j] = make_float2(ptx::ex2(fall.x + grow), ptx::ex2(fall.y + grow));
             m_neg[j] = make_float2(-mn.x, -mn.y);
             d[j] = add2(x[j], m_neg[j]);
-            alpha[j] = mul2(alpha[j], both(beta));
           }
           ptx::bar_sync(kSmBar + 2 + hh, kSmThreads / 2);  // the buffer is P's again
           if (live > 0 && !failed) {
