@@ -15,11 +15,15 @@
 //     2^-21 of that below;
 //   * p scale / u is split into three terms, P = t0 + t1 / 16 + t2 / 256, where u, the unit, is
 //     the largest scale of the first tile, but 2^-100 at least (a tile of zero tokens has 2^-126),
-//     raised when a later one passes it 16-fold.  P is 3.5 2^(x + log2(scale / u) - m) with a running maximum m
-//     that a value may pass by 2^7 before it is raised, so that P stays within e4m3's 448 and
-//     O is hardly ever rescaled.  Three terms round to 12 significant bits, and the third's
-//     smallest step is 2^-18.8 of a weight at m.  (Two terms, which allow 2^3, rescaled O in
-//     about half of the tiles.)
+//     raised when a later one passes it 16-fold.  P is 3.5 2^(x + log2(scale / u) - m) with a
+//     running maximum m of x + log2(scale / u) that a value may pass by 2^7 before m is raised, so
+//     that P stays within e4m3's 448 and O is hardly ever rescaled; a unit that rises lowers m by
+//     as much.  Three terms round to 12 significant bits, and the third's smallest step is
+//     2^-18.8 of a weight at m.  (Two terms, which allow 2^3, rescaled O in about half of the
+//     tiles.)  The sum l of 2^(x - m) has no scale in it: m stays so high that no score passes it by
+//     more than 2^96, so an entry that has a head's weight is held to these bits down to a scale
+//     of 2^-88 of the unit, and loses a bit with every halving below.  Scales up to 2^100 are
+//     within range (q . ckv_q8, up to 2^26, is multiplied by the scale before the query's unit).
 // The terms are extra columns of the same MMA (N = 2 NH and 3 NH): an M = 128 MMA costs about
 // the same from N = 16 to N = 64, so they are nearly free.
 //
@@ -96,7 +100,7 @@ constexpr int kScore = 5, kPv = 6, kKeeper = 7, kSm0 = 8;
 constexpr int kSmWarps = 8, kSmThreads = 256;
 constexpr uint32_t kSmBar = 1;  // all softmax warps; + 2 + half: those of a half of the heads
 constexpr float kTauQ8 = 7.f;         // log2: how far a weighted score may pass the running maximum
-constexpr float kTauL = 60.f;         // the same for a score alone: its exponential stays finite
+constexpr float kTauL = 96.f;         // the same for a score alone: the sum of 2^31 stays finite
 constexpr float kTauU = 16.f;         // how far a scale may pass the unit
 constexpr float kUnitMin = 7.888609e-31f;  // 2^-100, the smallest unit: its inverse, and an output's
                                            // weight u / L, are normal numbers
@@ -903,10 +907,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           // the maxima go through this tile's P buffer, whose last reader (PV) is done
           // (in the first term's rows of these heads, which only these warps write)
           float* tops = reinterpret_cast<float*>(sgen + C::OFF_P + (int)(n % C::kPBufs) * C::kPB + hh * kHT * 32);
+          // A maximum is one of x + log2(scale / u): it falls with a unit that rises, unless that
+          // would take l past 2^(kTauL - 8).
           const float over = fmaxf(lr, 8.f - kTauL);
 #pragma unroll
           for (int h = 0; h < kHT; ++h) {
-            const float v = ptx::warp_max(((h & 1) ? x[h / 2].y : x[h / 2].x) + over);
+            float v = ((h & 1) ? x[h / 2].y : x[h / 2].x) + over;
+            if (grow != 0.f) {
+              const float l = (h & 1) ? l_part[h / 2].y : l_part[h / 2].x;
+              v = fmaxf(v, ptx::lg2(l) - ((h & 1) ? m_neg[h / 2].y : m_neg[h / 2].x) + (8.f - kTauL));
+            }
+            v = ptx::warp_max(v);
             if (slot_ok && lane == 0) tops[qd * kHT + h] = v;
           }
           ptx::bar_sync(kSmBar + 2 + hh, kSmThreads / 2);
@@ -914,13 +925,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < kHT / 2; ++j) {
             const float2* t2 = reinterpret_cast<const float2*>(tops) + j;
-            float2 mn = make_float2(-m_neg[j].x, -m_neg[j].y);
+            float2 mn = make_float2(grow - m_neg[j].x, grow - m_neg[j].y);
 #pragma unroll
             for (int q = 0; q < kQuads; ++q) {
               const float2 t = t2[q * kHT / 2];
               mn = make_float2(fmaxf(mn.x, t.x), fmaxf(mn.y, t.y));
             }
-            // O is in old units: its factor has the unit's in the exponent, where neither can overflow
+            // l's factor is 2^(kTauL - 4) at most; O, in old units, takes the unit's growth beside it in
+            // the exponent, where neither can overflow
             const float2 fall = make_float2(-m_neg[j].x - mn.x, -m_neg[j].y - mn.y);
             l_part[j] = mul2(l_part[j], make_float2(ptx::ex2(fall.x), ptx::ex2(fall.y)));
             alpha[j] = make_float2(ptx::ex2(fall.x + grow), ptx::ex2(fall.y + grow));

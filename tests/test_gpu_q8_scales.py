@@ -46,6 +46,51 @@ def rope_queries(B, H):
     return qp
 
 
+@pytest.mark.parametrize("growth", [4, 6, 8, 10, 12, 14, 16, 20, 28, 40])
+@pytest.mark.parametrize("rows,heads,topk", SHAPES)
+def test_one_slot_of_a_far_larger_scale(rows, heads, topk, growth):
+    """Each row holds a slot whose scale is 2^growth times the others', at a place of its own from the
+    first tile to the last; heads give it nearly all of their weight, some, or none."""
+    g = torch.Generator().manual_seed(growth)
+    x = torch.rand(SLOTS, 512, generator=g) * 300 + 100  # of one sign, so that outputs do not cancel
+    x[0] *= torch.where(torch.rand(512, generator=g) < 0.5, -1.0, 1.0)
+    q8 = e4m3(x)
+    scale = torch.full((SLOTS,), 2.0 ** -9)
+    scale[0] = 2.0 ** (growth - 9)
+    kpe = (torch.randn(SLOTS // 16, 16, 64, generator=g) * 0.5).to(torch.bfloat16).cuda()
+    cache = (q8, scale.view(-1, 16).cuda(), kpe)
+    idx = torch.stack([torch.randperm(SLOTS - 1, generator=g)[:topk] + 1 for _ in range(rows)]).to(torch.int32)
+    at = torch.linspace(0, topk - 1, rows).long() if rows > 3 else torch.tensor([2, topk // 2 + 30, topk - 1])[:rows]
+    idx[torch.arange(rows), at] = 0
+    big = q8.view(-1, 512)[0].float().cpu() * scale[0]
+    q = 0.02 * torch.randn(rows, heads, 512, generator=g)
+    q -= (q @ big / (big @ big))[..., None] * big
+    aim = torch.linspace(-60, 20, rows * heads).view(rows, heads)
+    q += (aim / (SM * LOG2E * (big @ big)))[..., None] * big
+    q = (q.to(torch.bfloat16).cuda(), torch.randn(rows, heads, 64, generator=g).to(torch.bfloat16).cuda())
+    idx = idx.cuda()
+    q8_bounds.check(run(q, cache, idx), q, cache, idx, SM)
+
+
+@pytest.mark.parametrize("growth", [6, 12, 20, 40, 60, 80])
+@pytest.mark.parametrize("rows,heads,topk", SHAPES)
+def test_small_scales_with_the_weight(rows, heads, topk, growth):
+    """Entries of a small scale, in the first tiles, whose weight makes up for it: they and the
+    later ones share the output."""
+    g = torch.Generator().manual_seed(growth)
+    q8 = e4m3(torch.rand(SLOTS, 512, generator=g) * 300 + 100)
+    scale = torch.full((SLOTS,), 2.0 ** -growth)
+    scale[SLOTS // 2:] = 1
+    score = torch.rand(SLOTS, generator=g) * 2
+    score[:SLOTS // 2] += growth
+    cache = (q8, scale.view(-1, 16).cuda(), rope(score))
+    q = (torch.zeros(rows, heads, 512, dtype=torch.bfloat16, device="cuda"), rope_queries(rows, heads))
+    idx = torch.stack([torch.randperm(SLOTS, generator=g)[:topk].sort().values for _ in range(rows)]).to(torch.int32)
+    idx[0] = idx[0].flip(0)
+    idx = idx.cuda()
+    q8_bounds.check(run(q, cache, idx), q, cache, idx, SM)
+
+
 @pytest.mark.parametrize("late", [2.0 ** -60, 0.5, 1.0, 2.0, 4.0, 2.0 ** 20, 2.0 ** 60, 2.0 ** 90])
 @pytest.mark.parametrize("rows,heads,topk", SHAPES)
 def test_tokens_of_zeros_first(rows, heads, topk, late):
