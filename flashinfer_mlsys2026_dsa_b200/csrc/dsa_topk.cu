@@ -667,6 +667,21 @@ int run(const Params& p, int64_t num_rows, cudaStream_t st) {
              : launch<false, 1, kEvict>(p, num_rows, 0, st);
 }
 
+// Whether rows of `na` floats, `sa` apart from `a` on, and rows of `nb`, `sb` apart from `b` on, share
+// one.  Both walk up in memory, so the row that ends first can meet no later one of the other.
+bool rows_meet(const float* a, int64_t sa, int64_t na, const float* b, int64_t sb, int64_t nb,
+               int64_t rows) {
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
+  for (int64_t i = 0, j = 0; i < rows && j < rows;) {
+    const uintptr_t la = pa + (uintptr_t)(i * sa) * 4, lb = pb + (uintptr_t)(j * sb) * 4;
+    const uintptr_t ea = la + (uintptr_t)na * 4, eb = lb + (uintptr_t)nb * 4;
+    if (la < eb && lb < ea) return true;
+    if (ea <= lb) ++i;
+    else ++j;
+  }
+  return false;
+}
+
 }  // namespace topk
 }  // namespace dsa
 
@@ -717,9 +732,11 @@ extern "C" int dsa_evict_positions(const float* acc, int64_t acc_stride_b, const
   if ((!acc && max_len > 0) || !lengths || !keep || !new_lengths || acc_stride_b < 0 ||
       (num_rows > 1 && keep_stride_b < budget))
     return DSA_ERR_INVALID_ARGUMENT;
+  // new_acc is written while other CTAs still read acc
   if (new_acc != nullptr &&
-      (new_acc == acc || new_acc_cols < budget ||
-       (num_rows > 1 && new_acc_stride_b < new_acc_cols)))
+      (new_acc_cols < budget || (num_rows > 1 && new_acc_stride_b < new_acc_cols) ||
+       (max_len > 0 && dsa::topk::rows_meet(acc, acc_stride_b, max_len, new_acc, new_acc_stride_b,
+                                            new_acc_cols, num_rows))))
     return DSA_ERR_INVALID_ARGUMENT;
   dsa::topk::Params p;
   p.scores = acc;

@@ -79,6 +79,22 @@ def _unit(t):
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
+def _rows_meet(a, b):
+    """Whether the rows of two 2-D tensors of one type share memory (columns beside each other do not)."""
+    size = a.element_size()
+    i = j = 0
+    while i < a.shape[0] and j < b.shape[0] and a.shape[1] and b.shape[1]:
+        at, bt = a.data_ptr() + i * a.stride(0) * size, b.data_ptr() + j * b.stride(0) * size
+        ae, be = at + a.shape[1] * size, bt + b.shape[1] * size
+        if at < be and bt < ae:
+            return True
+        if ae <= bt:
+            i += 1
+        else:
+            j += 1
+    return False
+
+
 def _row_offsets(t, rows, dev):
     _need("row_offsets", t, torch.int32, 1, dev)
     if t.shape[0] != rows + 1:
@@ -362,7 +378,7 @@ def evict_positions(acc, lengths, budget, sinks=0, recent=0, new_acc=None):
         if new_acc.shape[0] != rows or new_acc.shape[1] < budget or new_acc.stride(1) != 1:
             raise ValueError(f"new_acc must be [{rows}, >= {budget}] with a unit inner stride, "
                              f"got {tuple(new_acc.shape)}, strides {new_acc.stride()}")
-        if new_acc.data_ptr() == acc.data_ptr():
+        if _rows_meet(new_acc, acc):
             raise ValueError("new_acc must not overlap acc")
         out = (new_acc.data_ptr(), new_acc.stride(0), new_acc.shape[1])
     lib = _native._lib or _native.load()

@@ -269,7 +269,7 @@ int dsa_accumulate_weights(const float* weights, int64_t weights_stride_t,
  * dsa_topk_slots orders scores; ties to the smaller positions); a row of at most `budget`
  * positions keeps them all.  keep [num_rows, >= budget] int32: the kept positions, ascending,
  * then -1.  new_lengths [num_rows]: how many.  new_acc (optional) [num_rows, >= new_acc_cols],
- * new_acc_cols >= budget: the kept positions' totals, then zeros; it does not overlap acc.
+ * new_acc_cols >= budget: the kept positions' totals, then zeros; refused where it overlaps acc.
  * sinks + recent <= budget.  Lengths past max_len count as max_len.
  */
 int dsa_evict_positions(const float* acc, int64_t acc_stride_b, const int32_t* lengths,
