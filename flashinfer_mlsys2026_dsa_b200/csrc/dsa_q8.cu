@@ -300,7 +300,9 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendParams 
 // the entries are independent and spread over CTAs of 256.  The adds are fire-and-forget
 // reductions, also right when a token names a position twice.  Measured: 16 rows of 8 x 1500
 // entries 4.6 us with eight CTAs a row (floor 0.4; the chain offsets -> entries -> eight barriers;
-// 7.1 us with one CTA a row); 64 rows of 2048 entries 1.9 us, an empty launch's time.
+// 7.1 us with one CTA a row); 64 rows of 2048 entries 1.9 us, an empty launch's time.  A row of
+// many tokens is serial: 512 tokens of 2048 entries in one row 201 us, 4096 1.68 ms, 64 in each
+// of 16 rows 29 us.
 
 struct AccumulateParams {
   const float* weights;
@@ -653,9 +655,13 @@ int prepare_device() {
   return n;
 }
 
-// CTAs per (row, head group).  Per CTA about 7 us are spent outside the tiles (first gather, end;
-// 8 with the merge) and 1.4 us (16 heads) or 1.75 us (32) per tile; a call whose units do not
-// fill the SMs splits them while that shortens the longest CTA.  Measured, us for S = 1, 2, 4, 8
+// CTAs per (row, head group).  Per CTA about 7 us are counted outside the tiles (first gather, end;
+// 8 with the merge) and 1.4 us (16 heads) or 1.75 us (32; measured 2.35 to 2.71) per tile; a
+// call whose units do not fill the SMs splits them while that shortens the longest CTA.  The rule
+// counts SMs, but a cluster must fit into a GPC, so where S G > 2 the last SMs of a wave can stay
+// idle and the call takes a second one: 16 rows of 16 heads and 2048 slots take 28.0 us in
+// splits of eight, 20 rows 18.0 in splits of four; 36 rows 34.0, 40 rows 24.5 (splits of
+// two); 16 rows of 128 heads 58.5, 19 rows 45.6 (unsplit).  Measured, us for S = 1, 2, 4, 8
 // (* chosen; -: a cluster of more than eight, or not measured):
 //     1 row, 16 heads, 2048 slots          35.4   21.9   15.5   12.1*
 //     64 rows, 16 heads, 2048 slots        37.9   26.4*  36.8     -

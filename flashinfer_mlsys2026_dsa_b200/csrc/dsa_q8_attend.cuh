@@ -39,17 +39,19 @@
 // the next one under the last one's end.
 //
 // What bounds it.  A tile of 16 heads needs 61 kB: 1.40 us a tile at 6.5 TB/s over 148 SMs, and
-// 120 copies of ~20 cycles of the SM's TMA unit, 1.2 us.  Measured: 1.3 us a tile for a row
-// alone on its SM, 1.54 us, 5.9 TB/s, with 148 SMs at work.  Fixed cost: about 6 us a call, 2
-// us for each further unit of a CTA.  64 rows of 16 heads and 2048 slots: 26.1 us (3.3 TB/s of
-// the 87 MB that they need; the bf16 kernel 42.5); 256 ragged rows: 76 us (44 tiles on the busiest
-// SM, 28 on average); 32 rows of 128 heads: 50 us (each slot is gathered by four groups, three
-// of them from L2; the bf16 kernel 58.4); one row in eight splits: 12 us.
+// 120 copies of ~20 cycles of the SM's TMA unit, 1.2 us.  Measured: 1.34 us a tile for a row
+// alone on its SMs, 1.50 us, 6.0 TB/s, with 148 SMs at work (32 heads: 2.35 and 2.71 us).  Fixed
+// cost: about 6 us a call, 2 us for each further unit of a CTA.  64 rows of 16 heads and 2048
+// slots: 26.8 us (3.2 TB/s of the 87 MB that they need; the bf16 kernel 42.5); 256 ragged rows: 76.7
+// us (44 tiles on the busiest SM, 28 on average); 32 rows of 128 heads: 49.9 us (each slot is
+// gathered by four groups, three of them from L2; the bf16 kernel 58.4); one row in eight splits:
+// 12.8 us.
 //
 // Per CTA (512 threads):
 //   warps 0-4    gather producers, one per 128-byte column block of the slots
-//   warp 5       score issuer: S^T[96 slots x (hi, lo, pe)], 16 f8 + 4 bf16 MMAs
-//   warp 6       PV issuer: O^T[512 x 3 terms] += V^T P^T, 12 f8 MMAs (V^T read in place)
+//   warp 5       score issuer: S^T[96 or 128 slots x (hi, lo, pe)], 16 f8 + 4 bf16 MMAs
+//   warp 6       PV issuer: O^T[512 x 3 terms] += V^T P^T, 12 f8 MMAs (16 for 128 slots; V^T read
+//                in place)
 //   warp 7       keeper: the slots of every tile with a valid entry, their scales and validity, and
 //                where the row's padding begins.  (Gatherers that each looked the slots up for
 //                themselves: 256 ragged rows 90.5 us, 64 rows 28.1, 32 rows of 128 heads 54.8.)
@@ -132,7 +134,7 @@ struct Cfg {
   static constexpr int OFF_CMD = OFF_MISC + 32;    // [stage][8]: validity words; [4] the tile (-1: end)
   static constexpr int OFF_SMAX = OFF_CMD + kStages * 32;  // [stage] largest scale of the tile
   static constexpr int OFF_QS = OFF_SMAX + 16;     // [NH] score units per query row
-  static constexpr int OFF_SC = OFF_QS + NH * 4;   // [stage][96] scales; at the end kMl floats
+  static constexpr int OFF_SC = OFF_QS + NH * 4;   // [stage][kTS] scales; at the end kMl floats
   static constexpr int kMl = 2 * NH + 1;           // a CTA's m, L and u, for the merge
   static constexpr int OFF_RED = OFF_SC + kStages * kTS * 4;  // [half][2 buffers][4 warps] votes
   static constexpr int OFF_LSE = OFF_RED + 16 * 4;  // [NH], for the weights

@@ -205,7 +205,8 @@ int dsa_sparse_mla_decode_grouped(
  *
  * Pools, bf16 inputs and their row strides are 16-byte aligned.  `workspace` is the decode's
  * (only its error word is used: an entry that names no slot, position or page of the call sets
- * DSA_DEVERR_BAD_INDEX and is left out).  Scales are expected to be finite and >= 0.
+ * DSA_DEVERR_BAD_INDEX and is left out).  Scales are expected to be finite and >= 0, for the decode
+ * at most 2^100.
  *
  * dsa_sparse_mla_decode_q8: dsa_sparse_mla_decode() over this cache.  With page_table NULL
  * `indices` holds flat slot ids, otherwise token positions that are translated as in
