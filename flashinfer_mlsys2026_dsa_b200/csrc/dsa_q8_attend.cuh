@@ -21,9 +21,10 @@
 //     as much.  Three terms round to 12 significant bits, and the third's smallest step is
 //     2^-18.8 of a weight at m.  (Two terms, which allow 2^3, rescaled O in about half of the
 //     tiles.)  The sum l of 2^(x - m) has no scale in it: m stays so high that no score passes it by
-//     more than 2^96, so an entry that has a head's weight is held to these bits down to a scale
-//     of 2^-88 of the unit, and loses a bit with every halving below.  Scales up to 2^100 are
-//     within range (q . ckv_q8, up to 2^26, is multiplied by the scale before the query's unit).
+//     more than 2^96.  That costs bits only where a head's weight lies on scales below 2^-88 of the
+//     unit, and then l is 2^88 or more, so that the third term's step is under 2^-106 u of the output.
+//     Scales up to 2^100 are within range (q . ckv_q8, up to 2^26, is multiplied by the scale
+//     before the query's unit).
 // The terms are extra columns of the same MMA (N = 2 NH and 3 NH): an M = 128 MMA costs about
 // the same from N = 16 to N = 64, so they are nearly free.
 //

@@ -215,7 +215,8 @@ def kernel_q8(q_nope, q_pe, ckv_q8, ckv_scale, kpe_cache, sparse_indices, sm_sca
     ``weights`` (optional) [B, topk] float32 receives each entry's attention probability summed
     over the heads, 0 for padding: what :func:`accumulate_weights` adds up.  Head counts,
     strides, padding and error bits are those of :func:`ops.kernel`.  The scales of a selection
-    may differ: an entry keeps 12 bits of its probability down to 2^-88 of the largest one.
+    may differ, up to 2^88-fold without any loss (beyond, a value may be off by 2^-106 of the
+    largest scale).
     """
     _attend(q_nope, q_pe, ckv_q8, ckv_scale, kpe_cache, None, sparse_indices, "sparse_indices",
             sm_scale, output, lse, weights)

@@ -19,7 +19,9 @@ def attend(q_nope, q_pe, q8, scale, kpe, slots, sm_scale):
       interval of each score, and the intervals of all scores one of each probability and of lse.
     * A probability times its scale is three e4m3 terms: each keeps 4 significant bits of what the
       one before left, 2^-12 in all, and the last one's step, 2^-9 / 2^8, rounds off at most
-      2^-18, where the largest of the row is 3.5 or more: 2^-19 of the largest (p scale).
+      2^-18, where the largest of the row is 3.5 or more: 2^-19 of the largest (p scale).  Only where
+      the weight lies on scales below 2^-88 of the largest one is the row's largest less; the sum of
+      the probabilities is then 2^88 or more: 2^-18 / 3.5 / 2^88 < 2^-107 of that scale.
     * Sums over the entries: a step of 32 entries adds a rounding of 2^-23 for itself and three for
       its products; exponentials (2^-22) and up to a rescale a tile: 2^-23 (topk / 8 + 64) in all.
     * lse is m + log2(l): each with 2^-22 of its size (log2 l is at most 100), 2^-20 for the sum.
@@ -37,7 +39,8 @@ def attend(q_nope, q_pe, q8, scale, kpe, slots, sm_scale):
     out = torch.zeros(B, H, 512, dtype=D, device=dev)
     lse = torch.full((B, H), -math.inf, dtype=D, device=dev)
     weights = torch.zeros(B, topk, dtype=D, device=dev)
-    out_tol, lse_tol, w_tol = torch.zeros_like(out), torch.zeros_like(lse), torch.zeros_like(weights)
+    # where there is nothing: the value itself
+    out_tol, lse_tol, w_tol = (torch.full_like(t, 1e-37) for t in (out, lse, weights))
     for b in range(B):
         at = torch.nonzero((idx[b] >= 0) & (idx[b] < raw.shape[0]))[:, 0]
         if not len(at):
@@ -70,7 +73,7 @@ def attend(q_nope, q_pe, q8, scale, kpe, slots, sm_scale):
         lse_own = 2.0 ** -20 + 2.0 ** -22 * (lse[b].abs() + 100)
         lse_tol[b] = torch.maximum(high - lse[b], lse[b] - lows) + lse_own
         rel = 2.0 ** -12 + (topk / 8 + 64) * 2.0 ** -23
-        last = 2.0 ** -19 * (p * sk).amax(1, keepdim=True) * x8.abs().sum(0)
+        last = (2.0 ** -19 * (p * sk).amax(1, keepdim=True) + 2.0 ** -107 * sk.max()) * x8.abs().sum(0)
         near = err @ v.abs() + rel * (p @ v.abs()) + last
         out_tol[b] = near + 2.0 ** -8 * (out[b].abs() + near) + 1e-37
         # a weight is 2^(score - lse): the exponential, the difference's rounding and lse's own

@@ -165,3 +165,24 @@ def test_ordinary_caches(rows, heads, topk):
     q = (q[..., :512].contiguous(), q[..., 512:].contiguous())
     idx = torch.stack([torch.randperm(SLOTS, generator=g)[:topk] for _ in range(rows)]).to(torch.int32).cuda()
     q8_bounds.check(run(q, cache, idx), q, cache, idx, SM)
+
+
+@pytest.mark.parametrize("above", [20, 80, 95, 110, 200])
+@pytest.mark.parametrize("rows,heads,topk", SHAPES)
+def test_zero_tokens_with_the_weight(rows, heads, topk, above):
+    """Zero tokens (scale 2^-126) whose scores lie 2^above over the others': the output is small, and off by
+    2^-107 of the others' values a slot at most; rows of padding and padded ones beside them."""
+    g = torch.Generator().manual_seed(above)
+    x = torch.rand(SLOTS, 512, generator=g) * 300 + 100
+    zero = torch.rand(SLOTS, generator=g) < 0.5
+    x[zero] = 0
+    scale = torch.where(zero, 2.0 ** -126, 0.25)
+    cache = (e4m3(x), scale.view(-1, 16).cuda(), rope(torch.where(zero, float(above), 0.0) + torch.rand(SLOTS, generator=g)))
+    q = (torch.zeros(rows, heads, 512, dtype=torch.bfloat16, device="cuda"), rope_queries(rows, heads))
+    idx = torch.stack([torch.randperm(SLOTS, generator=g)[:topk] for _ in range(rows)]).to(torch.int32)
+    idx[1, topk // 3:] = -1
+    idx[1, ::3] = -1
+    if rows > 2:
+        idx[2] = -1
+    idx = idx.cuda()
+    q8_bounds.check(run(q, cache, idx), q, cache, idx, SM)
