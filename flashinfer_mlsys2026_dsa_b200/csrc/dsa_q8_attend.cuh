@@ -105,8 +105,8 @@ constexpr uint32_t kSmBar = 1;  // all softmax warps; + 2 + half: those of a hal
 constexpr float kTauQ8 = 7.f;         // log2: how far a weighted score may pass the running maximum
 constexpr float kTauL = 96.f;         // the same for a score alone: the sum of 2^31 stays finite
 constexpr float kTauU = 16.f;         // how far a scale may pass the unit
-constexpr float kUnitMin = 7.888609e-31f;  // 2^-100, the smallest unit: its inverse, and an output's
-                                           // weight u / L, are normal numbers
+constexpr float kUnitMin = 7.888609e-31f;  // 2^-100, the smallest unit: its inverse is finite, and u / L
+                                           // of a sum L up to 2^24 keeps its bits
 constexpr float kNone = -3e38f;       // running maximum before the first score
 constexpr float kPScale = 3.5f;       // P <= 3.5 * 2^7 = 448, the largest e4m3 value
 constexpr int kMaxCluster = 8;
