@@ -62,6 +62,15 @@ _EVICT_ARGTYPES = [_PTR, _I64, _PTR, _I64, _I32,             # acc, stride_b, le
                    _PTR, _I64, _I32, _PTR]                   # new_acc, stride_b, cols, stream
 _COMPACT_Q8_ARGTYPES = ([_PTR, _I64, _I32, _I32] + _TABLE + _TABLE + [_I32] + _Q8_CACHE
                         + [_PTR, _PTR])
+_DENSE_Q_POOLS = _DECODE_ARGTYPES[:11] + [_I32]             # queries, pools; page_size
+_DENSE_ROWS = _TABLE + [_PTR, _PTR, _I32]                   # own pages; lengths, row_offsets, rows
+_DENSE_TAIL = ([_F32] + _DECODE_ARGTYPES[14:20]             # sm_scale, output, lse
+               + [_I64, _I32, _PTR, _SIZE, _PTR, _PTR])     # tokens, heads, scratch, ws, stream
+_WINDOW_ARGTYPES = _DENSE_Q_POOLS + _DENSE_ROWS + [_I32, _I32] + _DENSE_TAIL
+_SHARED_ARGTYPES = (_DENSE_Q_POOLS + _TABLE + [_PTR, _PTR, _I32]  # prefix pages, lengths, groups
+                    + _DENSE_ROWS + _DENSE_TAIL)
+_MERGE_ARGTYPES = ([_I32, _c.POINTER(_PTR), _c.POINTER(_I64), _c.POINTER(_PTR),
+                    _c.POINTER(_I64)] + _DECODE_ARGTYPES[14:20] + [_I64, _I32, _PTR])
 
 EXPORTED_SYMBOLS = (
     "dsa_sparse_mla_decode",
@@ -76,6 +85,10 @@ EXPORTED_SYMBOLS = (
     "dsa_accumulate_weights",
     "dsa_evict_positions",
     "dsa_compact_q8",
+    "dsa_mla_decode_window",
+    "dsa_mla_decode_shared",
+    "dsa_dense_scratch_size",
+    "dsa_merge_states",
     "dsa_sparse_mla_decode_workspace_size",
     "dsa_read_error_word",
     "dsa_selftest_bounded_wait",
@@ -135,11 +148,16 @@ def load(build_if_missing: bool = True):
                                ("dsa_append_q8", _APPEND_Q8_ARGTYPES),
                                ("dsa_accumulate_weights", _ACCUMULATE_ARGTYPES),
                                ("dsa_evict_positions", _EVICT_ARGTYPES),
-                               ("dsa_compact_q8", _COMPACT_Q8_ARGTYPES)):
+                               ("dsa_compact_q8", _COMPACT_Q8_ARGTYPES),
+                               ("dsa_mla_decode_window", _WINDOW_ARGTYPES),
+                               ("dsa_mla_decode_shared", _SHARED_ARGTYPES),
+                               ("dsa_merge_states", _MERGE_ARGTYPES)):
             getattr(lib, name).restype = _c.c_int
             getattr(lib, name).argtypes = argtypes
         lib.dsa_q8_scratch_size.restype = _c.c_size_t
         lib.dsa_q8_scratch_size.argtypes = [_c.c_int64, _c.c_int32, _c.c_int32]
+        lib.dsa_dense_scratch_size.restype = _c.c_size_t
+        lib.dsa_dense_scratch_size.argtypes = [_c.c_int64, _c.c_int32, _c.c_int32]
         lib.dsa_sparse_mla_decode_workspace_size.restype = _c.c_size_t
         lib.dsa_sparse_mla_decode_workspace_size.argtypes = [_c.c_int64, _c.c_int32, _c.c_int32,
                                                              _c.c_int32]

@@ -8,6 +8,8 @@
 // validates, raises the precise error or copies to a supported layout.
 #include <torch/extension.h>
 
+#include <vector>
+
 #include "dsa_b200.h"
 
 namespace {
@@ -211,6 +213,134 @@ int64_t compact_q8(const at::Tensor& keep, const at::Tensor& page_table,
                         ws.data_ptr(), reinterpret_cast<void*>(stream));
 }
 
+// Queries, pools and outputs of a dense call; page_size -1: the pools' page dimension.
+struct DenseArgs {
+  int64_t B = 0, H = 0, ckv_ss = -1, kpe_ss = -1, slots = 0, page = 0;
+  bool ok = false;
+  DenseArgs(const at::Tensor& q_nope, const at::Tensor& q_pe, const at::Tensor& ckv,
+            const at::Tensor& kpe, int64_t page_size, const at::Tensor& out,
+            const at::Tensor& lse, const at::Tensor& ws) {
+    const auto bf16 = at::kBFloat16;
+    if (!q_nope.is_cuda() || q_nope.dim() != 3 || q_nope.size(2) != 512) return;
+    B = q_nope.size(0);
+    H = q_nope.size(1);
+    const auto dev = q_nope.device();
+    for (const at::Tensor* t : {&q_pe, &ckv, &kpe, &out, &lse, &ws})
+      if (t->device() != dev) return;
+    for (const at::Tensor* t : {&q_nope, &q_pe, &ckv, &kpe, &out})
+      if (t->scalar_type() != bf16) return;
+    if (lse.scalar_type() != at::kFloat || q_pe.dim() != 3 || q_pe.size(0) != B ||
+        q_pe.size(1) != H || q_pe.size(2) != 64 || out.dim() != 3 || out.size(0) != B ||
+        out.size(1) != H || out.size(2) != 512 || lse.dim() != 2 || lse.size(0) != B ||
+        lse.size(1) != H || q_nope.stride(2) != 1 || q_pe.stride(2) != 1 || out.stride(2) != 1 ||
+        ckv.dim() < 2 || kpe.dim() < 2 || ckv.numel() == 0)
+      return;
+    ckv_ss = slot_stride(ckv, 512);
+    kpe_ss = slot_stride(kpe, 64);
+    if (ckv_ss < 0 || kpe_ss < 0) return;
+    slots = ckv.numel() / 512;
+    page = page_size;
+    if (page < 0 && ckv.dim() == 3) page = ckv.size(1);
+    ok = slots == kpe.numel() / 64 && page >= 1 && page <= (1 << 30);
+  }
+};
+
+// The rows of a dense call: page tables, lengths, and offsets or none (a token a row).
+bool plain_rows(const at::Tensor& table, const at::Tensor& lengths, const OptTensor& offsets,
+                int64_t tokens, const at::Device& dev) {
+  if (!plain_i32(table, dev, 2) || !plain_i32(lengths, dev, 1) ||
+      table.size(0) != lengths.size(0) || table.size(1) < 1)
+    return false;
+  if (!offsets.has_value()) return lengths.size(0) == tokens;
+  return plain_i32(*offsets, dev, 1) && offsets->size(0) == lengths.size(0) + 1;
+}
+
+at::Tensor dense_scratch(int64_t B, int64_t H, bool shared, const at::Device& dev) {
+  return at::empty({(int64_t)dsa_dense_scratch_size(B, (int32_t)H, shared ? 1 : 0)},
+                   at::TensorOptions().dtype(at::kByte).device(dev));
+}
+
+int64_t decode_window(const at::Tensor& q_nope, const at::Tensor& q_pe, const at::Tensor& ckv,
+                      const at::Tensor& kpe, int64_t page_size, const at::Tensor& page_table,
+                      const at::Tensor& lengths, const OptTensor& row_offsets, int64_t window,
+                      int64_t sinks, double sm_scale, const at::Tensor& out,
+                      const at::Tensor& lse, const at::Tensor& ws, int64_t stream) {
+  const DenseArgs a(q_nope, q_pe, ckv, kpe, page_size, out, lse, ws);
+  const auto dev = q_nope.device();
+  if (!a.ok || !plain_rows(page_table, lengths, row_offsets, a.B, dev)) return kNotHandled;
+  const at::Tensor scratch = dense_scratch(a.B, a.H, false, dev);
+  return dsa_mla_decode_window(
+      q_nope.data_ptr(), q_nope.stride(0), q_nope.stride(1), q_pe.data_ptr(), q_pe.stride(0),
+      q_pe.stride(1), ckv.data_ptr(), a.ckv_ss, kpe.data_ptr(), a.kpe_ss, a.slots,
+      (int32_t)a.page, i32(page_table), page_table.stride(0), (int32_t)page_table.size(1),
+      i32(lengths), row_offsets.has_value() ? i32(*row_offsets) : nullptr,
+      (int32_t)lengths.size(0), (int32_t)window, (int32_t)sinks, (float)sm_scale, out.data_ptr(),
+      out.stride(0), out.stride(1), f32(lse), lse.stride(0), lse.stride(1), a.B, (int32_t)a.H,
+      scratch.data_ptr(), (size_t)scratch.numel(), ws.data_ptr(), reinterpret_cast<void*>(stream));
+}
+
+int64_t decode_shared(const at::Tensor& q_nope, const at::Tensor& q_pe, const at::Tensor& ckv,
+                      const at::Tensor& kpe, int64_t page_size, const at::Tensor& prefix_table,
+                      const at::Tensor& prefix_lengths, const OptTensor& group_offsets,
+                      const at::Tensor& page_table, const at::Tensor& lengths,
+                      const OptTensor& row_offsets, double sm_scale, const at::Tensor& out,
+                      const at::Tensor& lse, const at::Tensor& ws, int64_t stream) {
+  const DenseArgs a(q_nope, q_pe, ckv, kpe, page_size, out, lse, ws);
+  const auto dev = q_nope.device();
+  if (!a.ok || !plain_rows(page_table, lengths, row_offsets, a.B, dev)) return kNotHandled;
+  const int64_t groups = prefix_lengths.numel();
+  if (!plain_i32(prefix_table, dev, 2) || !plain_i32(prefix_lengths, dev, 1) || groups < 1 ||
+      prefix_table.size(0) != groups || prefix_table.size(1) < 1)
+    return kNotHandled;
+  if (group_offsets.has_value()
+          ? !plain_i32(*group_offsets, dev, 1) || group_offsets->size(0) != groups + 1
+          : groups != 1)
+    return kNotHandled;
+  const at::Tensor scratch = dense_scratch(a.B, a.H, true, dev);
+  return dsa_mla_decode_shared(
+      q_nope.data_ptr(), q_nope.stride(0), q_nope.stride(1), q_pe.data_ptr(), q_pe.stride(0),
+      q_pe.stride(1), ckv.data_ptr(), a.ckv_ss, kpe.data_ptr(), a.kpe_ss, a.slots,
+      (int32_t)a.page, i32(prefix_table), prefix_table.stride(0), (int32_t)prefix_table.size(1),
+      i32(prefix_lengths), group_offsets.has_value() ? i32(*group_offsets) : nullptr,
+      (int32_t)groups, i32(page_table), page_table.stride(0), (int32_t)page_table.size(1),
+      i32(lengths), row_offsets.has_value() ? i32(*row_offsets) : nullptr,
+      (int32_t)lengths.size(0), (float)sm_scale, out.data_ptr(), out.stride(0), out.stride(1),
+      f32(lse), lse.stride(0), lse.stride(1), a.B, (int32_t)a.H, scratch.data_ptr(),
+      (size_t)scratch.numel(), ws.data_ptr(), reinterpret_cast<void*>(stream));
+}
+
+int64_t merge_states(const std::vector<at::Tensor>& outs, const std::vector<at::Tensor>& lses,
+                     const at::Tensor& out, const at::Tensor& lse, int64_t stream) {
+  constexpr size_t kMost = 8;
+  const size_t n = outs.size();
+  if (n < 1 || n > kMost || lses.size() != n || !out.is_cuda() || out.dim() != 3 ||
+      out.size(2) != 512 || out.scalar_type() != at::kBFloat16 || out.stride(2) != 1)
+    return kNotHandled;
+  const auto dev = out.device();
+  if (lse.device() != dev || lse.scalar_type() != at::kFloat || lse.dim() != 2 ||
+      lse.size(0) != out.size(0) || lse.size(1) != out.size(1))
+    return kNotHandled;
+  const void* o[kMost];
+  const float* z[kMost];
+  int64_t os[2 * kMost], zs[2 * kMost];
+  for (size_t i = 0; i < n; ++i) {
+    const at::Tensor &a = outs[i], &b = lses[i];
+    if (a.device() != dev || a.scalar_type() != at::kBFloat16 || a.sizes() != out.sizes() ||
+        a.stride(2) != 1 || b.device() != dev || b.scalar_type() != at::kFloat ||
+        b.sizes() != lse.sizes())
+      return kNotHandled;
+    o[i] = a.data_ptr();
+    z[i] = f32(b);
+    os[2 * i] = a.stride(0);
+    os[2 * i + 1] = a.stride(1);
+    zs[2 * i] = b.stride(0);
+    zs[2 * i + 1] = b.stride(1);
+  }
+  return dsa_merge_states((int32_t)n, o, os, z, zs, out.data_ptr(), out.stride(0), out.stride(1),
+                          f32(lse), lse.stride(0), lse.stride(1), out.size(0),
+                          (int32_t)out.size(1), reinterpret_cast<void*>(stream));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -219,5 +349,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("append_q8", &append_q8, "tokens into the 8-bit cache");
   m.def("accumulate_weights", &accumulate_weights, "attention weights into running totals");
   m.def("evict_positions", &evict_positions, "the positions an eviction keeps");
+  m.def("decode_window", &decode_window, "attention over a window and sinks");
+  m.def("decode_shared", &decode_shared, "attention of rows that share prefixes");
+  m.def("merge_states", &merge_states, "attention results joined");
   m.def("compact_q8", &compact_q8, "kept tokens of the 8-bit cache to new pages");
 }

@@ -295,6 +295,74 @@ int dsa_compact_q8(const int32_t* keep, int64_t keep_stride_b, int32_t num_rows,
                    void* workspace, void* stream);
 
 /*
+ * Dense attention over the bf16 latent cache.  No counterpart in the reference, whose rows name
+ * every position they read (fused.py:150); the mathematics is baseline.py:17-45 over the
+ * positions that a rule names.  Pools, queries, output, lse and workspace as for
+ * dsa_sparse_mla_decode(); output is 16-byte aligned, its strides too.
+ *
+ * Row r (num_rows of them) is a sequence: its pages are page_table row r (int32, page_size a power
+ * of two), its positions [0, lengths[r]).  Its tokens are [row_offsets[r], row_offsets[r + 1])
+ * (num_rows + 1 ascending int32) and stand at the sequence's last positions; row_offsets NULL: one
+ * token a row (num_rows == num_tokens).  Tokens before the first or behind the last offset are
+ * left as they are, in output and lse.  A token that sees nothing gets output 0 and lse -inf.  A
+ * position that the table has no page for is left out and sets DSA_DEVERR_BAD_INDEX.  Lengths and
+ * offsets are read on the device.
+ *
+ * dsa_mla_decode_window: the token at position p sees the positions q <= p with q < sinks or
+ * q > p - window.
+ *
+ * dsa_mla_decode_shared: groups of rows share a prefix.  Group g's prefix is the positions
+ * [0, prefix_lengths[g]) of prefix_table row g; its rows are [group_offsets[g],
+ * group_offsets[g + 1]) (num_groups + 1 ascending int32; NULL: num_groups == 1 and all rows; rows
+ * outside have no prefix).  page_table and lengths describe what follows the prefix, from
+ * position 0 of a row's own pages.  A token sees its group's prefix and the own positions up to
+ * its own; a row of length 0 with one token sees the prefix alone.
+ *
+ * Both need `scratch`, a device buffer of dsa_dense_scratch_size() bytes for this call alone
+ * (calls that may overlap on the GPU need one each).
+ */
+int dsa_mla_decode_window(
+    const void* q_nope, int64_t q_nope_stride_b, int64_t q_nope_stride_h, const void* q_pe,
+    int64_t q_pe_stride_b, int64_t q_pe_stride_h, const void* ckv_cache, int64_t ckv_slot_stride,
+    const void* kpe_cache, int64_t kpe_slot_stride, int64_t num_slots, int32_t page_size,
+    const int32_t* page_table, int64_t page_table_stride_b, int32_t page_table_cols,
+    const int32_t* lengths, const int32_t* row_offsets, int32_t num_rows, int32_t window,
+    int32_t sinks, float sm_scale, void* output, int64_t output_stride_b, int64_t output_stride_h,
+    float* lse, int64_t lse_stride_b, int64_t lse_stride_h, int64_t num_tokens, int32_t num_heads,
+    void* scratch, size_t scratch_bytes, void* workspace, void* stream);
+
+int dsa_mla_decode_shared(
+    const void* q_nope, int64_t q_nope_stride_b, int64_t q_nope_stride_h, const void* q_pe,
+    int64_t q_pe_stride_b, int64_t q_pe_stride_h, const void* ckv_cache, int64_t ckv_slot_stride,
+    const void* kpe_cache, int64_t kpe_slot_stride, int64_t num_slots, int32_t page_size,
+    const int32_t* prefix_table, int64_t prefix_table_stride_g, int32_t prefix_table_cols,
+    const int32_t* prefix_lengths, const int32_t* group_offsets, int32_t num_groups,
+    const int32_t* page_table, int64_t page_table_stride_b, int32_t page_table_cols,
+    const int32_t* lengths, const int32_t* row_offsets, int32_t num_rows, float sm_scale,
+    void* output, int64_t output_stride_b, int64_t output_stride_h, float* lse,
+    int64_t lse_stride_b, int64_t lse_stride_h, int64_t num_tokens, int32_t num_heads,
+    void* scratch, size_t scratch_bytes, void* workspace, void* stream);
+
+/* Bytes of scratch a window (shared == 0) or shared call needs on the current device; 0 for an
+ * unsupported shape. */
+size_t dsa_dense_scratch_size(int64_t num_tokens, int32_t num_heads, int32_t shared);
+
+/*
+ * Joins attention results over separate sets of positions: part i of num_parts (1 to 8) is
+ * outputs[i] [num_tokens, num_heads, 512] bf16 with strides output_strides[2 i], [2 i + 1] and its
+ * base-2 log-sum-exp lses[i] with strides lse_strides[2 i], [2 i + 1] (host arrays).  With M the
+ * largest lse and w_i = 2^(lse_i - M): output = sum w_i outputs[i] / sum w_i (summed in fp32),
+ * lse = M + log2 sum w_i.  A part of lse -inf is left out whatever its output holds; where all
+ * are, output is 0 and lse -inf.  Output and lse may each be a part's own; any other overlap with
+ * a part is refused.
+ */
+int dsa_merge_states(int32_t num_parts, const void* const* outputs,
+                     const int64_t* output_strides, const float* const* lses,
+                     const int64_t* lse_strides, void* output, int64_t output_stride_b,
+                     int64_t output_stride_h, float* lse, int64_t lse_stride_b,
+                     int64_t lse_stride_h, int64_t num_tokens, int32_t num_heads, void* stream);
+
+/*
  * Bytes of workspace dsa_sparse_mla_decode() needs for this problem on
  * `device` (split-K partials and the error word; the size depends only on
  * the device's SM count, so one workspace serves every shape).

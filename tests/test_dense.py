@@ -1,0 +1,158 @@
+"""The dense operators without a GPU: refusals, host checks of the C ABI, the 64-bit reference."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import dense_reference as ref
+from flashinfer_mlsys2026_dsa_b200 import _native, kernel_shared, kernel_window, merge_states
+
+
+def test_reference_window_is_softmax_over_the_visible_positions():
+    """attend() against torch.softmax with the rule written as loops."""
+    ckv, kpe = ref.pools(3, 8, 1, "cpu")
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32)
+    qn, qp = ref.queries(3, 16, 2, "cpu")
+    n, win, sinks = 19, 5, 2
+    out, lse, _, _ = ref.window(qn, qp, ckv, kpe, table, [n], [3], 0.1, win, sinks, 8)
+    keys = torch.cat([torch.cat([ckv[i], kpe[i]], 1) for i in (2, 0, 1)])[:n].double()
+    for j in range(3):
+        p = n - 3 + j
+        some = [i for i in range(n) if i <= p and (i < sinks or i > p - win)]
+        x = torch.cat([qn[j], qp[j]], 1).double() @ keys[some].T * 0.1
+        torch.testing.assert_close(out[j], torch.softmax(x, 1) @ keys[some][:, :512])
+        torch.testing.assert_close(lse[j], torch.logsumexp(x, 1) / math.log(2))
+
+
+def test_reference_shared_is_the_window_over_joined_pages():
+    ckv, kpe = ref.pools(6, 4, 3, "cpu")
+    qn, qp = ref.queries(3, 16, 4, "cpu")
+    pre, own = torch.tensor([[5, 1]], dtype=torch.int32), torch.tensor([[0, 2], [4, 3]], dtype=torch.int32)
+    got = ref.shared(qn, qp, ckv, kpe, pre, [8], [2], own, [5, 7], [1, 2], 0.1, 4)
+    whole = torch.cat([pre.expand(2, -1), own], 1)
+    want = ref.window(qn, qp, ckv, kpe, whole, [13, 15], [1, 2], 0.1, None, 0, 4)
+    torch.testing.assert_close(got[0], want[0])
+    torch.testing.assert_close(got[1], want[1])
+
+
+def test_reference_merge_joins_parts_of_one_softmax():
+    ckv, kpe = ref.pools(4, 8, 5, "cpu")
+    q = torch.cat(ref.queries(2, 16, 6, "cpu"), 2)
+    keys = ref.sequence(ckv, kpe, torch.arange(4), 30, 8)
+    seen = torch.ones(2, 30, dtype=torch.bool)
+    first = torch.arange(30) < 11
+    whole = ref.attend(q, keys, seen, 0.1)
+    parts = [ref.attend(q, keys, seen & first, 0.1), ref.attend(q, keys, seen & ~first, 0.1)]
+    out, lse, _, _ = ref.merge([x[0] for x in parts], [x[1] for x in parts])
+    torch.testing.assert_close(out, whole[0])
+    torch.testing.assert_close(lse, whole[1])
+
+
+def test_calls_without_a_gpu_are_refused():
+    ckv, kpe = ref.pools(2, 16, 1, "cpu")
+    qn, qp = ref.queries(1, 16, 2, "cpu")
+    out, lse = torch.empty_like(qn), torch.empty(1, 16)
+    table, n = torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        kernel_window(qn, qp, ckv, kpe, table, n, 0.1, out, lse, 4)
+    with pytest.raises(ValueError, match="CUDA"):
+        kernel_shared(qn, qp, ckv, kpe, table, n, table, n, 0.1, out, lse)
+    with pytest.raises(ValueError, match="CUDA"):
+        merge_states([out, out], [lse, lse], out, lse)
+    for bad in (dict(window=-1), dict(sinks=-1)):
+        with pytest.raises(ValueError, match=">= 0"):
+            kernel_window(qn, qp, ckv, kpe, table, n, 0.1, out, lse, **bad)
+    for outs, lses in (([], []), ([out] * 9, [lse] * 9), ([out], [lse, lse])):
+        with pytest.raises(ValueError, match="parts"):
+            merge_states(outs, lses, out, lse)
+
+
+# Host checks return before any CUDA call; 16 stands for an aligned pointer.
+Q = [16, 16 * 512, 512, 16, 16 * 64, 64]
+POOLS = [16, 512, 16, 64, 640]
+TABLE = [16, 4, 4]
+
+
+def _window(q=Q, pools=POOLS, page=64, table=TABLE, lengths=16, offsets=None, rows=2, window=8,
+            sinks=1, out=(16, 16 * 512, 512), lse=(16, 16, 1), tokens=2, heads=16, scratch=16,
+            nbytes=1 << 40, ws=16):
+    return _native.load().dsa_mla_decode_window(
+        *q, *pools, page, *table, lengths, offsets, rows, window, sinks, 0.1, *out, *lse, tokens,
+        heads, scratch, nbytes, ws, None)
+
+
+def _shared(prefix=TABLE, plens=16, goffs=None, groups=1, tokens=2, rows=2, table=TABLE, page=64,
+            ws=16, scratch=16):
+    return _native.load().dsa_mla_decode_shared(
+        *Q, *POOLS, page, *prefix, plens, goffs, groups, *table, 16, None, rows, 0.1,
+        16, 16 * 512, 512, 16, 16, 1, tokens, 16, scratch, 1 << 40, ws, None)
+
+
+def _with(values, i, x):
+    values = list(values)
+    values[i] = x
+    return values
+
+
+def test_window_arguments():
+    assert _window(tokens=0, rows=0) == 0 and _window(tokens=0) == 0
+    assert _window(heads=8) == 2 and _window(tokens=-1) == 1 and _window(rows=-1) == 1
+    assert _window(rows=3) == 1                        # a token a row
+    assert _window(window=-1) == 1 and _window(sinks=-1) == 1
+    assert _window(page=0) == 1 and _window(page=48) == 1
+    assert _window(lengths=None) == 1 and _window(ws=None) == 4
+    assert _window(tokens=1 << 40, rows=2, offsets=16) == 1
+    for i, bad, code in ((0, None, 1), (0, 24, 3), (1, 8193, 3), (2, 513, 3), (3, None, 1), (4, 1026, 3)):
+        assert _window(q=_with(Q, i, bad)) == code, (i, bad)
+    for i, bad, code in ((0, None, 1), (1, 511, 1), (1, 516, 3), (2, 8, 3), (3, 63, 1), (4, 0, 1),
+                         (4, 1 << 31, 1)):
+        assert _window(pools=_with(POOLS, i, bad)) == code, (i, bad)
+    for i, bad in ((0, None), (1, 3), (2, 0), (2, 1 << 26)):
+        assert _window(table=_with(TABLE, i, bad)) == 1, (i, bad)
+    assert _window(out=(24, 16 * 512, 512)) == 3 and _window(out=(None, 1, 1)) == 1
+    assert _window(lse=(None, 16, 1)) == 1
+
+
+def test_shared_arguments():
+    assert _shared(tokens=0, rows=0) == 0
+    assert _shared(groups=0) == 1 and _shared(groups=2) == 1 and _shared(plens=None) == 1
+    assert _shared(prefix=[None, 4, 4]) == 1 and _shared(prefix=[16, 3, 4]) == 1
+    assert _shared(prefix=[16, 1 << 26, 1 << 26]) == 1
+    assert _shared(rows=1) == 1 and _shared(ws=None) == 4 and _shared(page=3) == 1
+
+
+def test_scratch_size():
+    size = _native.load().dsa_dense_scratch_size
+    for bad in ((1, 8, 0), (-1, 16, 0), (1 << 40, 16, 1), (0, 16, 1)):
+        assert size(*bad) == 0
+
+
+def _merge(parts=2, outs=(1 << 20, 2 << 20), strides=(8192, 512) * 2, lses=(3 << 20, 4 << 20),
+           lse_strides=(16, 1) * 2, out=(5 << 20, 8192, 512), lse=(6 << 20, 16, 1), tokens=3, heads=16):
+    n = len(outs)
+    return _native.load().dsa_merge_states(
+        parts, (ctypes.c_void_p * n)(*outs), (ctypes.c_int64 * (2 * n))(*strides),
+        (ctypes.c_void_p * n)(*lses), (ctypes.c_int64 * (2 * n))(*lse_strides), *out, *lse, tokens,
+        heads, None)
+
+
+def test_merge_arguments():
+    assert _merge(tokens=0) == 0
+    assert _merge(parts=0) == 1 and _merge(parts=9) == 1 and _merge(tokens=-1) == 1 and _merge(heads=0) == 1
+    assert _merge(outs=(None, 16)) == 1 and _merge(lses=(16, None)) == 1
+    assert _merge(outs=(24, 1 << 20)) == 3 and _merge(strides=(8192, 513, 8192, 512)) == 3
+    assert _merge(out=(24, 8192, 512)) == 3 and _merge(out=(None, 1, 1)) == 1
+
+
+def test_merge_refuses_a_result_that_overlaps_a_part():
+    """A row of 16 heads is 16,384 bytes here, a token's lse 64."""
+    first = 1 << 20
+    for shift in (16, 1008, 1024, 16384, 2 * 16384, -1024, -16):
+        assert _merge(out=(first + shift, 8192, 512)) == 1, shift
+    for shift in (4, 60, 64, 128, -4):
+        assert _merge(lse=((3 << 20) + shift, 16, 1)) == 1, shift
+    # other strides over the same memory
+    assert _merge(out=(first, 16384, 512)) == 1
+    # interleaved with a part (rows between its rows, one of which would be met)
+    assert _merge(strides=(16384, 512) * 2, out=(first + 16384 + 512, 16384, 512)) == 1
