@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "dsa_b200.h"
 #include "dsa_common.cuh"
@@ -25,99 +26,36 @@ struct Table {
 };
 
 struct Params {
-  const __nv_bfloat16 *qn, *qp, *ckv, *kpe;
-  int64_t qn_sb, qn_sh, qp_sb, qp_sh, ckv_ss, kpe_ss, num_slots;
   Table own, pre;                  // pre.pt == nullptr: no prefixes
+  int64_t num_slots;
   int32_t page_shift;
   const int32_t *lengths, *row_offsets;     // row_offsets nullptr: a token a row
   const int32_t *pre_lengths, *group_offsets;  // group_offsets nullptr: one group of all rows
   int32_t rows, groups, tokens, heads;
+  int32_t head_shift, tpu;         // log2 heads; tokens of a unit
   int32_t window, sinks;
+  int64_t unit_tiles;              // tiles of a unit, at most
+  int32_t whole;                   // a pair for each unit
   float scale_log2;
   __nv_bfloat16* out;
   int64_t out_sb, out_sh;
   float* lse;
   int64_t lse_sb, lse_sh;
   uint32_t* err;
+  uint64_t wait_cycles;
+  // scratch: (tiles, pairs); where units lie in the line; partial results and their (max, sum)
+  int64_t *head, *cuts;
+  float2* sums;
+  float* part;
 };
 
-// The last i in [0, n) with offsets[i] <= x, -1 if there is none (ascending offsets).
-__device__ __forceinline__ int owner(const int32_t* offsets, int n, int x) {
-  int lo = -1, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(offsets + mid) <= x) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
+}  // namespace dense
+}  // namespace dsa
 
-// A warp is one head of one token: lane l holds 16 + 2 of the query's values and of the output's
-// 512; positions one after another with the running maximum and sum.
-__global__ void __launch_bounds__(256) attend_kernel(const Params p) {
-  const int t = blockIdx.x, h = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  int row = t, n = 1, j = 0;
-  if (p.row_offsets != nullptr) {
-    row = owner(p.row_offsets, p.rows + 1, t);
-    if (row < 0 || row >= p.rows) return;  // a token of no row: left as it is
-    j = t - p.row_offsets[row];
-    n = p.row_offsets[row + 1] - p.row_offsets[row];
-  }
-  float q[18], o[16];
-  for (int i = 0; i < 16; ++i) {
-    q[i] = __bfloat162float(p.qn[t * p.qn_sb + h * p.qn_sh + lane * 16 + i]);
-    o[i] = 0.f;
-  }
-  for (int i = 0; i < 2; ++i)
-    q[16 + i] = __bfloat162float(p.qp[t * p.qp_sb + h * p.qp_sh + lane * 2 + i]);
-  float m = -INFINITY, l = 0.f;
-  bool bad = false, any = false;
-  auto key = [&](const Table& tab, int r, int pos) {
-    const int pg = pos >> p.page_shift;
-    const int page = pg < tab.cols ? __ldg(tab.pt + r * tab.sb + pg) : -1;
-    const int64_t slot = ((int64_t)page << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
-    if (page < 0 || slot >= p.num_slots) {
-      bad = true;
-      return;
-    }
-    const __nv_bfloat16* k = p.ckv + slot * p.ckv_ss + lane * 16;
-    const __nv_bfloat16* e = p.kpe + slot * p.kpe_ss + lane * 2;
-    float v[16], s = 0.f;
-    for (int i = 0; i < 16; ++i) {
-      v[i] = __bfloat162float(k[i]);
-      s += q[i] * v[i];
-    }
-    for (int i = 0; i < 2; ++i) s += q[16 + i] * __bfloat162float(e[i]);
-    for (int i = 16; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
-    s *= p.scale_log2;
-    any = true;
-    const float mn = fmaxf(m, s);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float a = exp2f(m - base), w = exp2f(s - base);
-    l = l * a + w;
-    for (int i = 0; i < 16; ++i) o[i] = o[i] * a + w * v[i];
-    m = mn;
-  };
-  if (p.pre.pt != nullptr) {
-    int g = 0;
-    if (p.group_offsets != nullptr) g = owner(p.group_offsets, p.groups + 1, row);
-    if (g >= 0 && g < p.groups) {
-      const int len = p.pre_lengths[g];
-      const int cap = p.pre.cols << p.page_shift;
-      bad |= len > cap;
-      for (int i = 0; i < min(len, cap); ++i) key(p.pre, g, i);
-    }
-  }
-  const int pos = p.lengths[row] - n + j, cap = p.own.cols << p.page_shift;
-  bad |= pos >= cap;
-  const int last = min(pos, cap - 1), first = max(0, p.window >= pos + 1 ? 0 : pos - p.window + 1);
-  for (int i = 0; i <= min(last, min(p.sinks, first) - 1); ++i) key(p.own, row, i);
-  for (int i = first; i <= last; ++i) key(p.own, row, i);
-  if (bad && lane == 0) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
-  for (int i = 0; i < 16; ++i)
-    p.out[t * p.out_sb + h * p.out_sh + lane * 16 + i] = __float2bfloat16(any ? o[i] / l : 0.f);
-  if (lane == 0) p.lse[t * p.lse_sb + h * p.lse_sh] = any ? m + log2f(l) : -INFINITY;
-}
+#include "dsa_dense_attend.cuh"
+
+namespace dsa {
+namespace dense {
 
 // ------------------------------------------------------------------------------- the join
 
@@ -198,20 +136,6 @@ __global__ void __launch_bounds__(256) merge_kernel(const MergeParams p) {
   if (lane == 0) p.lse[t * p.lse_sb + h * p.lse_sh] = base + log2f(total);
 }
 
-template <typename P>
-int launch(void (*kern)(P), dim3 grid, unsigned threads, cudaStream_t st, const P& p) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
-}
-
 // Whether rows of `width` elements at a + t sb + h sh and at b + t sb + h sh meet, for any
 // (t, h) of either (bytes throughout).
 bool same_grid_meets(int64_t d, int64_t sb, int64_t sh, int64_t tokens, int64_t heads,
@@ -261,6 +185,8 @@ bool aligned_rows(const void* p, int64_t sb, int64_t sh) {
 // What window and shared have in common; `pre` fields are zero for a window call.
 struct Call {
   Params p;
+  const void *qn, *qp, *ckv, *kpe;
+  int64_t qn_sb, qn_sh, qp_sb, qp_sh, ckv_ss, kpe_ss;
   int32_t page_size;
   void* scratch;
   size_t scratch_bytes;
@@ -268,9 +194,79 @@ struct Call {
   void* stream;
 };
 
+constexpr int kMaxDevices = 64;
+
+// CTA pairs that the current device runs at once; 0 on an error.
+int max_pairs() {
+  static std::atomic<int> known[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+  int n = known[dev].load(std::memory_order_acquire);
+  if (n > 0) return n;
+  if (cudaFuncSetAttribute(attend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           SMEM_BYTES) != cudaSuccess)
+    return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, attend_kernel, &cfg) != cudaSuccess || n < 1) return 0;
+  known[dev].store(n, std::memory_order_release);
+  return n;
+}
+
+// Where scratch holds what.
+struct Layout {
+  size_t cuts, sums, part, total;
+  Layout(int64_t tokens, int32_t heads, bool shared, int pairs) {
+    const int64_t rows = shared ? 2 * tokens * heads + 128 * (int64_t)pairs : 256 * (int64_t)pairs;
+    cuts = 256;
+    sums = cuts + (size_t)((shared ? 48 * tokens : 32 * (int64_t)pairs) + 255) / 256 * 256;
+    part = sums + (size_t)(rows * 8 + 255) / 256 * 256;
+    total = part + (size_t)rows * kDCkv * 4;
+  }
+};
+
+int box_map(CUtensorMap* m, const void* base, int64_t stride, int width, int64_t rows, int box) {
+  const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
+  const cuuint32_t b[2] = {64, (cuuint32_t)box};
+  return encode(m, base, 2, dims, strides, b, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+int query_map(CUtensorMap* m, const void* base, int64_t sb, int64_t sh, int width, int heads,
+              int64_t tokens) {
+  const cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)heads, (cuuint64_t)tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
+  const cuuint32_t h = (cuuint32_t)std::min(heads, 64);
+  const cuuint32_t b[3] = {64, h, 64 / h};
+  return encode(m, base, 3, dims, strides, b, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 int check_table(const Table& t, int32_t page_size) {
   if (t.pt == nullptr || t.cols < 1 || (t.sb < t.cols)) return DSA_ERR_INVALID_ARGUMENT;
   return (int64_t)t.cols * page_size > INT32_MAX / 2 ? DSA_ERR_INVALID_ARGUMENT : DSA_OK;
+}
+
+template <typename... A>
+int launch_pdl(void (*kern)(A...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st,
+               A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
 }
 
 int attend(Call& c) {
@@ -279,26 +275,68 @@ int attend(Call& c) {
   if (!heads_supported(p.heads)) return DSA_ERR_UNSUPPORTED;
   if (p.tokens == 0 || p.rows == 0) return DSA_OK;
   if (p.row_offsets == nullptr && p.rows != p.tokens) return DSA_ERR_INVALID_ARGUMENT;
-  if (!p.qn || !p.qp || !p.ckv || !p.kpe || !p.lengths || !p.out || !p.lse ||
-      p.num_slots < 1 || p.num_slots > INT32_MAX - 64 || p.ckv_ss < kDCkv || p.kpe_ss < kDKpe ||
-      p.window < 0 || p.sinks < 0 || c.page_size < 1 || (c.page_size & (c.page_size - 1)))
+  if (!c.qn || !c.qp || !c.ckv || !c.kpe || !p.lengths || !p.out || !p.lse || p.num_slots < 1 ||
+      p.num_slots > INT32_MAX - 64 || c.ckv_ss < kDCkv || c.kpe_ss < kDKpe || p.window < 0 ||
+      p.sinks < 0 || c.page_size < 1 || (c.page_size & (c.page_size - 1)))
     return DSA_ERR_INVALID_ARGUMENT;
   int rc = check_table(p.own, c.page_size);
   if (rc == DSA_OK && p.pre.pt != nullptr) rc = check_table(p.pre, c.page_size);
   if (rc != DSA_OK) return rc;
-  if (!aligned_rows(p.qn, p.qn_sb, p.qn_sh) || !aligned_rows(p.qp, p.qp_sb, p.qp_sh) ||
-      !aligned_rows(p.ckv, p.ckv_ss, 0) || !aligned_rows(p.kpe, p.kpe_ss, 0) ||
+  if (!aligned_rows(c.qn, c.qn_sb, c.qn_sh) || !aligned_rows(c.qp, c.qp_sb, c.qp_sh) ||
+      !aligned_rows(c.ckv, c.ckv_ss, 0) || !aligned_rows(c.kpe, c.kpe_ss, 0) ||
       !aligned_rows(p.out, p.out_sb, p.out_sh))
     return DSA_ERR_MISALIGNED;
   if (c.workspace == nullptr) return DSA_ERR_WORKSPACE;
+  const bool shared = p.pre.pt != nullptr;
+  if (shared && 2 * (int64_t)p.tokens * p.heads > INT32_MAX / 2) return DSA_ERR_INVALID_ARGUMENT;
+  int pairs = max_pairs();
+  if (pairs < 1) return DSA_ERR_CUDA;
+  const Layout at(p.tokens, p.heads, shared, pairs);
+  if (c.scratch == nullptr || c.scratch_bytes < at.total) return DSA_ERR_WORKSPACE;
+
   p.page_shift = 0;
   while ((1 << p.page_shift) < c.page_size) ++p.page_shift;
+  p.head_shift = 0;
+  while ((1 << p.head_shift) < p.heads) ++p.head_shift;
+  p.tpu = 128 / p.heads;
   p.window = std::min(p.window, kAll);
   p.sinks = std::min(p.sinks, kAll);
+  // The chunks that T tokens' sinks and windows can touch.
+  const int64_t span = (int64_t)p.window + p.tpu - 1;
+  const int64_t chunks = ((int64_t)p.sinks + kChunk - 1) / kChunk + (span + 30) / kChunk + 1;
+  p.unit_tiles = (chunks + kTileChunks - 1) / kTileChunks;
   p.err = static_cast<uint32_t*>(c.workspace);
-  attend_kernel<<<dim3((unsigned)p.tokens, (unsigned)(p.heads / 8)), 256, 0,
-                  static_cast<cudaStream_t>(c.stream)>>>(p);
-  return cudaGetLastError() == cudaSuccess ? DSA_OK : DSA_ERR_CUDA;
+  p.wait_cycles = wait_limit_cycles();
+  uint8_t* scratch = static_cast<uint8_t*>(c.scratch);
+  p.head = reinterpret_cast<int64_t*>(scratch);
+  p.cuts = reinterpret_cast<int64_t*>(scratch + at.cuts);
+  p.sums = reinterpret_cast<float2*>(scratch + at.sums);
+  p.part = reinterpret_cast<float*>(scratch + at.part);
+
+  CUtensorMap ckv, kpe, ckv1, kpe1, qn, qp;
+  const int box = std::min(c.page_size, kChunk);
+  if ((rc = box_map(&ckv, c.ckv, c.ckv_ss, kDCkv, p.num_slots, box)) != DSA_OK ||
+      (rc = box_map(&kpe, c.kpe, c.kpe_ss, kDKpe, p.num_slots, box)) != DSA_OK ||
+      (rc = box_map(&ckv1, c.ckv, c.ckv_ss, kDCkv, p.num_slots, 1)) != DSA_OK ||
+      (rc = box_map(&kpe1, c.kpe, c.kpe_ss, kDKpe, p.num_slots, 1)) != DSA_OK ||
+      (rc = query_map(&qn, c.qn, c.qn_sb, c.qn_sh, kDCkv, p.heads, p.tokens)) != DSA_OK ||
+      (rc = query_map(&qp, c.qp, c.qp_sb, c.qp_sh, kDKpe, p.heads, p.tokens)) != DSA_OK)
+    return rc;
+
+  const cudaStream_t st = static_cast<cudaStream_t>(c.stream);
+  // One unit a row: where two would not fit side by side, each has a pair of its own and is cut
+  // nowhere.
+  p.whole = !shared && p.row_offsets == nullptr && p.rows <= pairs && 2 * p.rows > pairs;
+  if (p.whole) pairs = p.rows;
+  if ((rc = launch_pdl(attend_kernel, dim3(2 * (unsigned)pairs), kThreads, SMEM_BYTES, st, ckv, kpe,
+                       ckv1, kpe1, qn, qp, p)) != DSA_OK)
+    return rc;
+  if (shared)
+    return launch_pdl(join_tokens_kernel, dim3((unsigned)((int64_t)p.tokens * p.heads / 16), 4), 128,
+                      0, st, p);
+  if (!p.whole && pairs > 1)
+    return launch_pdl(join_cuts_kernel, dim3((unsigned)(pairs - 1), 8), 256, 0, st, p);
+  return DSA_OK;
 }
 
 }  // namespace dense
@@ -322,16 +360,16 @@ dense::Call common(const void* q_nope, int64_t q_nope_stride_b, int64_t q_nope_s
                    void* stream) {
   dense::Call c = {};
   dense::Params& p = c.p;
-  p.qn = static_cast<const __nv_bfloat16*>(q_nope);
-  p.qn_sb = q_nope_stride_b;
-  p.qn_sh = q_nope_stride_h;
-  p.qp = static_cast<const __nv_bfloat16*>(q_pe);
-  p.qp_sb = q_pe_stride_b;
-  p.qp_sh = q_pe_stride_h;
-  p.ckv = static_cast<const __nv_bfloat16*>(ckv_cache);
-  p.ckv_ss = ckv_slot_stride;
-  p.kpe = static_cast<const __nv_bfloat16*>(kpe_cache);
-  p.kpe_ss = kpe_slot_stride;
+  c.qn = q_nope;
+  c.qn_sb = q_nope_stride_b;
+  c.qn_sh = q_nope_stride_h;
+  c.qp = q_pe;
+  c.qp_sb = q_pe_stride_b;
+  c.qp_sh = q_pe_stride_h;
+  c.ckv = ckv_cache;
+  c.ckv_ss = ckv_slot_stride;
+  c.kpe = kpe_cache;
+  c.kpe_ss = kpe_slot_stride;
   p.num_slots = num_slots;
   p.own = {page_table, page_table_stride_b, page_table_cols};
   p.lengths = lengths;
@@ -361,8 +399,8 @@ extern "C" {
 
 size_t dsa_dense_scratch_size(int64_t num_tokens, int32_t num_heads, int32_t shared) {
   if (!heads_supported(num_heads) || clamp32(num_tokens) < 1) return 0;
-  (void)shared;
-  return 16;
+  const int pairs = dense::max_pairs();
+  return pairs < 1 ? 0 : dense::Layout(num_tokens, num_heads, shared != 0, pairs).total;
 }
 
 int dsa_mla_decode_window(
@@ -453,7 +491,7 @@ int dsa_merge_states(int32_t num_parts, const void* const* outputs,
       merge_kernel<1>, merge_kernel<2>, merge_kernel<3>, merge_kernel<4>,
       merge_kernel<5>, merge_kernel<6>, merge_kernel<7>, merge_kernel<8>};
   const dim3 grid((unsigned)((p.rows + 7) / 8));
-  return launch(kern[num_parts - 1], grid, 256, static_cast<cudaStream_t>(stream), p);
+  return launch_pdl(kern[num_parts - 1], grid, 256, 0, static_cast<cudaStream_t>(stream), p);
 }
 
 }  // extern "C"
