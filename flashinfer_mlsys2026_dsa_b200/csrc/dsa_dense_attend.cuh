@@ -173,28 +173,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Bounded wait for what the other CTA may have signalled.
-struct PairWaiter {
-  volatile uint32_t* abort_flag;
-  uint32_t* err;
-  uint64_t limit;
-  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) const {
-    if (ptx::mbar_test_wait_cluster(bar, parity)) return true;
-    const uint64_t t0 = ptx::cycles();
-    for (uint32_t it = 1;; ++it) {
-      if (ptx::mbar_test_wait_cluster(bar, parity)) return true;
-      if ((it & 63u) == 0) {
-        if (*abort_flag) return false;
-        if (ptx::cycles() - t0 > limit) {
-          *abort_flag = 1;
-          atomicOr(err, (uint32_t)DSA_DEVERR_TIMEOUT);
-          return false;
-        }
-      }
-    }
-  }
-};
-
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     attend_kernel(const __grid_constant__ CUtensorMap m_ckv, const __grid_constant__ CUtensorMap m_kpe,
                   const __grid_constant__ CUtensorMap m_ckv1,
@@ -605,7 +583,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ tensor cores
     if (rank == 0) {
-      const PairWaiter pwait{misc + 2, p.err, p.wait_cycles};
+      const Waiter pwait{misc + 2, p.err, p.wait_cycles, true};
       constexpr uint32_t kIdS = idesc_bf16(128, kTile, false), kIdO = idesc_bf16(128, 256, false, true);
       const uint64_t dq = desc(sbase + OFF_Q, 16, 1024, kSw128);
       const uint64_t dp = desc(sbase + OFF_P, 16, 1024, kSw128);
