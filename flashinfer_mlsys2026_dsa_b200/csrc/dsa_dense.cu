@@ -34,7 +34,7 @@ struct Params {
   int32_t rows, groups, tokens, heads;
   int32_t head_shift, tpu;         // log2 heads; tokens of a unit
   int32_t window, sinks;
-  int64_t unit_tiles;              // tiles of a unit, at most
+  int32_t unit_tiles;              // tiles of a unit, at most
   int32_t whole;                   // a pair for each unit
   float scale_log2;
   __nv_bfloat16* out;
@@ -304,7 +304,7 @@ int attend(Call& c) {
   // The chunks that T tokens' sinks and windows can touch.
   const int64_t span = (int64_t)p.window + p.tpu - 1;
   const int64_t chunks = ((int64_t)p.sinks + kChunk - 1) / kChunk + (span + 30) / kChunk + 1;
-  p.unit_tiles = (chunks + kTileChunks - 1) / kTileChunks;
+  p.unit_tiles = (int32_t)((chunks + kTileChunks - 1) / kTileChunks);
   p.err = static_cast<uint32_t*>(c.workspace);
   p.wait_cycles = wait_limit_cycles();
   uint8_t* scratch = static_cast<uint8_t*>(c.scratch);

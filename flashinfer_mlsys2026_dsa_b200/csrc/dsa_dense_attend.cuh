@@ -17,9 +17,10 @@
 // The units of all rows form one line of tiles, cut into equal parts, one for each pair.  A unit
 // that is cut leaves partial results (O, maximum, sum) that combine kernels join.
 //
-// Warps of a CTA:  0 loads keys and values, 1 issues the tensor-core work (rank 0 alone), 2 loads
-// queries, 3 walks the units, 4-11 softmax and output: a thread is a row and a quarter of a
-// tile's keys (its lane quadrant holds half of them, two warps share a quadrant).
+// Warps of a CTA:  0 and 12 load keys and values (64 columns each of a slot's 128), 1 issues the
+// tensor-core work (rank 0 alone), 2 loads queries, 3 walks the units, 4-11 softmax and output: a
+// thread is a row and a quarter of a tile's keys (its lane quadrant holds half of them, two warps
+// share a quadrant).
 #pragma once
 
 namespace dsa {
@@ -32,8 +33,9 @@ constexpr int kSlots = 5;                  // ring of 24 KB: [96 keys x 128 colu
 constexpr int kBlkB = 96 * 128;            // [96 keys x 64 columns], 128-byte swizzle
 constexpr int kSlotB = 2 * kBlkB;
 constexpr int kQBlk = 64 * 128;            // [64 rows x 64 columns]
-constexpr int kThreads = 384;
-constexpr int kLoadWarp = 0, kMmaWarp = 1, kQWarp = 2, kWalkWarp = 3, kSm0 = 4, kSmWarps = 8;
+constexpr int kThreads = 416;
+constexpr int kLoadWarp = 0, kMmaWarp = 1, kQWarp = 2, kWalkWarp = 3, kSm0 = 4, kSmWarps = 8,
+              kLoadWarp2 = 12;
 constexpr int kSegs = 4;                   // units that the walker is ahead
 constexpr float kTau = 8.f;                // a maximum that grows by less leaves O as it is
 
@@ -46,8 +48,9 @@ constexpr int OFF_MASK = OFF_SEG + kSegs * 64;   // [4 tiles][8] visible positio
 constexpr int OFF_POS = OFF_MASK + 4 * 8 * 4;    // [4 tiles][8] a chunk's first position
 constexpr int OFF_MAX = OFF_POS + 4 * 8 * 4;     // [2][4][64] row maxima of the quarters
 constexpr int OFF_SUM = OFF_MAX + 2 * 4 * 64 * 4;  // [4][64] row sums of the quarters
-constexpr int OFF_SCAN = OFF_SUM + 4 * 64 * 4;   // the start's scan: 12 x (tiles, units), result
-constexpr int OFF_MISC = OFF_SCAN + 256;
+constexpr int OFF_SCAN = OFF_SUM + 4 * 64 * 4;   // the start's scan: 13 x (tiles, units), result
+constexpr int OFF_ROWS = OFF_SCAN + 320;         // [2 loaders][2 tiles][32 + 192] slots
+constexpr int OFF_MISC = OFF_ROWS + 2 * 2 * 224 * 4;
 constexpr int SMEM_BYTES = OFF_MISC + 64 + 1024;
 static_assert(OFF_P % 1024 == 0 && OFF_KV % 1024 == 0 && kBlkB % 1024 == 0, "swizzle atoms");
 static_assert(SMEM_BYTES <= 232448, "shared memory budget");
@@ -77,10 +80,10 @@ struct Seg {
   int row, own;      // row of the page table; own positions (tokens differ in what they see) or a prefix
   int p_lo;          // the first token's position (a prefix: its last one, for all tokens)
   int t0, t1, nt;    // tiles of nt
-  int chunks, cs;    // chunks: the first cs from position 0 on, the others from `base` on
-  int base;
+  int per, rem;      // chunks of a tile; so many tiles have one more
+  int cs, base;      // the first cs chunks are from position 0 on, the others from chunk `base` on
   int slot;          // partial result's first row, -1: the unit is whole
-  int pad[4];
+  int pad[3];
 };
 static_assert(sizeof(Seg) == 64, "ring entry");
 
@@ -88,7 +91,7 @@ __device__ __forceinline__ int chunk_pos(const Seg& s, int k) {
   return kChunk * (k < s.cs ? k : s.base + k - s.cs);
 }
 __device__ __forceinline__ int seg_chunk(const Seg& s, int t) {  // first chunk of tile t
-  return (int)((int64_t)s.chunks * t / s.nt);
+  return s.per * t + min(t, s.rem);
 }
 
 // Bits 0 .. x.
@@ -132,26 +135,49 @@ __device__ __forceinline__ Entry load_entry(const Params& p, int e) {
   }
   return x;
 }
-__device__ __forceinline__ int entry_units(const Params& p, const Entry& x) {
-  return (x.tok1 - x.tok0 + p.tpu - 1) / p.tpu;
-}
 __device__ __forceinline__ int cap_of(const Params& p, int own) {
   return (own ? p.own.cols : p.pre.cols) << p.page_shift;
 }
 // Tiles of units 0 .. x - 1 of a sequence whose unit i ends at position (i + 1) T: ceil((i + 1) / D)
-// each (D = 192 / T units a tile), `most` at most.
-__device__ __forceinline__ int64_t tiles_to(int64_t x, int d, int64_t most) {
-  const int64_t y = min(x, most * (int64_t)d), q = y / d, r = y % d;
-  return d * (q * (q + 1) / 2) + r * (q + 1) + (x - y) * most;
+// each (D = 192 / T = 3 x 2^shift units a tile), `most` at most.
+__device__ __forceinline__ int64_t tiles_to(uint32_t x, int shift, uint32_t most) {
+  const uint32_t whole = (x >> shift) / 3u;  // units that fill their last tile
+  if (whole >= most) {
+    const uint32_t y = (3u * most) << shift;
+    return (int64_t)y * (most + 1) / 2 + (int64_t)(x - y) * most;
+  }
+  const uint32_t r = x - ((3u * whole) << shift);
+  return ((int64_t)((3u * whole) << shift) >> 1) * (whole + 1) + (int64_t)r * (whole + 1);
 }
-// Tiles of the first j units of an entry.
-__device__ __forceinline__ int64_t entry_tiles(const Params& p, const Entry& x, int j) {
-  const int cap = cap_of(p, x.own);
-  if (!x.own) return (int64_t)j * max(1, (min(x.len, cap) + kTile - 1) / kTile);
-  const int64_t most = min(p.unit_tiles, (int64_t)max(1, (cap + kTile - 1) / kTile));
-  const int d = kTile / p.tpu;
-  const int64_t a = ((int64_t)max(0, x.len - (x.tok1 - x.tok0)) + p.tpu - 1) / p.tpu;
-  return tiles_to(a + j, d, most) - tiles_to(a, d, most);
+// An entry with what its units' tiles follow from.
+struct Line {
+  int units;
+  uint32_t a, most;  // own: units that would fit before the first token; tiles of a unit, at most
+  int own, shift;
+};
+__device__ __forceinline__ Line line_of(const Params& p, const Entry& x) {
+  Line y;
+  const int tpu_shift = 7 - p.head_shift, cap = cap_of(p, x.own), n = x.tok1 - x.tok0;
+  y.units = (n + p.tpu - 1) >> tpu_shift;
+  y.own = x.own;
+  y.shift = p.head_shift - 1;
+  if (x.own) {
+    y.a = ((uint32_t)max(0, x.len - n) + p.tpu - 1) >> tpu_shift;
+    y.most = (uint32_t)min(p.unit_tiles, max(1, (cap + kTile - 1) / kTile));
+  } else {
+    y.a = 0;
+    y.most = (uint32_t)max(1, (min(x.len, cap) + kTile - 1) / kTile);
+  }
+  return y;
+}
+// Tiles of its first j units.
+__device__ __forceinline__ int64_t line_tiles(const Line& y, int j) {
+  if (!y.own) return (int64_t)j * y.most;
+  return tiles_to(y.a + j, y.shift, y.most) - (y.a ? tiles_to(y.a, y.shift, y.most) : 0);
+}
+// Tiles of unit j.
+__device__ __forceinline__ int unit_tiles(const Line& y, int j) {
+  return y.own ? (int)min(y.most, ((y.a + j) >> y.shift) / 3u + 1u) : (int)y.most;
 }
 
 __device__ __forceinline__ int64_t cut_at(int64_t tiles, int pairs, int64_t c) {
@@ -168,10 +194,53 @@ __device__ __forceinline__ int64_t part_at(int64_t row, int d) {
   return (row >> 4) * (16 * kDCkv) + (d >> 2) * 64 + (row & 15) * 4;
 }
 
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
+        "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+
+// Bounded wait on an mbarrier.  What follows a first look that fails is out of line: the kernel's
+// roles run side by side, and their code has to fit the instruction caches together (174 KB with
+// every wait and loop inline: 1,450 cycles to fill a slot; see the figures above for now).
+__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                     uint32_t* err, uint64_t limit) {
+  const uint64_t t0 = ptx::cycles();
+#pragma unroll 1
+  for (uint32_t it = 1;; ++it) {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    if ((it & 63u) == 0) {
+      if (*abort_flag) return false;
+      if (ptx::cycles() - t0 > limit) {
+        *abort_flag = 1;
+        atomicOr(err, (uint32_t)DSA_DEVERR_TIMEOUT);
+        return false;
+      }
+    }
+  }
+}
+struct Wait {
+  volatile uint32_t* abort_flag;
+  uint32_t* err;
+  uint64_t limit;
+  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) const {
+    return ptx::mbar_try_wait(bar, parity) || wait_on(bar, parity, abort_flag, err, limit);
+  }
+};
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     attend_kernel(const __grid_constant__ CUtensorMap m_ckv, const __grid_constant__ CUtensorMap m_kpe,
@@ -192,7 +261,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) {
-      ptx::mbar_init(bar(B_FULL + s), 2);
+      ptx::mbar_init(bar(B_FULL + s), 4);
       ptx::mbar_init(bar(B_EMPTY + s), 1);
     }
     ptx::mbar_init(bar(B_QF), 2);
@@ -208,8 +277,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < kSegs; ++i) {
       ptx::mbar_init(bar(B_GF + i), 1);
-      // loader, query loader, softmax warps and, in rank 0, the issuer
-      ptx::mbar_init(bar(B_GE + i), 2 + kSmWarps + (rank == 0 ? 1 : 0));
+      // loaders, query loader, softmax warps and, in rank 0, the issuer
+      ptx::mbar_init(bar(B_GE + i), 3 + kSmWarps + (rank == 0 ? 1 : 0));
     }
     ptx::mbar_init(bar(B_RX), 4);
     ptx::mbar_init(bar(B_RX + 1), 4);
@@ -237,23 +306,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   int64_t* scan = reinterpret_cast<int64_t*>(sgen + OFF_SCAN);
   if (p.whole) {
     // a pair for each row's one unit
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 32 * kWalkWarp) {
       const Entry x = load_entry(p, pair);
-      scan[24] = pair;
-      scan[25] = scan[26] = 0;
-      scan[27] = entry_tiles(p, x, entry_units(p, x));
+      scan[26] = pair;
+      scan[27] = scan[28] = 0;
+      scan[29] = line_tiles(line_of(p, x), x.tok1 - x.tok0);
     }
-    __syncthreads();
   } else {
     const int per = (entries + kThreads - 1) / kThreads;
     const int e0 = min(entries, (int)threadIdx.x * per), e1 = min(entries, e0 + per);
     int64_t mine = 0;
     int units = 0;
     for (int e = e0; e < e1; ++e) {
-      const Entry x = load_entry(p, e);
-      const int n = entry_units(p, x);
-      mine += entry_tiles(p, x, n);
-      units += n;
+      const Line y = line_of(p, load_entry(p, e));
+      mine += line_tiles(y, y.units);
+      units += y.units;
     }
     int64_t run = mine;
 #pragma unroll
@@ -263,14 +330,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       units += __shfl_xor_sync(0xffffffffu, units, o);
     }
     if (lane == 31) scan[warp] = run;
-    if (lane == 0) scan[12 + warp] = units;
+    if (lane == 0) scan[13 + warp] = units;
     __syncthreads();
     int64_t tiles = 0, before = run - mine;
     int all = 0;
     for (int w = 0; w < kThreads / 32; ++w) {
       if (w < warp) before += scan[w];
       tiles += scan[w];
-      all += (int)scan[12 + w];
+      all += (int)scan[13 + w];
     }
     // A window's units cost about the same: whole ones, or equal parts of each, while they fit.
     int pairs = (int)(gridDim.x >> 1);
@@ -281,23 +348,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (lo < hi && lo >= before && lo < before + mine) {
       int e = e0;
       for (;; ++e) {
-        const Entry x = load_entry(p, e);
-        const int64_t n = entry_tiles(p, x, entry_units(p, x));
+        const Line y = line_of(p, load_entry(p, e));
+        const int64_t n = line_tiles(y, y.units);
         if (lo < before + n) break;
         before += n;
       }
-      scan[24] = e;
-      scan[25] = before;
+      scan[26] = e;
+      scan[27] = before;
     }
     if (threadIdx.x == 0) {
-      scan[26] = lo;
-      scan[27] = hi;
-      scan[28] = tiles;
-      scan[29] = pairs;
+      scan[28] = lo;
+      scan[29] = hi;
+      scan[30] = tiles;
+      scan[31] = pairs;
     }
     __syncthreads();
   }
-  const Waiter wait{misc + 2, p.err, p.wait_cycles};
+  const Wait wait{misc + 2, p.err, p.wait_cycles};
   // One unit record after another; false at the line's end or when a wait gave up.
   auto next_seg = [&](Seg& s, int n) -> bool {
     const bool ok = wait(bar(B_GF + (n % kSegs)), (uint32_t)((n / kSegs) & 1));
@@ -313,11 +380,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == kWalkWarp) {
     // ------------------------------------------------------------------ units
     if (lane == 0) {
-      int64_t x = scan[26];
-      const int64_t hi = scan[27];
+      const int64_t start = scan[28], hi = scan[29];
+      int64_t x = start;
       if (rank == 0 && pair == 0 && !p.whole) {
-        p.head[0] = scan[28];
-        p.head[1] = scan[29];
+        p.head[0] = scan[30];
+        p.head[1] = scan[31];
       }
       int n = 0;
       bool ok = true;
@@ -328,36 +395,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ptx::mbar_arrive(bar(B_GF + (n % kSegs)));
         ++n;
       };
-      int e = x < hi ? (int)scan[24] : 0;
-      int64_t ebase = x < hi ? scan[25] : 0;
+      int e = x < hi ? (int)scan[26] : 0;
+      int64_t ebase = x < hi ? scan[27] : 0;
       const int heads = p.heads;
-      while (ok && x < hi) {
+      for (; ok && x < hi; ++e) {
         const Entry en = load_entry(p, e);
-        const int units = entry_units(p, en);
-        const int64_t etiles = entry_tiles(p, en, units);
-        if (x >= ebase + etiles) {
-          ebase += etiles;
-          ++e;
-          continue;
-        }
-        // the unit that holds tile x
-        int j = 0, top = units;
-        while (top - j > 1) {
-          const int mid = (j + top) >> 1;
-          if (ebase + entry_tiles(p, en, mid) <= x) j = mid;
-          else top = mid;
+        const Line y = line_of(p, en);
+        int j = 0;
+        int64_t ubase = ebase;
+        if (x > ebase) {  // the line's first entry: the unit that holds tile x
+          int top = y.units;
+          while (top - j > 1) {
+            const int mid = (j + top) >> 1;
+            if (ebase + line_tiles(y, mid) <= x) j = mid;
+            else top = mid;
+          }
+          ubase = ebase + line_tiles(y, j);
         }
         const int cap = cap_of(p, en.own);
-        for (; ok && j < units && x < hi; ++j) {
+        for (; ok && j < y.units && x < hi; ++j) {
           Seg s = {};
-          const int64_t ubase = ebase + entry_tiles(p, en, j);
-          s.nt = (int)(ebase + entry_tiles(p, en, j + 1) - ubase);
+          s.nt = unit_tiles(y, j);
           s.tok0 = en.tok0 + j * p.tpu;
           s.ntok = min(p.tpu, en.tok1 - s.tok0);
           s.own = en.own;
           s.row = en.own ? e - p.groups : e;
           s.t0 = (int)(x - ubase);
           s.t1 = (int)min((int64_t)s.nt, hi - ubase);
+          int chunks;
           if (en.own) {
             s.p_lo = en.len - (en.tok1 - en.tok0) + j * p.tpu;
             const int p_hi = s.p_lo + s.ntok - 1, last = min(p_hi, cap - 1);
@@ -365,20 +430,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int all = last < 0 ? 0 : last / kChunk + 1;
             const int base = lo / kChunk, sink = (p.sinks + kChunk - 1) / kChunk;
             const int near = last >= lo ? last / kChunk - base + 1 : 0;
-            s.chunks = min(all, sink + near);
+            chunks = min(all, sink + near);
             s.cs = all <= sink + near ? all : sink;
             s.base = base;
             if (p_hi >= cap) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
           } else {
             s.p_lo = min(en.len, cap) - 1;
-            s.chunks = s.cs = (min(en.len, cap) + kChunk - 1) / kChunk;
+            chunks = s.cs = (min(en.len, cap) + kChunk - 1) / kChunk;
             if (en.len > cap) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
           }
+          s.per = chunks / s.nt;
+          s.rem = chunks - s.per * s.nt;
           const bool whole = s.t0 == 0 && s.t1 == s.nt;
           if (p.groups == 0) {
             // two partial results of a pair at most: its line's first unit and its last
             s.slot = whole ? -1 : 128 * (2 * pair + (s.t0 == 0 ? 1 : 0));
-            if (rank == 0 && x == scan[26] && !p.whole) {
+            if (rank == 0 && x == start && !p.whole) {
               int64_t* m = p.cuts + 4 * pair;
               m[0] = ubase;
               m[1] = ubase + s.nt;
@@ -397,7 +464,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
           put(s);
           x = ubase + s.t1;
+          ubase += s.nt;
         }
+        ebase = ubase;
       }
       if (ok) put(Seg{});
     }
@@ -421,10 +490,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       __syncwarp();
     }
     __syncwarp();
-  } else if (warp == kLoadWarp) {
+  } else if (warp == kLoadWarp || warp == kLoadWarp2) {
     // ------------------------------------------------------------------ keys and values
     // A tile's keys are looked up once; K and V slots then follow in the order in which the
-    // issuer reads them: K of tile i + 1 before V of tile i.
+    // issuer reads them: K of tile i + 1 before V of tile i.  Both warps look the keys up.
+    const int blk = warp == kLoadWarp ? 0 : 1;
+    const bool el = ptx::elect_one();  // warp-uniform loops around one issuing thread
     const int hbs = min(5, p.page_shift);      // log2 of a box's rows
     const bool by_row = p.page_shift < 3;      // pages too small for boxes: four rows at a time
     const int nbs = by_row ? 0 : 5 - hbs;      // log2 of the boxes in a chunk
@@ -432,20 +503,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int64_t num_pages = p.num_slots >> p.page_shift;
     volatile uint32_t* masks = reinterpret_cast<volatile uint32_t*>(sgen + OFF_MASK);
     volatile int* poss = reinterpret_cast<volatile int*>(sgen + OFF_POS);
+    // Of a tile's keys, for this warp, [2 tiles]: the slots of its boxes, and of its rows where a
+    // chunk goes row by row.
+    int* boxes = reinterpret_cast<int*>(sgen + OFF_ROWS) + blk * (2 * 224);
     struct Keys {
-      int nc;                        // chunks
-      int box;                       // lane: the slot of box `lane` (chunk lane >> nbs)
-      uint32_t w[kTileChunks];       // visible positions of each chunk
-      int rows[kTileChunks];         // by_row: lane: the slot of row `lane` of each chunk
+      int nc;          // chunks
+      uint32_t whole;  // chunks seen whole (bits)
+      int at;          // in boxes
+      int row[6];      // pages of 32 and more: the chunks' slots
     };
-    int cnt = 0, tile = 0;
+    int slot = 0, tile = 0;
+    uint32_t turn = 1;  // parity of the slot's last reading
     bool ok = true;
+    const uint32_t full0 = ptx::mapa(bar(B_FULL), 0);
+    const uint32_t dst0 = sbase + OFF_KV + blk * kBlkB;
 
     auto look_up = [&](const Seg& s, int t, Keys& k) {
       const Table& tab = s.own ? p.own : p.pre;
       const int32_t* pages = tab.pt + (int64_t)s.row * tab.sb;
       const int c0 = seg_chunk(s, t);
       k.nc = seg_chunk(s, t + 1) - c0;
+      k.at = (tile & 1) * 224;
+      k.whole = 0;
       const int p_hi = s.own ? s.p_lo + s.ntok - 1 : s.p_lo;
       auto slot_of = [&](int pos) -> int {
         const int pg = pos >> p.page_shift;
@@ -454,127 +533,156 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                          : none;
       };
       bool bad = false;
-      k.box = none;
+      int box = none;
       uint32_t absent = 0;  // boxes without a page
       if (!by_row) {
         const int c = lane >> nbs;
-        if (c < k.nc) k.box = slot_of(chunk_pos(s, c0 + c) + ((lane & ((1 << nbs) - 1)) << hbs));
-        absent = __ballot_sync(0xffffffffu, c < k.nc && k.box == none);
+        if (c < k.nc) box = slot_of(chunk_pos(s, c0 + c) + ((lane & ((1 << nbs) - 1)) << hbs));
+        absent = __ballot_sync(0xffffffffu, c < k.nc && box == none);
+        boxes[k.at + lane] = box;
       }
-#pragma unroll
-      for (int c = 0; c < kTileChunks; ++c) {
-        k.w[c] = 0;
-        if (c >= k.nc) continue;
+      uint32_t mask = 0;
+#pragma unroll 1
+      for (int c = 0; c < k.nc; ++c) {
         const int pos = chunk_pos(s, c0 + c);
         uint32_t w = s.own ? visible(p, pos, s.p_lo, p_hi) : bits_to(p_hi - pos);
+        int row = none;
         if (by_row) {
-          k.rows[c] = (w >> lane) & 1u ? slot_of(pos + lane) : none;
-          const uint32_t have = __ballot_sync(0xffffffffu, k.rows[c] != none);
-          bad |= (have != w);
+          if ((w >> lane) & 1u) row = slot_of(pos + lane);
+          const uint32_t have = __ballot_sync(0xffffffffu, row != none);
+          bad |= have != w;
           w = have;
-        } else if (absent) {
-          uint32_t gone = 0;
-          for (int b = 0; b < (1 << nbs); ++b)
-            if ((absent >> ((c << nbs) + b)) & 1u)
-              gone |= (hbs == 5 ? 0xFFFFFFFFu : ((1u << (1 << hbs)) - 1u)) << (b << hbs);
-          bad |= (w & gone) != 0u;
-          w &= ~gone;
+        } else {
+          if ((absent >> (c << nbs)) & ((1u << (1 << nbs)) - 1u)) {
+            const uint32_t here = __ballot_sync(
+                0xffffffffu, !((absent >> ((c << nbs) + (lane >> hbs))) & 1u));
+            bad |= (w & ~here) != 0u;
+            w &= here;
+          }
+          if (w == 0xFFFFFFFFu) k.whole |= 1u << c;
+          else {
+            const int b = __shfl_sync(0xffffffffu, box, (c << nbs) + (lane >> hbs));
+            if ((w >> lane) & 1u) row = b + (lane & ((1 << hbs) - 1));
+          }
         }
-        k.w[c] = w;
-        if (lane == c) {
-          masks[(tile & 3) * 8 + c] = w;
-          poss[(tile & 3) * 8 + c] = pos;
-        }
+        if (!((k.whole >> c) & 1u)) boxes[k.at + 32 + kChunk * c + lane] = row;
+        if (lane == c) mask = w;
+        if (blk == 0 && lane == c) poss[(tile & 3) * 8 + c] = pos;
       }
-      if (bad && lane == 0) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
-      if (lane >= k.nc && lane < kTileChunks) masks[(tile & 3) * 8 + lane] = 0;
+#pragma unroll
+      for (int c = 0; c < kTileChunks; ++c) k.row[c] = __shfl_sync(0xffffffffu, box, c);
+      if (blk == 0) {
+        if (lane < kTileChunks) masks[(tile & 3) * 8 + lane] = mask;
+        if (bad && lane == 0) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
+      }
+      __syncwarp();
     };
 
-    // Fills the next slot: chunks c3 .. c3 + 2 (3 x `hi`), columns col .. of 64 x blocks.
-    auto fill = [&](const Keys& k, bool hi, const CUtensorMap* map, const CUtensorMap* map1,
-                    int col, int blocks_shift, bool values) {
-      const int slot = cnt % kSlots;
-      if (cnt >= kSlots) ok = ok && wait(bar(B_EMPTY + slot), (uint32_t)((cnt / kSlots - 1) & 1));
-      ok = __all_sync(0xffffffffu, ok);
-      ++cnt;
-      if (!ok) return;
-      const uint32_t full = ptx::mapa(bar(B_FULL + slot), 0);
-      const int c3 = hi ? 3 : 0;
-      const int n = min(3, max(0, k.nc - c3));
-      if (lane == 0) {
-        if (n) ptx::mbar_arrive_expect_tx_cluster(full, (uint32_t)(n * kChunk * 128) << blocks_shift);
+    // The next slot, free again; n chunks will land in this warp's block of it.
+    auto claim = [&](int n) -> uint32_t {
+      const uint32_t full = full0 + 8u * (uint32_t)slot;
+      ok = __all_sync(0xffffffffu, wait(bar(B_EMPTY) + 8u * (uint32_t)slot, turn));
+      if (el && ok) {
+        if (n > 0) ptx::mbar_arrive_expect_tx_cluster(full, (uint32_t)(n * kChunk * 128));
         else ptx::mbar_arrive_cluster(full);
       }
-      __syncwarp();
-      const uint32_t dst = sbase + OFF_KV + slot * kSlotB;
-      const int blk = lane & ((1 << blocks_shift) - 1);
-      const int bx = lane >> blocks_shift;
-      if (!by_row) {
-        const int row = __shfl_sync(0xffffffffu, k.box, ((c3 << nbs) + bx) & 31);
-        const int c = bx >> nbs;
-        bool mine = bx < (n << nbs);
-        // values of a chunk that is not seen whole: row by row below, zeros for the rest
-        if (values && mine) {
-          const uint32_t w = c == 0 ? (hi ? k.w[3] : k.w[0])
-                             : c == 1 ? (hi ? k.w[4] : k.w[1]) : (hi ? k.w[5] : k.w[2]);
-          mine = w == 0xFFFFFFFFu;
-        }
-        if (mine)
-          ptx::pair_load_2d(dst + blk * kBlkB + (bx << hbs) * 128, map, col + 64 * blk, row, full);
-      }
-      if (by_row || values) {
-#pragma unroll
-        for (int c = 0; c < 3; ++c) {
-          const uint32_t w = hi ? k.w[3 + c] : k.w[c];
-          if (c >= n || (!by_row && w == 0xFFFFFFFFu)) continue;
-          int row;
-          if (by_row) row = hi ? k.rows[3 + c] : k.rows[c];
-          else {
-            const int b = __shfl_sync(0xffffffffu, k.box, ((c3 + c) << nbs) + (lane >> hbs));
-            row = (w >> lane) & 1u ? b + (lane & ((1 << hbs) - 1)) : none;
-          }
-          const int g = bx & 7;
-          int4 r;
-          r.x = __shfl_sync(0xffffffffu, row, 4 * g);
-          r.y = __shfl_sync(0xffffffffu, row, 4 * g + 1);
-          r.z = __shfl_sync(0xffffffffu, row, 4 * g + 2);
-          r.w = __shfl_sync(0xffffffffu, row, 4 * g + 3);
-          if (bx < 8)
-            ptx::pair_gather4(dst + blk * kBlkB + (c * kChunk + 4 * g) * 128, map1, col + 64 * blk, r,
-                              full);
-        }
-      }
-      __syncwarp();
+      return full;
     };
-    auto load_k = [&](const Keys& k) {
-      if (k.nc == 0) return;
+    auto next_slot = [&]() {
+      if (++slot == kSlots) {
+        slot = 0;
+        turn ^= 1u;
+      }
+    };
+    // Three chunks of which n are there, a box each.
+    auto fill = [&](int n, int r0, int r1, int r2, const CUtensorMap* map, int col) {
+      const uint32_t full = claim(n);
+      if (el && ok) {
+        const uint32_t dst = dst0 + (uint32_t)(slot * kSlotB);
+        if (n > 0) ptx::pair_load_2d(dst, map, col, r0, full);
+        if (n > 1) ptx::pair_load_2d(dst + kChunk * 128, map, col, r1, full);
+        if (n > 2) ptx::pair_load_2d(dst + 2 * kChunk * 128, map, col, r2, full);
+      }
+      next_slot();
+    };
+    // The same for chunks c3 .. of smaller pages, or with values that are not seen whole: those
+    // row by row, zeros where there is nothing to see.
+    auto fill_parts = [&](const Keys& k, int c3, int n, bool rope, int col, bool values) {
+      const uint32_t full = claim(n);
+      if (ok) {
+        uint32_t dst = dst0 + (uint32_t)(slot * kSlotB);
 #pragma unroll 1
-      for (int b = 0; b < 4; ++b) fill(k, rank == 1, &m_ckv, &m_ckv1, 128 * b, 1, false);
-      fill(k, rank == 1, &m_kpe, &m_kpe1, 0, 0, false);
+        for (int c = c3; c < c3 + n; ++c, dst += kChunk * 128) {
+          if (!by_row && (!values || ((k.whole >> c) & 1u))) {
+            const CUtensorMap* map = rope ? &m_kpe : &m_ckv;
+            const int* b = boxes + k.at + (c << nbs);
+#pragma unroll 1
+            for (int j = 0; j < (1 << nbs); ++j) {
+              const int row = b[j];
+              if (el) ptx::pair_load_2d(dst + ((j << hbs) * 128), map, col, row, full);
+            }
+          } else {
+            const CUtensorMap* map = rope ? &m_kpe1 : &m_ckv1;
+            const int4* rows = reinterpret_cast<const int4*>(boxes + k.at + 32 + kChunk * c);
+#pragma unroll 1
+            for (int g = 0; g < 8; ++g) {
+              const int4 r = rows[g];
+              if (el) ptx::pair_gather4(dst + 512 * g, map, col, r, full);
+            }
+          }
+        }
+      }
+      next_slot();
+    };
+    // A tile's slots: five of K (this CTA's keys; four of 128 latent columns, the rope keys), then
+    // up to four of V of the tile before (both halves of its keys, this CTA's columns).
+    auto load_k = [&](const Keys& k) {
+      const int c3 = 3 * (int)rank, n = min(3, max(0, k.nc - c3));
+      if (k.nc == 0) return;
+      if (nbs == 0 && !by_row) {
+        const int r0 = rank ? k.row[3] : k.row[0], r1 = rank ? k.row[4] : k.row[1],
+                  r2 = rank ? k.row[5] : k.row[2];
+#pragma unroll 1
+        for (int b = 0; ok && b < 4; ++b) fill(n, r0, r1, r2, &m_ckv, 128 * b + 64 * blk);
+        if (ok) fill(blk == 0 ? n : 0, r0, r1, r2, &m_kpe, 0);
+      } else {
+#pragma unroll 1
+        for (int b = 0; ok && b < 5; ++b)
+          fill_parts(k, c3, b == 4 && blk ? 0 : n, b == 4, b < 4 ? 128 * b + 64 * blk : 0, false);
+      }
     };
     auto load_v = [&](const Keys& k) {
+      const int col = 256 * (int)rank + 64 * blk;
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
-        if (k.nc <= 3 * h) break;
+        const int n = min(3, k.nc - 3 * h);
+        if (n <= 0) break;
+        const uint32_t all = (1u << n) - 1u;
+        if (nbs == 0 && ((k.whole >> (3 * h)) & all) == all) {
+          const int r0 = h ? k.row[3] : k.row[0], r1 = h ? k.row[4] : k.row[1],
+                    r2 = h ? k.row[5] : k.row[2];
+          if (ok) fill(n, r0, r1, r2, &m_ckv, col);
+          if (ok) fill(n, r0, r1, r2, &m_ckv, col + 128);
+        } else {
 #pragma unroll 1
-        for (int d = 0; d < 2; ++d)
-          fill(k, h == 1, &m_ckv, &m_ckv1, 256 * (int)rank + 128 * d, 1, true);
+          for (int d = 0; ok && d < 2; ++d) fill_parts(k, 3 * h, n, false, col + 128 * d, true);
+        }
       }
     };
 
     Seg s;
     for (int n = 0; ok && next_seg(s, n); ++n) {
       seg_read(n);
-      Keys prev, now;
+      Keys prev = {}, now = {};
       for (int t = s.t0; ok && t < s.t1; ++t, ++tile) {
-        if (tile >= 4)
+        if (tile >= 4 && blk == 0)
           ok = __all_sync(0xffffffffu, wait(bar(B_ME + (tile & 3)), (uint32_t)(((tile >> 2) - 1) & 1)));
         if (!ok) break;
         look_up(s, t, now);
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar(B_MF + (tile & 3)));
+        if (lane == 0 && blk == 0) ptx::mbar_arrive(bar(B_MF + (tile & 3)));
         load_k(now);
-        if (t > s.t0) load_v(prev);
+        if (ok && t > s.t0) load_v(prev);
         prev = now;
       }
       if (ok) load_v(prev);
@@ -583,91 +691,100 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ tensor cores
     if (rank == 0) {
-      const Waiter pwait{misc + 2, p.err, p.wait_cycles, true};
       constexpr uint32_t kIdS = idesc_bf16(128, kTile, false), kIdO = idesc_bf16(128, 256, false, true);
       const uint64_t dq = desc(sbase + OFF_Q, 16, 1024, kSw128);
       const uint64_t dp = desc(sbase + OFF_P, 16, 1024, kSw128);
       const uint64_t dk = desc(sbase + OFF_KV, 16, 1024, kSw128);
       const uint64_t dv = desc(sbase + OFF_KV, kBlkB, 1024, kSw128);
-      int cnt = 0, i = 0;  // slots and tiles so far
+      const bool el = ptx::elect_one();  // warp-uniform loops around one issuing thread
+      int slot = 0, i = 0;               // the ring's, tiles so far
+      uint32_t turn = 0;
       bool ok = true;
+      auto landed = [&]() {
+        ok = __all_sync(0xffffffffu, wait(bar(B_FULL) + 8u * (uint32_t)slot, turn));
+        ptx::tc_fence_after();
+      };
+      auto next_slot = [&]() {
+        if (el) ptx::pair_commit(bar(B_EMPTY) + 8u * (uint32_t)slot);
+        if (++slot == kSlots) {
+          slot = 0;
+          turn ^= 1u;
+        }
+      };
+      auto scores = [&](int nc) {
+        const uint32_t d = tmem + S_COL + 96 * (i & 1);
+        if (nc > 0) {
+#pragma unroll 1
+          for (int b = 0; b < 5; ++b) {
+            landed();
+            if (!ok) return;
+            const uint64_t ko = dk + (uint64_t)((slot * kSlotB) >> 4);
+            if (el) {
+              const uint64_t qo = dq + (uint64_t)((2 * b * kQBlk) >> 4);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                if (k == 4 && b == 4) break;
+                ptx::pair_umma_bf16(d, qo + (uint64_t)(((k >> 2) * kQBlk + (k & 3) * 32) >> 4),
+                                    ko + (uint64_t)(((k >> 2) * kBlkB + (k & 3) * 32) >> 4), kIdS,
+                                    (b | k) ? 1u : 0u);
+              }
+            }
+            next_slot();
+          }
+        }
+        if (el) ptx::pair_commit(bar(B_SF + (i & 1)));
+      };
+      bool o_init = false;
+      auto values = [&](int tile, int nc) {
+        ok = __all_sync(0xffffffffu, wait(bar(B_PF), (uint32_t)(tile & 1)));
+        if (!ok) return;
+#pragma unroll 1
+        for (int hd = 0; hd < (nc > 3 ? 4 : nc > 0 ? 2 : 0); ++hd) {
+            const int h = hd >> 1, dd = hd & 1, steps = 2 * min(3, nc - 3 * h);
+            landed();
+            if (!ok) return;
+            const uint64_t vo = dv + (uint64_t)((slot * kSlotB) >> 4);
+            if (el) {
+#pragma unroll
+              for (int k = 0; k < 6; ++k) {
+                if (k >= steps) break;
+                // P's 16 keys 6 h + k: block (6 h + k) / 4 of 64 keys
+                const uint32_t po = h ? (uint32_t)(((6 + k) >> 2) * kQBlk + ((6 + k) & 3) * 32)
+                                      : (uint32_t)((k >> 2) * kQBlk + (k & 3) * 32);
+                ptx::pair_umma_bf16(tmem + O_COL + 128 * dd, dp + (uint64_t)(po >> 4),
+                                    vo + (uint64_t)((k * 2048) >> 4), kIdO,
+                                    (o_init || (h | k)) ? 1u : 0u);
+              }
+            }
+            next_slot();
+        }
+        o_init = o_init || nc > 0;
+        if (el) ptx::pair_commit(bar(B_PD));
+      };
       Seg s;
       for (int n = 0; ok && next_seg(s, n); ++n) {
         seg_read(n);
-        if (lane == 0) {
-          bool o_init = false;
-          auto scores = [&](int nc) {
-            const uint32_t d = tmem + S_COL + 96 * (i & 1);
-            if (nc > 0) {
-#pragma unroll 1
-              for (int b = 0; b < 5 && ok; ++b, ++cnt) {
-                const int slot = cnt % kSlots;
-                ok = pwait(bar(B_FULL + slot), (uint32_t)((cnt / kSlots) & 1));
-                if (!ok) return;
-                ptx::tc_fence_after();
-                const uint64_t ko = (uint64_t)((slot * kSlotB) >> 4);
-                const uint64_t qo = (uint64_t)((2 * b * kQBlk) >> 4);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  ptx::pair_umma_bf16(d, dq + qo + (uint64_t)((k * 32) >> 4),
-                                      dk + ko + (uint64_t)((k * 32) >> 4), kIdS, (b | k) ? 1u : 0u);
-                if (b < 4) {
-#pragma unroll
-                  for (int k = 0; k < 4; ++k)
-                    ptx::pair_umma_bf16(d, dq + qo + (uint64_t)((kQBlk + k * 32) >> 4),
-                                        dk + ko + (uint64_t)((kBlkB + k * 32) >> 4), kIdS, 1u);
-                }
-                ptx::pair_commit(bar(B_EMPTY + slot));
-              }
-            }
-            ptx::pair_commit(bar(B_SF + (i & 1)));
-          };
-          auto values = [&](int tile, int nc, bool first) {
-            ok = ok && pwait(bar(B_PF), (uint32_t)(tile & 1));
-            if (ok && first && n > 0) ok = pwait(bar(B_OE), (uint32_t)((n - 1) & 1));
-            if (!ok) return;
-            ptx::tc_fence_after();
-#pragma unroll 1
-            for (int h = 0; h < 2 && nc > 3 * h; ++h) {
-              const int steps = 2 * min(3, nc - 3 * h);
-#pragma unroll 1
-              for (int dd = 0; dd < 2; ++dd, ++cnt) {
-                const int slot = cnt % kSlots;
-                ok = pwait(bar(B_FULL + slot), (uint32_t)((cnt / kSlots) & 1));
-                if (!ok) return;
-                ptx::tc_fence_after();
-                const uint64_t vo = (uint64_t)((slot * kSlotB) >> 4);
-#pragma unroll
-                for (int k = 0; k < 6; ++k) {
-                  if (k < steps) {
-                    const int kk = 6 * h + k;
-                    ptx::pair_umma_bf16(tmem + O_COL + 128 * dd,
-                                        dp + (uint64_t)(((kk >> 2) * kQBlk + (kk & 3) * 32) >> 4),
-                                        dv + vo + (uint64_t)((k * 2048) >> 4), kIdO,
-                                        (o_init || kk > 0) ? 1u : 0u);
-                  }
-                }
-                ptx::pair_commit(bar(B_EMPTY + slot));
-              }
-            }
-            if (nc > 0) o_init = true;
-            ptx::pair_commit(bar(B_PD));
-          };
-          ok = pwait(bar(B_QF), (uint32_t)(n & 1));
-          int before = 0;
-          for (int t = s.t0; ok && t < s.t1; ++t, ++i) {
-            const int nc = seg_chunk(s, t + 1) - seg_chunk(s, t);
+        ok = __all_sync(0xffffffffu, wait(bar(B_QF), (uint32_t)(n & 1)));
+        o_init = false;
+        int before = 0;
+        for (int t = s.t0; ok && t <= s.t1; ++t) {
+          const int nc = seg_chunk(s, t + 1) - seg_chunk(s, t);
+          if (t < s.t1) {
             scores(nc);
             if (!ok) break;
-            if (t == s.t1 - 1) ptx::pair_commit(bar(B_QE));
-            if (t > s.t0) values(i - 1, before, t - 1 == s.t0);
-            before = nc;
+            if (t == s.t1 - 1 && el) ptx::pair_commit(bar(B_QE));
+            ++i;
           }
-          if (ok) values(i - 1, before, s.t1 - s.t0 == 1);
+          if (t == s.t0) {
+            before = nc;
+            continue;
+          }
+          // the last unit's output has been read
+          if (t == s.t0 + 1 && n > 0)
+            ok = __all_sync(0xffffffffu, wait(bar(B_OE), (uint32_t)((n - 1) & 1)));
+          if (ok) values(t < s.t1 ? i - 2 : i - 1, before);
+          before = nc;
         }
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-        i = __shfl_sync(0xffffffffu, i, 0);
-        cnt = __shfl_sync(0xffffffffu, cnt, 0);
       }
     }
     __syncwarp();
@@ -682,6 +799,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     float* maxes = reinterpret_cast<float*>(sgen + OFF_MAX);
     float* sums = reinterpret_cast<float*>(sgen + OFF_SUM);
     const int part = 2 * half + ch;
+    const float size = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
     int i = 0, shared = 0;
     bool ok = true;
     // The four warps that share these rows have written what they exchange.
@@ -725,40 +843,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           ptx::tmem_ld32(sc + 64 * ch, a);
           ptx::tmem_ld16(sc + 32 + 16 * ch, b);
           ptx::tmem_wait_ld();
-          float mt = -INFINITY;
-          if (__all_sync(0xffffffffu, wa == 0xFFFFFFFFu && wb == 0xFFFFu)) {
+          // Values of the row's largest score are taken before the scale; a scale below zero turns
+          // the scores round first, zero makes them all alike.
+          if (p.scale_log2 <= 0.f) {
+            const float turn = p.scale_log2 < 0.f ? -1.f : 0.f;
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float x = __uint_as_float(a[k]) * p.scale_log2;
-              a[k] = __float_as_uint(x);
-              mt = fmaxf(mt, x);
-            }
+            for (int k = 0; k < 32; ++k) a[k] = __float_as_uint(__uint_as_float(a[k]) * turn);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const float x = __uint_as_float(b[k]) * p.scale_log2;
-              b[k] = __float_as_uint(x);
-              mt = fmaxf(mt, x);
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float x = (wa >> k) & 1u ? __uint_as_float(a[k]) * p.scale_log2 : -INFINITY;
-              a[k] = __float_as_uint(x);
-              mt = fmaxf(mt, x);
-            }
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const float x = (wb >> k) & 1u ? __uint_as_float(b[k]) * p.scale_log2 : -INFINITY;
-              b[k] = __float_as_uint(x);
-              mt = fmaxf(mt, x);
-            }
+            for (int k = 0; k < 16; ++k) b[k] = __float_as_uint(__uint_as_float(b[k]) * turn);
           }
+          if (!__all_sync(0xffffffffu, wa == 0xFFFFFFFFu && wb == 0xFFFFu)) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (!((wa >> k) & 1u)) a[k] = 0xFF800000u;  // -inf
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              if (!((wb >> k) & 1u)) b[k] = 0xFF800000u;
+          }
+          float mp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int k = 0; k < 32; k += 8)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              mp[j] = fmaxf(mp[j], fmaxf(__uint_as_float(a[k + j]), __uint_as_float(a[k + j + 4])));
+#pragma unroll
+          for (int k = 0; k < 16; k += 8)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              mp[j] = fmaxf(mp[j], fmaxf(__uint_as_float(b[k + j]), __uint_as_float(b[k + j + 4])));
+          float mt = fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3]));
           // the row's maximum over the four threads that share it
           float* mx = maxes + (i & 1) * 256;
           mx[part * 64 + row] = mt;
           ok = exchange();
           if (!ok) break;
-          mt = fmaxf(fmaxf(mx[row], mx[64 + row]), fmaxf(mx[128 + row], mx[192 + row]));
+          mt = fmaxf(fmaxf(mx[row], mx[64 + row]), fmaxf(mx[128 + row], mx[192 + row])) * size;
           float alpha = 1.f;
           const bool need = mt > m + kTau;
           if (need) {
@@ -767,26 +886,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             m = mt;
           }
           const float me = m == -INFINITY ? 0.f : m;
-          float l0 = 0.f, l1 = 0.f;
+          const float2 size2 = make_float2(size, size), me2 = make_float2(-me, -me);
+          float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          auto numerator = [&](uint32_t u, uint32_t v, int j) -> uint32_t {
+            const float2 x = fma2(make_float2(__uint_as_float(u), __uint_as_float(v)), size2, me2);
+            const float2 e = make_float2(ptx::ex2(x.x), ptx::ex2(x.y));
+            l2[j & 1] = add2(l2[j & 1], e);
+            // P is rounded to bf16, as the values are (2^-8 of each at most, independent of one
+            // another); a second term would double the tensor cores' work on it
+            return pack2(e.x, e.y);
+          };
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const float x = ptx::ex2(__uint_as_float(a[2 * k]) - me);
-            const float y = ptx::ex2(__uint_as_float(a[2 * k + 1]) - me);
-            l0 += x;
-            l1 += y;
-            // P is rounded to bf16 (2^-9 of a value on average less, the values' own type): a
-            // second term would double the tensor cores' work on it
-            a[k] = pack2(x, y);
-          }
+          for (int k = 0; k < 16; ++k) a[k] = numerator(a[2 * k], a[2 * k + 1], k);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float x = ptx::ex2(__uint_as_float(b[2 * k]) - me);
-            const float y = ptx::ex2(__uint_as_float(b[2 * k + 1]) - me);
-            l0 += x;
-            l1 += y;
-            b[k] = pack2(x, y);
-          }
-          l += l0 + l1;
+          for (int k = 0; k < 8; ++k) b[k] = numerator(b[2 * k], b[2 * k + 1], k);
+          l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
           // P V of the tile before has read P and written O
           if (i > 0) ok = __all_sync(0xffffffffu, wait(bar(B_PD), (uint32_t)((i - 1) & 1)));
           if (!ok) break;
