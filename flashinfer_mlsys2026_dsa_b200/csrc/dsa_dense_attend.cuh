@@ -17,10 +17,10 @@
 // The units of all rows form one line of tiles, cut into equal parts, one for each pair.  A unit
 // that is cut leaves partial results (O, maximum, sum) that combine kernels join.
 //
-// Warps of a CTA:  0 and 12 load keys and values (64 columns each of a slot's 128), 1 issues the
-// tensor-core work (rank 0 alone), 2 loads queries, 3 walks the units, 4-11 softmax and output: a
-// thread is a row and a quarter of a tile's keys (its lane quadrant holds half of them, two warps
-// share a quadrant).
+// Warps of a CTA:  0 and 12 load keys, 13 and 14 values (64 columns each of a slot's 128), 1 issues
+// the tensor-core work (rank 0 alone), 2 loads queries, 3 walks the units, 4-11 softmax and output:
+// a thread is a row and a quarter of a tile's keys (its lane quadrant holds half of them, two
+// warps share a quadrant).
 #pragma once
 
 namespace dsa {
@@ -33,9 +33,9 @@ constexpr int kSlots = 5;                  // ring of 24 KB: [96 keys x 128 colu
 constexpr int kBlkB = 96 * 128;            // [96 keys x 64 columns], 128-byte swizzle
 constexpr int kSlotB = 2 * kBlkB;
 constexpr int kQBlk = 64 * 128;            // [64 rows x 64 columns]
-constexpr int kThreads = 416;
+constexpr int kThreads = 480;
 constexpr int kLoadWarp = 0, kMmaWarp = 1, kQWarp = 2, kWalkWarp = 3, kSm0 = 4, kSmWarps = 8,
-              kLoadWarp2 = 12;
+              kLoadWarp2 = 12;  // and the two behind it
 constexpr int kSegs = 4;                   // units that the walker is ahead
 constexpr float kTau = 8.f;                // a maximum that grows by less leaves O as it is
 
@@ -48,9 +48,9 @@ constexpr int OFF_MASK = OFF_SEG + kSegs * 64;   // [4 tiles][8] visible positio
 constexpr int OFF_POS = OFF_MASK + 4 * 8 * 4;    // [4 tiles][8] a chunk's first position
 constexpr int OFF_MAX = OFF_POS + 4 * 8 * 4;     // [2][4][64] row maxima of the quarters
 constexpr int OFF_SUM = OFF_MAX + 2 * 4 * 64 * 4;  // [4][64] row sums of the quarters
-constexpr int OFF_SCAN = OFF_SUM + 4 * 64 * 4;   // the start's scan: 13 x (tiles, units), result
-constexpr int OFF_ROWS = OFF_SCAN + 320;         // [2 loaders][2 tiles][32 + 192] slots
-constexpr int OFF_MISC = OFF_ROWS + 2 * 2 * 224 * 4;
+constexpr int OFF_SCAN = OFF_SUM + 4 * 64 * 4;   // the start's scan: 15 x (tiles, units), result
+constexpr int OFF_ROWS = OFF_SCAN + 320;         // 6 x [32 + 192] slots, for the loaders
+constexpr int OFF_MISC = OFF_ROWS + 6 * 224 * 4;
 constexpr int SMEM_BYTES = OFF_MISC + 64 + 1024;
 static_assert(OFF_P % 1024 == 0 && OFF_KV % 1024 == 0 && kBlkB % 1024 == 0, "swizzle atoms");
 static_assert(SMEM_BYTES <= 232448, "shared memory budget");
@@ -278,7 +278,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int i = 0; i < kSegs; ++i) {
       ptx::mbar_init(bar(B_GF + i), 1);
       // loaders, query loader, softmax warps and, in rank 0, the issuer
-      ptx::mbar_init(bar(B_GE + i), 3 + kSmWarps + (rank == 0 ? 1 : 0));
+      ptx::mbar_init(bar(B_GE + i), 5 + kSmWarps + (rank == 0 ? 1 : 0));
     }
     ptx::mbar_init(bar(B_RX), 4);
     ptx::mbar_init(bar(B_RX + 1), 4);
@@ -308,9 +308,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // a pair for each row's one unit
     if (threadIdx.x == 32 * kWalkWarp) {
       const Entry x = load_entry(p, pair);
-      scan[26] = pair;
-      scan[27] = scan[28] = 0;
-      scan[29] = line_tiles(line_of(p, x), x.tok1 - x.tok0);
+      scan[30] = pair;
+      scan[31] = scan[32] = 0;
+      scan[33] = line_tiles(line_of(p, x), x.tok1 - x.tok0);
     }
   } else {
     const int per = (entries + kThreads - 1) / kThreads;
@@ -330,14 +330,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       units += __shfl_xor_sync(0xffffffffu, units, o);
     }
     if (lane == 31) scan[warp] = run;
-    if (lane == 0) scan[13 + warp] = units;
+    if (lane == 0) scan[15 + warp] = units;
     __syncthreads();
     int64_t tiles = 0, before = run - mine;
     int all = 0;
     for (int w = 0; w < kThreads / 32; ++w) {
       if (w < warp) before += scan[w];
       tiles += scan[w];
-      all += (int)scan[13 + w];
+      all += (int)scan[15 + w];
     }
     // A window's units cost about the same: whole ones, or equal parts of each, while they fit.
     int pairs = (int)(gridDim.x >> 1);
@@ -353,14 +353,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (lo < before + n) break;
         before += n;
       }
-      scan[26] = e;
-      scan[27] = before;
+      scan[30] = e;
+      scan[31] = before;
     }
     if (threadIdx.x == 0) {
-      scan[28] = lo;
-      scan[29] = hi;
-      scan[30] = tiles;
-      scan[31] = pairs;
+      scan[32] = lo;
+      scan[33] = hi;
+      scan[34] = tiles;
+      scan[35] = pairs;
     }
     __syncthreads();
   }
@@ -380,11 +380,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == kWalkWarp) {
     // ------------------------------------------------------------------ units
     if (lane == 0) {
-      const int64_t start = scan[28], hi = scan[29];
+      const int64_t start = scan[32], hi = scan[33];
       int64_t x = start;
       if (rank == 0 && pair == 0 && !p.whole) {
-        p.head[0] = scan[30];
-        p.head[1] = scan[31];
+        p.head[0] = scan[34];
+        p.head[1] = scan[35];
       }
       int n = 0;
       bool ok = true;
@@ -395,8 +395,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ptx::mbar_arrive(bar(B_GF + (n % kSegs)));
         ++n;
       };
-      int e = x < hi ? (int)scan[26] : 0;
-      int64_t ebase = x < hi ? scan[27] : 0;
+      int e = x < hi ? (int)scan[30] : 0;
+      int64_t ebase = x < hi ? scan[31] : 0;
       const int heads = p.heads;
       for (; ok && x < hi; ++e) {
         const Entry en = load_entry(p, e);
@@ -439,6 +439,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             chunks = s.cs = (min(en.len, cap) + kChunk - 1) / kChunk;
             if (en.len > cap) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
           }
+          // Every tile has a chunk: where there are too few, further ones of which nothing is seen.
+          if (s.cs == chunks) s.base = s.cs;
+          chunks = max(chunks, s.nt);
           s.per = chunks / s.nt;
           s.rem = chunks - s.per * s.nt;
           const bool whole = s.t0 == 0 && s.t1 == s.nt;
@@ -490,11 +493,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       __syncwarp();
     }
     __syncwarp();
-  } else if (warp == kLoadWarp || warp == kLoadWarp2) {
+  } else if (warp == kLoadWarp || warp >= kLoadWarp2) {
     // ------------------------------------------------------------------ keys and values
-    // A tile's keys are looked up once; K and V slots then follow in the order in which the
-    // issuer reads them: K of tile i + 1 before V of tile i.  Both warps look the keys up.
-    const int blk = warp == kLoadWarp ? 0 : 1;
+    // The ring holds, in the order in which the issuer reads them, K of tile i + 1 (this CTA's half
+    // of the keys; slots of 128 latent columns, the rope keys third of five), then V of tile i (four
+    // slots: half of the keys, half of this CTA's columns; two where it has up to 96 keys).  Two
+    // warps load the latent keys, two the rope keys and V: one chain of wait, arrive and copy is too
+    // long for every slot.  A warp passes the others' slots without a look.  Parities still tell a
+    // slot's readings apart: no slot is read without this warp's own part, and the next one that it
+    // fills is at most five further on, so that the reading before last is over (at the end of a
+    // unit, where the keys' warps pass eight slots of V, they wait for the last scores instead).
+    const bool vals = warp > kLoadWarp2;
+    const int blk = vals ? warp - kLoadWarp2 - 1 : warp == kLoadWarp2, me = vals ? 2 + blk : blk;
     const bool el = ptx::elect_one();  // warp-uniform loops around one issuing thread
     const int hbs = min(5, p.page_shift);      // log2 of a box's rows
     const bool by_row = p.page_shift < 3;      // pages too small for boxes: four rows at a time
@@ -503,13 +513,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int64_t num_pages = p.num_slots >> p.page_shift;
     volatile uint32_t* masks = reinterpret_cast<volatile uint32_t*>(sgen + OFF_MASK);
     volatile int* poss = reinterpret_cast<volatile int*>(sgen + OFF_POS);
-    // Of a tile's keys, for this warp, [2 tiles]: the slots of its boxes, and of its rows where a
-    // chunk goes row by row.
-    int* boxes = reinterpret_cast<int*>(sgen + OFF_ROWS) + blk * (2 * 224);
+    // Of a tile's keys, for this warp: the slots of its boxes, and of its rows where a chunk goes
+    // row by row (a value warp holds two tiles).
     struct Keys {
       int nc;          // chunks
       uint32_t whole;  // chunks seen whole (bits)
-      int at;          // in boxes
+      int* boxes;
       int row[6];      // pages of 32 and more: the chunks' slots
     };
     int slot = 0, tile = 0;
@@ -518,62 +527,74 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t full0 = ptx::mapa(bar(B_FULL), 0);
     const uint32_t dst0 = sbase + OFF_KV + blk * kBlkB;
 
-    auto look_up = [&](const Seg& s, int t, Keys& k) {
+    // The page of this lane's box of tile t (-1: no box, or none in the table).
+    auto page_of = [&](const Seg& s, int t) -> int {
       const Table& tab = s.own ? p.own : p.pre;
-      const int32_t* pages = tab.pt + (int64_t)s.row * tab.sb;
+      const int c0 = seg_chunk(s, t), c = lane >> nbs;
+      if (by_row || c >= seg_chunk(s, t + 1) - c0) return -1;
+      const int pg = (chunk_pos(s, c0 + c) + ((lane & ((1 << nbs) - 1)) << hbs)) >> p.page_shift;
+      return pg < tab.cols ? tab.pt[(int64_t)s.row * tab.sb + pg] : -1;
+    };
+    auto look_up = [&](const Seg& s, int t, int page, Keys& k) {
       const int c0 = seg_chunk(s, t);
       k.nc = seg_chunk(s, t + 1) - c0;
-      k.at = (tile & 1) * 224;
-      k.whole = 0;
       const int p_hi = s.own ? s.p_lo + s.ntok - 1 : s.p_lo;
-      auto slot_of = [&](int pos) -> int {
-        const int pg = pos >> p.page_shift;
-        const int id = pg < tab.cols ? pages[pg] : -1;
-        return id >= 0 && id < num_pages ? (id << p.page_shift) + (pos & ((1 << p.page_shift) - 1))
-                                         : none;
-      };
-      bool bad = false;
+      const int in_page = (1 << p.page_shift) - 1;
+      int* boxes = reinterpret_cast<int*>(sgen + OFF_ROWS) +
+                   224 * (vals ? 2 + 2 * blk + (tile & 1) : blk);
+      k.boxes = boxes;
+      __syncwarp();
       int box = none;
-      uint32_t absent = 0;  // boxes without a page
-      if (!by_row) {
-        const int c = lane >> nbs;
-        if (c < k.nc) box = slot_of(chunk_pos(s, c0 + c) + ((lane & ((1 << nbs) - 1)) << hbs));
-        absent = __ballot_sync(0xffffffffu, c < k.nc && box == none);
-        boxes[k.at + lane] = box;
-      }
-      uint32_t mask = 0;
-#pragma unroll 1
-      for (int c = 0; c < k.nc; ++c) {
-        const int pos = chunk_pos(s, c0 + c);
-        uint32_t w = s.own ? visible(p, pos, s.p_lo, p_hi) : bits_to(p_hi - pos);
-        int row = none;
-        if (by_row) {
-          if ((w >> lane) & 1u) row = slot_of(pos + lane);
-          const uint32_t have = __ballot_sync(0xffffffffu, row != none);
-          bad |= have != w;
-          w = have;
-        } else {
-          if ((absent >> (c << nbs)) & ((1u << (1 << nbs)) - 1u)) {
-            const uint32_t here = __ballot_sync(
-                0xffffffffu, !((absent >> ((c << nbs) + (lane >> hbs))) & 1u));
-            bad |= (w & ~here) != 0u;
-            w &= here;
-          }
-          if (w == 0xFFFFFFFFu) k.whole |= 1u << c;
-          else {
-            const int b = __shfl_sync(0xffffffffu, box, (c << nbs) + (lane >> hbs));
-            if ((w >> lane) & 1u) row = b + (lane & ((1 << hbs) - 1));
-          }
-        }
-        if (!((k.whole >> c) & 1u)) boxes[k.at + 32 + kChunk * c + lane] = row;
-        if (lane == c) mask = w;
-        if (blk == 0 && lane == c) poss[(tile & 3) * 8 + c] = pos;
-      }
+      if (page >= 0 && page < num_pages)
+        box = (page << p.page_shift) +
+              ((chunk_pos(s, c0 + (lane >> nbs)) + ((lane & ((1 << nbs) - 1)) << hbs)) & in_page);
+      boxes[lane] = box;
 #pragma unroll
       for (int c = 0; c < kTileChunks; ++c) k.row[c] = __shfl_sync(0xffffffffu, box, c);
-      if (blk == 0) {
-        if (lane < kTileChunks) masks[(tile & 3) * 8 + lane] = mask;
-        if (bad && lane == 0) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
+      // lane c: chunk c's first position and what of it is seen
+      const int pos = chunk_pos(s, c0 + min(lane, kTileChunks - 1));
+      const uint32_t want = lane >= k.nc ? 0u : s.own ? visible(p, pos, s.p_lo, p_hi) : bits_to(p_hi - pos);
+      uint32_t w = want;
+      if (nbs == 0 && !by_row) {
+        if (box == none) w = 0;
+      } else if (!by_row) {
+        const uint32_t have = __ballot_sync(0xffffffffu, box != none);
+        for (int b = 0; b < (1 << nbs); ++b)
+          if (!((have >> ((min(lane, kTileChunks - 1) << nbs) + b)) & 1u)) w &= ~(((1u << (1 << hbs)) - 1u) << (b << hbs));
+        if (lane >= k.nc) w = 0;
+      }
+      k.whole = __ballot_sync(0xffffffffu, w == 0xFFFFFFFFu);
+      if (by_row) k.whole = 0;
+      // the rows of the chunks that are not seen whole
+      if (vals || by_row) {
+        uint32_t todo = ((1u << k.nc) - 1u) & ~k.whole;
+        while (todo) {
+          const int c = __ffs(todo) - 1;
+          todo &= todo - 1;
+          const uint32_t wc = __shfl_sync(0xffffffffu, w, c);
+          const int pc = __shfl_sync(0xffffffffu, pos, c) + lane;
+          int row = none;
+          if (by_row) {
+            const Table& tab = s.own ? p.own : p.pre;
+            const int pg = pc >> p.page_shift;
+            const int id = ((wc >> lane) & 1u) && pg < tab.cols ? tab.pt[(int64_t)s.row * tab.sb + pg] : -1;
+            if (id >= 0 && id < num_pages) row = (id << p.page_shift) + (pc & in_page);
+            const uint32_t have = __ballot_sync(0xffffffffu, row != none);
+            if (lane == c) w = have;
+          } else {
+            const int b = __shfl_sync(0xffffffffu, box, (c << nbs) + (lane >> hbs));
+            if ((wc >> lane) & 1u) row = b + (lane & ((1 << hbs) - 1));
+          }
+          boxes[32 + kChunk * c + lane] = row;
+        }
+      }
+      if (me == 0) {
+        if (lane < kTileChunks) {
+          masks[(tile & 3) * 8 + lane] = w;
+          poss[(tile & 3) * 8 + lane] = pos;
+        }
+        // a position that should be there has no page
+        if (w != want) atomicOr(p.err, (uint32_t)DSA_DEVERR_BAD_INDEX);
       }
       __syncwarp();
     };
@@ -588,9 +609,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       return full;
     };
-    auto next_slot = [&]() {
-      if (++slot == kSlots) {
-        slot = 0;
+    auto skip = [&](int n) {
+      slot += n;
+      if (slot >= kSlots) {
+        slot -= kSlots;
         turn ^= 1u;
       }
     };
@@ -603,7 +625,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (n > 1) ptx::pair_load_2d(dst + kChunk * 128, map, col, r1, full);
         if (n > 2) ptx::pair_load_2d(dst + 2 * kChunk * 128, map, col, r2, full);
       }
-      next_slot();
+      skip(1);
     };
     // The same for chunks c3 .. of smaller pages, or with values that are not seen whole: those
     // row by row, zeros where there is nothing to see.
@@ -615,7 +637,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int c = c3; c < c3 + n; ++c, dst += kChunk * 128) {
           if (!by_row && (!values || ((k.whole >> c) & 1u))) {
             const CUtensorMap* map = rope ? &m_kpe : &m_ckv;
-            const int* b = boxes + k.at + (c << nbs);
+            const int* b = k.boxes + (c << nbs);
 #pragma unroll 1
             for (int j = 0; j < (1 << nbs); ++j) {
               const int row = b[j];
@@ -623,7 +645,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
           } else {
             const CUtensorMap* map = rope ? &m_kpe1 : &m_ckv1;
-            const int4* rows = reinterpret_cast<const int4*>(boxes + k.at + 32 + kChunk * c);
+            const int4* rows = reinterpret_cast<const int4*>(k.boxes + 32 + kChunk * c);
 #pragma unroll 1
             for (int g = 0; g < 8; ++g) {
               const int4 r = rows[g];
@@ -632,40 +654,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
       }
-      next_slot();
+      skip(1);
     };
-    // A tile's slots: five of K (this CTA's keys; four of 128 latent columns, the rope keys), then
-    // up to four of V of the tile before (both halves of its keys, this CTA's columns).
-    auto load_k = [&](const Keys& k) {
-      const int c3 = 3 * (int)rank, n = min(3, max(0, k.nc - c3));
-      if (k.nc == 0) return;
-      if (nbs == 0 && !by_row) {
-        const int r0 = rank ? k.row[3] : k.row[0], r1 = rank ? k.row[4] : k.row[1],
-                  r2 = rank ? k.row[5] : k.row[2];
-#pragma unroll 1
-        for (int b = 0; ok && b < 4; ++b) fill(n, r0, r1, r2, &m_ckv, 128 * b + 64 * blk);
-        if (ok) fill(blk == 0 ? n : 0, r0, r1, r2, &m_kpe, 0);
-      } else {
-#pragma unroll 1
-        for (int b = 0; ok && b < 5; ++b)
-          fill_parts(k, c3, b == 4 && blk ? 0 : n, b == 4, b < 4 ? 128 * b + 64 * blk : 0, false);
-      }
+    const bool by_box = nbs == 0 && !by_row;  // a box is a chunk
+    // 64 columns of this CTA's keys.
+    auto load_keys = [&](const Keys& k, bool rope, int col) {
+      const int c3 = 3 * (int)rank, n = rope && blk ? 0 : min(3, max(0, k.nc - c3));
+      if (by_box)
+        fill(n, rank ? k.row[3] : k.row[0], rank ? k.row[4] : k.row[1], rank ? k.row[5] : k.row[2],
+             rope ? &m_kpe : &m_ckv, col);
+      else
+        fill_parts(k, c3, n, rope, col, false);
     };
-    auto load_v = [&](const Keys& k) {
+    auto load_values = [&](const Keys& k) {
       const int col = 256 * (int)rank + 64 * blk;
 #pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; ok && h < 2; ++h) {
         const int n = min(3, k.nc - 3 * h);
         if (n <= 0) break;
         const uint32_t all = (1u << n) - 1u;
-        if (nbs == 0 && ((k.whole >> (3 * h)) & all) == all) {
-          const int r0 = h ? k.row[3] : k.row[0], r1 = h ? k.row[4] : k.row[1],
-                    r2 = h ? k.row[5] : k.row[2];
-          if (ok) fill(n, r0, r1, r2, &m_ckv, col);
-          if (ok) fill(n, r0, r1, r2, &m_ckv, col + 128);
-        } else {
+        const bool whole = by_box && ((k.whole >> (3 * h)) & all) == all;
 #pragma unroll 1
-          for (int d = 0; ok && d < 2; ++d) fill_parts(k, 3 * h, n, false, col + 128 * d, true);
+        for (int d = 0; ok && d < 2; ++d) {
+          if (whole)
+            fill(n, h ? k.row[3] : k.row[0], h ? k.row[4] : k.row[1], h ? k.row[5] : k.row[2], &m_ckv,
+                 col + 128 * d);
+          else
+            fill_parts(k, 3 * h, n, false, col + 128 * d, true);
         }
       }
     };
@@ -673,19 +688,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     Seg s;
     for (int n = 0; ok && next_seg(s, n); ++n) {
       seg_read(n);
-      Keys prev = {}, now = {};
-      for (int t = s.t0; ok && t < s.t1; ++t, ++tile) {
-        if (tile >= 4 && blk == 0)
-          ok = __all_sync(0xffffffffu, wait(bar(B_ME + (tile & 3)), (uint32_t)(((tile >> 2) - 1) & 1)));
-        if (!ok) break;
-        look_up(s, t, now);
-        __syncwarp();
-        if (lane == 0 && blk == 0) ptx::mbar_arrive(bar(B_MF + (tile & 3)));
-        load_k(now);
-        if (ok && t > s.t0) load_v(prev);
-        prev = now;
+      Keys k, prev;
+      prev.nc = 0;
+      int page = page_of(s, s.t0);
+      for (int t = s.t0; ok && t <= s.t1; ++t) {
+        if (t < s.t1) {
+          if (tile >= 4 && me == 0)
+            ok = __all_sync(0xffffffffu, wait(bar(B_ME + (tile & 3)), (uint32_t)(((tile >> 2) - 1) & 1)));
+          if (!ok) break;
+          const int here = page;
+          page = t + 1 < s.t1 ? page_of(s, t + 1) : -1;  // on its way meanwhile
+          look_up(s, t, here, k);
+          if (me == 0 && lane == 0) ptx::mbar_arrive(bar(B_MF + (tile & 3)));
+          ++tile;
+          if (vals) {
+            skip(2);
+            load_keys(k, true, 0);
+            skip(2);
+          } else {
+#pragma unroll 1
+            for (int b = 0; ok && b < 4; ++b) {
+              if (b == 2) skip(1);
+              load_keys(k, false, 128 * b + 64 * blk);
+            }
+          }
+        } else if (!vals) {
+          ok = __all_sync(0xffffffffu, wait(bar(B_SF + ((tile - 1) & 1)), (uint32_t)(((tile - 1) >> 1) & 1)));
+        }
+        if (t > s.t0) {
+          if (vals) load_values(prev);
+          else skip(prev.nc > 3 ? 4 : 2);
+        }
+        prev = k;
       }
-      if (ok) load_v(prev);
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
@@ -711,26 +746,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           turn ^= 1u;
         }
       };
-      auto scores = [&](int nc) {
+      auto scores = [&]() {
         const uint32_t d = tmem + S_COL + 96 * (i & 1);
-        if (nc > 0) {
 #pragma unroll 1
-          for (int b = 0; b < 5; ++b) {
-            landed();
-            if (!ok) return;
-            const uint64_t ko = dk + (uint64_t)((slot * kSlotB) >> 4);
-            if (el) {
-              const uint64_t qo = dq + (uint64_t)((2 * b * kQBlk) >> 4);
+        for (int b = 0; b < 5; ++b) {
+          landed();
+          if (!ok) return;
+          const uint64_t ko = dk + (uint64_t)((slot * kSlotB) >> 4);
+          const uint64_t qo = dq + (uint64_t)(((b < 2 ? 2 * b : b == 2 ? 8 : 2 * b - 2) * kQBlk) >> 4);
+          if (el) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                if (k == 4 && b == 4) break;
-                ptx::pair_umma_bf16(d, qo + (uint64_t)(((k >> 2) * kQBlk + (k & 3) * 32) >> 4),
-                                    ko + (uint64_t)(((k >> 2) * kBlkB + (k & 3) * 32) >> 4), kIdS,
-                                    (b | k) ? 1u : 0u);
-              }
+            for (int k = 0; k < 8; ++k) {
+              if (k == 4 && b == 2) break;
+              ptx::pair_umma_bf16(d, qo + (uint64_t)(((k >> 2) * kQBlk + (k & 3) * 32) >> 4),
+                                  ko + (uint64_t)(((k >> 2) * kBlkB + (k & 3) * 32) >> 4), kIdS,
+                                  (b | k) ? 1u : 0u);
             }
-            next_slot();
           }
+          next_slot();
         }
         if (el) ptx::pair_commit(bar(B_SF + (i & 1)));
       };
@@ -739,7 +772,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, wait(bar(B_PF), (uint32_t)(tile & 1)));
         if (!ok) return;
 #pragma unroll 1
-        for (int hd = 0; hd < (nc > 3 ? 4 : nc > 0 ? 2 : 0); ++hd) {
+        for (int hd = 0; hd < (nc > 3 ? 4 : 2); ++hd) {
             const int h = hd >> 1, dd = hd & 1, steps = 2 * min(3, nc - 3 * h);
             landed();
             if (!ok) return;
@@ -758,7 +791,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
             next_slot();
         }
-        o_init = o_init || nc > 0;
+        o_init = true;
         if (el) ptx::pair_commit(bar(B_PD));
       };
       Seg s;
@@ -770,7 +803,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int t = s.t0; ok && t <= s.t1; ++t) {
           const int nc = seg_chunk(s, t + 1) - seg_chunk(s, t);
           if (t < s.t1) {
-            scores(nc);
+            scores();
             if (!ok) break;
             if (t == s.t1 - 1 && el) ptx::pair_commit(bar(B_QE));
             ++i;
@@ -835,7 +868,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ok = ok && wait(bar(B_SF + (i & 1)), (uint32_t)((i >> 1) & 1));
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const int nc = seg_chunk(s, t + 1) - seg_chunk(s, t);
         if (live) {
           ptx::tc_fence_after();
           uint32_t a[32], b[16];
@@ -938,7 +970,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive_cluster(pf);
-        o_valid = o_valid || nc > 0;
+        o_valid = true;
       }
       if (!ok) break;
       // the unit's (or its part's) output
