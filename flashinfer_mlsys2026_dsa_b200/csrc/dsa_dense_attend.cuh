@@ -180,12 +180,17 @@ __device__ __forceinline__ int unit_tiles(const Line& y, int j) {
   return y.own ? (int)min(y.most, ((y.a + j) >> y.shift) / 3u + 1u) : (int)y.most;
 }
 
+// a / b, both at least 0 and b above; 64 bits only where they are needed (a tenth of the time).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((uint64_t)a | (uint64_t)b) >> 32) return (int64_t)((uint64_t)a / (uint64_t)b);
+  return (uint32_t)a / (uint32_t)b;
+}
 __device__ __forceinline__ int64_t cut_at(int64_t tiles, int pairs, int64_t c) {
-  return tiles * c / pairs;
+  return quotient(tiles * c, pairs);
 }
 // The pair whose part holds tile x.
 __device__ __forceinline__ int pair_of(int64_t tiles, int pairs, int64_t x) {
-  return (int)(((x + 1) * pairs - 1) / tiles);
+  return (int)quotient((x + 1) * pairs - 1, tiles);
 }
 
 // Where a partial result's values and (maximum, sum) lie: blocks of 16 rows, so that a warp's
@@ -347,7 +352,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int64_t hi = pair < pairs ? cut_at(tiles, pairs, pair + 1) : tiles;
     if (lo < hi && lo >= before && lo < before + mine) {
       int e = e0;
-      for (;; ++e) {
+      for (; e + 1 < e1; ++e) {
         const Line y = line_of(p, load_entry(p, e));
         const int64_t n = line_tiles(y, y.units);
         if (lo < before + n) break;
@@ -631,8 +636,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // row by row, zeros where there is nothing to see.
     auto fill_parts = [&](const Keys& k, int c3, int n, bool rope, int col, bool values) {
       const uint32_t full = claim(n);
-      if (ok) {
-        uint32_t dst = dst0 + (uint32_t)(slot * kSlotB);
+      const uint32_t all = ((1u << n) - 1u) << c3;
+      uint32_t dst = dst0 + (uint32_t)(slot * kSlotB);
+      if (ok && !by_row && nbs > 0 && (!values || (k.whole & all) == all)) {
+        const CUtensorMap* map = rope ? &m_kpe : &m_ckv;
+        const int2* b = reinterpret_cast<const int2*>(k.boxes + (c3 << nbs));
+#pragma unroll 2
+        for (int j = 0; j < (n << nbs) / 2; ++j, dst += 256 << hbs) {
+          const int2 row = b[j];
+          if (el) {
+            ptx::pair_load_2d(dst, map, col, row.x, full);
+            ptx::pair_load_2d(dst + (128 << hbs), map, col, row.y, full);
+          }
+        }
+      } else if (ok) {
 #pragma unroll 1
         for (int c = c3; c < c3 + n; ++c, dst += kChunk * 128) {
           if (!by_row && (!values || ((k.whole >> c) & 1u))) {
@@ -646,7 +663,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           } else {
             const CUtensorMap* map = rope ? &m_kpe1 : &m_ckv1;
             const int4* rows = reinterpret_cast<const int4*>(k.boxes + 32 + kChunk * c);
-#pragma unroll 1
+#pragma unroll 2
             for (int g = 0; g < 8; ++g) {
               const int4 r = rows[g];
               if (el) ptx::pair_gather4(dst + 512 * g, map, col, r, full);
@@ -982,46 +999,69 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ok = exchange();
         if (!ok) break;
         l = sums[row] + sums[64 + row] + sums[128 + row] + sums[192 + row];
-        const bool mine = r < (s.ntok << p.head_shift);
-        const int64_t tok = s.tok0 + (r >> p.head_shift);
-        const int head = r & (p.heads - 1);
+        const int rows = s.ntok << p.head_shift;
+        const bool mine = r < rows;
         const int d0 = 256 * half + 128 * ch;
         const bool empty = l == 0.f;  // nothing was visible; NaN is not empty
+        const uint32_t oc = tmem + lanes + O_COL + 128 * ch;
         if (s.slot < 0) {
-          const float inv = 1.f / l;
-          __nv_bfloat16* out = p.out + tok * p.out_sb + head * p.out_sh + d0;
-#pragma unroll 1
+          // 32 columns at a time through this warp's share of P's memory, so that four lanes write
+          // 64 consecutive bytes of a row instead of 32 lanes 16 bytes of 32 rows
+          const float inv = empty ? 0.f : 1.f / l;
+          uint8_t* stage = sgen + OFF_P + 2048 * (warp - kSm0);
+          __nv_bfloat16* out[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int rr = 64 * (int)rank + 32 * (quad & 1) + 8 * k + (lane >> 2);
+            out[k] = p.out + (int64_t)(s.tok0 + (rr >> p.head_shift)) * p.out_sb +
+                     (int64_t)(rr & (p.heads - 1)) * p.out_sh + d0 + 8 * (lane & 3);
+            if (rr >= rows) out[k] = nullptr;
+          }
+          uint32_t o[2][32];
+          ptx::tmem_ld32(oc, o[0]);
+#pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            ptx::tmem_ld32(tmem + lanes + O_COL + 128 * ch + 32 * c, o);
             ptx::tmem_wait_ld();
-            if (mine) {
+            if (c < 3) ptx::tmem_ld32(oc + 32 * (c + 1), o[(c + 1) & 1]);
+            __syncwarp();
 #pragma unroll
-              for (int v = 0; v < 4; ++v) {
-                uint32_t w[4];
+            for (int v = 0; v < 4; ++v) {
+              uint32_t w[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  w[k] = empty ? 0u : pack2(__uint_as_float(o[8 * v + 2 * k]) * inv,
-                                            __uint_as_float(o[8 * v + 2 * k + 1]) * inv);
-                *reinterpret_cast<uint4*>(out + 32 * c + 8 * v) = make_uint4(w[0], w[1], w[2], w[3]);
-              }
+              for (int k = 0; k < 4; ++k)
+                w[k] = empty ? 0u : pack2(__uint_as_float(o[c & 1][8 * v + 2 * k]) * inv,
+                                          __uint_as_float(o[c & 1][8 * v + 2 * k + 1]) * inv);
+              *reinterpret_cast<uint4*>(stage + lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4)) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int row8 = 8 * k + (lane >> 2);
+              const uint4 x = *reinterpret_cast<const uint4*>(
+                  stage + row8 * 64 + (((lane & 3) ^ ((row8 >> 1) & 3)) << 4));
+              if (out[k] != nullptr) *reinterpret_cast<uint4*>(out[k] + 32 * c) = x;
             }
           }
           if (mine && part == 0)
-            p.lse[tok * p.lse_sb + head * p.lse_sh] =
+            p.lse[(int64_t)(s.tok0 + (r >> p.head_shift)) * p.lse_sb +
+                  (int64_t)(r & (p.heads - 1)) * p.lse_sh] =
                 empty ? -INFINITY : (m == -INFINITY ? 0.f : m) + ptx::lg2(l);
         } else {
           const int64_t at = (int64_t)s.slot + r;
-#pragma unroll 1
+          uint32_t o[2][32];
+          ptx::tmem_ld32(oc, o[0]);
+#pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            ptx::tmem_ld32(tmem + lanes + O_COL + 128 * ch + 32 * c, o);
             ptx::tmem_wait_ld();
+            if (c < 3) ptx::tmem_ld32(oc + 32 * (c + 1), o[(c + 1) & 1]);
             if (mine) {
+              float* to = p.part + part_at(at, d0 + 32 * c);
 #pragma unroll
               for (int v = 0; v < 8; ++v)
-                *reinterpret_cast<uint4*>(p.part + part_at(at, d0 + 32 * c + 4 * v)) =
-                    make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+                *reinterpret_cast<uint4*>(to + 64 * v) =
+                    make_uint4(o[c & 1][4 * v], o[c & 1][4 * v + 1], o[c & 1][4 * v + 2],
+                               o[c & 1][4 * v + 3]);
             }
           }
           if (mine && part == 0)
