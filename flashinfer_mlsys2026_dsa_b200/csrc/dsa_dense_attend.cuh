@@ -199,6 +199,8 @@ __device__ __forceinline__ int64_t part_at(int64_t row, int d) {
   return (row >> 4) * (16 * kDCkv) + (d >> 2) * 64 + (row & 15) * 4;
 }
 
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;"
@@ -257,7 +259,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t raw = ptx::smem_u32(smem_raw);
   const uint32_t sbase = (raw + 1023u) & ~1023u;
   uint8_t* sgen = smem_raw + (sbase - raw);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // What a warp's lanes hold alike is taken from lane 0 where it comes out of memory or the thread's
+  // number: only then does the compiler keep it, and the loops and operands that follow from it,
+  // in uniform registers, where copies and tensor-core instructions want them.
+  const int warp = uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31;
   const uint32_t rank = ptx::cluster_ctarank();
   const int pair = blockIdx.x >> 1;
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sgen + OFF_MISC);
@@ -302,7 +307,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::tc_fence_before();
   ptx::cluster_sync();
   ptx::tc_fence_after();
-  const uint32_t tmem = misc[0];
+  const uint32_t tmem = (uint32_t)uniform((int)misc[0]);
   ptx::grid_dep_wait();
   ptx::launch_dependents();
 
@@ -373,8 +378,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   // One unit record after another; false at the line's end or when a wait gave up.
   auto next_seg = [&](Seg& s, int n) -> bool {
     const bool ok = wait(bar(B_GF + (n % kSegs)), (uint32_t)((n / kSegs) & 1));
-    s = *reinterpret_cast<const Seg*>(sgen + OFF_SEG + 64 * (n % kSegs));
-    __syncwarp();
+    const int v = reinterpret_cast<const int*>(sgen + OFF_SEG + 64 * (n % kSegs))[lane & 15];
+    int w[sizeof(Seg) / 4];
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Seg) / 4); ++i) w[i] = __shfl_sync(0xffffffffu, v, i);
+    s = *reinterpret_cast<const Seg*>(w);
     return __all_sync(0xffffffffu, ok) && s.t0 < s.t1;
   };
   auto seg_read = [&](int n) {
@@ -752,9 +760,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int slot = 0, i = 0;               // the ring's, tiles so far
       uint32_t turn = 0;
       bool ok = true;
+      // The tensor cores' queue is short: what the issuing warp does between two slots' instructions
+      // leaves them idle.  So the next slot is looked at amid a slot's instructions, and the answer
+      // is there when they are issued (the waits took 1,200 cycles a tile).
+      bool ready = false;
       auto landed = [&]() {
-        ok = __all_sync(0xffffffffu, wait(bar(B_FULL) + 8u * (uint32_t)slot, turn));
-        ptx::tc_fence_after();
+        if (!ready) ok = __all_sync(0xffffffffu, wait(bar(B_FULL) + 8u * (uint32_t)slot, turn));
+      };
+      auto look_ahead = [&]() {
+        const bool wrap = slot + 1 == kSlots;
+        ready = __all_sync(0xffffffffu,
+                           ptx::mbar_test_wait(bar(B_FULL) + 8u * (uint32_t)(wrap ? 0 : slot + 1),
+                                               turn ^ (wrap ? 1u : 0u)));
       };
       auto next_slot = [&]() {
         if (el) ptx::pair_commit(bar(B_EMPTY) + 8u * (uint32_t)slot);
@@ -773,12 +790,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint64_t qo = dq + (uint64_t)(((b < 2 ? 2 * b : b == 2 ? 8 : 2 * b - 2) * kQBlk) >> 4);
           if (el) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              if (k == 4 && b == 2) break;
-              ptx::pair_umma_bf16(d, qo + (uint64_t)(((k >> 2) * kQBlk + (k & 3) * 32) >> 4),
-                                  ko + (uint64_t)(((k >> 2) * kBlkB + (k & 3) * 32) >> 4), kIdS,
-                                  (b | k) ? 1u : 0u);
-            }
+            for (int k = 0; k < 4; ++k)
+              ptx::pair_umma_bf16(d, qo + (uint64_t)((k * 32) >> 4), ko + (uint64_t)((k * 32) >> 4),
+                                  kIdS, (b | k) ? 1u : 0u);
+          }
+          look_ahead();
+          if (el && b != 2) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              ptx::pair_umma_bf16(d, qo + (uint64_t)((kQBlk + k * 32) >> 4),
+                                  ko + (uint64_t)((kBlkB + k * 32) >> 4), kIdS, 1u);
           }
           next_slot();
         }
@@ -788,24 +809,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       auto values = [&](int tile, int nc) {
         ok = __all_sync(0xffffffffu, wait(bar(B_PF), (uint32_t)(tile & 1)));
         if (!ok) return;
+        // S was read and O rescaled through tensor memory; copies need no such fence
+        ptx::tc_fence_after();
 #pragma unroll 1
         for (int hd = 0; hd < (nc > 3 ? 4 : 2); ++hd) {
             const int h = hd >> 1, dd = hd & 1, steps = 2 * min(3, nc - 3 * h);
             landed();
             if (!ok) return;
             const uint64_t vo = dv + (uint64_t)((slot * kSlotB) >> 4);
-            if (el) {
+            // P's 16 keys 6 h + k lie in block (6 h + k) / 4 of 64 keys
+            const uint64_t po = dp + (uint64_t)((h * (kQBlk + 64)) >> 4);
+            const uint32_t o = tmem + O_COL + 128 * dd;
+            auto two = [&](int k0) {
 #pragma unroll
-              for (int k = 0; k < 6; ++k) {
-                if (k >= steps) break;
-                // P's 16 keys 6 h + k: block (6 h + k) / 4 of 64 keys
-                const uint32_t po = h ? (uint32_t)(((6 + k) >> 2) * kQBlk + ((6 + k) & 3) * 32)
-                                      : (uint32_t)((k >> 2) * kQBlk + (k & 3) * 32);
-                ptx::pair_umma_bf16(tmem + O_COL + 128 * dd, dp + (uint64_t)(po >> 4),
-                                    vo + (uint64_t)((k * 2048) >> 4), kIdO,
+              for (int k = k0; k < k0 + 2; ++k) {
+                // blocks of the two halves break at other places: 0-3, 4-5 and 6-7, 8-11
+                const uint64_t at = h ? (k < 2 ? k * 32 : kQBlk - 64 + (k - 2) * 32)
+                                      : (k >> 2) * kQBlk + (k & 3) * 32;
+                ptx::pair_umma_bf16(o, po + (at >> 4), vo + (uint64_t)((k * 2048) >> 4), kIdO,
                                     (o_init || (h | k)) ? 1u : 0u);
               }
-            }
+            };
+            if (el) two(0);
+            look_ahead();
+            if (el && steps > 2) two(2);
+            if (el && steps > 4) two(4);
             next_slot();
         }
         o_init = true;
