@@ -17,10 +17,10 @@
 // The units of all rows form one line of tiles, cut into equal parts, one for each pair.  A unit
 // that is cut leaves partial results (O, maximum, sum) that combine kernels join.
 //
-// Warps of a CTA:  0 and 12 load keys, 13 and 14 values (64 columns each of a slot's 128), 1 issues
-// the tensor-core work (rank 0 alone), 2 loads queries, 3 walks the units, 4-11 softmax and output:
-// a thread is a row and a quarter of a tile's keys (its lane quadrant holds half of them, two
-// warps share a quadrant).
+// Warps of a CTA:  0 and 12 load keys, 13 and 14 values (64 columns each of a slot's 128), 1 and 15
+// issue the tensor-core work for S and for O (rank 0 alone), 2 loads queries, 3 walks the units,
+// 4-11 softmax and output: a thread is a row and a quarter of a tile's keys (its lane quadrant
+// holds half of them, two warps share a quadrant).
 #pragma once
 
 namespace dsa {
@@ -30,12 +30,14 @@ constexpr int kChunk = 32;                 // positions that are looked up and m
 constexpr int kTileChunks = 6;
 constexpr int kTile = kChunk * kTileChunks;
 constexpr int kSlots = 5;                  // ring of 24 KB: [96 keys x 128 columns]
+constexpr int kTurns = 2 * kSlots;         // two barriers a slot, for its fillings in turn
 constexpr int kBlkB = 96 * 128;            // [96 keys x 64 columns], 128-byte swizzle
 constexpr int kSlotB = 2 * kBlkB;
 constexpr int kQBlk = 64 * 128;            // [64 rows x 64 columns]
-constexpr int kThreads = 480;
+constexpr int kThreads = 512;
 constexpr int kLoadWarp = 0, kMmaWarp = 1, kQWarp = 2, kWalkWarp = 3, kSm0 = 4, kSmWarps = 8,
-              kLoadWarp2 = 12;  // and the two behind it
+              kLoadWarp2 = 12,  // and the two behind it
+              kPvWarp = 15;
 constexpr int kSegs = 4;                   // units that the walker is ahead
 constexpr float kTau = 8.f;                // a maximum that grows by less leaves O as it is
 
@@ -48,7 +50,7 @@ constexpr int OFF_MASK = OFF_SEG + kSegs * 64;   // [4 tiles][8] visible positio
 constexpr int OFF_POS = OFF_MASK + 4 * 8 * 4;    // [4 tiles][8] a chunk's first position
 constexpr int OFF_MAX = OFF_POS + 4 * 8 * 4;     // [2][4][64] row maxima of the quarters
 constexpr int OFF_SUM = OFF_MAX + 2 * 4 * 64 * 4;  // [4][64] row sums of the quarters
-constexpr int OFF_SCAN = OFF_SUM + 4 * 64 * 4;   // the start's scan: 15 x (tiles, units), result
+constexpr int OFF_SCAN = OFF_SUM + 4 * 64 * 4;   // the start's scan: 16 x (tiles, units), result
 constexpr int OFF_ROWS = OFF_SCAN + 320;         // 6 x [32 + 192] slots, for the loaders
 constexpr int OFF_MISC = OFF_ROWS + 6 * 224 * 4;
 constexpr int SMEM_BYTES = OFF_MISC + 64 + 1024;
@@ -57,13 +59,13 @@ static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 constexpr int S_COL = 0, O_COL = 256;      // S [2 x 96 columns], O [256]
 
 enum : int {
-  B_FULL = 0,                   // [slot] landed in both CTAs (rank 0's)
-  B_EMPTY = B_FULL + kSlots,    // [slot] read by the tensor cores
-  B_QF = B_EMPTY + kSlots,      // queries landed in both CTAs (rank 0's)
+  B_FULL = 0,                   // [turn] landed in both CTAs (rank 0's)
+  B_EMPTY = B_FULL + kTurns,    // [turn] read by the tensor cores
+  B_QF = B_EMPTY + kTurns,      // queries landed in both CTAs (rank 0's)
   B_QE,                         // ... read
   B_SF,                         // [2] S written
-  B_PF = B_SF + 2,              // P written by both CTAs (rank 0's)
-  B_PD,                         // P V done
+  B_PF = B_SF + 2,              // [2] P written by both CTAs (rank 0's)
+  B_PD = B_PF + 2,              // P V done
   B_OE,                         // O read by both CTAs (rank 0's)
   B_MF,                         // [4] masks of a tile written
   B_ME = B_MF + 4,              // [4] ... read
@@ -270,7 +272,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #define bar(k) (bar0 + 8u * (uint32_t)(k))
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kSlots; ++s) {
+    for (int s = 0; s < kTurns; ++s) {
       ptx::mbar_init(bar(B_FULL + s), 4);
       ptx::mbar_init(bar(B_EMPTY + s), 1);
     }
@@ -279,6 +281,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ptx::mbar_init(bar(B_SF), 1);
     ptx::mbar_init(bar(B_SF + 1), 1);
     ptx::mbar_init(bar(B_PF), 2 * kSmWarps);
+    ptx::mbar_init(bar(B_PF + 1), 2 * kSmWarps);
     ptx::mbar_init(bar(B_PD), 1);
     ptx::mbar_init(bar(B_OE), 2 * kSmWarps);
     for (int i = 0; i < 4; ++i) {
@@ -287,8 +290,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < kSegs; ++i) {
       ptx::mbar_init(bar(B_GF + i), 1);
-      // loaders, query loader, softmax warps and, in rank 0, the issuer
-      ptx::mbar_init(bar(B_GE + i), 5 + kSmWarps + (rank == 0 ? 1 : 0));
+      // loaders, query loader, softmax warps and, in rank 0, the issuers
+      ptx::mbar_init(bar(B_GE + i), 5 + kSmWarps + (rank == 0 ? 2 : 0));
     }
     ptx::mbar_init(bar(B_RX), 4);
     ptx::mbar_init(bar(B_RX + 1), 4);
@@ -340,14 +343,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       units += __shfl_xor_sync(0xffffffffu, units, o);
     }
     if (lane == 31) scan[warp] = run;
-    if (lane == 0) scan[15 + warp] = units;
+    if (lane == 0) scan[16 + warp] = units;
     __syncthreads();
     int64_t tiles = 0, before = run - mine;
     int all = 0;
     for (int w = 0; w < kThreads / 32; ++w) {
       if (w < warp) before += scan[w];
       tiles += scan[w];
-      all += (int)scan[15 + w];
+      all += (int)scan[16 + w];
     }
     // A window's units cost about the same: whole ones, or equal parts of each, while they fit.
     int pairs = (int)(gridDim.x >> 1);
@@ -506,16 +509,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       __syncwarp();
     }
     __syncwarp();
-  } else if (warp == kLoadWarp || warp >= kLoadWarp2) {
+  } else if (warp == kLoadWarp || (warp >= kLoadWarp2 && warp != kPvWarp)) {
     // ------------------------------------------------------------------ keys and values
     // The ring holds, in the order in which the issuer reads them, K of tile i + 1 (this CTA's half
     // of the keys; slots of 128 latent columns, the rope keys third of five), then V of tile i (four
     // slots: half of the keys, half of this CTA's columns; two where it has up to 96 keys).  Two
     // warps load the latent keys, two the rope keys and V: one chain of wait, arrive and copy is too
-    // long for every slot.  A warp passes the others' slots without a look.  Parities still tell a
-    // slot's readings apart: no slot is read without this warp's own part, and the next one that it
-    // fills is at most five further on, so that the reading before last is over (at the end of a
-    // unit, where the keys' warps pass eight slots of V, they wait for the last scores instead).
+    // long for every slot.  A warp passes the others' slots without a look, and the two issuers do
+    // not read in one order, so a slot has two pairs of barriers in turn: a wait tells a barrier's
+    // fillings apart by their parity, and with ten slots' fillings between two of one barrier the
+    // one before is always over (with five it need not be: a model of the five warps and the
+    // issuers in random steps finds both).
     const bool vals = warp > kLoadWarp2;
     const int blk = vals ? warp - kLoadWarp2 - 1 : warp == kLoadWarp2, me = vals ? 2 + blk : blk;
     const bool el = ptx::elect_one();  // warp-uniform loops around one issuing thread
@@ -534,11 +538,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int* boxes;
       int row[6];      // pages of 32 and more: the chunks' slots
     };
-    int slot = 0, tile = 0;
-    uint32_t turn = 1;  // parity of the slot's last reading
+    int at = 0, tile = 0;  // the ring's turn, 0 .. 9; tiles so far
+    uint32_t round = 0;    // rounds of ten, as a parity
     bool ok = true;
     const uint32_t full0 = ptx::mapa(bar(B_FULL), 0);
-    const uint32_t dst0 = sbase + OFF_KV + blk * kBlkB;
+    const uint32_t ring0 = sbase + OFF_KV + blk * kBlkB;
 
     // The page of this lane's box of tile t (-1: no box, or none in the table).
     auto page_of = [&](const Seg& s, int t) -> int {
@@ -612,10 +616,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       __syncwarp();
     };
 
-    // The next slot, free again; n chunks will land in this warp's block of it.
+    // The next slot, free again (its filling before, five turns ago, has been read); n chunks will
+    // land in this warp's block of it.
+    uint32_t dst0 = 0;
     auto claim = [&](int n) -> uint32_t {
-      const uint32_t full = full0 + 8u * (uint32_t)slot;
-      ok = __all_sync(0xffffffffu, wait(bar(B_EMPTY) + 8u * (uint32_t)slot, turn));
+      const bool wrapped = at >= kSlots;
+      const uint32_t full = full0 + 8u * (uint32_t)at;
+      dst0 = ring0 + (uint32_t)((wrapped ? at - kSlots : at) * kSlotB);
+      ok = __all_sync(0xffffffffu, wait(bar(B_EMPTY) + 8u * (uint32_t)(wrapped ? at - kSlots : at + kSlots),
+                                        wrapped ? round : round ^ 1u));
       if (el && ok) {
         if (n > 0) ptx::mbar_arrive_expect_tx_cluster(full, (uint32_t)(n * kChunk * 128));
         else ptx::mbar_arrive_cluster(full);
@@ -623,17 +632,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       return full;
     };
     auto skip = [&](int n) {
-      slot += n;
-      if (slot >= kSlots) {
-        slot -= kSlots;
-        turn ^= 1u;
+      at += n;
+      if (at >= kTurns) {
+        at -= kTurns;
+        round ^= 1u;
       }
     };
     // Three chunks of which n are there, a box each.
     auto fill = [&](int n, int r0, int r1, int r2, const CUtensorMap* map, int col) {
       const uint32_t full = claim(n);
       if (el && ok) {
-        const uint32_t dst = dst0 + (uint32_t)(slot * kSlotB);
+        const uint32_t dst = dst0;
         if (n > 0) ptx::pair_load_2d(dst, map, col, r0, full);
         if (n > 1) ptx::pair_load_2d(dst + kChunk * 128, map, col, r1, full);
         if (n > 2) ptx::pair_load_2d(dst + 2 * kChunk * 128, map, col, r2, full);
@@ -645,7 +654,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     auto fill_parts = [&](const Keys& k, int c3, int n, bool rope, int col, bool values) {
       const uint32_t full = claim(n);
       const uint32_t all = ((1u << n) - 1u) << c3;
-      uint32_t dst = dst0 + (uint32_t)(slot * kSlotB);
+      uint32_t dst = dst0;
       if (ok && !by_row && nbs > 0 && (!values || (k.whole & all) == all)) {
         const CUtensorMap* map = rope ? &m_kpe : &m_ckv;
         const int2* b = reinterpret_cast<const int2*>(k.boxes + (c3 << nbs));
@@ -737,8 +746,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               load_keys(k, false, 128 * b + 64 * blk);
             }
           }
-        } else if (!vals) {
-          ok = __all_sync(0xffffffffu, wait(bar(B_SF + ((tile - 1) & 1)), (uint32_t)(((tile - 1) >> 1) & 1)));
         }
         if (t > s.t0) {
           if (vals) load_values(prev);
@@ -748,120 +755,133 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp == kMmaWarp) {
+  } else if (warp == kMmaWarp || warp == kPvWarp) {
     // ------------------------------------------------------------------ tensor cores
+    // One warp issues S = Q K^T, the other O += P V.  The tensor cores' queue is short, so what an
+    // issuer does between two slots' instructions would leave them idle if it were alone (one
+    // issuer: 5,100 cycles a tile of 3,270), and the scores of the next unit start behind the last
+    // ones of this.  Each looks at its next slot amid a slot's instructions, so that the answer is
+    // there when they are issued.
     if (rank == 0) {
-      constexpr uint32_t kIdS = idesc_bf16(128, kTile, false), kIdO = idesc_bf16(128, 256, false, true);
-      const uint64_t dq = desc(sbase + OFF_Q, 16, 1024, kSw128);
-      const uint64_t dp = desc(sbase + OFF_P, 16, 1024, kSw128);
-      const uint64_t dk = desc(sbase + OFF_KV, 16, 1024, kSw128);
-      const uint64_t dv = desc(sbase + OFF_KV, kBlkB, 1024, kSw128);
       const bool el = ptx::elect_one();  // warp-uniform loops around one issuing thread
-      int slot = 0, i = 0;               // the ring's, tiles so far
-      uint32_t turn = 0;
-      bool ok = true;
-      // The tensor cores' queue is short: what the issuing warp does between two slots' instructions
-      // leaves them idle.  So the next slot is looked at amid a slot's instructions, and the answer
-      // is there when they are issued (the waits took 1,200 cycles a tile).
-      bool ready = false;
+      int at = 0, i = 0;                 // the ring's turn, tiles so far
+      uint32_t round = 0;
+      bool ok = true, ready = false;
       auto landed = [&]() {
-        if (!ready) ok = __all_sync(0xffffffffu, wait(bar(B_FULL) + 8u * (uint32_t)slot, turn));
+        if (!ready) ok = __all_sync(0xffffffffu, wait(bar(B_FULL) + 8u * (uint32_t)at, round));
+        ready = false;
       };
       auto look_ahead = [&]() {
-        const bool wrap = slot + 1 == kSlots;
+        const bool wrap = at + 1 == kTurns;
         ready = __all_sync(0xffffffffu,
-                           ptx::mbar_test_wait(bar(B_FULL) + 8u * (uint32_t)(wrap ? 0 : slot + 1),
-                                               turn ^ (wrap ? 1u : 0u)));
+                           ptx::mbar_test_wait(bar(B_FULL) + 8u * (uint32_t)(wrap ? 0 : at + 1),
+                                               round ^ (wrap ? 1u : 0u)));
       };
-      auto next_slot = [&]() {
-        if (el) ptx::pair_commit(bar(B_EMPTY) + 8u * (uint32_t)slot);
-        if (++slot == kSlots) {
-          slot = 0;
-          turn ^= 1u;
+      auto skip = [&](int n) {
+        at += n;
+        if (at >= kTurns) {
+          at -= kTurns;
+          round ^= 1u;
         }
       };
-      auto scores = [&]() {
-        const uint32_t d = tmem + S_COL + 96 * (i & 1);
-#pragma unroll 1
-        for (int b = 0; b < 5; ++b) {
-          landed();
-          if (!ok) return;
-          const uint64_t ko = dk + (uint64_t)((slot * kSlotB) >> 4);
-          const uint64_t qo = dq + (uint64_t)(((b < 2 ? 2 * b : b == 2 ? 8 : 2 * b - 2) * kQBlk) >> 4);
-          if (el) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              ptx::pair_umma_bf16(d, qo + (uint64_t)((k * 32) >> 4), ko + (uint64_t)((k * 32) >> 4),
-                                  kIdS, (b | k) ? 1u : 0u);
-          }
-          look_ahead();
-          if (el && b != 2) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              ptx::pair_umma_bf16(d, qo + (uint64_t)((kQBlk + k * 32) >> 4),
-                                  ko + (uint64_t)((kBlkB + k * 32) >> 4), kIdS, 1u);
-          }
-          next_slot();
-        }
-        if (el) ptx::pair_commit(bar(B_SF + (i & 1)));
-      };
-      bool o_init = false;
-      auto values = [&](int tile, int nc) {
-        ok = __all_sync(0xffffffffu, wait(bar(B_PF), (uint32_t)(tile & 1)));
-        if (!ok) return;
-        // S was read and O rescaled through tensor memory; copies need no such fence
-        ptx::tc_fence_after();
-#pragma unroll 1
-        for (int hd = 0; hd < (nc > 3 ? 4 : 2); ++hd) {
-            const int h = hd >> 1, dd = hd & 1, steps = 2 * min(3, nc - 3 * h);
-            landed();
-            if (!ok) return;
-            const uint64_t vo = dv + (uint64_t)((slot * kSlotB) >> 4);
-            // P's 16 keys 6 h + k lie in block (6 h + k) / 4 of 64 keys
-            const uint64_t po = dp + (uint64_t)((h * (kQBlk + 64)) >> 4);
-            const uint32_t o = tmem + O_COL + 128 * dd;
-            auto two = [&](int k0) {
-#pragma unroll
-              for (int k = k0; k < k0 + 2; ++k) {
-                // blocks of the two halves break at other places: 0-3, 4-5 and 6-7, 8-11
-                const uint64_t at = h ? (k < 2 ? k * 32 : kQBlk - 64 + (k - 2) * 32)
-                                      : (k >> 2) * kQBlk + (k & 3) * 32;
-                ptx::pair_umma_bf16(o, po + (at >> 4), vo + (uint64_t)((k * 2048) >> 4), kIdO,
-                                    (o_init || (h | k)) ? 1u : 0u);
-              }
-            };
-            if (el) two(0);
-            look_ahead();
-            if (el && steps > 2) two(2);
-            if (el && steps > 4) two(4);
-            next_slot();
-        }
-        o_init = true;
-        if (el) ptx::pair_commit(bar(B_PD));
+      auto slot_at = [&]() -> uint64_t {
+        return (uint64_t)(((at >= kSlots ? at - kSlots : at) * kSlotB) >> 4);
       };
       Seg s;
-      for (int n = 0; ok && next_seg(s, n); ++n) {
-        seg_read(n);
-        ok = __all_sync(0xffffffffu, wait(bar(B_QF), (uint32_t)(n & 1)));
-        o_init = false;
-        int before = 0;
-        for (int t = s.t0; ok && t <= s.t1; ++t) {
-          const int nc = seg_chunk(s, t + 1) - seg_chunk(s, t);
-          if (t < s.t1) {
-            scores();
+      if (warp == kMmaWarp) {
+        constexpr uint32_t kIdS = idesc_bf16(128, kTile, false);
+        const uint64_t dq = desc(sbase + OFF_Q, 16, 1024, kSw128);
+        const uint64_t dk = desc(sbase + OFF_KV, 16, 1024, kSw128);
+        for (int n = 0; ok && next_seg(s, n); ++n) {
+          seg_read(n);
+          ok = __all_sync(0xffffffffu, wait(bar(B_QF), (uint32_t)(n & 1)));
+          for (int t = s.t0; ok && t < s.t1; ++t, ++i) {
+            // P of two tiles before is written, so its S has been read
+            if (i >= 2) {
+              ok = __all_sync(0xffffffffu, wait(bar(B_PF + (i & 1)), (uint32_t)(((i - 2) >> 1) & 1)));
+              ptx::tc_fence_after();
+            }
+            const uint32_t d = tmem + S_COL + 96 * (i & 1);
+#pragma unroll 1
+            for (int b = 0; ok && b < 5; ++b) {
+              landed();
+              if (!ok) break;
+              const uint64_t ko = dk + slot_at();
+              const uint64_t qo = dq + (uint64_t)(((b < 2 ? 2 * b : b == 2 ? 8 : 2 * b - 2) * kQBlk) >> 4);
+              if (el) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  ptx::pair_umma_bf16(d, qo + (uint64_t)((k * 32) >> 4), ko + (uint64_t)((k * 32) >> 4),
+                                      kIdS, (b | k) ? 1u : 0u);
+              }
+              if (b < 4) look_ahead();
+              if (el) {
+                if (b != 2) {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k)
+                    ptx::pair_umma_bf16(d, qo + (uint64_t)((kQBlk + k * 32) >> 4),
+                                        ko + (uint64_t)((kBlkB + k * 32) >> 4), kIdS, 1u);
+                }
+                ptx::pair_commit(bar(B_EMPTY) + 8u * (uint32_t)at);
+              }
+              skip(1);
+            }
+            if (ok && el) {
+              ptx::pair_commit(bar(B_SF + (i & 1)));
+              if (t == s.t1 - 1) ptx::pair_commit(bar(B_QE));
+            }
+            // V of the tile before, at the end of the unit of the last one too
+            if (t > s.t0) skip(seg_chunk(s, t) - seg_chunk(s, t - 1) > 3 ? 4 : 2);
+            if (t == s.t1 - 1) skip(seg_chunk(s, t + 1) - seg_chunk(s, t) > 3 ? 4 : 2);
+          }
+        }
+      } else {
+        constexpr uint32_t kIdO = idesc_bf16(128, 256, false, true);
+        const uint64_t dp = desc(sbase + OFF_P, 16, 1024, kSw128);
+        const uint64_t dv = desc(sbase + OFF_KV, kBlkB, 1024, kSw128);
+        for (int n = 0; ok && next_seg(s, n); ++n) {
+          seg_read(n);
+          for (int t = s.t0; ok && t < s.t1; ++t, ++i) {
+            skip(t == s.t0 ? 5 : 0);            // K of this tile
+            skip(t + 1 < s.t1 ? 5 : 0);         // and of the next
+            ok = __all_sync(0xffffffffu, wait(bar(B_PF + (i & 1)), (uint32_t)((i >> 1) & 1)));
+            // the last unit's output has been read
+            if (ok && t == s.t0 && n > 0)
+              ok = __all_sync(0xffffffffu, wait(bar(B_OE), (uint32_t)((n - 1) & 1)));
             if (!ok) break;
-            if (t == s.t1 - 1 && el) ptx::pair_commit(bar(B_QE));
-            ++i;
+            // S was read and O rescaled through tensor memory
+            ptx::tc_fence_after();
+            const int nc = seg_chunk(s, t + 1) - seg_chunk(s, t);
+#pragma unroll 1
+            for (int hd = 0; ok && hd < (nc > 3 ? 4 : 2); ++hd) {
+              const int h = hd >> 1, dd = hd & 1, steps = 2 * min(3, nc - 3 * h);
+              landed();
+              if (!ok) break;
+              const uint64_t vo = dv + slot_at();
+              // P's 16 keys 6 h + k lie in block (6 h + k) / 4 of 64 keys
+              const uint64_t po = dp + (uint64_t)((h * (kQBlk + 64)) >> 4);
+              const uint32_t o = tmem + O_COL + 128 * dd;
+              const bool add = t > s.t0 || h > 0;
+              auto two = [&](int k0) {
+#pragma unroll
+                for (int k = k0; k < k0 + 2; ++k) {
+                  // blocks of the two halves break at other places: 0-3, 4-5 and 6-7, 8-11
+                  const uint64_t in = h ? (k < 2 ? k * 32 : kQBlk - 64 + (k - 2) * 32)
+                                        : (k >> 2) * kQBlk + (k & 3) * 32;
+                  ptx::pair_umma_bf16(o, po + (in >> 4), vo + (uint64_t)((k * 2048) >> 4), kIdO,
+                                      (add || k) ? 1u : 0u);
+                }
+              };
+              if (el) two(0);
+              if (hd < 3) look_ahead();
+              if (el && steps > 2) two(2);
+              if (el && steps > 4) two(4);
+              if (el) ptx::pair_commit(bar(B_EMPTY) + 8u * (uint32_t)at);
+              skip(1);
+            }
+            ready = false;
+            if (ok && el) ptx::pair_commit(bar(B_PD));
           }
-          if (t == s.t0) {
-            before = nc;
-            continue;
-          }
-          // the last unit's output has been read
-          if (t == s.t0 + 1 && n > 0)
-            ok = __all_sync(0xffffffffu, wait(bar(B_OE), (uint32_t)((n - 1) & 1)));
-          if (ok) values(t < s.t1 ? i - 2 : i - 1, before);
-          before = nc;
         }
       }
     }
@@ -871,7 +891,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int quad = warp & 3, ch = (warp - kSm0) >> 2;  // lanes 32 quad ..; which half of their keys
     const int half = quad >> 1, row = (quad & 1) * 32 + lane;
     const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-    const uint32_t pf = ptx::mapa(bar(B_PF), 0), oe = ptx::mapa(bar(B_OE), 0);
+    const uint32_t pf0 = ptx::mapa(bar(B_PF), 0), oe = ptx::mapa(bar(B_OE), 0);
     volatile uint32_t* masks = reinterpret_cast<volatile uint32_t*>(sgen + OFF_MASK);
     volatile int* poss = reinterpret_cast<volatile int*>(sgen + OFF_POS);
     float* maxes = reinterpret_cast<float*>(sgen + OFF_MAX);
@@ -1014,7 +1034,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (!ok) break;
         }
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive_cluster(pf);
+        if (lane == 0) ptx::mbar_arrive_cluster(pf0 + 8u * (uint32_t)(i & 1));
         o_valid = true;
       }
       if (!ok) break;
