@@ -43,8 +43,9 @@ struct Params {
   int64_t lse_sb, lse_sh;
   uint32_t* err;
   uint64_t wait_cycles;
-  // scratch: (tiles, pairs); where units lie in the line; partial results and their (max, sum)
-  int64_t *head, *cuts;
+  // scratch: where units are cut; partial results and their (maximum, sum)
+  int4* cuts;  // window: each pair's first unit; shared: each token's units, the prefix's and its own
+  int32_t pairs;
   float2* sums;
   float* part;
 };
@@ -223,11 +224,10 @@ int max_pairs() {
 
 // Where scratch holds what.
 struct Layout {
-  size_t cuts, sums, part, total;
+  size_t sums, part, total;
   Layout(int64_t tokens, int32_t heads, bool shared, int pairs) {
     const int64_t rows = shared ? 2 * tokens * heads + 128 * (int64_t)pairs : 256 * (int64_t)pairs;
-    cuts = 256;
-    sums = cuts + (size_t)((shared ? 48 * tokens : 32 * (int64_t)pairs) + 255) / 256 * 256;
+    sums = (size_t)(16 * (shared ? tokens : (int64_t)pairs) + 255) / 256 * 256;
     part = sums + (size_t)(rows * 8 + 255) / 256 * 256;
     total = part + (size_t)rows * kDCkv * 4;
   }
@@ -308,8 +308,7 @@ int attend(Call& c) {
   p.err = static_cast<uint32_t*>(c.workspace);
   p.wait_cycles = wait_limit_cycles();
   uint8_t* scratch = static_cast<uint8_t*>(c.scratch);
-  p.head = reinterpret_cast<int64_t*>(scratch);
-  p.cuts = reinterpret_cast<int64_t*>(scratch + at.cuts);
+  p.cuts = reinterpret_cast<int4*>(scratch);
   p.sums = reinterpret_cast<float2*>(scratch + at.sums);
   p.part = reinterpret_cast<float*>(scratch + at.part);
 
@@ -328,6 +327,7 @@ int attend(Call& c) {
   // nowhere.
   p.whole = !shared && p.row_offsets == nullptr && p.rows <= pairs && 2 * p.rows > pairs;
   if (p.whole) pairs = p.rows;
+  p.pairs = pairs;
   if ((rc = launch_pdl(attend_kernel, dim3(2 * (unsigned)pairs), kThreads, SMEM_BYTES, st, ckv, kpe,
                        ckv1, kpe1, qn, qp, p)) != DSA_OK)
     return rc;

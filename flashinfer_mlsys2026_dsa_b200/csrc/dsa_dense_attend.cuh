@@ -172,10 +172,13 @@ __device__ __forceinline__ Line line_of(const Params& p, const Entry& x) {
   }
   return y;
 }
-// Tiles of its first j units.
+// Places of its first j units: their tiles, and kExtra for what a unit takes besides (its queries,
+// its output, the first softmax before there is a P).
+constexpr int kExtra = 1;
 __device__ __forceinline__ int64_t line_tiles(const Line& y, int j) {
-  if (!y.own) return (int64_t)j * y.most;
-  return tiles_to(y.a + j, y.shift, y.most) - (y.a ? tiles_to(y.a, y.shift, y.most) : 0);
+  if (!y.own) return (int64_t)j * (y.most + kExtra);
+  return tiles_to(y.a + j, y.shift, y.most) - (y.a ? tiles_to(y.a, y.shift, y.most) : 0) +
+         (int64_t)j * kExtra;
 }
 // Tiles of unit j.
 __device__ __forceinline__ int unit_tiles(const Line& y, int j) {
@@ -398,10 +401,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       const int64_t start = scan[32], hi = scan[33];
       int64_t x = start;
-      if (rank == 0 && pair == 0 && !p.whole) {
-        p.head[0] = scan[34];
-        p.head[1] = scan[35];
-      }
+      const int64_t tiles = p.whole ? 1 : scan[34];
+      const int pairs = p.whole ? 1 : (int)scan[35];
+      int4 cut = make_int4(0, 0, 0, 0);
       int n = 0;
       bool ok = true;
       auto put = [&](const Seg& s) {
@@ -432,6 +434,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (; ok && j < y.units && x < hi; ++j) {
           Seg s = {};
           s.nt = unit_tiles(y, j);
+          const int64_t next = ubase + s.nt + kExtra;
+          if (x - ubase >= s.nt) {  // a cut behind its last tile
+            x = ubase = next;
+            continue;
+          }
           s.tok0 = en.tok0 + j * p.tpu;
           s.ntok = min(p.tpu, en.tok1 - s.tok0);
           s.own = en.own;
@@ -460,33 +467,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           chunks = max(chunks, s.nt);
           s.per = chunks / s.nt;
           s.rem = chunks - s.per * s.nt;
-          const bool whole = s.t0 == 0 && s.t1 == s.nt;
           if (p.groups == 0) {
             // two partial results of a pair at most: its line's first unit and its last
-            s.slot = whole ? -1 : 128 * (2 * pair + (s.t0 == 0 ? 1 : 0));
-            if (rank == 0 && x == start && !p.whole) {
-              int64_t* m = p.cuts + 4 * pair;
-              m[0] = ubase;
-              m[1] = ubase + s.nt;
-              m[2] = s.tok0;
-              m[3] = s.ntok;
+            s.slot = s.t0 == 0 && s.t1 == s.nt ? -1 : 128 * (2 * pair + (s.t0 == 0 ? 1 : 0));
+            if (s.t0 > 0) {
+              cut = make_int4(pair_of(tiles, pairs, ubase), pair_of(tiles, pairs, ubase + s.nt - 1),
+                              s.tok0, s.ntok);
+              if (cut.x != pair - 1) cut.w = 0;  // joined at its first cut
             }
           } else {
             s.slot = heads * (s.tok0 + (en.own ? p.tokens : 0)) + 128 * pair;
-            if (rank == 0 && s.t0 == 0)
-              for (int i = 0; i < s.ntok; ++i) {
-                int64_t* m = p.cuts + 3 * (2 * (int64_t)(s.tok0 + i) + en.own);
-                m[0] = ubase;
-                m[1] = ubase + s.nt;
-                m[2] = s.tok0;
-              }
+            if (rank == 0 && s.t0 == 0) {
+              const int2 where = make_int2(pair_of(tiles, pairs, ubase),
+                                           pair_of(tiles, pairs, ubase + s.nt - 1));
+              for (int i = 0; i < s.ntok; ++i)
+                reinterpret_cast<int2*>(p.cuts)[2 * (int64_t)(s.tok0 + i) + en.own] = where;
+            }
           }
           put(s);
-          x = ubase + s.t1;
-          ubase += s.nt;
+          x = min(hi, next);
+          ubase = next;
         }
         ebase = ubase;
       }
+      if (p.groups == 0 && rank == 0 && !p.whole) p.cuts[pair] = cut;
       if (ok) put(Seg{});
     }
     __syncwarp();
@@ -909,6 +913,91 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       ++shared;
       return __all_sync(0xffffffffu, done);
     };
+    // A unit's (or a part's) output, written when the next unit's first P has been: its scores and
+    // softmax run while the last P V of this one does, and P V of the next waits for this alone.
+    struct Last {
+      int tok0, rows, slot;
+      bool live, open;
+      float m, l;
+    } last = {};
+    auto finish = [&]() {
+      last.open = false;
+      if (last.live) {
+        ptx::tc_fence_after();
+        sums[part * 64 + row] = last.l;
+        ok = exchange();
+        if (!ok) return;
+        const float l = sums[row] + sums[64 + row] + sums[128 + row] + sums[192 + row], m = last.m;
+        const int r = 64 * (int)rank + row;
+        const bool mine = r < last.rows;
+        const int d0 = 256 * half + 128 * ch;
+        const bool empty = l == 0.f;  // nothing was visible; NaN is not empty
+        const uint32_t oc = tmem + lanes + O_COL + 128 * ch;
+        uint32_t o[2][32];
+        ptx::tmem_ld32(oc, o[0]);
+        if (last.slot < 0) {
+          const float inv = empty ? 0.f : 1.f / l;
+          const int q = lane & 3;
+          __nv_bfloat16* out[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int rr = 64 * (int)rank + 32 * (quad & 1) + (lane & 28) + (q ^ k);
+            out[k] = p.out + (int64_t)(last.tok0 + (rr >> p.head_shift)) * p.out_sb +
+                     (int64_t)(rr & (p.heads - 1)) * p.out_sh + d0 + 8 * q;
+            if (rr >= last.rows) out[k] = nullptr;
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            ptx::tmem_wait_ld();
+            if (c < 3) ptx::tmem_ld32(oc + 32 * (c + 1), o[(c + 1) & 1]);
+            uint32_t w[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              w[k] = empty ? 0u : pack2(__uint_as_float(o[c & 1][2 * k]) * inv,
+                                        __uint_as_float(o[c & 1][2 * k + 1]) * inv);
+            // Four lanes swap pieces of 16 bytes, so that they write 64 consecutive bytes of each of
+            // their rows in turn instead of 16 bytes of four: lane q gets piece q of row q ^ k from
+            // its holder, which sends piece (its own q) ^ k.
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t x[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const bool b0 = ((q ^ k) & 1) != 0, b1 = ((q ^ k) & 2) != 0;
+                const uint32_t lo = b0 ? w[4 + j] : w[j], hi = b0 ? w[12 + j] : w[8 + j];
+                x[j] = __shfl_xor_sync(0xffffffffu, b1 ? hi : lo, k);
+              }
+              if (out[k] != nullptr)
+                *reinterpret_cast<uint4*>(out[k] + 32 * c) = make_uint4(x[0], x[1], x[2], x[3]);
+            }
+          }
+          if (mine && part == 0)
+            p.lse[(int64_t)(last.tok0 + (r >> p.head_shift)) * p.lse_sb +
+                  (int64_t)(r & (p.heads - 1)) * p.lse_sh] =
+                empty ? -INFINITY : (m == -INFINITY ? 0.f : m) + ptx::lg2(l);
+        } else {
+          const int64_t at = (int64_t)last.slot + r;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            ptx::tmem_wait_ld();
+            if (c < 3) ptx::tmem_ld32(oc + 32 * (c + 1), o[(c + 1) & 1]);
+            if (mine) {
+              float* to = p.part + part_at(at, d0 + 32 * c);
+#pragma unroll
+              for (int v = 0; v < 8; ++v)
+                *reinterpret_cast<uint4*>(to + 64 * v) =
+                    make_uint4(o[c & 1][4 * v], o[c & 1][4 * v + 1], o[c & 1][4 * v + 2],
+                               o[c & 1][4 * v + 3]);
+            }
+          }
+          if (mine && part == 0)
+            p.sums[at] = make_float2(m == -INFINITY ? 0.f : m, l);
+        }
+        ptx::tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(oe);
+    };
     Seg s;
     for (int n = 0; ok && next_seg(s, n); ++n) {
       seg_read(n);
@@ -1036,89 +1125,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive_cluster(pf0 + 8u * (uint32_t)(i & 1));
         o_valid = true;
-      }
-      if (!ok) break;
-      // the unit's (or its part's) output
-      ok = __all_sync(0xffffffffu, wait(bar(B_PD), (uint32_t)((i - 1) & 1)));
-      if (!ok) break;
-      if (live) {
-        ptx::tc_fence_after();
-        sums[part * 64 + row] = l;
-        ok = exchange();
-        if (!ok) break;
-        l = sums[row] + sums[64 + row] + sums[128 + row] + sums[192 + row];
-        const int rows = s.ntok << p.head_shift;
-        const bool mine = r < rows;
-        const int d0 = 256 * half + 128 * ch;
-        const bool empty = l == 0.f;  // nothing was visible; NaN is not empty
-        const uint32_t oc = tmem + lanes + O_COL + 128 * ch;
-        if (s.slot < 0) {
-          // 32 columns at a time through this warp's share of P's memory, so that four lanes write
-          // 64 consecutive bytes of a row instead of 32 lanes 16 bytes of 32 rows
-          const float inv = empty ? 0.f : 1.f / l;
-          uint8_t* stage = sgen + OFF_P + 2048 * (warp - kSm0);
-          __nv_bfloat16* out[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int rr = 64 * (int)rank + 32 * (quad & 1) + 8 * k + (lane >> 2);
-            out[k] = p.out + (int64_t)(s.tok0 + (rr >> p.head_shift)) * p.out_sb +
-                     (int64_t)(rr & (p.heads - 1)) * p.out_sh + d0 + 8 * (lane & 3);
-            if (rr >= rows) out[k] = nullptr;
-          }
-          uint32_t o[2][32];
-          ptx::tmem_ld32(oc, o[0]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            ptx::tmem_wait_ld();
-            if (c < 3) ptx::tmem_ld32(oc + 32 * (c + 1), o[(c + 1) & 1]);
-            __syncwarp();
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              uint32_t w[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                w[k] = empty ? 0u : pack2(__uint_as_float(o[c & 1][8 * v + 2 * k]) * inv,
-                                          __uint_as_float(o[c & 1][8 * v + 2 * k + 1]) * inv);
-              *reinterpret_cast<uint4*>(stage + lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4)) =
-                  make_uint4(w[0], w[1], w[2], w[3]);
-            }
-            __syncwarp();
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int row8 = 8 * k + (lane >> 2);
-              const uint4 x = *reinterpret_cast<const uint4*>(
-                  stage + row8 * 64 + (((lane & 3) ^ ((row8 >> 1) & 3)) << 4));
-              if (out[k] != nullptr) *reinterpret_cast<uint4*>(out[k] + 32 * c) = x;
-            }
-          }
-          if (mine && part == 0)
-            p.lse[(int64_t)(s.tok0 + (r >> p.head_shift)) * p.lse_sb +
-                  (int64_t)(r & (p.heads - 1)) * p.lse_sh] =
-                empty ? -INFINITY : (m == -INFINITY ? 0.f : m) + ptx::lg2(l);
-        } else {
-          const int64_t at = (int64_t)s.slot + r;
-          uint32_t o[2][32];
-          ptx::tmem_ld32(oc, o[0]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            ptx::tmem_wait_ld();
-            if (c < 3) ptx::tmem_ld32(oc + 32 * (c + 1), o[(c + 1) & 1]);
-            if (mine) {
-              float* to = p.part + part_at(at, d0 + 32 * c);
-#pragma unroll
-              for (int v = 0; v < 8; ++v)
-                *reinterpret_cast<uint4*>(to + 64 * v) =
-                    make_uint4(o[c & 1][4 * v], o[c & 1][4 * v + 1], o[c & 1][4 * v + 2],
-                               o[c & 1][4 * v + 3]);
-            }
-          }
-          if (mine && part == 0)
-            p.sums[at] = make_float2(m == -INFINITY ? 0.f : m, l);
+        if (last.open) {  // P V of its last tile is done: P was written behind it
+          finish();
+          if (!ok) break;
         }
-        ptx::tc_fence_before();
       }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(oe);
+      if (!ok) break;
+      last = {s.tok0, s.ntok << p.head_shift, s.slot, live, true, m, l};
+    }
+    if (ok && last.open) {
+      ok = __all_sync(0xffffffffu, wait(bar(B_PD), (uint32_t)((i - 1) & 1)));
+      if (ok) finish();
     }
   }
 
@@ -1145,101 +1162,86 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------- partial results joined
-// Rows 16 at a time, a thread a row and kCols consecutive columns: the parts' maxima and sums
-// first, then sum_i 2^(m_i - M) O_i over 2^(m_i - M) l_i.
+// Rows 16 at a time, a thread a row and kCols consecutive columns, with the running maximum and
+// sum, so that a part's values are on their way together with its maximum.
+template <int kCols>
+struct Joined {
+  float o[kCols] = {};
+  float m = -INFINITY, l = 0.f;
 
-template <int kCols, typename Rows>
-__device__ __forceinline__ void join_rows(const Params& p, int64_t tok, int head, int d0,
-                                          const Rows& each) {
-  float m = -INFINITY;
-  each([&](int64_t at) {
+  __device__ __forceinline__ void add(const Params& p, int64_t at, int d0) {
     const float2 z = p.sums[at];
-    if (z.y != 0.f) m = fmaxf(m, z.x);
-  });
-  const float base = m == -INFINITY ? 0.f : m;
-  float o[kCols] = {}, l = 0.f;
-  each([&](int64_t at) {
-    const float2 z = p.sums[at];
-    if (z.y == 0.f) return;
-    const float w = ptx::ex2(z.x - base);
-    l += w * z.y;
+    float4 v[kCols / 4];
+#pragma unroll
+    for (int k = 0; k < kCols / 4; ++k)
+      v[k] = *reinterpret_cast<const float4*>(p.part + part_at(at, d0 + 4 * k));
+    if (z.y == 0.f) return;  // nothing was visible: its values are none
+    const float top = fmaxf(m, z.x), a = m == -INFINITY ? 0.f : ptx::ex2(m - top),
+                w = ptx::ex2(z.x - top);
+    m = top;
+    l = l * a + w * z.y;
 #pragma unroll
     for (int k = 0; k < kCols / 4; ++k) {
-      const float4 v = *reinterpret_cast<const float4*>(p.part + part_at(at, d0 + 4 * k));
-      o[4 * k] += w * v.x;
-      o[4 * k + 1] += w * v.y;
-      o[4 * k + 2] += w * v.z;
-      o[4 * k + 3] += w * v.w;
+      o[4 * k] = o[4 * k] * a + w * v[k].x;
+      o[4 * k + 1] = o[4 * k + 1] * a + w * v[k].y;
+      o[4 * k + 2] = o[4 * k + 2] * a + w * v[k].z;
+      o[4 * k + 3] = o[4 * k + 3] * a + w * v[k].w;
     }
-  });
-  const float inv = 1.f / l;
-  const bool empty = l == 0.f;
-  __nv_bfloat16* out = p.out + tok * p.out_sb + head * p.out_sh + d0;
-#pragma unroll
-  for (int k = 0; k < kCols / 8; ++k) {
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      w[j] = empty ? 0u : pack2(o[8 * k + 2 * j] * inv, o[8 * k + 2 * j + 1] * inv);
-    *reinterpret_cast<uint4*>(out + 8 * k) = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  if (d0 == 0) p.lse[tok * p.lse_sb + head * p.lse_sh] = empty ? -INFINITY : base + ptx::lg2(l);
-}
+  __device__ __forceinline__ void write(const Params& p, int64_t tok, int head, int d0) const {
+    const float inv = 1.f / l;
+    const bool empty = l == 0.f;
+    __nv_bfloat16* out = p.out + tok * p.out_sb + head * p.out_sh + d0;
+#pragma unroll
+    for (int k = 0; k < kCols / 8; ++k) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = empty ? 0u : pack2(o[8 * k + 2 * j] * inv, o[8 * k + 2 * j + 1] * inv);
+      *reinterpret_cast<uint4*>(out + 8 * k) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (d0 == 0) p.lse[tok * p.lse_sb + head * p.lse_sh] = empty ? -INFINITY : m + ptx::lg2(l);
+  }
+};
 
-// Window calls: the units that a cut goes through.  Block (c, rows 16 y ..): the unit that pair c
-// goes on with, if pair c - 1 began it.
+// Window calls: the units that a cut goes through.  Block (c, rows 16 y ..): the unit that pair
+// c + 1 goes on with, if pair c began it.
 __global__ void __launch_bounds__(256) join_cuts_kernel(const Params p) {
   ptx::grid_dep_wait();
   ptx::launch_dependents();
-  const int64_t tiles = p.head[0];
-  const int pairs = (int)p.head[1], c = (int)blockIdx.x + 1;
-  if (c >= pairs) return;
-  const int64_t *m = p.cuts + 4 * (int64_t)c, lo = m[0], hi = m[1];
-  const int first = pair_of(tiles, pairs, lo), last = pair_of(tiles, pairs, hi - 1);
-  if (first != c - 1 || cut_at(tiles, pairs, c) == lo) return;
+  const int4 cut = p.cuts[blockIdx.x + 1];  // first and last pair, first token, tokens
   const int r = 16 * (int)blockIdx.y + ((int)threadIdx.x & 15);
-  if (r >= (int)m[3] << p.head_shift) return;
-  join_rows<32>(p, m[2] + (r >> p.head_shift), r & (p.heads - 1), 32 * ((int)threadIdx.x >> 4),
-                [&](auto&& f) {
-                  f((int64_t)128 * (2 * first + 1) + r);
-                  for (int k = first + 1; k <= last; ++k) f((int64_t)256 * k + r);
-                });
+  if (r >= cut.w << p.head_shift) return;
+  const int d0 = 32 * ((int)threadIdx.x >> 4);
+  Joined<32> x;
+  x.add(p, (int64_t)128 * (2 * cut.x + 1) + r, d0);
+#pragma unroll 2
+  for (int k = cut.x + 1; k <= cut.y; ++k) x.add(p, (int64_t)256 * k + r, d0);
+  x.write(p, cut.z + (r >> p.head_shift), r & (p.heads - 1), d0);
 }
 
 // Shared calls: every token, its prefix's parts and its own.  Block (16 rows, 128 columns).
 __global__ void __launch_bounds__(128) join_tokens_kernel(const Params p) {
   ptx::grid_dep_wait();
   ptx::launch_dependents();
-  const int64_t tiles = p.head[0];
-  const int pairs = (int)p.head[1];
   const int64_t r = 16 * (int64_t)blockIdx.x + (threadIdx.x & 15);
-  const int tok = (int)(r >> p.head_shift);
+  const int tok = (int)(r >> p.head_shift), d0 = 128 * blockIdx.y + 16 * (threadIdx.x >> 4);
+  const int2* where = reinterpret_cast<const int2*>(p.cuts) + 2 * (int64_t)tok;
+  const int2 pre = where[0], own = where[1];  // first and last pair of each
   if (tok < row_token(p, 0) || tok >= row_token(p, p.rows)) return;
   int r0 = 0, r1 = p.rows;  // rows with a prefix
   if (p.group_offsets != nullptr) {
     r0 = clampi(p.group_offsets[0], 0, p.rows);
     r1 = clampi(p.group_offsets[p.groups], r0, p.rows);
   }
-  const bool prefixed = tok >= row_token(p, r0) && tok < row_token(p, r1);
-  const int64_t* rec = p.cuts + 6 * (int64_t)tok;
-  int64_t at[2];
-  int first[2], last[2];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    first[k] = 0;
-    last[k] = -1;
-    if (k == 0 && !prefixed) continue;
-    const int64_t lo = rec[3 * k], hi = rec[3 * k + 1];
-    first[k] = max(0, pair_of(tiles, pairs, lo));
-    last[k] = min(pairs - 1, pair_of(tiles, pairs, hi - 1));
-    at[k] = r + (k ? (int64_t)p.tokens * p.heads : 0);
-  }
-  join_rows<16>(p, tok, (int)(r & (p.heads - 1)), 128 * blockIdx.y + 16 * (threadIdx.x >> 4),
-                [&](auto&& f) {
-#pragma unroll
-                  for (int k = 0; k < 2; ++k)
-                    for (int c = first[k]; c <= last[k]; ++c) f(at[k] + 128 * (int64_t)c);
-                });
+  Joined<16> x;
+  if (tok >= row_token(p, r0) && tok < row_token(p, r1))
+#pragma unroll 2
+    for (int c = max(pre.x, 0); c <= min(pre.y, p.pairs - 1); ++c) x.add(p, r + 128 * (int64_t)c, d0);
+  const int64_t mine = r + (int64_t)p.tokens * p.heads;
+#pragma unroll 2
+  for (int c = max(own.x, 0); c <= min(own.y, p.pairs - 1); ++c) x.add(p, mine + 128 * (int64_t)c, d0);
+  x.write(p, tok, (int)(r & (p.heads - 1)), d0);
 }
 
 }  // namespace dense
