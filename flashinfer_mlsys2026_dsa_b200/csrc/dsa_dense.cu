@@ -327,6 +327,15 @@ int attend(Call& c) {
   // nowhere.
   p.whole = !shared && p.row_offsets == nullptr && p.rows <= pairs && 2 * p.rows > pairs;
   if (p.whole) pairs = p.rows;
+  // No more pairs than there can be places in the line, which are counted in 32 bits.
+  const bool single = p.row_offsets == nullptr;
+  auto places = [&](int64_t units, int64_t most, const Table& t) {
+    return units * (std::min<int64_t>(most, ((int64_t)t.cols * c.page_size + kTile - 1) / kTile) + kExtra);
+  };
+  int64_t line = places(single ? p.rows : p.tokens / p.tpu + p.rows, p.unit_tiles, p.own);
+  if (shared) line += places(p.tokens / p.tpu + p.groups, INT32_MAX, p.pre);
+  if (line > INT32_MAX / 2) return DSA_ERR_INVALID_ARGUMENT;
+  pairs = (int)std::min<int64_t>(pairs, line);
   p.pairs = pairs;
   if ((rc = launch_pdl(attend_kernel, dim3(2 * (unsigned)pairs), kThreads, SMEM_BYTES, st, ckv, kpe,
                        ckv1, kpe1, qn, qp, p)) != DSA_OK)
@@ -335,7 +344,8 @@ int attend(Call& c) {
     return launch_pdl(join_tokens_kernel, dim3((unsigned)((int64_t)p.tokens * p.heads / 16), 4), 128,
                       0, st, p);
   if (!p.whole && pairs > 1)
-    return launch_pdl(join_cuts_kernel, dim3((unsigned)(pairs - 1), 8), 256, 0, st, p);
+    return launch_pdl(join_cuts_kernel, dim3((unsigned)(pairs - 1), single ? p.heads / 16 : 8), 256,
+                      0, st, p);
   return DSA_OK;
 }
 

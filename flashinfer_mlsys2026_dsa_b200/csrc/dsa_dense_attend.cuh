@@ -141,15 +141,12 @@ __device__ __forceinline__ int cap_of(const Params& p, int own) {
   return (own ? p.own.cols : p.pre.cols) << p.page_shift;
 }
 // Tiles of units 0 .. x - 1 of a sequence whose unit i ends at position (i + 1) T: ceil((i + 1) / D)
-// each (D = 192 / T = 3 x 2^shift units a tile), `most` at most.
-__device__ __forceinline__ int64_t tiles_to(uint32_t x, int shift, uint32_t most) {
-  const uint32_t whole = (x >> shift) / 3u;  // units that fill their last tile
-  if (whole >= most) {
-    const uint32_t y = (3u * most) << shift;
-    return (int64_t)y * (most + 1) / 2 + (int64_t)(x - y) * most;
-  }
-  const uint32_t r = x - ((3u * whole) << shift);
-  return ((int64_t)((3u * whole) << shift) >> 1) * (whole + 1) + (int64_t)r * (whole + 1);
+// each (D = 192 / T = 3 x 2^shift units a tile), `most` at most.  The host refuses calls whose line
+// could pass 2^30 places.
+__device__ __forceinline__ int tiles_to(uint32_t x, int shift, uint32_t most) {
+  const uint32_t whole = min((x >> shift) / 3u, most);  // units that fill their last tile, in D
+  const uint32_t y = (3u * whole) << shift;
+  return (int)((y >> 1) * (whole + 1) + (x - y) * min(whole + 1, most));
 }
 // An entry with what its units' tiles follow from.
 struct Line {
@@ -175,27 +172,37 @@ __device__ __forceinline__ Line line_of(const Params& p, const Entry& x) {
 // Places of its first j units: their tiles, and kExtra for what a unit takes besides (its queries,
 // its output, the first softmax before there is a P).
 constexpr int kExtra = 1;
-__device__ __forceinline__ int64_t line_tiles(const Line& y, int j) {
-  if (!y.own) return (int64_t)j * (y.most + kExtra);
-  return tiles_to(y.a + j, y.shift, y.most) - (y.a ? tiles_to(y.a, y.shift, y.most) : 0) +
-         (int64_t)j * kExtra;
+__device__ __forceinline__ int line_tiles(const Line& y, int j) {
+  if (!y.own) return j * (int)(y.most + kExtra);
+  return tiles_to(y.a + j, y.shift, y.most) - tiles_to(y.a, y.shift, y.most) + j * kExtra;
 }
 // Tiles of unit j.
 __device__ __forceinline__ int unit_tiles(const Line& y, int j) {
   return y.own ? (int)min(y.most, ((y.a + j) >> y.shift) / 3u + 1u) : (int)y.most;
 }
 
-// a / b, both at least 0 and b above; 64 bits only where they are needed (a tenth of the time).
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-  if (((uint64_t)a | (uint64_t)b) >> 32) return (int64_t)((uint64_t)a / (uint64_t)b);
-  return (uint32_t)a / (uint32_t)b;
+// Places of entries e0 .. e1 - 1, and their units.
+__device__ __noinline__ int2 count_entries(const Params& p, int e0, int e1) {
+  int2 n = make_int2(0, 0);
+#pragma unroll 1
+  for (int e = e0; e < e1; ++e) {
+    const Line y = line_of(p, load_entry(p, e));
+    n.x += line_tiles(y, y.units);
+    n.y += y.units;
+  }
+  return n;
 }
-__device__ __forceinline__ int64_t cut_at(int64_t tiles, int pairs, int64_t c) {
-  return quotient(tiles * c, pairs);
+
+// Where part c of `pairs` equal ones begins, and the part that place x lies in.
+__device__ __forceinline__ int cut_at(int tiles, int pairs, int c) {
+  const uint32_t q = (uint32_t)tiles / (uint32_t)pairs, r = (uint32_t)tiles - q * pairs;
+  return (int)(q * c + r * c / (uint32_t)pairs);
 }
-// The pair whose part holds tile x.
-__device__ __forceinline__ int pair_of(int64_t tiles, int pairs, int64_t x) {
-  return (int)quotient((x + 1) * pairs - 1, tiles);
+__device__ __forceinline__ int pair_of(int tiles, int pairs, int x) {
+  int c = min(pairs - 1, (int)((float)x * (float)pairs / (float)tiles));  // one off at most
+  if (cut_at(tiles, pairs, c) > x) --c;
+  else if (c + 1 < pairs && cut_at(tiles, pairs, c + 1) <= x) ++c;
+  return c;
 }
 
 // Where a partial result's values and (maximum, sum) lie: blocks of 16 rows, so that a warp's
@@ -317,67 +324,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   ptx::grid_dep_wait();
   ptx::launch_dependents();
 
-  // ---------------------------------------------------------------- this pair's tiles
-  const int entries = p.groups + p.rows;
-  int64_t* scan = reinterpret_cast<int64_t*>(sgen + OFF_SCAN);
-  if (p.whole) {
-    // a pair for each row's one unit
-    if (threadIdx.x == 32 * kWalkWarp) {
-      const Entry x = load_entry(p, pair);
-      scan[30] = pair;
-      scan[31] = scan[32] = 0;
-      scan[33] = line_tiles(line_of(p, x), x.tok1 - x.tok0);
-    }
-  } else {
-    const int per = (entries + kThreads - 1) / kThreads;
+  // ---------------------------------------------------------------- the line's length
+  // Up to 32 entries are counted by the walker itself, more by all warps, for the walker.
+  const int entries = p.groups + p.rows, per = (entries + kThreads - 1) / kThreads;
+  int2* scan = reinterpret_cast<int2*>(sgen + OFF_SCAN);
+  if (entries > 32 && !p.whole) {
     const int e0 = min(entries, (int)threadIdx.x * per), e1 = min(entries, e0 + per);
-    int64_t mine = 0;
-    int units = 0;
-    for (int e = e0; e < e1; ++e) {
-      const Line y = line_of(p, load_entry(p, e));
-      mine += line_tiles(y, y.units);
-      units += y.units;
-    }
-    int64_t run = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += up;
-      units += __shfl_xor_sync(0xffffffffu, units, o);
-    }
-    if (lane == 31) scan[warp] = run;
-    if (lane == 0) scan[16 + warp] = units;
-    __syncthreads();
-    int64_t tiles = 0, before = run - mine;
-    int all = 0;
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) before += scan[w];
-      tiles += scan[w];
-      all += (int)scan[16 + w];
-    }
-    // A window's units cost about the same: whole ones, or equal parts of each, while they fit.
-    int pairs = (int)(gridDim.x >> 1);
-    if (p.groups == 0 && all <= pairs && all > 0) pairs = all * (pairs / all);
-    pairs = (int)min((int64_t)pairs, tiles);
-    const int64_t lo = pair < pairs ? cut_at(tiles, pairs, pair) : tiles;
-    const int64_t hi = pair < pairs ? cut_at(tiles, pairs, pair + 1) : tiles;
-    if (lo < hi && lo >= before && lo < before + mine) {
-      int e = e0;
-      for (; e + 1 < e1; ++e) {
-        const Line y = line_of(p, load_entry(p, e));
-        const int64_t n = line_tiles(y, y.units);
-        if (lo < before + n) break;
-        before += n;
-      }
-      scan[30] = e;
-      scan[31] = before;
-    }
-    if (threadIdx.x == 0) {
-      scan[32] = lo;
-      scan[33] = hi;
-      scan[34] = tiles;
-      scan[35] = pairs;
-    }
+    const int2 n = count_entries(p, e0, e1);
+    const int places = __reduce_add_sync(0xffffffffu, n.x), units = __reduce_add_sync(0xffffffffu, n.y);
+    if (lane == 0) scan[warp] = make_int2(places, units);
     __syncthreads();
   }
   const Wait wait{misc + 2, p.err, p.wait_cycles};
@@ -398,11 +353,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (warp == kWalkWarp) {
     // ------------------------------------------------------------------ units
+    // This pair's part of the line, and the entry where that begins.
+    int tiles = 0, pairs = 1, start = 0, hi = 0, e = pair, ebase = 0;
+    if (p.whole) {
+      hi = count_entries(p, e, e + 1).x;  // a pair for each row's one unit
+    } else {
+      auto up = [&](int x) {  // sums of the lanes up to this one
+#pragma unroll 1
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        return x;
+      };
+      const bool alone = entries <= 32;
+      const int step = alone ? 1 : per;
+      int2 mine = make_int2(0, 0);
+      if (!alone) {
+        if (lane < kThreads / 32) mine = scan[lane];
+      } else if (lane < entries) {
+        mine = count_entries(p, lane, lane + 1);
+      }
+      tiles = __reduce_add_sync(0xffffffffu, mine.x);
+      const int units = __reduce_add_sync(0xffffffffu, mine.y);
+      // A window's units cost about the same: whole ones, or equal parts of each, while they fit.
+      pairs = p.pairs;
+      if (p.groups == 0 && units <= pairs && units > 0) pairs = units * (pairs / units);
+      pairs = min(pairs, tiles);
+      start = pair < pairs ? cut_at(tiles, pairs, pair) : tiles;
+      hi = pair < pairs ? cut_at(tiles, pairs, pair + 1) : tiles;
+      e = 0;
+#pragma unroll 1
+      for (int level = alone ? 1 : 0; level < 2; ++level) {
+        // the warp's entries that hold `start`, then the lane's
+        const int from = ebase + up(mine.x) - mine.x;
+        const uint32_t here = __ballot_sync(0xffffffffu, start >= from && start < from + mine.x);
+        const int at = max(0, __ffs(here) - 1);
+        ebase = __shfl_sync(0xffffffffu, from, at);
+        e += at * (level ? step : 32 * step);
+        if (level == 0) {
+          const int e0 = min(entries, e + lane * step);
+          mine = count_entries(p, e0, min(entries, e0 + step));
+        }
+      }
+    }
     if (lane == 0) {
-      const int64_t start = scan[32], hi = scan[33];
-      int64_t x = start;
-      const int64_t tiles = p.whole ? 1 : scan[34];
-      const int pairs = p.whole ? 1 : (int)scan[35];
+      int x = start;
       int4 cut = make_int4(0, 0, 0, 0);
       int n = 0;
       bool ok = true;
@@ -413,16 +409,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ptx::mbar_arrive(bar(B_GF + (n % kSegs)));
         ++n;
       };
-      int e = x < hi ? (int)scan[30] : 0;
-      int64_t ebase = x < hi ? scan[31] : 0;
       const int heads = p.heads;
-      for (; ok && x < hi; ++e) {
+#pragma unroll 1
+      for (; ok && x < hi && e < entries; ++e) {
         const Entry en = load_entry(p, e);
         const Line y = line_of(p, en);
-        int j = 0;
-        int64_t ubase = ebase;
-        if (x > ebase) {  // the line's first entry: the unit that holds tile x
+        if (x >= ebase + line_tiles(y, y.units)) {  // an entry before the one sought, or empty
+          ebase += line_tiles(y, y.units);
+          continue;
+        }
+        int j = 0, ubase = ebase;
+        if (x > ebase) {  // the first entry: the unit that holds place x
           int top = y.units;
+#pragma unroll 1
           while (top - j > 1) {
             const int mid = (j + top) >> 1;
             if (ebase + line_tiles(y, mid) <= x) j = mid;
@@ -431,10 +430,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           ubase = ebase + line_tiles(y, j);
         }
         const int cap = cap_of(p, en.own);
+#pragma unroll 1
         for (; ok && j < y.units && x < hi; ++j) {
           Seg s = {};
           s.nt = unit_tiles(y, j);
-          const int64_t next = ubase + s.nt + kExtra;
+          const int next = ubase + s.nt + kExtra;
           if (x - ubase >= s.nt) {  // a cut behind its last tile
             x = ubase = next;
             continue;
@@ -443,8 +443,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           s.ntok = min(p.tpu, en.tok1 - s.tok0);
           s.own = en.own;
           s.row = en.own ? e - p.groups : e;
-          s.t0 = (int)(x - ubase);
-          s.t1 = (int)min((int64_t)s.nt, hi - ubase);
+          s.t0 = x - ubase;
+          s.t1 = min(s.nt, hi - ubase);
           int chunks;
           if (en.own) {
             s.p_lo = en.len - (en.tok1 - en.tok0) + j * p.tpu;
@@ -467,24 +467,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           chunks = max(chunks, s.nt);
           s.per = chunks / s.nt;
           s.rem = chunks - s.per * s.nt;
-          if (p.groups == 0) {
-            // two partial results of a pair at most: its line's first unit and its last
-            s.slot = s.t0 == 0 && s.t1 == s.nt ? -1 : 128 * (2 * pair + (s.t0 == 0 ? 1 : 0));
-            if (s.t0 > 0) {
-              cut = make_int4(pair_of(tiles, pairs, ubase), pair_of(tiles, pairs, ubase + s.nt - 1),
-                              s.tok0, s.ntok);
-              if (cut.x != pair - 1) cut.w = 0;  // joined at its first cut
-            }
-          } else {
-            s.slot = heads * (s.tok0 + (en.own ? p.tokens : 0)) + 128 * pair;
-            if (rank == 0 && s.t0 == 0) {
-              const int2 where = make_int2(pair_of(tiles, pairs, ubase),
-                                           pair_of(tiles, pairs, ubase + s.nt - 1));
-              for (int i = 0; i < s.ntok; ++i)
-                reinterpret_cast<int2*>(p.cuts)[2 * (int64_t)(s.tok0 + i) + en.own] = where;
-            }
-          }
+          // a window's pair leaves two partial results at most: its part's first unit and its last
+          s.slot = p.groups > 0 ? heads * (s.tok0 + (en.own ? p.tokens : 0)) + 128 * pair
+                   : s.t0 == 0 && s.t1 == s.nt ? -1 : 128 * (2 * pair + (s.t0 == 0 ? 1 : 0));
           put(s);
+          // where the joins find the unit's parts
+          if (rank == 0 && (p.groups > 0 ? s.t0 == 0 : s.t0 > 0)) {
+            const int first = pair_of(tiles, pairs, ubase), last = pair_of(tiles, pairs, ubase + s.nt - 1);
+            if (p.groups > 0)
+              for (int i = 0; i < s.ntok; ++i)
+                reinterpret_cast<int2*>(p.cuts)[2 * (int64_t)(s.tok0 + i) + en.own] = make_int2(first, last);
+            else if (first == pair - 1)  // at its first cut
+              cut = make_int4(first, last, s.tok0, s.ntok);
+          }
           x = min(hi, next);
           ubase = next;
         }
@@ -998,16 +993,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive_cluster(oe);
     };
-    Seg s;
-    for (int n = 0; ok && next_seg(s, n); ++n) {
+    Seg s = {};
+    int n = 0, t = 0, pos = 0;
+    bool live = false, differ = false;
+    float m = -INFINITY, l = 0.f;
+    auto open_unit = [&]() -> bool {
+      if (!next_seg(s, n)) return false;
       seg_read(n);
+      ++n;
       const int r = 64 * (int)rank + row;  // row of the unit: token r >> head_shift
-      const bool live = 64 * (int)rank + 32 * (quad & 1) < (s.ntok << p.head_shift);
-      const int pos = s.own ? s.p_lo + (r >> p.head_shift) : s.p_lo;
-      const bool differ = s.own && s.ntok > 1;
-      float m = -INFINITY, l = 0.f;
-      bool o_valid = false;
-      for (int t = s.t0; t < s.t1; ++t, ++i) {
+      live = 64 * (int)rank + 32 * (quad & 1) < (s.ntok << p.head_shift);
+      pos = s.own ? s.p_lo + (r >> p.head_shift) : s.p_lo;
+      differ = s.own && s.ntok > 1;
+      t = s.t0;
+      m = -INFINITY;
+      l = 0.f;
+      return true;
+    };
+#pragma unroll 1
+    for (bool more = true;; ++i, ++t) {
+      if (t == s.t1) {  // at the start too: both are 0
+        if (i > 0) last = {s.tok0, s.ntok << p.head_shift, s.slot, live, true, m, l};
+        more = open_unit();
+      }
+      if (more) {
         ok = wait(bar(B_MF + (i & 3)), (uint32_t)((i >> 2) & 1));
         // keys: chunk 3 half + 2 ch whole (A), and 16 positions of chunk 3 half + 1 (B)
         const int ca = 3 * half + 2 * ch, cb = 3 * half + 1;
@@ -1090,7 +1099,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           // P V of the tile before has read P and written O
           if (i > 0) ok = __all_sync(0xffffffffu, wait(bar(B_PD), (uint32_t)((i - 1) & 1)));
           if (!ok) break;
-          if (__any_sync(0xffffffffu, need) && o_valid) {
+          if (__any_sync(0xffffffffu, need) && t > s.t0) {
             ptx::tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
@@ -1124,18 +1133,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive_cluster(pf0 + 8u * (uint32_t)(i & 1));
-        o_valid = true;
-        if (last.open) {  // P V of its last tile is done: P was written behind it
-          finish();
-          if (!ok) break;
-        }
+      } else {
+        if (!last.open) break;
+        ok = __all_sync(0xffffffffu, wait(bar(B_PD), (uint32_t)((i - 1) & 1)));
+        if (!ok) break;
       }
-      if (!ok) break;
-      last = {s.tok0, s.ntok << p.head_shift, s.slot, live, true, m, l};
-    }
-    if (ok && last.open) {
-      ok = __all_sync(0xffffffffu, wait(bar(B_PD), (uint32_t)((i - 1) & 1)));
-      if (ok) finish();
+      if (last.open) {  // P V of its last tile is done: P was written behind it
+        finish();
+        if (!ok) break;
+      }
+      if (!more) break;
     }
   }
 
