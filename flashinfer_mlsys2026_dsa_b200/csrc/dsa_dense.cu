@@ -249,7 +249,8 @@ int query_map(CUtensorMap* m, const void* base, int64_t sb, int64_t sh, int widt
 }
 
 int check_table(const Table& t, int32_t page_size) {
-  if (t.pt == nullptr || t.cols < 1 || (t.sb < t.cols)) return DSA_ERR_INVALID_ARGUMENT;
+  // a stride of 0: all rows share one list of pages
+  if (t.pt == nullptr || t.cols < 1 || (t.sb < t.cols && t.sb != 0)) return DSA_ERR_INVALID_ARGUMENT;
   return (int64_t)t.cols * page_size > INT32_MAX / 2 ? DSA_ERR_INVALID_ARGUMENT : DSA_OK;
 }
 
@@ -286,13 +287,10 @@ int attend(Call& c) {
       !aligned_rows(c.ckv, c.ckv_ss, 0) || !aligned_rows(c.kpe, c.kpe_ss, 0) ||
       !aligned_rows(p.out, p.out_sb, p.out_sh))
     return DSA_ERR_MISALIGNED;
-  if (c.workspace == nullptr) return DSA_ERR_WORKSPACE;
-  const bool shared = p.pre.pt != nullptr;
+  if (c.workspace == nullptr || c.scratch == nullptr) return DSA_ERR_WORKSPACE;
+  if (!aligned16(c.scratch)) return DSA_ERR_MISALIGNED;
+  const bool shared = p.pre.pt != nullptr, single = p.row_offsets == nullptr;
   if (shared && 2 * (int64_t)p.tokens * p.heads > INT32_MAX / 2) return DSA_ERR_INVALID_ARGUMENT;
-  int pairs = max_pairs();
-  if (pairs < 1) return DSA_ERR_CUDA;
-  const Layout at(p.tokens, p.heads, shared, pairs);
-  if (c.scratch == nullptr || c.scratch_bytes < at.total) return DSA_ERR_WORKSPACE;
 
   p.page_shift = 0;
   while ((1 << p.page_shift) < c.page_size) ++p.page_shift;
@@ -305,6 +303,18 @@ int attend(Call& c) {
   const int64_t span = (int64_t)p.window + p.tpu - 1;
   const int64_t chunks = ((int64_t)p.sinks + kChunk - 1) / kChunk + (span + 30) / kChunk + 1;
   p.unit_tiles = (int32_t)((chunks + kTileChunks - 1) / kTileChunks);
+  // The most places that the line can have, which the kernel counts in 32 bits.
+  auto places = [&](int64_t units, int64_t most, const Table& t) {
+    return units * (std::min<int64_t>(most, ((int64_t)t.cols * c.page_size + kTile - 1) / kTile) + kExtra);
+  };
+  int64_t line = places(single ? p.rows : p.tokens / p.tpu + p.rows, p.unit_tiles, p.own);
+  if (shared) line += places(p.tokens / p.tpu + p.groups, INT32_MAX, p.pre);
+  if (line > INT32_MAX / 2) return DSA_ERR_INVALID_ARGUMENT;
+
+  int pairs = max_pairs();
+  if (pairs < 1) return DSA_ERR_CUDA;
+  const Layout at(p.tokens, p.heads, shared, pairs);
+  if (c.scratch_bytes < at.total) return DSA_ERR_WORKSPACE;
   p.err = static_cast<uint32_t*>(c.workspace);
   p.wait_cycles = wait_limit_cycles();
   uint8_t* scratch = static_cast<uint8_t*>(c.scratch);
@@ -325,17 +335,9 @@ int attend(Call& c) {
   const cudaStream_t st = static_cast<cudaStream_t>(c.stream);
   // One unit a row: where two would not fit side by side, each has a pair of its own and is cut
   // nowhere.
-  p.whole = !shared && p.row_offsets == nullptr && p.rows <= pairs && 2 * p.rows > pairs;
+  p.whole = !shared && single && p.rows <= pairs && 2 * p.rows > pairs;
   if (p.whole) pairs = p.rows;
-  // No more pairs than there can be places in the line, which are counted in 32 bits.
-  const bool single = p.row_offsets == nullptr;
-  auto places = [&](int64_t units, int64_t most, const Table& t) {
-    return units * (std::min<int64_t>(most, ((int64_t)t.cols * c.page_size + kTile - 1) / kTile) + kExtra);
-  };
-  int64_t line = places(single ? p.rows : p.tokens / p.tpu + p.rows, p.unit_tiles, p.own);
-  if (shared) line += places(p.tokens / p.tpu + p.groups, INT32_MAX, p.pre);
-  if (line > INT32_MAX / 2) return DSA_ERR_INVALID_ARGUMENT;
-  pairs = (int)std::min<int64_t>(pairs, line);
+  pairs = (int)std::min<int64_t>(pairs, line);  // no more than there can be places
   p.pairs = pairs;
   if ((rc = launch_pdl(attend_kernel, dim3(2 * (unsigned)pairs), kThreads, SMEM_BYTES, st, ckv, kpe,
                        ckv1, kpe1, qn, qp, p)) != DSA_OK)

@@ -112,6 +112,18 @@ def test_window_arguments():
         assert _window(table=_with(TABLE, i, bad)) == 1, (i, bad)
     assert _window(out=(24, 16 * 512, 512)) == 3 and _window(out=(None, 1, 1)) == 1
     assert _window(lse=(None, 16, 1)) == 1
+    assert _window(scratch=None) == 4 and _window(scratch=24) == 3
+
+
+def test_lines_past_32_bits_are_refused():
+    """A call's tiles are counted in 32 bits: 2^22 rows behind 2^19 positions pass them, with a
+    window that leaves a tile of each they do not (and reach the device, which is not there)."""
+    many = dict(tokens=1 << 22, rows=1 << 22, table=(16, 1 << 13, 1 << 13))
+    assert _window(**many, window=1 << 30) == 1
+    if not torch.cuda.is_available():
+        assert _window(**many, window=10) == 5
+    # a prefix of 2^26 positions for as many tokens as the call takes
+    assert _shared(tokens=1 << 22, rows=1 << 22, prefix=(16, 1 << 20, 1 << 20)) == 1
 
 
 def test_shared_arguments():

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import dense_reference as ref
-from flashinfer_mlsys2026_dsa_b200 import (kernel, kernel_shared, kernel_window, merge_states,
+from flashinfer_mlsys2026_dsa_b200 import (_native, kernel, kernel_shared, kernel_window, merge_states,
                                            read_device_errors)
 
 pytestmark = pytest.mark.gpu
@@ -411,6 +411,123 @@ def test_streams_overlap():
     for a, b in got:
         ref.check(a[0], want[0], want[2], "output")
         ref.check(b[0], want2[0], want2[2], "output")
+
+
+@pytest.mark.parametrize("rows", [33, 513, 1025, 1600])
+def test_window_many_rows(rows):
+    """More rows than lanes, than threads and than twice that; every ninth sees nothing."""
+    lens = [0 if r % 9 == 4 else (53 * r) % 400 + 1 for r in range(rows)]
+    args, want = window_case([max(n, 1) for n in lens], [1] * rows, 16, 64, 150, 2)
+    out, lse = outputs(rows, 16)
+    kernel_window(*args[:5], i32(lens), SM, out, lse, 150, 2)
+    live = torch.tensor([n > 0 for n in lens], device="cuda")
+    ref.check(out[live], want[0][live], want[2][live], "output")
+    ref.check(lse[live], want[1][live], want[3][live], "lse")
+    assert not out[~live].any() and (lse[~live] == -math.inf).all()
+
+
+@pytest.mark.parametrize("groups", [20, 40, 300, 700])
+def test_shared_many_groups(groups):
+    """Groups of 0 to 3 rows of 1 to 3 tokens; 40 and more with their rows are over 32 entries."""
+    sizes = [g % 4 for g in range(groups)]
+    rows = sum(sizes)
+    run_shared([(29 * g) % 330 + 1 for g in range(groups)], sizes, [(37 * r) % 90 + 3 for r in range(rows)],
+               [1 + r % 3 for r in range(rows)], 32, 32)
+
+
+def test_queries_and_tables_that_rows_share():
+    """Strides of 0: one token's query and one page list for all rows."""
+    args, _ = window_case([400], [1], 16, 64, 120, 3, poison=False)
+    qn, qp, ckv, kpe, table, _ = args
+    lens = [400, 1, 77, 300]
+    q = qn.expand(4, -1, -1), qp.expand(4, -1, -1)
+    out, lse = outputs(4, 16)
+    kernel_window(*q, ckv, kpe, table.expand(4, -1), i32([400]).expand(4).clone(), SM, out, lse, 120, 3)
+    want = ref.window(*q, ckv, kpe, table.expand(4, -1), [400] * 4, [1] * 4, SM, 120, 3, 64)
+    ref.check(out, want[0], want[2], "output")
+    kernel_window(*q, ckv, kpe, table.expand(4, -1), i32(lens), SM, out, lse, 120, 3)
+    want = ref.window(*q, ckv, kpe, table.expand(4, -1), lens, [1] * 4, SM, 120, 3, 64)
+    ref.check(out, want[0], want[2], "output")
+    ref.check(lse, want[1], want[3], "lse")
+
+
+def test_slots_behind_the_last_whole_page():
+    """A flat pool of three pages and a half: what lies behind the third is no page."""
+    ckv, kpe = (x.view(-1, w)[:3 * 64 + 32] for x, w in zip(ref.pools(4, 64, 3), (512, 64)))
+    qn, qp = ref.queries(1, 16, 4)
+    read_device_errors()
+    out, lse = outputs(1, 16)
+    kernel_window(qn, qp, ckv, kpe, i32([[2, 3, 0]]), i32([192]), SM, out, lse, page_size=64)
+    assert read_device_errors() == 1
+    pools = ckv[:192].view(3, 64, 512), kpe[:192].view(3, 64, 64)
+    keys = ref.sequence(*pools, i32([2, 0, 0]), 192, 64)
+    seen = torch.arange(192, device="cuda") // 64 != 1
+    want = ref.attend(torch.cat([qn, qp], 2), keys, seen[None], SM)
+    ref.check(out, want[0], want[2], "output")
+    ref.check(lse, want[1], want[3], "lse")
+
+
+def test_two_graphs_at_once():
+    """Two graphs captured on one stream, replayed in turn on it and side by side on two."""
+    w, want = window_case([3000, 50, 700], [1, 9, 33], 16, 64, 2000, 4, poison=False)
+    s, want2 = shared_case([2000], [9], [100] * 9, [1] * 9, 32, 64, poison=False)
+    off = offsets([1, 9, 33])
+    a, b = outputs(43, 16), outputs(9, 32)
+    stream, other = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def one():
+        kernel_window(*w, SM, *a, 2000, 4, row_offsets=off)
+
+    def two():
+        kernel_shared(*s, SM, *b)
+
+    torch.cuda.synchronize()
+    graphs = []
+    with torch.cuda.stream(stream):
+        for step in (one, two):
+            step()
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=stream):
+                step()
+    torch.cuda.synchronize()
+    for apart in (False, True):
+        for x in (*a, *b):
+            x.fill_(7)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            with torch.cuda.stream(stream):
+                graphs[0].replay()
+            with torch.cuda.stream(other if apart else stream):
+                graphs[1].replay()
+        torch.cuda.synchronize()
+        for got, exp in ((a, want), (b, want2)):
+            ref.check(got[0], exp[0], exp[2], "output")
+            ref.check(got[1], exp[1], exp[3], "lse")
+
+
+def test_scratch_that_is_too_small_is_refused():
+    lib = _native.load()
+    args, _ = window_case([100], [1], 16, 64, 10, 0, poison=False)
+    qn, qp, ckv, kpe, table, n = args
+    out, lse = outputs(1, 16)
+    ws = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    for shared in (0, 1):
+        size = lib.dsa_dense_scratch_size(1, 16, shared)
+        assert size > 0
+        scratch = torch.empty(size, dtype=torch.uint8, device="cuda")
+        for nbytes in (size - 1, 0):
+            head = (qn.data_ptr(), 8192, 512, qp.data_ptr(), 1024, 64, ckv.data_ptr(), 512,
+                    kpe.data_ptr(), 64, ckv.shape[0] * 64, 64)
+            own = (table.data_ptr(), table.stride(0), table.shape[1], n.data_ptr(), None, 1)
+            tail = (0.1, out.data_ptr(), 8192, 512, lse.data_ptr(), 16, 1, 1, 16, scratch.data_ptr(),
+                    nbytes, ws.data_ptr(), torch.cuda.current_stream().cuda_stream)
+            if shared:
+                rc = lib.dsa_mla_decode_shared(*head, *own[:4], None, 1, *own, *tail)
+            else:
+                rc = lib.dsa_mla_decode_window(*head, *own, 10, 0, *tail)
+            assert rc == 4
+    torch.cuda.synchronize()
+    assert (out == 7).all() and (lse == 7).all()
 
 
 # --------------------------------------------------------------------------------- the join
