@@ -493,10 +493,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------ queries
     const uint32_t qf = ptx::mapa(bar(B_QF), 0);
     Seg s;
-    for (int n = 0; next_seg(s, n); ++n) {
+    bool ok = true;
+    for (int n = 0; ok && next_seg(s, n); ++n) {
       seg_read(n);
-      if (lane == 0) {
-        if (n > 0 && !wait(bar(B_QE), (uint32_t)((n - 1) & 1))) break;
+      if (n > 0) ok = __all_sync(0xffffffffu, wait(bar(B_QE), (uint32_t)((n - 1) & 1)));
+      if (ok && lane == 0) {
         ptx::mbar_arrive_expect_tx_cluster(qf, 9 * kQBlk);
         const int hb = min(64, p.heads);
         const int tok = s.tok0 + (p.heads == 128 ? 0 : (int)rank * (64 / hb));
