@@ -233,9 +233,10 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Bounded wait on an mbarrier.  What follows a first look that fails is out of line: the kernel's
-// roles run side by side, and their code has to fit the instruction caches together (174 KB with
-// every wait and loop inline: 1,450 cycles to fill a slot; see the figures above for now).
+// Bounded wait on an mbarrier.  The kernel's roles run side by side, and their code has to fit the
+// instruction caches together: 256 rows behind 32768 shared positions took 614 us with 174 KB of it,
+// 331 with 109 KB, 317 with 85 KB.  So what follows a first look that fails is out of line, but for
+// the walker, whose loops are 25 KB longer with a call in them.
 __device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
                                      uint32_t* err, uint64_t limit) {
   const uint64_t t0 = ptx::cycles();
@@ -258,6 +259,19 @@ struct Wait {
   uint64_t limit;
   __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) const {
     return ptx::mbar_try_wait(bar, parity) || wait_on(bar, parity, abort_flag, err, limit);
+  }
+  __device__ __forceinline__ bool here(uint32_t bar, uint32_t parity) const {
+    const uint64_t t0 = ptx::cycles();
+#pragma unroll 1
+    while (!ptx::mbar_try_wait(bar, parity)) {
+      if (*abort_flag) return false;
+      if (ptx::cycles() - t0 > limit) {
+        *abort_flag = 1;
+        atomicOr(err, (uint32_t)DSA_DEVERR_TIMEOUT);
+        return false;
+      }
+    }
+    return true;
   }
 };
 
@@ -403,7 +417,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int n = 0;
       bool ok = true;
       auto put = [&](const Seg& s) {
-        if (n >= kSegs) ok = wait(bar(B_GE + (n % kSegs)), (uint32_t)(((n / kSegs) - 1) & 1));
+        ok = wait.here(bar(B_GE + (n % kSegs)), (uint32_t)((n / kSegs + 1) & 1));
         if (!ok) return;
         *reinterpret_cast<Seg*>(sgen + OFF_SEG + 64 * (n % kSegs)) = s;
         ptx::mbar_arrive(bar(B_GF + (n % kSegs)));
