@@ -319,7 +319,13 @@ int dsa_compact_q8(const int32_t* keep, int64_t keep_stride_b, int32_t num_rows,
  * its own; a row of length 0 with one token sees the prefix alone.
  *
  * Both need `scratch`, a device buffer of dsa_dense_scratch_size() bytes for this call alone
- * (calls that may overlap on the GPU need one each).
+ * (calls that may overlap on the GPU need one each), 16-byte aligned.
+ *
+ * Only whole pages of the pool count.  A page table's stride may be 0 (rows that share one list).
+ * Where a row has several tokens, a NaN or infinity that one of them sees may reach the others.
+ * A call whose tiles (192 positions for up to 128 / num_heads tokens) could pass 2^30, with two
+ * more for each such unit, is refused.  Where a wait runs out (DSA_DEVERR_TIMEOUT) the call's
+ * outputs are unspecified.
  */
 int dsa_mla_decode_window(
     const void* q_nope, int64_t q_nope_stride_b, int64_t q_nope_stride_h, const void* q_pe,
