@@ -50,7 +50,7 @@ constexpr int OFF_MASK = OFF_SEG + kSegs * 64;   // [4 tiles][8] visible positio
 constexpr int OFF_POS = OFF_MASK + 4 * 8 * 4;    // [4 tiles][8] a chunk's first position
 constexpr int OFF_MAX = OFF_POS + 4 * 8 * 4;     // [2][4][64] row maxima of the quarters
 constexpr int OFF_SUM = OFF_MAX + 2 * 4 * 64 * 4;  // [4][64] row sums of the quarters
-constexpr int OFF_SCAN = OFF_SUM + 4 * 64 * 4;   // the start's scan: 16 x (tiles, units), result
+constexpr int OFF_SCAN = OFF_SUM + 4 * 64 * 4;   // the start's scan: 16 x (tiles, units); Part
 constexpr int OFF_ROWS = OFF_SCAN + 320;         // 6 x [32 + 192] slots, for the loaders
 constexpr int OFF_MISC = OFF_ROWS + 6 * 224 * 4;
 constexpr int SMEM_BYTES = OFF_MISC + 64 + 1024;
@@ -233,6 +233,52 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// A pair's part of the line, as the walker found it.
+struct Part {
+  int start, end;     // places
+  int entry, before;  // the entry that holds the first, and the places before that entry
+};
+
+// What a pair that gave up leaves: NaN in all query rows of its part, in output and lse where no
+// other pair works on their unit, and as the statistics of its partial results, which every join of
+// their rows meets.
+__device__ __noinline__ void spoil(const Params& p, const Part& x, int pair) {
+  const int entries = x.start < x.end ? p.groups + p.rows : 0;
+  int ubase = x.before;
+#pragma unroll 1
+  for (int e = x.entry; e < entries && ubase < x.end; ++e) {
+    const Entry en = load_entry(p, e);
+    const Line y = line_of(p, en);
+#pragma unroll 1
+    for (int j = 0; j < y.units && ubase < x.end; ++j) {
+      const int nt = unit_tiles(y, j), t0 = max(0, x.start - ubase), t1 = min(nt, x.end - ubase);
+      const int tok0 = en.tok0 + j * p.tpu, ntok = min(p.tpu, en.tok1 - tok0);
+      const int rows = t0 < t1 ? ntok << p.head_shift : 0;
+      const int nan = 0x7fffffff;  // two of bf16 also
+      if (p.groups == 0 && t0 == 0 && t1 == nt) {
+#pragma unroll 1
+        for (int i = threadIdx.x; i < rows * (kDCkv / 8); i += kThreads) {
+          const int r = i / (kDCkv / 8), tok = tok0 + (r >> p.head_shift), h = r & (p.heads - 1);
+          *reinterpret_cast<int4*>(p.out + (int64_t)tok * p.out_sb + (int64_t)h * p.out_sh +
+                                   8 * (i % (kDCkv / 8))) = make_int4(nan, nan, nan, nan);
+          if (i % (kDCkv / 8) == 0)
+            p.lse[(int64_t)tok * p.lse_sb + (int64_t)h * p.lse_sh] = __int_as_float(nan);
+        }
+      } else {
+        const int64_t slot = p.groups > 0 ? p.heads * (tok0 + (en.own ? p.tokens : 0)) + 128 * pair
+                                          : 128 * (2 * pair + (t0 == 0 ? 1 : 0));
+#pragma unroll 1
+        for (int r = threadIdx.x; r < rows; r += kThreads)
+          p.sums[slot + r] = make_float2(__int_as_float(nan), __int_as_float(nan));
+        if (p.groups > 0 && t0 == 0 && (int)threadIdx.x < ntok && rows > 0)
+          reinterpret_cast<int2*>(p.cuts)[2 * (int64_t)(tok0 + threadIdx.x) + en.own] =
+              make_int2(pair, pair);
+      }
+      ubase += nt + kExtra;
+    }
+  }
+}
+
 // Bounded wait on an mbarrier.  The kernel's roles run side by side, and their code has to fit the
 // instruction caches together: 256 rows behind 32768 shared positions took 614 us with 174 KB of it,
 // 331 with 109 KB, 317 with 85 KB.  So what follows a first look that fails is out of line, but for
@@ -412,6 +458,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
     if (lane == 0) {
+      *reinterpret_cast<Part*>(scan + 16) = {start, hi, e, ebase};
       int x = start;
       int4 cut = make_int4(0, 0, 0, 0);
       int n = 0;
@@ -1184,6 +1231,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     __syncthreads();
     ptx::cluster_sync();
+    if (rank == 0) spoil(p, *reinterpret_cast<const Part*>(scan + 16), pair);
   }
   if (warp == kMmaWarp) {
     ptx::tc_fence_after();

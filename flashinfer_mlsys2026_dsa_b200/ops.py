@@ -54,7 +54,7 @@ def _strict_check(device: torch.device, what: str) -> None:
         if word & _native.DEVERR_BAD_INDEX:
             bits.append("an index outside [-1, num_slots) was treated as padding")
         if word & _native.DEVERR_TIMEOUT:
-            bits.append("a wait in the kernel ran out (rows whose split-K merge gave up are NaN)")
+            bits.append("a wait in the kernel ran out (the rows that it gave up on are NaN)")
         raise DSAError(f"{what}: device error word {word:#x}: " + "; ".join(bits))
 
 

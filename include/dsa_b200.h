@@ -324,8 +324,8 @@ int dsa_compact_q8(const int32_t* keep, int64_t keep_stride_b, int32_t num_rows,
  * Only whole pages of the pool count.  A page table's stride may be 0 (rows that share one list).
  * Where a row has several tokens, a NaN or infinity that one of them sees may reach the others.
  * A call whose tiles (192 positions for up to 128 / num_heads tokens) could pass 2^30, with two
- * more for each such unit, is refused.  Where a wait runs out (DSA_DEVERR_TIMEOUT) the call's
- * outputs are unspecified.
+ * more for each such unit, is refused.  Where a wait runs out (DSA_DEVERR_TIMEOUT) all that its CTA
+ * pair worked on is NaN, in output and lse; the rest is as without it.
  */
 int dsa_mla_decode_window(
     const void* q_nope, int64_t q_nope_stride_b, int64_t q_nope_stride_h, const void* q_pe,
