@@ -137,46 +137,48 @@ __global__ void __launch_bounds__(256) merge_kernel(const MergeParams p) {
   if (lane == 0) p.lse[t * p.lse_sb + h * p.lse_sh] = base + log2f(total);
 }
 
-// Whether rows of `width` elements at a + t sb + h sh and at b + t sb + h sh meet, for any
-// (t, h) of either (bytes throughout).
-bool same_grid_meets(int64_t d, int64_t sb, int64_t sh, int64_t tokens, int64_t heads,
-                     int64_t width) {
+// The rows of a [tokens, heads] tensor (bytes throughout).
+struct Rows2 {
+  const void* p;
+  int64_t sb, sh, width;
+};
+
+// Whether rows of a and b meet, for any (t, h) of either; strides are those of a.
+bool same_grid_meets(const Rows2& a, const Rows2& b, int64_t tokens, int64_t heads) {
+  const int64_t d = (int64_t) reinterpret_cast<intptr_t>(a.p) - (int64_t) reinterpret_cast<intptr_t>(b.p);
   for (int64_t dh = -(heads - 1); dh < heads; ++dh) {
-    const int64_t rest = d - dh * sh;
-    if (sb == 0 || tokens == 1) {
-      if (std::abs(rest) < width) return true;
-      continue;
+    const int64_t rest = d + dh * a.sh;
+    // the tokens' distance that brings them closest, and its neighbours
+    const int64_t q = a.sb == 0 ? 0 : std::clamp(-rest / a.sb, -(tokens - 1), tokens - 1);
+    for (int64_t dt = q - 1; dt <= q + 1; ++dt) {
+      const int64_t x = rest + dt * a.sb;
+      if (std::abs(dt) < tokens && x < b.width && -x < a.width) return true;
     }
-    const int64_t q = rest / sb;
-    for (int64_t dt = q - 1; dt <= q + 1; ++dt)
-      if (std::abs(dt) < tokens && std::abs(rest - dt * sb) < width) return true;
   }
   return false;
 }
 
-struct Rows2 {
-  const void* p;
-  int64_t sb, sh;  // bytes
-};
-
-// Whether writing `out` may change what is still to be read of `part`: they overlap without
-// being the same rows.
-bool overlaps(const Rows2& out, const Rows2& part, int64_t tokens, int64_t heads, int64_t width) {
-  if (out.p == part.p && out.sb == part.sb && out.sh == part.sh) return false;
-  auto range = [&](const Rows2& r, int64_t& lo, int64_t& hi) {
-    const int64_t b = (tokens - 1) * r.sb, h = (heads - 1) * r.sh;
-    lo = (int64_t) reinterpret_cast<intptr_t>(r.p) + std::min<int64_t>(b, 0) + std::min<int64_t>(h, 0);
-    hi = (int64_t) reinterpret_cast<intptr_t>(r.p) + std::max<int64_t>(b, 0) +
-         std::max<int64_t>(h, 0) + width;
+// Whether a and b share memory.  Exact where they have the same strides; otherwise all that lies
+// between a token's first and last row counts (between the first and last of all, where the tokens'
+// strides differ too).
+bool overlaps(Rows2 a, Rows2 b, int64_t tokens, int64_t heads) {
+  if (a.sb == b.sb && a.sh == b.sh) return same_grid_meets(a, b, tokens, heads);
+  auto whole = [](Rows2& r, int64_t n, int64_t stride) {
+    const int64_t span = (n - 1) * stride;
+    if (span < 0) r.p = static_cast<const char*>(r.p) + span;
+    r.width += std::abs(span);
   };
-  int64_t a0, a1, b0, b1;
-  range(out, a0, a1);
-  range(part, b0, b1);
-  if (a1 <= b0 || b1 <= a0) return false;
-  if (out.sb != part.sb || out.sh != part.sh) return true;
-  return same_grid_meets((int64_t) reinterpret_cast<intptr_t>(out.p) -
-                             (int64_t) reinterpret_cast<intptr_t>(part.p),
-                         out.sb, out.sh, tokens, heads, width);
+  for (Rows2* r : {&a, &b}) whole(*r, heads, r->sh);
+  a.sh = b.sh = 0;
+  if (a.sb == b.sb) return same_grid_meets(a, b, tokens, 1);
+  for (Rows2* r : {&a, &b}) whole(*r, tokens, r->sb);
+  a.sb = b.sb = 0;
+  return same_grid_meets(a, b, 1, 1);
+}
+
+// Whether they are the same rows.
+bool same_rows(const Rows2& a, const Rows2& b) {
+  return a.p == b.p && a.sb == b.sb && a.sh == b.sh;
 }
 
 bool aligned_rows(const void* p, int64_t sb, int64_t sh) {
@@ -475,6 +477,8 @@ int dsa_merge_states(int32_t num_parts, const void* const* outputs,
       num_tokens > INT64_MAX / num_heads || num_tokens * num_heads > (int64_t)INT32_MAX * 8)
     return DSA_ERR_INVALID_ARGUMENT;
   if (!aligned_rows(output, output_stride_b, output_stride_h)) return DSA_ERR_MISALIGNED;
+  const Rows2 out_rows = {output, 2 * output_stride_b, 2 * output_stride_h, 2 * kDCkv},
+              lse_rows = {lse, 4 * lse_stride_b, 4 * lse_stride_h, 4};
   MergeParams p = {};
   for (int i = 0; i < num_parts; ++i) {
     if (!outputs[i] || !lses[i]) return DSA_ERR_INVALID_ARGUMENT;
@@ -485,10 +489,14 @@ int dsa_merge_states(int32_t num_parts, const void* const* outputs,
     p.z_sb[i] = lse_strides[2 * i];
     p.z_sh[i] = lse_strides[2 * i + 1];
     if (!aligned_rows(p.o[i], p.o_sb[i], p.o_sh[i])) return DSA_ERR_MISALIGNED;
-    if (overlaps({output, 2 * output_stride_b, 2 * output_stride_h},
-                 {p.o[i], 2 * p.o_sb[i], 2 * p.o_sh[i]}, num_tokens, num_heads, 2 * kDCkv) ||
-        overlaps({lse, 4 * lse_stride_b, 4 * lse_stride_h}, {p.z[i], 4 * p.z_sb[i], 4 * p.z_sh[i]},
-                 num_tokens, num_heads, 4))
+    const Rows2 o = {p.o[i], 2 * p.o_sb[i], 2 * p.o_sh[i], 2 * kDCkv},
+                z = {p.z[i], 4 * p.z_sb[i], 4 * p.z_sh[i], 4};
+    // a warp reads its own rows of all parts before it writes them, and no others
+    auto spoils = [&](const Rows2& to, const Rows2& own, const Rows2& other) {
+      return overlaps(to, other, num_tokens, num_heads) ||
+             (!same_rows(to, own) && overlaps(to, own, num_tokens, num_heads));
+    };
+    if (spoils(out_rows, o, z) || spoils(lse_rows, z, o))
       return DSA_ERR_INVALID_ARGUMENT;
   }
   p.out = static_cast<__nv_bfloat16*>(output);

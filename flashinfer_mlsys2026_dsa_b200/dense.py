@@ -209,7 +209,7 @@ def merge_states(outputs, lses, output, lse) -> None:
     positions: with M the largest lse and ``w_i = 2 ** (lse_i - M)``, ``output = sum w_i outputs_i /
     sum w_i`` (summed in fp32) and ``lse = M + log2(sum w_i)``.  A part of lse -inf is left out
     whatever its output holds; where all are, output is 0 and lse -inf.  ``output`` and ``lse`` may
-    each be one of the parts themselves; another overlap with a part is refused.
+    each be one of the parts themselves; another overlap with a part's output or lse is refused.
     """
     what = "dsa_merge_states"
     outputs, lses = list(outputs), list(lses)

@@ -360,7 +360,8 @@ size_t dsa_dense_scratch_size(int64_t num_tokens, int32_t num_heads, int32_t sha
  * largest lse and w_i = 2^(lse_i - M): output = sum w_i outputs[i] / sum w_i (summed in fp32),
  * lse = M + log2 sum w_i.  A part of lse -inf is left out whatever its output holds; where all
  * are, output is 0 and lse -inf.  Output and lse may each be a part's own; any other overlap with
- * a part is refused.
+ * a part's output or lse is refused (rows of other strides count from a token's first to its last,
+ * or from the first of all to the last).
  */
 int dsa_merge_states(int32_t num_parts, const void* const* outputs,
                      const int64_t* output_strides, const float* const* lses,

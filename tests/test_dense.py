@@ -1,6 +1,7 @@
 """The dense operators without a GPU: refusals, host checks of the C ABI, the 64-bit reference."""
 import ctypes
 import math
+import random
 
 import pytest
 import torch
@@ -168,3 +169,52 @@ def test_merge_refuses_a_result_that_overlaps_a_part():
     assert _merge(out=(first, 16384, 512)) == 1
     # interleaved with a part (rows between its rows, one of which would be met)
     assert _merge(strides=(16384, 512) * 2, out=(first + 16384 + 512, 16384, 512)) == 1
+
+
+def test_merge_refuses_a_result_over_the_other_kind_of_part():
+    """An lse inside a part's output, and an output over a part's lse."""
+    first, z = 1 << 20, 3 << 20
+    for at in (first, first + 512, first + 3 * 16384 - 4, (2 << 20) + 1024):
+        assert _merge(lse=(at, 16, 1)) == 1, at
+    for at in (z, z - 1008, z - 3 * 16384 + 16, (4 << 20) + 176):
+        assert _merge(out=(at, 8192, 512)) == 1, at
+    # beside each other in one buffer of 16 x (1024 + 16) bytes a token: the lse of the next head
+    packed = dict(outs=(first, 2 << 20), strides=(8320, 520) * 2)
+    assert _merge(**packed, lse=(first + 1020, 4160, 260)) == 1
+    assert _merge(**packed, lse=(first + 1040 + 1020, 4160, 260)) == 1
+    if not torch.cuda.is_available():  # what is no overlap reaches the device, which is not there
+        assert _merge(lse=(first - 192, 16, 1)) == 5 and _merge(lse=(first + 3 * 16384, 16, 1)) == 5
+        assert _merge(out=(z - 3 * 16384, 8192, 512)) == 5 and _merge(out=(z + 192, 8192, 512)) == 5
+        assert _merge(**packed, lse=(first + 1024, 4160, 260)) == 5
+        # a token's lses behind its outputs
+        assert _merge(outs=(first, 2 << 20), strides=(8224, 512) * 2, lse=(first + 16384, 4112, 1)) == 5
+
+
+def test_merge_overlaps_against_every_byte():
+    """Random layouts near one another: what shares a byte is refused; with equal strides nothing else is."""
+    if torch.cuda.is_available():
+        pytest.skip("calls that are taken would run")
+    rng = random.Random(1)
+    taken = 0
+
+    def rows(p, sb, sh, tokens, heads, width):
+        return {p + t * sb + h * sh + i for t in range(tokens) for h in range(heads) for i in range(0, width, 4)}
+
+    for _ in range(1500):
+        tokens, heads = rng.choice((1, 2, 3)), rng.choice((1, 2, 3))
+        sh = rng.choice((512, 520, 1040, 16)) if rng.random() < 0.8 else 3 * 520
+        sb = rng.choice((512, heads * 520, heads * 1040 + 520, 520, 64))
+        lse_at = (1 << 20) + 4 * rng.randrange(-400, 1200 * tokens)
+        lb, lh = rng.choice(((sb // 2, sh // 2), (heads, 1), (sb // 2, 1), (3, 7)))
+        got = _merge(parts=1, outs=(1 << 20,), strides=(sb, sh), lses=(8 << 20,), lse_strides=(lb, lh),
+                     out=(16 << 20, sb, sh), lse=(lse_at, lb, lh), tokens=tokens, heads=heads)
+        a = rows(1 << 20, 2 * sb, 2 * sh, tokens, heads, 1024)
+        meets = not a.isdisjoint(rows(lse_at, 4 * lb, 4 * lh, tokens, heads, 4))
+        assert got == (1 if meets else 5) or (got == 1 and (lb, lh) != (sb // 2, sh // 2))
+        out_at = (1 << 20) + 16 * rng.randrange(-200, 300 * tokens)
+        other = _merge(parts=1, outs=(1 << 20,), strides=(sb, sh), lses=(8 << 20,), lse_strides=(lb, lh),
+                       out=(out_at, sb, sh), lse=(8 << 20, lb, lh), tokens=tokens, heads=heads)
+        meets = not a.isdisjoint(rows(out_at, 2 * sb, 2 * sh, tokens, heads, 1024))
+        assert other == (1 if meets and out_at != 1 << 20 else 5)
+        taken += (got == 5) + (other == 5)
+    assert taken > 500

@@ -660,3 +660,24 @@ def test_sparse_and_window_attention_joined():
         more = 2.0 ** -8 * (p @ k[:, :512].abs())
         ref.check(out[0][r:r + 1], want[0], want[2] + more + 2.0 ** -18, "output")
         ref.check(out[1][r:r + 1], want[1], want[3] + 2.0 ** -18, "lse")
+
+
+def test_merge_in_one_buffer():
+    """Outputs and lses of a token in one row."""
+    for tokens in (1, 5):
+        g = torch.Generator(device="cuda").manual_seed(tokens)
+        outs = [torch.randn(tokens, 16, 512, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2)]
+        lses = [torch.randn(tokens, 16, generator=g, device="cuda") for _ in range(2)]
+        want = ref.merge(outs, lses)
+        buf = torch.zeros(tokens, 16, 520, dtype=torch.bfloat16, device="cuda")
+        out, lse = buf[..., :512], buf.view(torch.float32)[..., 256]
+        merge_states(outs, lses, out, lse)
+        ref.check(out, want[0], want[2], "output")
+        ref.check(lse, want[1], want[3], "lse")
+        out.copy_(outs[0])
+        lse.copy_(lses[0])
+        merge_states([out, outs[1]], [lse, lses[1]], out, lse)
+        ref.check(out, want[0], want[2], "output in place")
+        ref.check(lse, want[1], want[3], "lse in place")
+        with pytest.raises(ValueError, match="overlap"):
+            merge_states([out, outs[1]], lses, out, out[..., 0:2].view(torch.float32)[..., 0])
