@@ -162,6 +162,8 @@ bool same_grid_meets(const Rows2& a, const Rows2& b, int64_t tokens, int64_t hea
 // between a token's first and last row counts (between the first and last of all, where the tokens'
 // strides differ too).
 bool overlaps(Rows2 a, Rows2 b, int64_t tokens, int64_t heads) {
+  if (tokens == 1) a.sb = b.sb = 0;
+  if (heads == 1) a.sh = b.sh = 0;
   if (a.sb == b.sb && a.sh == b.sh) return same_grid_meets(a, b, tokens, heads);
   auto whole = [](Rows2& r, int64_t n, int64_t stride) {
     const int64_t span = (n - 1) * stride;
@@ -177,8 +179,8 @@ bool overlaps(Rows2 a, Rows2 b, int64_t tokens, int64_t heads) {
 }
 
 // Whether they are the same rows.
-bool same_rows(const Rows2& a, const Rows2& b) {
-  return a.p == b.p && a.sb == b.sb && a.sh == b.sh;
+bool same_rows(const Rows2& a, const Rows2& b, int64_t tokens, int64_t heads) {
+  return a.p == b.p && (a.sb == b.sb || tokens == 1) && (a.sh == b.sh || heads == 1);
 }
 
 bool aligned_rows(const void* p, int64_t sb, int64_t sh) {
@@ -494,7 +496,7 @@ int dsa_merge_states(int32_t num_parts, const void* const* outputs,
     // a warp reads its own rows of all parts before it writes them, and no others
     auto spoils = [&](const Rows2& to, const Rows2& own, const Rows2& other) {
       return overlaps(to, other, num_tokens, num_heads) ||
-             (!same_rows(to, own) && overlaps(to, own, num_tokens, num_heads));
+             (!same_rows(to, own, num_tokens, num_heads) && overlaps(to, own, num_tokens, num_heads));
     };
     if (spoils(out_rows, o, z) || spoils(lse_rows, z, o))
       return DSA_ERR_INVALID_ARGUMENT;

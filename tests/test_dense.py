@@ -190,6 +190,16 @@ def test_merge_refuses_a_result_over_the_other_kind_of_part():
         assert _merge(outs=(first, 2 << 20), strides=(8224, 512) * 2, lse=(first + 16384, 4112, 1)) == 5
 
 
+def test_merge_takes_a_part_whose_unused_strides_differ():
+    """With one token or one head, that stride says nothing."""
+    first, z = 1 << 20, 3 << 20
+    for tokens, heads, out, lse in ((1, 16, (first, 9999 * 8, 512), (z, 5, 1)), (3, 1, (first, 8192, 8), (z, 16, 77)),
+                                    (1, 1, (first, 8, 16), (z, 9, 9))):
+        if not torch.cuda.is_available():
+            assert _merge(tokens=tokens, heads=heads, out=out, lse=lse) == 5
+        assert _merge(tokens=tokens, heads=heads, out=(out[0] + 16, *out[1:])) == 1
+
+
 def test_merge_overlaps_against_every_byte():
     """Random layouts near one another: what shares a byte is refused; with equal strides nothing else is."""
     if torch.cuda.is_available():

@@ -662,8 +662,8 @@ def test_sparse_and_window_attention_joined():
         ref.check(out[1][r:r + 1], want[1], want[3] + 2.0 ** -18, "lse")
 
 
-def test_merge_in_one_buffer():
-    """Outputs and lses of a token in one row."""
+def test_merge_in_place_through_another_view_and_in_one_buffer():
+    """One token whose part has another (unused) stride; outputs and lses of a token in one row."""
     for tokens in (1, 5):
         g = torch.Generator(device="cuda").manual_seed(tokens)
         outs = [torch.randn(tokens, 16, 512, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2)]
@@ -676,7 +676,8 @@ def test_merge_in_one_buffer():
         ref.check(lse, want[1], want[3], "lse")
         out.copy_(outs[0])
         lse.copy_(lses[0])
-        merge_states([out, outs[1]], [lse, lses[1]], out, lse)
+        own = out.as_strided(out.shape, (8 * 999, *out.stride()[1:])) if tokens == 1 else out
+        merge_states([own, outs[1]], [lse, lses[1]], out, lse)
         ref.check(out, want[0], want[2], "output in place")
         ref.check(lse, want[1], want[3], "lse in place")
         with pytest.raises(ValueError, match="overlap"):
