@@ -138,7 +138,7 @@ def kernel_window(q_nope, q_pe, ckv_cache, kpe_cache, page_table, lengths, sm_sc
         ext, ws, stream = fast
         try:
             rc = ext.decode_window(q_nope, q_pe, ckv_cache, kpe_cache,
-                                   -1 if page_size is None else int(page_size), page_table,
+                                   -1 if page_size is None else max(0, int(page_size)), page_table,
                                    lengths, row_offsets, reach, sinks, float(sm_scale), output,
                                    lse, ws, stream)
         except TypeError:
@@ -172,7 +172,7 @@ def kernel_shared(q_nope, q_pe, ckv_cache, kpe_cache, prefix_table, prefix_lengt
         ext, ws, stream = fast
         try:
             rc = ext.decode_shared(q_nope, q_pe, ckv_cache, kpe_cache,
-                                   -1 if page_size is None else int(page_size), prefix_table,
+                                   -1 if page_size is None else max(0, int(page_size)), prefix_table,
                                    prefix_lengths, group_offsets, page_table, lengths,
                                    row_offsets, float(sm_scale), output, lse, ws, stream)
         except TypeError:

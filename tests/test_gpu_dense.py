@@ -682,3 +682,16 @@ def test_merge_in_place_through_another_view_and_in_one_buffer():
         ref.check(lse, want[1], want[3], "lse in place")
         with pytest.raises(ValueError, match="overlap"):
             merge_states([out, outs[1]], lses, out, out[..., 0:2].view(torch.float32)[..., 0])
+
+
+def test_page_sizes_below_one_are_refused():
+    """By the direct route of a second call too, which writes "the pools' page size" as -1."""
+    args, _ = window_case([100], [1], 16, 64, 10, 0, poison=False)
+    s, _ = shared_case([70], [1], [100], [1], 16, 64, poison=False)
+    out, lse = outputs(1, 16)
+    kernel_window(*args, SM, out, lse, 10)
+    for size in (0, -1, -64):
+        with pytest.raises(ValueError, match="power of two"):
+            kernel_window(*args, SM, out, lse, 10, page_size=size)
+        with pytest.raises(ValueError, match="power of two"):
+            kernel_shared(*s, SM, out, lse, page_size=size)
