@@ -688,7 +688,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                         wrapped ? round : round ^ 1u));
       if (el && ok) {
         if (n > 0) ptx::mbar_arrive_expect_tx_cluster(full, (uint32_t)(n * kChunk * 128));
-        else ptx::mbar_arrive_cluster(full);
+        else ptx::mbar_arrive_relaxed_cluster(full);
       }
       return full;
     };
@@ -845,6 +845,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           round ^= 1u;
         }
       };
+      // The wait that also acquires at cluster scope: P and what the softmax warps of rank 1 read.
+      auto pair_wait = [&](uint32_t b, uint32_t parity) {
+        return wait(b, parity) && ptx::mbar_test_wait_cluster(b, parity);
+      };
       auto slot_at = [&]() -> uint64_t {
         return (uint64_t)(((at >= kSlots ? at - kSlots : at) * kSlotB) >> 4);
       };
@@ -859,7 +863,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int t = s.t0; ok && t < s.t1; ++t, ++i) {
             // P of two tiles before is written, so its S has been read
             if (i >= 2) {
-              ok = __all_sync(0xffffffffu, wait(bar(B_PF + (i & 1)), (uint32_t)(((i - 2) >> 1) & 1)));
+              ok = __all_sync(0xffffffffu, pair_wait(bar(B_PF + (i & 1)), (uint32_t)(((i - 2) >> 1) & 1)));
               ptx::tc_fence_after();
             }
             const uint32_t d = tmem + S_COL + 96 * (i & 1);
@@ -905,10 +909,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int t = s.t0; ok && t < s.t1; ++t, ++i) {
             skip(t == s.t0 ? 5 : 0);            // K of this tile
             skip(t + 1 < s.t1 ? 5 : 0);         // and of the next
-            ok = __all_sync(0xffffffffu, wait(bar(B_PF + (i & 1)), (uint32_t)((i >> 1) & 1)));
+            ok = __all_sync(0xffffffffu, pair_wait(bar(B_PF + (i & 1)), (uint32_t)((i >> 1) & 1)));
             // the last unit's output has been read
             if (ok && t == s.t0 && n > 0)
-              ok = __all_sync(0xffffffffu, wait(bar(B_OE), (uint32_t)((n - 1) & 1)));
+              ok = __all_sync(0xffffffffu, pair_wait(bar(B_OE), (uint32_t)((n - 1) & 1)));
             if (!ok) break;
             // S was read and O rescaled through tensor memory
             ptx::tc_fence_after();
@@ -1017,7 +1021,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
           ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive_cluster(oe);
+          if (lane == 0) ptx::mbar_arrive_relaxed_cluster(oe);
           // Four lanes swap pieces of 16 bytes, so that they write 64 consecutive bytes of each of
           // their rows in turn instead of 16 bytes of four: lane q gets piece q of row q ^ k from its
           // holder, which sends piece (its own q) ^ k.
@@ -1062,7 +1066,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ptx::tc_fence_before();
       }
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(oe);
+      if (lane == 0) ptx::mbar_arrive_relaxed_cluster(oe);
     };
     Seg s = {};
     int n = 0, t = 0, pos = 0;
@@ -1203,7 +1207,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (!ok) break;
         }
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive_cluster(pf0 + 8u * (uint32_t)(i & 1));
+        if (lane == 0) {
+          ptx::fence_release_smem_cluster();  // P of all lanes
+          ptx::mbar_arrive_relaxed_cluster(pf0 + 8u * (uint32_t)(i & 1));
+        }
       } else {
         if (!last.open) break;
         ok = __all_sync(0xffffffffu, wait(bar(B_PD), (uint32_t)((i - 1) & 1)));

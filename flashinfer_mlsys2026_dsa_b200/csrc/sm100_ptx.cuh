@@ -390,12 +390,29 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
       "h"((uint16_t)3)
       : "memory");
 }
-// Arrivals on an mbarrier of either CTA (a shared::cluster address).  Their order (release at CTA
-// scope, none for the expected bytes) is all that is needed where the data is this CTA's shared
-// memory, made visible to the async proxy before, or a copy's.  Release at cluster scope, and an
-// acquire at cluster scope in the wait, cost the issuing warp about 2,000 cycles each.
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// Arrivals on an mbarrier of either CTA (a shared::cluster address), and the look at one that takes
+// over what the other CTA's threads did before theirs.  The arrivals are relaxed: a copy completes its
+// own bytes on the barrier, and tcgen05 operations are ordered by tcgen05.fence on both sides.  What a
+// thread wrote to its own shared memory is handed over by the fence before its arrival, which is a
+// release at cluster scope of shared memory alone.  For 256 rows behind 32768 positions that costs 1 to
+// 2 % against arrivals that release at CTA scope only, which promises the other CTA nothing (321 us ->
+// 324-327); a release of all memory on the arrival itself costs 15 % (328 -> 377), the acquire nothing.
+__device__ __forceinline__ void mbar_arrive_relaxed_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_release_smem_cluster() {
+  asm volatile("fence.release.sync_restrict::shared::cta.cluster;" ::: "memory");
+}
+__device__ __forceinline__ bool mbar_test_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 __device__ __forceinline__ void mbar_arrive_expect_tx_cluster(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar),
