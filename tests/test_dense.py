@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import dense_reference as ref
+import dense_targets as aimed
 from flashinfer_mlsys2026_dsa_b200 import _native, kernel_shared, kernel_window, merge_states
 
 
@@ -228,3 +229,26 @@ def test_merge_overlaps_against_every_byte():
         assert other == (1 if meets and out_at != 1 << 20 else 5)
         taken += (got == 5) + (other == 5)
     assert taken > 500
+
+
+def test_aimed_queries_show_a_value_from_a_wrong_place():
+    """With a query for every eighth position, a chunk of 32 values that is left out, read as zero or
+    taken from elsewhere is far outside the bound, and a chunk counted twice outside lse's."""
+    n = 4096
+    ckv, kpe = ref.pools(n // 64, 64, 1, "cpu")
+    keys = ref.sequence(ckv, kpe, torch.arange(n // 64), n, 64)
+    at = aimed.spread(n // 8, n)
+    assert len(set(at.tolist())) == n // 8 and len(set((at // 32).tolist())) == n // 32
+    qn, qp = aimed.aim(keys, at.view(1, n // 8))
+    q = torch.cat([qn, qp], 2)
+    sm = 1 / math.sqrt(192.0)
+    out, lse, otol, ltol = ref.attend(q, keys, torch.ones(1, n, dtype=torch.bool), sm)
+    p = torch.softmax(q[0].double() @ keys.T * sm, 1)
+    assert p.gather(1, at[:, None]).min() > 0.9
+    for a in (0, 32 * 77, n - 32):
+        for values in (torch.zeros(32, 512, dtype=torch.float64), keys[(a + 192) % n:][:32, :512]):
+            wrong = (out[0] + p[:, a:a + 32] @ (values - keys[a:a + 32, :512])).to(torch.bfloat16)
+            off = ((wrong.double() - out[0]).abs() / otol[0]).amax(1)
+            assert (off > 10).sum() >= 2, a
+        twice = lse[0] + torch.log2(1 + p[:, a:a + 32].sum(1))
+        assert (((twice - lse[0]) / ltol[0]) > 10).sum() >= 2
