@@ -8,14 +8,17 @@
 //   O[128 x 512] += P V     2 x 12 instructions, N = 256; each CTA holds 256 of the value columns
 // O (fp32) fills half of each CTA's tensor memory, which no smaller group could: one CTA with
 // 128 rows would need all of it, and 64 rows in one CTA run the tensor cores at half rate.  In
-// this form S needs no exchange between the CTAs, Q and P stay with their rows, and a key passes
-// each CTA's shared memory 1.9 times (as K: its own half of the keys; as V: its half of the
-// columns), 63 bytes a cycle at the tensor cores' full rate, which L2 delivers.
+// this form S needs no exchange between the CTAs, Q and P stay with their rows, and each CTA takes
+// 1,088 of a key's 1,152 bytes into its shared memory (as K: its own half of the keys; as V: its half
+// of the columns), 63 bytes a cycle at the tensor cores' full rate, which L2 delivers.
 // Measured instruction costs (cycles): N = 64 .. 128 45, N = 192 48, N = 256 64; so 192 keys a
 // tile is the smallest at full rate, 17 cycles a key.
 //
-// The units of all rows form one line of tiles, cut into equal parts, one for each pair.  A unit
-// that is cut leaves partial results (O, maximum, sum) that combine kernels join.
+// The units of all rows form one line of tiles, cut into equal parts, one for each pair (window
+// calls with no more units than pairs: for as many pairs as are a multiple of the units; with a token
+// a row and more than half as many rows as pairs, a pair for each row and no cut).  A unit that is cut
+// leaves partial results (O, maximum, sum) that combine kernels join, and so does every unit of a
+// shared call.
 //
 // Warps of a CTA:  0 and 12 load keys, 13 and 14 values (64 columns each of a slot's 128), 1 and 15
 // issue the tensor-core work for S and for O (rank 0 alone), 2 loads queries, 3 walks the units,
@@ -280,9 +283,9 @@ __device__ __noinline__ void spoil(const Params& p, const Part& x, int pair) {
 }
 
 // Bounded wait on an mbarrier.  The kernel's roles run side by side, and their code has to fit the
-// instruction caches together: 256 rows behind 32768 shared positions took 614 us with 174 KB of it,
-// 331 with 109 KB, 317 with 85 KB.  So what follows a first look that fails is out of line, but for
-// the walker, whose loops are 25 KB longer with a call in them.
+// instruction caches together: 256 rows behind 32768 shared positions took 345 us with 109 KB of it and
+// 317 with 85 KB.  So what follows a first look that fails is out of line, but for the walker, whose
+// loops are 25 KB longer with a call in them.
 __device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
                                      uint32_t* err, uint64_t limit) {
   const uint64_t t0 = ptx::cycles();
@@ -436,7 +439,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       tiles = __reduce_add_sync(0xffffffffu, mine.x);
       const int units = __reduce_add_sync(0xffffffffu, mine.y);
-      // A window's units cost about the same: whole ones, or equal parts of each, while they fit.
+      // Windows that the rows fill cost about the same, and as many parts of each unit as of the
+      // others cut each of them the same number of times.  (Units of unequal length are cut where
+      // the line's equal parts end; up to half of the pairs have none.)
       pairs = p.pairs;
       if (p.groups == 0 && units <= pairs && units > 0) pairs = units * (pairs / units);
       pairs = min(pairs, tiles);

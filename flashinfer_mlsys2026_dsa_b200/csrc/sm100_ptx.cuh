@@ -85,7 +85,7 @@ __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* m) {
 // Four rows (row coordinates r.x..r.w) of `box[0]` elements starting at column
 // `col` land as four consecutive 128-byte rows at `dst` (swizzle applied by the
 // tensor map).  A row coordinate outside [0, dim1) reads nothing from global
-// memory; callers must not rely on the bytes that land for such a row.
+// memory and lands as the map's fill, zeros.
 __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* m, int32_t col,
                                             int4 r, uint32_t bar, uint64_t policy) {
   asm volatile(

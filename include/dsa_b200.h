@@ -319,7 +319,14 @@ int dsa_compact_q8(const int32_t* keep, int64_t keep_stride_b, int32_t num_rows,
  * its own; a row of length 0 with one token sees the prefix alone.
  *
  * Both need `scratch`, a device buffer of dsa_dense_scratch_size() bytes for this call alone
- * (calls that may overlap on the GPU need one each), 16-byte aligned.
+ * (calls that may overlap on the GPU need one each), 16-byte aligned.  A window call's does not
+ * depend on the tokens (39 MB for the 74 CTA pairs of a B200).  A shared call's grows with them: 4,112
+ * bytes for each (token, head) and 16 a token, beside 19 MB (64 tokens of 16 heads 24 MB, 8,192 tokens
+ * of 128 heads 4.3 GB); long prompts go in chunks.
+ *
+ * With row_offsets NULL and more than half as many rows as the GPU has CTA pairs, but no more than
+ * pairs, dsa_mla_decode_window() gives each row one pair.  Rows of very unequal length are faster with
+ * row_offsets 0, 1, 2, .. num_rows, which spread each row over several pairs.
  *
  * Only whole pages of the pool count.  A page table's stride may be 0 (rows that share one list).
  * Where a row has several tokens, a NaN or infinity that one of them sees may reach the others.
