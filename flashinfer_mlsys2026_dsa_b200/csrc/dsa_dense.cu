@@ -164,18 +164,22 @@ bool same_grid_meets(const Rows2& a, const Rows2& b, int64_t tokens, int64_t hea
 bool overlaps(Rows2 a, Rows2 b, int64_t tokens, int64_t heads) {
   if (tokens == 1) a.sb = b.sb = 0;
   if (heads == 1) a.sh = b.sh = 0;
-  if (a.sb == b.sb && a.sh == b.sh) return same_grid_meets(a, b, tokens, heads);
   auto whole = [](Rows2& r, int64_t n, int64_t stride) {
     const int64_t span = (n - 1) * stride;
     if (span < 0) r.p = static_cast<const char*>(r.p) + span;
     r.width += std::abs(span);
   };
-  for (Rows2* r : {&a, &b}) whole(*r, heads, r->sh);
-  a.sh = b.sh = 0;
-  if (a.sb == b.sb) return same_grid_meets(a, b, tokens, 1);
-  for (Rows2* r : {&a, &b}) whole(*r, tokens, r->sb);
-  a.sb = b.sb = 0;
-  return same_grid_meets(a, b, 1, 1);
+  Rows2 ta = a, tb = b;  // a row for each token
+  whole(ta, heads, a.sh);
+  whole(tb, heads, b.sh);
+  ta.sh = tb.sh = 0;
+  Rows2 all_a = ta, all_b = tb;
+  whole(all_a, tokens, a.sb);
+  whole(all_b, tokens, b.sb);
+  all_a.sb = all_b.sb = 0;
+  if (!same_grid_meets(all_a, all_b, 1, 1)) return false;  // apart, as most are
+  if (a.sb != b.sb) return true;
+  return a.sh == b.sh ? same_grid_meets(a, b, tokens, heads) : same_grid_meets(ta, tb, tokens, 1);
 }
 
 // Whether they are the same rows.
